@@ -54,8 +54,8 @@ typedef struct {
  * (src/main.rs:42-60).  Fails if the device is not gfx950. */
 int qh_create(int device, qh_ctx **out);
 void qh_destroy(qh_ctx *ctx);
-/* Message of the last failure on this context (or of qh_create when ctx is
- * NULL). */
+/* Message of the last failure on this context (or, when ctx is NULL, of
+ * qh_create and of this thread's calls without a context). */
 const char *qh_last_error(const qh_ctx *ctx);
 
 /* Parses and validates a GGUF image held in host memory and uploads every
@@ -337,6 +337,145 @@ int qh_bench_matvec(qh_ctx *ctx, const void *data, size_t len, uint32_t kind, si
  * launch by a plain streaming kernel; mean and median launch times as for
  * qh_bench_matvec (empty_ms is 0).  The matvec bandwidths are read against it. */
 int qh_bench_read(qh_ctx *ctx, size_t bytes, size_t copies, size_t iters, qh_matvec_timing_t *out);
+
+/* ---- operators on device tensors --------------------------------------- *
+ * For a program that serves several sequences from device memory of its own
+ * (no counterpart in the reference, which holds one sequence): a key-value
+ * cache in pages (append, attention of one new token per sequence, eviction)
+ * and the log probabilities of tokens.  They allocate nothing and keep nothing;
+ * what they read and write is device memory of the context's device.
+ *
+ *   - element kinds: 0 F32, 1 F16, 30 BF16 (GGML's ids), and in a cache 8 Q8_0;
+ *   - strides count elements; the last dimension is contiguous; a tensor is
+ *     aligned to its elements (kernels for tensors and strides aligned to 16
+ *     bytes are faster);
+ *   - stream NULL: the context's stream, and the call returns when its outputs
+ *     are written (its inputs must be there); QH_NULL_STREAM: the device's null
+ *     stream; else that HIP stream.  With a stream the call returns at once,
+ *     and may be captured into a graph.  A workspace belongs to one call at a
+ *     time: calls that may overlap, and graphs that may be replayed beside
+ *     each other, need one each;
+ *   - arguments on the host are checked, with an error; what lies in device
+ *     memory (lengths, page ids, targets) is checked by the kernels, which read
+ *     and write nothing out of range: each call says what it does instead;
+ *   - the calling thread's current HIP device is left as it was. */
+#define QH_NULL_STREAM ((void *)(intptr_t)-1)
+#define QH_BF16 30u
+
+/* A cache: element j of KV head g of slot s of page p is element p *
+ * page_stride + s * token_stride + g * head_stride + j of k and of v.  Q8_0
+ * (kind 8): k and v hold int8 codes, and k_scale and v_scale the f16 scale of
+ * each 32 of them at that offset / 32; dim and the strides are multiples of 32.
+ * dim is at most 256. */
+typedef struct {
+    void *k, *v;
+    void *k_scale, *v_scale; /* kind 8 only */
+    uint32_t kind, page, kvheads, dim;
+    uint64_t pages;
+    size_t page_stride, token_stride, head_stride;
+} qh_pages_t;
+
+/* Sequences: key t of sequence b is in slot t % page of page table[b *
+ * table_stride + t / page], t < length[b].  most: no length is above it (and
+ * table_pages pages hold that many); a sequence whose length is negative or
+ * above it counts as out of range.  A length of 0 is a row of padding. */
+typedef struct {
+    const int32_t *table;
+    const int32_t *length;
+    size_t table_stride, table_pages;
+    uint32_t batch, most;
+} qh_sequences_t;
+
+/* [rows][heads][dim] of F32, F16 or BF16. */
+typedef struct {
+    void *data;
+    uint32_t kind;
+    size_t row_stride, head_stride;
+} qh_heads_t;
+
+/* Q/K norm and RoPE on the way into the cache, and the queries that go with
+ * the keys.  q NULL data: no queries.  q_norm / k_norm: RMSNorm weights [dim]
+ * (NULL: none).  rope: (cos, sin) pairs [rope_rows][dim / 2], NeoX pairing
+ * (NULL: none; dim even); position: the row of each token (NULL: its place in
+ * its sequence).  A position outside the table makes the token's q and k NaN. */
+typedef struct {
+    qh_heads_t q, q_out;
+    uint32_t heads;
+    const float *q_norm, *k_norm;
+    float eps;
+    const float *rope;
+    size_t rope_rows;
+    const int32_t *position;
+} qh_append_t;
+
+/* Appends n tokens' k and v ([n][kvheads][dim]).  The lengths count them:
+ * sequence b's tokens are first[b] .. first[b + 1] - 1 of k and v (first:
+ * batch + 1 ascending numbers; NULL: one token each, n = batch), the last of
+ * them at length[b] - 1.  Values are rounded once to the cache's kind (Q8_0:
+ * scale max |x| / 127 of each 32, rounded to f16; a block with a value that is
+ * not finite becomes NaN).  Tokens without a place (in front of first[0] or
+ * behind first[batch], a length of 0 or out of range) leave every output as it
+ * was, those of a page id outside the cache leave the cache as it was.  Two
+ * sequences must not append to the same slot.  more: nullable. */
+int qh_paged_append(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,
+                    const qh_heads_t *k, const qh_heads_t *v, const qh_append_t *more, void *stream);
+
+/* Softmax weights of a cache's keys, summed over each KV head's query heads:
+ * in ([batch][kvheads][most], NULL: zeros) plus this call's to out, for every
+ * key of a sequence; out behind a sequence's keys is left as it was.  in and
+ * out may be the same. */
+typedef struct {
+    const float *in;
+    float *out;
+    size_t in_row, in_head, out_row, out_head; /* strides of sequences and KV heads */
+} qh_key_weights_t;
+
+/* Attention of one token per sequence over its cached keys (qh_attention's
+ * formula with a scale of the caller's): q and out [batch][heads][dim], heads a
+ * multiple of kvheads, query head h reading KV head h / (heads / kvheads).
+ * Sums in 32 bits, out rounded once to its kind.  A sequence without keys, or
+ * whose scores are all -inf, gives zeros; one with a length or a page id out of
+ * range NaN.  weights nullable; the weights of a sequence whose length is out of
+ * range are left as they were. */
+int qh_paged_attention(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const qh_heads_t *q,
+                       uint32_t heads, float scale, const qh_heads_t *out, const qh_key_weights_t *weights,
+                       void *workspace, size_t workspace_bytes, void *stream);
+/* Bytes of workspace that a call of these shapes needs (0: none; its pointer
+ * may then be NULL, else it is aligned to 16 bytes). */
+int qh_paged_attention_bytes(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, uint32_t heads,
+                             int with_weights, size_t *out);
+
+/* Brings every sequence to at most keep keys: of a longer one every KV head
+ * keeps its first `first` keys, its last `recent` and the heaviest of those
+ * between by weights ([batch][kvheads][most], strides weight_row and
+ * weight_head; total order as f32::total_cmp, the lower index on ties).  Kept
+ * keys move in ascending order to the slots 0.. of the pages to[b * to_stride +
+ * i] (to_pages of them a row), which no sequence of the call may read.  Outputs:
+ * kept[batch][kvheads][keep] their indexes (-1 behind them), kept_weights
+ * [batch][kvheads][keep] their weights (0 behind them), new_length[batch].  A
+ * sequence with a length or a page id out of range keeps nothing (length 0). */
+int qh_paged_evict(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const float *weights,
+                   size_t weight_row, size_t weight_head, size_t keep, size_t first, size_t recent, const int32_t *to,
+                   size_t to_stride, size_t to_pages, int32_t *kept, float *kept_weights, int32_t *new_length,
+                   void *stream);
+
+/* Rows of logits ([rows][vocab], row_stride) of F32, F16 or BF16: logp[rows] =
+ * log softmax at target[rows] (both nullable), entropy[rows] (nullable), and the
+ * top (0-128, at most vocab) ids of each row in descending total order, the
+ * lower id on ties, with their log probabilities (top_ids, top_logp
+ * [rows][top]).  valid: nullable [vocab] mask, ids with 0 read as f32::MIN (as
+ * in qh_sample_logits).  Sums in 32 bits.  A row that holds NaN or +inf gives
+ * NaN, one of -inf alone log probabilities of -inf and an entropy of 0, a target
+ * outside the vocabulary NaN.  At most 2^24 logits a row. */
+int qh_logprobs(qh_ctx *ctx, const void *logits, uint32_t kind, size_t rows, size_t vocab, size_t row_stride,
+                const int32_t *target, const uint8_t *valid, size_t top, float *logp, float *entropy, int32_t *top_ids,
+                float *top_logp, void *workspace, size_t workspace_bytes, void *stream);
+int qh_logprobs_bytes(qh_ctx *ctx, size_t rows, size_t vocab, size_t top, size_t *out);
+/* The same for the logits of the last token step (with qh_set_valid_tokens'
+ * mask), read where they are: target nullable, outputs on the host (top_ids and
+ * top_logp hold top values). */
+int qh_last_logprobs(qh_ctx *ctx, const uint32_t *target, size_t top, float *logp, float *entropy, uint32_t *top_ids,
+                     float *top_logp);
 
 #ifdef __cplusplus
 }

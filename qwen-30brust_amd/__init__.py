@@ -52,6 +52,35 @@ class _Inspect(C.Structure):
                 ("kv_f32_bytes_at_context", C.c_uint64)]
 
 
+class _Pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("kind", C.c_uint32), ("page", C.c_uint32), ("kvheads", C.c_uint32), ("dim", C.c_uint32),
+                ("pages", C.c_uint64), ("page_stride", C.c_size_t), ("token_stride", C.c_size_t),
+                ("head_stride", C.c_size_t)]
+
+
+class _Sequences(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("length", C.c_void_p), ("table_stride", C.c_size_t),
+                ("table_pages", C.c_size_t), ("batch", C.c_uint32), ("most", C.c_uint32)]
+
+
+class _Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("kind", C.c_uint32), ("row_stride", C.c_size_t), ("head_stride", C.c_size_t)]
+
+
+class _Append(C.Structure):
+    _fields_ = [("q", _Heads), ("q_out", _Heads), ("heads", C.c_uint32), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float), ("rope", C.c_void_p), ("rope_rows", C.c_size_t),
+                ("position", C.c_void_p)]
+
+
+class _KeyWeights(C.Structure):
+    _fields_ = [("before", C.c_void_p), ("after", C.c_void_p), ("before_row", C.c_size_t),
+                ("before_head", C.c_size_t), ("after_row", C.c_size_t), ("after_head", C.c_size_t)]
+
+
+NULL_STREAM = C.c_void_p(-1).value  # QH_NULL_STREAM
+
 _SIGS = {
     "qh_create": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),
     "qh_inspect": (C.c_int, [C.c_char_p, C.c_size_t, C.POINTER(_Inspect)]),
@@ -115,6 +144,22 @@ _SIGS = {
     "qh_bench_matvec": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_uint32, C.c_size_t,
                                   C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t,
                                   C.c_void_p]),
+    "qh_paged_append": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.c_void_p, C.c_size_t,
+                                  C.POINTER(_Heads), C.POINTER(_Heads), C.POINTER(_Append), C.c_void_p]),
+    "qh_paged_attention_bytes": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.c_uint32, C.c_int,
+                                           C.POINTER(C.c_size_t)]),
+    "qh_paged_attention": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.POINTER(_Heads),
+                                     C.c_uint32, C.c_float, C.POINTER(_Heads), C.POINTER(_KeyWeights), C.c_void_p,
+                                     C.c_size_t, C.c_void_p]),
+    "qh_paged_evict": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.c_void_p, C.c_size_t,
+                                 C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t,
+                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "qh_logprobs": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p,
+                              C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                              C.c_size_t, C.c_void_p]),
+    "qh_logprobs_bytes": (C.c_int, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.POINTER(C.c_size_t)]),
+    "qh_last_logprobs": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32), C.c_size_t, C.POINTER(C.c_float),
+                                   C.POINTER(C.c_float), C.c_void_p, C.c_void_p]),
 }
 
 _lib = None
@@ -232,6 +277,7 @@ class Device:
         if lib().qh_create(device, C.byref(h)) != 0:
             raise EngineError(lib().qh_last_error(None).decode())
         self.h = h
+        self.index = device
         _open_devices.add(self)
 
     def close(self):
@@ -416,6 +462,18 @@ class Model:
         out = C.c_uint32()
         self.dev._check(lib().qh_sample(self.dev.h, sampler.h, C.byref(out)))
         return out.value
+
+    def logprobs(self, target=None, top=0):
+        """Log probabilities after the last step, read on the device (with the
+        valid-token mask): (of target or None, entropy, ids of the top
+        alternatives, their log probabilities)."""
+        self._live()
+        t = None if target is None else C.c_uint32(target)
+        lp, h = C.c_float(), C.c_float()
+        ids, alt = np.zeros(top, np.uint32), np.zeros(top, np.float32)
+        self.dev._check(lib().qh_last_logprobs(self.dev.h, t, top, None if t is None else C.byref(lp), C.byref(h),
+                                               _ptr(ids), _ptr(alt)))
+        return None if t is None else lp.value, h.value, ids, alt
 
     def set_valid_tokens(self, valid):
         """Padding-vocab mask (src/main.rs:262-266); None clears it."""

@@ -24,6 +24,7 @@
 #include "kernels.hpp"
 #include "qh_rows.hpp"
 #include "qh_tile.hpp"
+#include "serving.hpp"
 
 namespace qh {
 // Kernels (kernels.hip).
@@ -424,7 +425,7 @@ template <class F> int guarded(qh_ctx* c, F f) {
         f();
         return 0;
     } catch (const std::exception& e) {
-        if (c) c->err = e.what();
+        (c ? c->err : g_create_err) = e.what();
         return 1;
     }
 }
@@ -2476,6 +2477,356 @@ int qh_bench_matvec(qh_ctx* c, const void* data, size_t len, uint32_t kind, size
         sync(c);
         for (float v : y)
             if (!std::isfinite(v)) throw Error("benchmark matvec produced a non-finite value");
+    });
+}
+
+// ------------------------------------------- operators on device tensors --
+// Checks of the host-side arguments; the kernels check what lies in device
+// memory.
+namespace {
+
+void need_ctx(const qh_ctx* c) {
+    if (!c) throw Error("null context");
+}
+
+// The context's device as the current one, and the caller's again at the end.
+struct OnDevice {
+    int before = 0;
+    explicit OnDevice(int device) {
+        HIP_OK(hipGetDevice(&before));
+        if (before != device) HIP_OK(hipSetDevice(device));
+        else before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+hipStream_t stream_of(const qh_ctx* c, void* stream) {
+    return stream == QH_NULL_STREAM ? nullptr : stream ? static_cast<hipStream_t>(stream) : c->s;
+}
+
+size_t kind_bytes(uint32_t kind, const char* what) {
+    if (kind == F32) return 4;
+    if (kind == F16 || kind == BF16) return 2;
+    throw Error(std::string(what) + ": unsupported element kind " + std::to_string(kind));
+}
+
+void need_ptr(const void* p, size_t align, const char* what) {
+    if (!p) throw Error(std::string("null ") + what);
+    if ((uintptr_t)p % align) throw Error(std::string(what) + " is not aligned to its elements");
+}
+
+// sum of (count - 1) * stride + last stays below 2^60 elements
+void need_extent(std::initializer_list<std::pair<uint64_t, uint64_t>> dims, const char* what) {
+    unsigned __int128 e = 0;
+    for (const auto& [count, stride] : dims) e += (unsigned __int128)(count ? count - 1 : 0) * stride;
+    if (e >> 60) throw Error(std::string(what) + ": strides beyond the address space");
+}
+
+Pages pages_of(const qh_pages_t* p) {
+    if (!p) throw Error("null cache");
+    if (!p->page || !p->kvheads || !p->dim || !p->pages) throw Error("empty cache shape");
+    if (p->dim > kPageMaxDim) throw Error("cache heads are at most " + std::to_string(kPageMaxDim) + " wide");
+    if (p->pages > 0x7fffffffu) throw Error("too many pages");
+    if (p->kvheads > 65535 || p->page > (1u << 30)) throw Error("cache shape out of range");
+    const bool q8 = p->kind == Q8_0;
+    const size_t es = q8 ? 1 : kind_bytes(p->kind, "cache");
+    need_ptr(p->k, es, "cache keys");
+    need_ptr(p->v, es, "cache values");
+    if (q8) {
+        need_ptr(p->k_scale, 2, "cache key scales");
+        need_ptr(p->v_scale, 2, "cache value scales");
+        if (p->dim % 32 || p->page_stride % 32 || p->token_stride % 32 || p->head_stride % 32)
+            throw Error("a Q8_0 cache's head width and strides are multiples of 32");
+    }
+    need_extent({{p->pages, p->page_stride}, {p->page, p->token_stride}, {p->kvheads, p->head_stride}}, "cache");
+    Pages c{};
+    c.k = static_cast<uint8_t*>(p->k);
+    c.v = static_cast<uint8_t*>(p->v);
+    c.ks = q8 ? static_cast<_Float16*>(p->k_scale) : nullptr;
+    c.vs = q8 ? static_cast<_Float16*>(p->v_scale) : nullptr;
+    c.ps = p->page_stride;
+    c.ts = p->token_stride;
+    c.hs = p->head_stride;
+    c.kind = p->kind;
+    c.page = p->page;
+    c.kvheads = p->kvheads;
+    c.dim = p->dim;
+    c.count = (uint32_t)p->pages;
+    return c;
+}
+
+Rows rows_of(const qh_sequences_t* q, const Pages& c) {
+    if (!q) throw Error("null sequences");
+    if (q->batch > 65535) throw Error("at most 65535 sequences");
+    if (q->most > 0x7fffffffu - (1u << 20)) throw Error("sequences are too long");
+    if (q->batch) {
+        need_ptr(q->length, 4, "lengths");
+        if (q->most) need_ptr(q->table, 4, "page table");
+        if ((uint64_t)q->table_pages * c.page < q->most) throw Error("the page table's rows hold fewer keys than the longest length");
+        need_extent({{q->batch, q->table_stride}, {q->table_pages, 1}}, "page table");
+    }
+    Rows r{};
+    r.table = q->table;
+    r.length = q->length;
+    r.stride = q->table_stride;
+    r.batch = q->batch;
+    r.most = q->most;
+    return r;
+}
+
+Heads heads_of(const qh_heads_t* h, uint64_t rows, uint64_t heads, const char* what) {
+    if (!h) throw Error(std::string("null ") + what);
+    const size_t es = kind_bytes(h->kind, what);
+    if (rows) need_ptr(h->data, es, what);
+    need_extent({{rows, h->row_stride}, {heads, h->head_stride}}, what);
+    Heads r{};
+    r.p = static_cast<uint8_t*>(h->data);
+    r.row = h->row_stride;
+    r.head = h->head_stride;
+    r.kind = h->kind;
+    return r;
+}
+
+void need_heads(uint32_t heads, uint32_t kvheads) {
+    if (!heads || heads % kvheads || heads > 65535) throw Error("query heads are a multiple of the KV heads");
+}
+
+PageAttn attn_of(const qh_pages_t* cache, const qh_sequences_t* seqs, uint32_t heads) {
+    PageAttn a{};
+    a.c = pages_of(cache);
+    a.r = rows_of(seqs, a.c);
+    need_heads(heads, a.c.kvheads);
+    if ((uint64_t)a.r.batch * heads > (1u << 24)) throw Error("too many sequences and heads");
+    a.heads = heads;
+    return a;
+}
+
+void need_workspace(const void* p, size_t have, size_t need) {
+    if (!need) return;
+    if (have < need) throw Error("workspace of " + std::to_string(have) + " bytes, " + std::to_string(need) + " needed");
+    need_ptr(p, 16, "workspace");
+}
+
+// The call's kernels are launched; without a stream of the caller's, waits.
+void launched(const qh_ctx* c, void* stream) {
+    HIP_OK(hipGetLastError());
+    if (!stream) HIP_OK(hipStreamSynchronize(c->s));
+}
+
+Logprobs logprobs_of(const void* logits, uint32_t kind, size_t rows, size_t vocab, size_t stride, size_t top) {
+    const size_t es = kind_bytes(kind, "logits");
+    if (!vocab || vocab > (1u << 24)) throw Error("a row holds 1 to 16777216 logits");
+    if (rows > 0x7fffffffu / 256) throw Error("too many rows");
+    if (top > kLogprobMaxTop || top > vocab) throw Error("at most " + std::to_string(kLogprobMaxTop) + " alternatives, and no more than logits");
+    if (rows) need_ptr(logits, es, "logits");
+    need_extent({{rows, stride}}, "logits");
+    Logprobs a{};
+    a.x = logits;
+    a.kind = kind;
+    a.rows = (uint32_t)rows;
+    a.vocab = (uint32_t)vocab;
+    a.stride = stride;
+    a.top = (uint32_t)top;
+    return a;
+}
+
+}  // namespace
+
+int qh_paged_append(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, const int32_t* first, size_t n,
+                    const qh_heads_t* k, const qh_heads_t* v, const qh_append_t* more, void* stream) {
+    return guarded(c, [&] {
+        PageAppend a{};
+        a.c = pages_of(cache);
+        a.r = rows_of(seqs, a.c);
+        if (n > (1u << 24)) throw Error("at most 16777216 tokens");
+        if (!first && n != a.r.batch) throw Error("one token per sequence needs as many tokens as sequences");
+        if (first) need_ptr(first, 4, "first tokens");
+        a.first = first;
+        a.n = (uint32_t)n;
+        a.k = heads_of(k, n, a.c.kvheads, "keys");
+        a.v = heads_of(v, n, a.c.kvheads, "values");
+        if (more) {
+            if (more->q.data) {
+                need_heads(more->heads, a.c.kvheads);
+                a.heads = more->heads;
+                a.q = heads_of(&more->q, n, a.heads, "queries");
+                a.qo = heads_of(&more->q_out, n, a.heads, "query outputs");
+            }
+            a.qw = more->q_norm;
+            a.kw = more->k_norm;
+            if (a.qw) need_ptr(a.qw, 4, "query norm weights");
+            if (a.kw) need_ptr(a.kw, 4, "key norm weights");
+            a.eps = more->eps;
+            if (more->rope) {
+                if (a.c.dim % 2) throw Error("RoPE needs an even head width");
+                if (!more->rope_rows || more->rope_rows > 0x7fffffffu) throw Error("table of angles out of range");
+                need_ptr(more->rope, 8, "table of angles");
+                a.rope = reinterpret_cast<const float2*>(more->rope);
+                a.rope_rows = (uint32_t)more->rope_rows;
+                a.pos = more->position;
+                if (a.pos) need_ptr(a.pos, 4, "positions");
+            }
+        }
+        if ((uint64_t)n * (a.heads + 2ull * a.c.kvheads) > 0x7fffffffu) throw Error("too many tokens and heads");
+        if (!n || !a.r.batch || !a.r.most) return;
+        need_ctx(c);
+        const OnDevice on(c->device);
+        launch_page_append(a, stream_of(c, stream));
+        launched(c, stream);
+    });
+}
+
+int qh_paged_attention_bytes(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, uint32_t heads,
+                             int with_weights, size_t* out) {
+    return guarded(c, [&] {
+        if (!out) throw Error("null output buffer");
+        PageAttn a = attn_of(cache, seqs, heads);
+        *out = a.r.batch ? page_attn_plan(a, with_weights) : 0;
+    });
+}
+
+int qh_paged_attention(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, const qh_heads_t* q,
+                       uint32_t heads, float scale, const qh_heads_t* out, const qh_key_weights_t* weights,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded(c, [&] {
+        PageAttn a = attn_of(cache, seqs, heads);
+        a.q = heads_of(q, a.r.batch, heads, "queries");
+        a.out = heads_of(out, a.r.batch, heads, "attention outputs");
+        a.scale = scale;
+        if (!a.r.batch) return;
+        if (weights && a.r.most) {
+            need_ptr(weights->out, 4, "weight outputs");
+            if (weights->in) need_ptr(weights->in, 4, "weights");
+            need_extent({{a.r.batch, weights->in_row}, {a.c.kvheads, weights->in_head}, {a.r.most, 1}}, "weights");
+            need_extent({{a.r.batch, weights->out_row}, {a.c.kvheads, weights->out_head}, {a.r.most, 1}}, "weight outputs");
+            a.win = weights->in;
+            a.wout = weights->out;
+            a.win_row = weights->in_row;
+            a.win_head = weights->in_head;
+            a.wout_row = weights->out_row;
+            a.wout_head = weights->out_head;
+        }
+        need_workspace(workspace, workspace_bytes, page_attn_plan(a, weights));
+        page_attn_place(a, workspace, weights);
+        need_ctx(c);
+        const OnDevice on(c->device);
+        launch_page_attn(a, stream_of(c, stream));
+        launched(c, stream);
+    });
+}
+
+int qh_paged_evict(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, const float* weights,
+                   size_t weight_row, size_t weight_head, size_t keep, size_t first, size_t recent, const int32_t* to,
+                   size_t to_stride, size_t to_pages, int32_t* kept, float* kept_weights, int32_t* new_length,
+                   void* stream) {
+    return guarded(c, [&] {
+        PageEvict a{};
+        a.c = pages_of(cache);
+        a.r = rows_of(seqs, a.c);
+        if (!keep || keep > 0x7fffffffu / 2) throw Error("keys to keep out of range");
+        if (first > keep || recent > keep - first) throw Error("the first and recent keys are more than those kept");
+        if (!a.r.batch) return;
+        const uint64_t most = std::min<uint64_t>(keep, a.r.most);
+        if ((uint64_t)to_pages * a.c.page < most) throw Error("the new pages hold fewer keys than those kept");
+        if (a.r.most) {
+            need_ptr(weights, 4, "weights");
+            need_ptr(to, 4, "new pages");
+        }
+        need_ptr(kept, 4, "kept indexes");
+        need_ptr(kept_weights, 4, "kept weights");
+        need_ptr(new_length, 4, "new lengths");
+        need_extent({{a.r.batch, weight_row}, {a.c.kvheads, weight_head}, {a.r.most, 1}}, "weights");
+        need_extent({{a.r.batch, to_stride}, {to_pages, 1}}, "new pages");
+        a.w = weights;
+        a.w_row = weight_row;
+        a.w_head = weight_head;
+        a.keep = (uint32_t)keep;
+        a.first = (uint32_t)first;
+        a.recent = (uint32_t)recent;
+        a.to = to;
+        a.to_stride = to_stride;
+        a.kept = kept;
+        a.wout = kept_weights;
+        a.length = new_length;
+        need_ctx(c);
+        const OnDevice on(c->device);
+        launch_page_evict(a, stream_of(c, stream));
+        launched(c, stream);
+    });
+}
+
+int qh_logprobs_bytes(qh_ctx* c, size_t rows, size_t vocab, size_t top, size_t* out) {
+    return guarded(c, [&] {
+        if (!out) throw Error("null output buffer");
+        const Logprobs a = logprobs_of(nullptr, F32, 0, vocab, vocab, top);
+        if (rows > 0x7fffffffu / 256) throw Error("too many rows");
+        *out = rows ? logprobs_bytes((uint32_t)rows, a.vocab, a.top) : 0;
+    });
+}
+
+int qh_logprobs(qh_ctx* c, const void* logits, uint32_t kind, size_t rows, size_t vocab, size_t row_stride,
+                const int32_t* target, const uint8_t* valid, size_t top, float* logp, float* entropy, int32_t* top_ids,
+                float* top_logp, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded(c, [&] {
+        Logprobs a = logprobs_of(logits, kind, rows, vocab, row_stride, top);
+        if (!target != !logp) throw Error("targets and their log probabilities go together");
+        if (!rows) return;
+        if (target) {
+            need_ptr(target, 4, "targets");
+            need_ptr(logp, 4, "log probabilities");
+        }
+        if (entropy) need_ptr(entropy, 4, "entropies");
+        if (top) {
+            need_ptr(top_ids, 4, "alternatives");
+            need_ptr(top_logp, 4, "log probabilities of the alternatives");
+        }
+        need_workspace(workspace, workspace_bytes, logprobs_bytes(a.rows, a.vocab, a.top));
+        a.target = target;
+        a.valid = valid;
+        a.logp = logp;
+        a.entropy = entropy;
+        a.ids = top_ids;
+        a.alt = top_logp;
+        a.work = workspace;
+        need_ctx(c);
+        const OnDevice on(c->device);
+        launch_logprobs(a, stream_of(c, stream));
+        launched(c, stream);
+    });
+}
+
+int qh_last_logprobs(qh_ctx* c, const uint32_t* target, size_t top, float* logp, float* entropy, uint32_t* top_ids,
+                     float* top_logp) {
+    return guarded(c, [&] {
+        need_model(c);
+        if (c->pos == 0) throw Error("no logits: run a token step first");
+        if (!target != !logp) throw Error("targets and their log probabilities go together");
+        if (target && *target >= c->cfg.vocab) throw Error("token outside vocabulary");
+        if (top && (!top_ids || !top_logp)) throw Error("null output buffer");
+        Logprobs a = logprobs_of(c->acts.logits, F32, 1, c->cfg.vocab, c->cfg.vocab, top);
+        const OnDevice on(c->device);
+        // [target][logp][entropy][ids][their log probabilities][workspace]
+        const size_t head = (12 + 8 * top + 255) / 256 * 256;
+        c->samp_big.reserve(head + logprobs_bytes(1, a.vocab, a.top));
+        uint8_t* p = static_cast<uint8_t*>(c->samp_big.p);
+        const int32_t id = target ? (int32_t)*target : 0;
+        copy_in(c, p, &id, 4);
+        a.target = reinterpret_cast<int32_t*>(p);
+        a.valid = c->valid_n ? c->valid.as<uint8_t>() : nullptr;
+        a.logp = reinterpret_cast<float*>(p + 4);
+        a.entropy = reinterpret_cast<float*>(p + 8);
+        a.ids = reinterpret_cast<int32_t*>(p + 12);
+        a.alt = reinterpret_cast<float*>(p + 12 + 4 * top);
+        a.work = p + head;
+        launch_logprobs(a, c->s);
+        HIP_OK(hipGetLastError());
+        if (target) copy_out(c, logp, a.logp, 4);
+        if (entropy) copy_out(c, entropy, a.entropy, 4);
+        copy_out(c, top_ids, a.ids, 4 * top);
+        copy_out(c, top_logp, a.alt, 4 * top);
+        sync(c);
     });
 }
 
