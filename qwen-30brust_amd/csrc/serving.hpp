@@ -73,6 +73,7 @@ struct PageAttn {
     uint32_t heads;
     float scale;
     uint32_t span, splits;
+    uint32_t groups, per;  // a KV head's query heads, `per` to a workgroup
     float *ml, *o;          // null: one part, written to out
     float* score;           // [batch][heads][score_row] scaled scores, or null
     size_t score_row;
@@ -80,7 +81,8 @@ struct PageAttn {
     float* wout;            // and with this call's added
     size_t win_row, win_head, wout_row, wout_head;
 };
-// Sets span and splits; bytes of workspace.
+// Chooses the parts and head groups, whatever the queries' kind; bytes of
+// workspace.
 size_t page_attn_plan(PageAttn& a, bool weights);
 void page_attn_place(PageAttn& a, void* work, bool weights);
 void launch_page_attn(const PageAttn& a, hipStream_t s);
