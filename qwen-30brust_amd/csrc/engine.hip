@@ -2489,6 +2489,8 @@ void need_ctx(const qh_ctx* c) {
     if (!c) throw Error("null context");
 }
 
+uint32_t cus_of(const qh_ctx* c) { return c ? c->num_cu : 256; }
+
 // The context's device as the current one, and the caller's again at the end.
 struct OnDevice {
     int before = 0;
@@ -2683,7 +2685,11 @@ int qh_paged_attention_bytes(qh_ctx* c, const qh_pages_t* cache, const qh_sequen
     return guarded(c, [&] {
         if (!out) throw Error("null output buffer");
         PageAttn a = attn_of(cache, seqs, heads);
-        *out = a.r.batch ? page_attn_plan(a, with_weights) : 0;
+        *out = 0;
+        for (const bool fast : {false, true}) {  // the queries' kind decides
+            page_attn_plan(a, fast, cus_of(c));
+            if (a.r.batch) *out = std::max(*out, page_attn_bytes(a, with_weights));
+        }
     });
 }
 
@@ -2708,7 +2714,8 @@ int qh_paged_attention(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t*
             a.wout_row = weights->out_row;
             a.wout_head = weights->out_head;
         }
-        need_workspace(workspace, workspace_bytes, page_attn_plan(a, weights));
+        page_attn_plan(a, page_attn_fast(a), cus_of(c));
+        need_workspace(workspace, workspace_bytes, page_attn_bytes(a, weights));
         page_attn_place(a, workspace, weights);
         need_ctx(c);
         const OnDevice on(c->device);

@@ -137,115 +137,234 @@ void launch_page_append(const PageAppend& a, hipStream_t s) {
 // --------------------------------------------------------------- attention --
 //   s_t = scale * log2(e) * q . k_t,  m = max s_t,  l = sum 2^(s_t - m),
 //   o = sum 2^(s_t - m) v_t / l
-// over the keys of one sequence, in parts of `span` keys whose (m, l, o) are
-// folded by k_page_join; everything in 32 bits.  A row with no keys, or whose
-// scores are all -inf, is zeros.
+// over the keys of one sequence, everything in 32 bits.  A row with no keys, or
+// whose scores are all -inf, is zeros.
+//
+// Work is counted in steps of 32 keys of a unit (a sequence, one of its KV heads
+// and `per` of that head's query heads), a sequence without keys as one, and
+// kUnitCost more for its start and end.  All units' steps, one behind the other, are dealt to the workgroups in equal runs,
+// whatever the lengths: a ragged batch and one long sequence both fill the
+// chip.  A run may hold several units; one that it holds whole goes straight to
+// out, and at most the first and the last it holds in part: their (m, l, o) go
+// to the workgroup's two slots, and k_page_join folds them.  Lengths are known on
+// the device only, so every workgroup finds its run from them (a wave per 64
+// lengths and pass).
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kStep = 32, kRunMin = 4;  // keys; steps of a run at least
+constexpr uint32_t kUnitCost = 4;            // steps in front of a unit's own that are not work
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32
 
-// One head and part per workgroup, any head width up to 8 E: eight lanes share
-// a key, with E elements of its row each, and keep the (m, l, o) of their own
-// keys, so there is no barrier before the merge at the end.
+__device__ __forceinline__ uint32_t steps_of(int32_t len) {
+    return (len <= 0 ? 1u : ((uint32_t)len + kStep - 1) / kStep) + kUnitCost;
+}
+__device__ __forceinline__ uint64_t div64(uint64_t a, uint64_t b) {
+    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+}
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t same64(uint64_t v) { return (uint64_t)same((uint32_t)(v >> 32)) << 32 | same((uint32_t)v); }
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) { return __shfl((unsigned long long)v, lane, 64); }
+
+// The steps of sequences [0, end), by a wave.
+__device__ __forceinline__ uint64_t steps_before(const PageAttn& a, uint32_t end) {
+    uint64_t n = 0;
+    for (uint32_t j = threadIdx.x & 63; j < end; j += 64) n += steps_of(length_of(a.r, j));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor((unsigned long long)n, o, 64);
+    return same64(n);
+}
+// Run i of `total` steps in all holds the steps [total i / runs, total (i + 1) /
+// runs); fewer runs where they would be too short.
+__device__ __forceinline__ uint64_t runs_of(const PageAttn& a, uint64_t total) {
+    const uint64_t n = (total + kRunMin - 1) / kRunMin;
+    return n < a.runs ? n : a.runs;
+}
+__device__ __forceinline__ uint64_t run_begin(uint64_t total, uint64_t runs, uint64_t i) { return div64(total * i, runs); }
+__device__ __forceinline__ uint64_t run_with(uint64_t total, uint64_t runs, uint64_t x) {  // the run of step x
+    return div64((x + 1) * runs + total - 1, total) - 1;
+}
+
+// A workgroup's run: unit u (of a.units) of sequence b, from step r of its
+// `steps`; `left` steps to go.  Of a unit in hand: key(), the first key, and
+// end(), behind the last.
+struct Run {
+    uint32_t b, u, r, steps;
+    int32_t len;
+    uint64_t x, left;  // the step's number
+    __device__ __forceinline__ bool start(const PageAttn& a) {
+        const uint32_t lane = threadIdx.x & 63;
+        const uint64_t total = a.units * steps_before(a, a.r.batch), runs = runs_of(a, total);
+        if (blockIdx.x >= runs) return false;
+        x = run_begin(total, runs, blockIdx.x);
+        left = run_begin(total, runs, blockIdx.x + 1) - x;
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.begin[a.r.batch] = total;
+        uint64_t base = 0;
+        for (uint32_t j = 0;; j += 64) {  // ends: x lies in a sequence
+            const uint32_t n = j + lane < a.r.batch ? steps_of(length_of(a.r, j + lane)) : 0;
+            uint64_t sum = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint64_t t = __shfl_up((unsigned long long)sum, o, 64);
+                if (lane >= (uint32_t)o) sum += t;
+            }
+            const uint64_t past = __ballot(a.units * (base + sum) > x);
+            if (past) {
+                const int at = __ffsll((unsigned long long)past) - 1;
+                b = same(j + at);
+                steps = same(__shfl(n, at, 64));
+                const uint64_t rest = same64(x - a.units * (base + shfl64(sum - n, at)));
+                u = (uint32_t)div64(rest, steps);
+                r = (uint32_t)(rest - (uint64_t)u * steps);
+                break;
+            }
+            base += same64(shfl64(sum, 63));
+        }
+        len = (int32_t)same(length_of(a.r, b));
+        note(a);
+        return true;
+    }
+    // for k_page_join
+    __device__ __forceinline__ void note(const PageAttn& a) const {
+        if (u == 0 && r == 0 && threadIdx.x == 0) a.begin[b] = x;
+    }
+    // steps of the unit in hand
+    __device__ __forceinline__ uint32_t here() const { return (uint32_t)min((uint64_t)(steps - r), left); }
+    __device__ __forceinline__ uint32_t key() const { return (max(r, kUnitCost) - kUnitCost) * kStep; }
+    __device__ __forceinline__ uint32_t end() const {
+        const uint32_t n = len < 0 ? 0u : (uint32_t)len, s = max(r + here(), kUnitCost) - kUnitCost;
+        return r + here() == steps ? n : min(n, s * kStep);
+    }
+    __device__ __forceinline__ bool none() const { return r + here() <= kUnitCost; }  // no step of its own
+    __device__ __forceinline__ bool head() const { return r <= kUnitCost; }           // its first step
+    __device__ __forceinline__ bool whole() const { return head() && r + here() == steps; }
+    __device__ __forceinline__ bool next(const PageAttn& a) {
+        x += here();
+        left -= here();
+        if (left == 0) return false;
+        r = 0;
+        if (++u == a.units) {
+            u = 0;
+            len = (int32_t)same(length_of(a.r, ++b));
+            steps = steps_of(len);
+            note(a);
+        }
+        return true;
+    }
+};
+
+// Where head n of a unit goes: a whole unit to out, a part to a slot of the
+// workgroup (0: a part that starts inside its unit, 1: one that starts with it).
+__device__ __forceinline__ void store_part(const PageAttn& a, const Run& w, uint32_t h, uint32_t n, uint32_t j, float M,
+                                           float L, float O) {
+    if (w.whole()) {
+        put_kind(a.out.kind, a.out.p, w.b * a.out.row + h * a.out.head + j, L == 0.f ? 0.f : O / L);
+        if (a.sum && j == 0) a.sum[(size_t)w.b * a.heads + h] = make_float2(M, L);
+        return;
+    }
+    const size_t slot = ((size_t)blockIdx.x * 2 + w.head()) * a.per + n;
+    a.o[slot * a.c.dim + j] = O;
+    if (j == 0) a.ml[slot] = make_float2(M, L);
+}
+
+// One query head, any head width up to 8 E: eight lanes share a key, with E
+// elements of its row each, and keep the (m, l, o) of their own keys, so there is
+// no barrier before the merge at the end.
 template <uint32_t K, int E>
 __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
     __shared__ float red[kWaves][8 * E], rm[kWaves], rl[kWaves];
-    const uint32_t h = blockIdx.x, part = blockIdx.y, b = blockIdx.z, d = a.c.dim;
-    const uint32_t g = h / (a.heads / a.c.kvheads);
-    const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, kl = lane >> 3, p = lane & 7;
-    const int32_t len = length_of(a.r, b);
-    const uint32_t n = len < 0 ? 0u : (uint32_t)len, k0 = part * a.span;
-    if (part && k0 >= n) return;  // k_page_join does not read it
-    const uint32_t k1 = min(n, k0 + a.span);
-    float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; i++) {
-        const uint32_t e = p + 8 * i;
-        q[i] = e < d ? elem_kind(a.q.kind, a.q.p, b * a.q.row + h * a.q.head + e) : 0.f;
-        o[i] = 0.f;
-    }
-    bool bad = len < 0;
-    for (uint32_t t = k0 + 8 * wv + kl; t - kl < k1; t += 8 * kWaves) {  // wave-uniform
-        const uint32_t tt = min(t, k1 - 1);
-        int32_t page = gld<int32_t>(a.r.table + b * a.r.stride + tt / a.c.page);
-        if (page < 0 || (uint32_t)page >= a.c.count) {
-            bad = true;
-            page = 0;
-        }
-        const size_t at = (size_t)page * a.c.ps + (size_t)(tt % a.c.page) * a.c.ts + g * a.c.hs;
-        float kr[E], vr[E];
+    const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, kl = lane >> 3, p = lane & 7, d = a.c.dim;
+    Run w;
+    if (!w.start(a)) return;
+    do {
+        const uint32_t h = w.u, b = w.b, g = h / (a.heads / a.c.kvheads);
+        const uint32_t k0 = w.key(), k1 = w.end();
+        if (w.none()) continue;
+        float q[E], o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < E; i++) {
             const uint32_t e = p + 8 * i;
-            kr[i] = vr[i] = 0.f;
-            if (e < d) {
-                kr[i] = elem<K>(a.c.k, at + e);
-                vr[i] = elem<K>(a.c.v, at + e);
-                if constexpr (K == Q8_0) {
-                    kr[i] *= (float)gld<_Float16>(a.c.ks + (at + e) / 32);
-                    vr[i] *= (float)gld<_Float16>(a.c.vs + (at + e) / 32);
+            q[i] = e < d ? elem_kind(a.q.kind, a.q.p, b * a.q.row + h * a.q.head + e) : 0.f;
+            o[i] = 0.f;
+        }
+        bool bad = w.len < 0;
+        for (uint32_t t = k0 + 8 * wv + kl; t - kl < k1; t += 8 * kWaves) {  // wave-uniform
+            const uint32_t tt = min(t, k1 - 1);
+            int32_t page = gld<int32_t>(a.r.table + b * a.r.stride + tt / a.c.page);
+            if (page < 0 || (uint32_t)page >= a.c.count) {
+                bad = true;
+                page = 0;
+            }
+            const size_t at = (size_t)page * a.c.ps + (size_t)(tt % a.c.page) * a.c.ts + g * a.c.hs;
+            float kr[E], vr[E];
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const uint32_t e = p + 8 * i;
+                kr[i] = vr[i] = 0.f;
+                if (e < d) {
+                    kr[i] = elem<K>(a.c.k, at + e);
+                    vr[i] = elem<K>(a.c.v, at + e);
+                    if constexpr (K == Q8_0) {
+                        kr[i] *= (float)gld<_Float16>(a.c.ks + (at + e) / 32);
+                        vr[i] *= (float)gld<_Float16>(a.c.vs + (at + e) / 32);
+                    }
                 }
             }
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < E; i++) s = fmaf(q[i], kr[i], s);
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) s += __shfl_xor(s, x, 64);
+            s *= a.scale * kLog2e;
+            if (t >= k1) continue;  // not 0 times the value of a key past the end
+            if (a.score && p == 0) a.score[((size_t)b * a.heads + h) * a.score_row + t] = s;
+            const float M = fmaxf(m, s), Mf = M == -INFINITY ? 0.f : M;
+            const float alpha = exp2_of(m - Mf), e = exp2_of(s - Mf);
+            m = M;
+            l = fmaf(l, alpha, e);
+#pragma unroll
+            for (int i = 0; i < E; i++) o[i] = fmaf(e, vr[i], o[i] * alpha);
         }
-        float s = 0.f;
+        if (bad) l = __builtin_nanf("");
+        // the wave's eight lane groups, then the waves
+        float M = m;
 #pragma unroll
-        for (int i = 0; i < E; i++) s = fmaf(q[i], kr[i], s);
+        for (int x = 8; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+        const float e = exp2_of(m - (M == -INFINITY ? 0.f : M));
+        l *= e;
 #pragma unroll
-        for (int x = 1; x < 8; x <<= 1) s += __shfl_xor(s, x, 64);
-        s *= a.scale * kLog2e;
-        if (t >= k1) continue;  // not 0 times the value of a key past the end
-        if (a.score && p == 0) a.score[((size_t)b * a.heads + h) * a.score_row + t] = s;
-        const float M = fmaxf(m, s), Mf = M == -INFINITY ? 0.f : M;
-        const float alpha = exp2_of(m - Mf), e = exp2_of(s - Mf);
-        m = M;
-        l = fmaf(l, alpha, e);
+        for (int i = 0; i < E; i++) o[i] *= e;
 #pragma unroll
-        for (int i = 0; i < E; i++) o[i] = fmaf(e, vr[i], o[i] * alpha);
-    }
-    if (bad) l = __builtin_nanf("");
-    // the wave's eight lane groups, then the waves
-    float M = m;
+        for (int x = 8; x < 64; x <<= 1) {
+            l += __shfl_xor(l, x, 64);
 #pragma unroll
-    for (int x = 8; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-    const float e = exp2_of(m - (M == -INFINITY ? 0.f : M));
-    l *= e;
+            for (int i = 0; i < E; i++) o[i] += __shfl_xor(o[i], x, 64);
+        }
+        __syncthreads();  // the unit before has been stored
+        if (kl == 0) {
 #pragma unroll
-    for (int i = 0; i < E; i++) o[i] *= e;
-#pragma unroll
-    for (int x = 8; x < 64; x <<= 1) {
-        l += __shfl_xor(l, x, 64);
-#pragma unroll
-        for (int i = 0; i < E; i++) o[i] += __shfl_xor(o[i], x, 64);
-    }
-    if (kl == 0) {
-#pragma unroll
-        for (int i = 0; i < E; i++) red[wv][p + 8 * i] = o[i];
-    }
-    if (lane == 0) {
-        rm[wv] = M;
-        rl[wv] = l;
-    }
-    __syncthreads();
-    float Ma = -INFINITY, L = 0.f;
-    for (int x = 0; x < kWaves; x++) Ma = fmaxf(Ma, rm[x]);
-    const float Mf = Ma == -INFINITY ? 0.f : Ma;
-    for (int x = 0; x < kWaves; x++) L = fmaf(rl[x], exp2_of(rm[x] - Mf), L);
-    const size_t slot = ((size_t)b * a.heads + h) * a.splits + part;
-    for (uint32_t j = threadIdx.x; j < d; j += kBlock) {
-        float O = 0.f;
-        for (int x = 0; x < kWaves; x++) O = fmaf(red[x][j], exp2_of(rm[x] - Mf), O);
-        if (a.ml) a.o[slot * d + j] = O;
-        else put_kind(a.out.kind, a.out.p, b * a.out.row + h * a.out.head + j, L == 0.f ? 0.f : O / L);
-    }
-    if (a.ml && threadIdx.x == 0) {
-        a.ml[2 * slot] = Ma;
-        a.ml[2 * slot + 1] = L;
-    }
+            for (int i = 0; i < E; i++) red[wv][p + 8 * i] = o[i];
+        }
+        if (lane == 0) {
+            rm[wv] = M;
+            rl[wv] = l;
+        }
+        __syncthreads();
+        float Ma = -INFINITY, L = 0.f;
+        for (int x = 0; x < kWaves; x++) Ma = fmaxf(Ma, rm[x]);
+        const float Mf = Ma == -INFINITY ? 0.f : Ma;
+        for (int x = 0; x < kWaves; x++) L = fmaf(rl[x], exp2_of(rm[x] - Mf), L);
+        for (uint32_t j = threadIdx.x; j < d; j += kBlock) {
+            float O = 0.f;
+            for (int x = 0; x < kWaves; x++) O = fmaf(red[x][j], exp2_of(rm[x] - Mf), O);
+            store_part(a, w, h, 0, j, Ma, L, O);
+        }
+    } while (w.next(a));
 }
 
-// The waves' parts of heads h0 .. h0 + nh - 1 folded: to the part's slot, or,
-// where it is the only one, to out.  After a barrier.
+// The waves' (m, l, o) of a unit's heads h0 .. h0 + nh - 1, folded and stored.
+// After a barrier.
 template <int H, int D>
-__device__ __forceinline__ void merge_waves(const PageAttn& a, uint32_t b, uint32_t h0, uint32_t nh, uint32_t part,
+__device__ __forceinline__ void merge_waves(const PageAttn& a, const Run& w, uint32_t h0, uint32_t nh,
                                             const float (*red)[H][D + 4], const float (*rm)[H], const float (*rl)[H]) {
     for (uint32_t i = threadIdx.x; i < nh * D; i += kBlock) {
         const uint32_t n = i / D, j = i % D;
@@ -259,16 +378,7 @@ __device__ __forceinline__ void merge_waves(const PageAttn& a, uint32_t b, uint3
             L = fmaf(rl[x][n], f, L);
             O = fmaf(red[x][n][j], f, O);
         }
-        if (!a.ml) {
-            put_kind(a.out.kind, a.out.p, b * a.out.row + (h0 + n) * a.out.head + j, L == 0.f ? 0.f : O / L);
-            continue;
-        }
-        const size_t slot = ((size_t)b * a.heads + h0 + n) * a.splits + part;
-        a.o[slot * D + j] = O;
-        if (j == 0) {
-            a.ml[2 * slot] = M;
-            a.ml[2 * slot + 1] = L;
-        }
+        store_part(a, w, h0 + n, n, j, M, L, O);
     }
 }
 
@@ -305,7 +415,19 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kWindow = 1024;
+template <int N> struct Words { typedef uint32_t type __attribute__((ext_vector_type(N))); };
+template <int N> using words = typename Words<N>::type;
+// A load of what no other workgroup reads (58 us for 268 MB of rows; 61 without
+// the hint).
+template <typename T> __device__ __forceinline__ T once(const uint8_t* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_nontemporal_load((gptr<T>)p);
+#else
+    return *reinterpret_cast<const T*>(p);  // host pass: never executed
+#endif
+}
+
+constexpr uint32_t kWindow = 2048;
 
 template <uint32_t C> __device__ __forceinline__ f4 mfma32(u4 a, u4 b, f4 c) {
     if constexpr (C == BF16)
@@ -358,286 +480,335 @@ __global__ __launch_bounds__(kBlock, 2) void k_page_attn16(PageAttn a) {
     __shared__ uint32_t off[kWindow];
     __shared__ float red[kWaves][8][D + 4], rm[kWaves][8], rl[kWaves][8];
     const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
-    const uint32_t kv = blockIdx.x / a.groups, G = a.heads / a.c.kvheads, part = blockIdx.y, b = blockIdx.z;
-    const uint32_t in = blockIdx.x % a.groups * a.per, h0 = kv * G + in, nh = min(a.per, G - in);
-    const int32_t len = length_of(a.r, b);
-    const uint32_t len0 = len < 0 ? 0u : (uint32_t)len, k0 = part * a.span, k1 = min(len0, k0 + a.span);
-    if (part && k0 >= len0) return;  // k_page_join does not read it
-    // queries: lane (g, n) holds dims 32 c + 8 g .. + 7 of head n % 8
-    u4 q[NC];
-    float qs = a.scale * kLog2e;
-    {
-        const uint32_t h = h0 + min(n & 7, nh - 1);
-        const bool on = (n & 7) < nh;
-        const uint8_t* row = a.q.p + 2 * (b * a.q.row + h * a.q.head + 8 * g);
-        const bool whole = (((uintptr_t)a.q.p | 2 * a.q.row | 2 * a.q.head) & 15) == 0;
+    const uint32_t G = a.heads / a.c.kvheads;
+    Run run;
+    if (!run.start(a)) return;
+    do {
+        const uint32_t kv = run.u / a.groups, in = run.u % a.groups * a.per, h0 = kv * G + in, nh = min(a.per, G - in);
+        const uint32_t b = run.b, k0 = run.key(), k1 = run.end();
+        if (run.none()) continue;
+        // queries: lane (g, n) holds dims 32 c + 8 g .. + 7 of head n % 8
+        u4 q[NC];
+        float qs = a.scale * kLog2e;
+        {
+            const uint32_t h = h0 + min(n & 7, nh - 1);
+            const bool on = (n & 7) < nh;
+            const uint8_t* row = a.q.p + 2 * (b * a.q.row + h * a.q.head + 8 * g);
+            const bool whole = (((uintptr_t)a.q.p | 2 * a.q.row | 2 * a.q.head) & 15) == 0;
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            u4 w;
-            if (whole) {
-                w = gld<u4>(row + 64 * c);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    w[i] = gld<uint16_t>(row + 64 * c + 4 * i) | (uint32_t)gld<uint16_t>(row + 64 * c + 4 * i + 2) << 16;
-            }
-            q[c] = on ? w : u4{0u, 0u, 0u, 0u};
-        }
-        if constexpr (C == Q8_0) {
-            float x[NC][8], top = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 y = a.q.kind == BF16 ? unpack2<BF16>(q[c][i]) : unpack2<F16>(q[c][i]);
-                    x[c][2 * i] = y.x;
-                    x[c][2 * i + 1] = y.y;
-                    top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
-                }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // 2^-exponent of the largest; its inverse goes to the scores
-            const uint32_t e = __float_as_uint(top) >> 23;
-            const bool scaled = e > 1 && e < 253;
-            const float f = scaled ? __uint_as_float((254 - e) << 23) : 1.f;
-            qs *= scaled ? __uint_as_float(e << 23) : 1.f;
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) q[c][i] = pack2<F16>(x[c][2 * i] * f, x[c][2 * i + 1] * f);
-        }
-    }
-    f4 o[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) o[t] = f4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    bool bad = len < 0;
-    const uint8_t* kb = a.c.k + kv * a.c.hs * ES + 8 * ES * g;
-    const uint8_t* vb = a.c.v + kv * a.c.hs * ES + (D / 16) * ES * n;
-    const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.c.ks) + kv * a.c.hs / 16;
-    const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.c.vs) + kv * a.c.hs / 16 + (D / 16 * n / 32) * 2;
-    for (uint32_t w0 = k0; w0 < k1; w0 += kWindow) {
-        if (w0 != k0) __syncthreads();  // off is still read
-        if (window_offsets(a, b, w0, k1, ES, off)) {
-            bad = true;
-            break;
-        }
-        const uint32_t end = min(k1, w0 + kWindow);
-        for (uint32_t t0 = w0 + 32 * wv; t0 < end; t0 += 32 * kWaves) {
-            const uint32_t* of = off + (t0 - w0);
-            // every load of the step, K first
-            uint32_t kr[2][NC][KW], vr[8][VW];
-            uint32_t vs[8];
-            uint64_t ksc[2][4];
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-                const uint8_t* row = kb + (size_t)of[16 * kt + n] * 16;
-#pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    if constexpr (KW == 4) {
-                        const u4 w = gld<u4>(row + 64 * c);
-                        kr[kt][c][0] = w.x, kr[kt][c][1] = w.y, kr[kt][c][2] = w.z, kr[kt][c][3] = w.w;
-                    } else {
-                        const uint2 w = gld<uint2>(row + 32 * c);
-                        kr[kt][c][0] = w.x, kr[kt][c][1] = w.y;
-                    }
-                }
-            }
-            uint32_t vo[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) vo[j] = of[(j & 4) * 4 + 4 * g + (j & 3)];
-            if constexpr (C == Q8_0) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {  // of the keys that the lane's scores belong to
-                    if constexpr (NC == 4) ksc[j / 4][j % 4] = gld<uint64_t>(ksb + vo[j]);
-                    else ksc[j / 4][j % 4] = gld<uint32_t>(ksb + vo[j]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint8_t* row = vb + (size_t)vo[j] * 16;
-                if constexpr (VW == 4) {
-                    const u4 w = gld<u4>(row);
-                    vr[j][0] = w.x, vr[j][1] = w.y, vr[j][2] = w.z, vr[j][3] = w.w;
-                } else if constexpr (VW == 2) {
-                    const uint2 w = gld<uint2>(row);
-                    vr[j][0] = w.x, vr[j][1] = w.y;
+            for (int c = 0; c < NC; c++) {
+                u4 w;
+                if (whole) {
+                    w = gld<u4>(row + 64 * c);
                 } else {
-                    vr[j][0] = gld<uint32_t>(row);
-                }
-                if constexpr (C == Q8_0) vs[j] = gld<uint16_t>(vsb + vo[j]);
-            }
-            f4 s[2];
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-                s[kt] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    if constexpr (C == Q8_0) {
-                        u4 k16;
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const uint32_t x = kr[kt][c][i] ^ 0x80808080u;
-                            k16[2 * i] = bits_of(codes2(__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)));
-                            k16[2 * i + 1] = bits_of(codes2(__builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)));
-                        }
-                        const f4 acc = mfma32<F16>(k16, q[c], f4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            s[kt][r] = fmaf(acc[r], (float)__builtin_bit_cast(_Float16, (uint16_t)(ksc[kt][r] >> (16 * c))),
-                                            s[kt][r]);
-                    } else {
-                        s[kt] = mfma32<C>(u4{kr[kt][c][0], kr[kt][c][1], kr[kt][c][2], kr[kt][c][3]}, q[c], s[kt]);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; r++) s[kt][r] *= qs;
-            }
-            if (a.score && n < nh) {  // nh is at most 8; the row holds whole steps
-#pragma unroll
-                for (int kt = 0; kt < 2; kt++)
-                    *reinterpret_cast<f4*>(a.score + ((size_t)b * a.heads + h0 + n) * a.score_row + t0 + 16 * kt + 4 * g) = s[kt];
-            }
-            if (t0 + 32 > k1) {  // no weight, and no value, past the end
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const bool past = t0 + (j & 4) * 4 + 4 * g + (j & 3) >= k1;
-                    if (past) s[j / 4][j % 4] = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < VW; i++) vr[j][i] = past ? 0u : vr[j][i];
-                    if constexpr (C == Q8_0) vs[j] = past ? 0u : vs[j];
-                }
-            }
-            float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-            if (__any(top > m + 15.f)) {
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float M = fmaxf(m, top - 7.f), alpha = M == -INFINITY ? 1.f : exp2_of(m - M);
-                m = M;
-                l *= alpha;
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) o[t][r] *= alpha;
-            }
-            const float mf = m == -INFINITY ? 0.f : m;
-            u4 p;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float x = exp2_of(s[i / 2][2 * (i % 2)] - mf), y = exp2_of(s[i / 2][2 * (i % 2) + 1] - mf);
-                l += x + y;
-                const uint32_t hi = pack2<C>(x, y);
-                const float2 back = unpack2<C>(hi);
-                const uint32_t lo = pack2<C>(x - back.x, y - back.y);
-                p[i] = n < 8 ? hi : lo;
-            }
-            if constexpr (C == Q8_0) {
-                h2 d[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(h2, vs[2 * i] | vs[2 * i + 1] << 16);
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int i = 0; i < VW; i++) vr[j][i] ^= 0x80808080u;
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    u4 hi, lo;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t sel = 0x0c000c00u | (uint32_t)(t % 4) | (uint32_t)(4 + t % 4) << 16;
-                        const h2 c = codes2(__builtin_amdgcn_perm(vr[2 * i + 1][t / 4], vr[2 * i][t / 4], sel) | 0x64006400u);
-                        const h2 v = c * d[i];
-                        hi[i] = bits_of(v);
-                        lo[i] = bits_of(__builtin_elementwise_fma(c, d[i], -v));
-                    }
-                    o[t] = mfma32<F16>(hi, p, o[t]);
-                    o[t] = mfma32<F16>(lo, p, o[t]);
-                }
-            } else {
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    u4 v;
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        v[i] = __builtin_amdgcn_perm(vr[2 * i + 1][t / 2], vr[2 * i][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
-                    o[t] = mfma32<C>(v, p, o[t]);
+                        w[i] = gld<uint16_t>(row + 64 * c + 4 * i) | (uint32_t)gld<uint16_t>(row + 64 * c + 4 * i + 2) << 16;
                 }
+                q[c] = on ? w : u4{0u, 0u, 0u, 0u};
+            }
+            if constexpr (C == Q8_0) {
+                float x[NC][8], top = 0.f;
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float2 y = a.q.kind == BF16 ? unpack2<BF16>(q[c][i]) : unpack2<F16>(q[c][i]);
+                        x[c][2 * i] = y.x;
+                        x[c][2 * i + 1] = y.y;
+                        top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+                    }
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                // 2^-exponent of the largest; its inverse goes to the scores
+                const uint32_t e = __float_as_uint(top) >> 23;
+                const bool scaled = e > 1 && e < 253;
+                const float f = scaled ? __uint_as_float((254 - e) << 23) : 1.f;
+                qs *= scaled ? __uint_as_float(e << 23) : 1.f;
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) q[c][i] = pack2<F16>(x[c][2 * i] * f, x[c][2 * i + 1] * f);
             }
         }
-    }
-    if (bad) l = __builtin_nanf("");
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+        f4 o[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++)
+        for (int t = 0; t < NT; t++) o[t] = f4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        bool bad = run.len < 0;
+        const uint8_t* kb = a.c.k + kv * a.c.hs * ES + 8 * ES * g;
+        const uint8_t* vb = a.c.v + kv * a.c.hs * ES + (D / 16) * ES * n;
+        const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.c.ks) + kv * a.c.hs / 16;
+        const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.c.vs) + kv * a.c.hs / 16 + (D / 16 * n / 32) * 2;
+        for (uint32_t w0 = k0; w0 < k1; w0 += kWindow) {
+            __syncthreads();  // off is still read
+            if (window_offsets(a, b, w0, k1, ES, off)) {
+                bad = true;
+                break;
+            }
+            const uint32_t end = min(k1, w0 + kWindow);
+            words<KW> kr[2][NC];
+            words<VW> vr[8];
+            uint32_t vs[8];
+            uint64_t ksc[2][4];
+            auto load_k = [&](uint32_t t0) {
+                const uint32_t* of = off + (t0 - w0);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {  // the lo parts' sums, from column n + 8
-            const float lo = __shfl_xor(o[t][r], 8, 64);
-            if (finite_f(o[t][r])) o[t][r] += lo;
+                for (int kt = 0; kt < 2; kt++) {
+                    const uint8_t* row = kb + (size_t)of[16 * kt + n] * 16;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) kr[kt][c] = once<words<KW>>(row + 16 * KW * c);
+                }
+                if constexpr (C == Q8_0) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {  // of the keys that the lane's scores belong to
+                        const uint8_t* at = ksb + of[(j & 4) * 4 + 4 * g + (j & 3)];
+                        if constexpr (NC == 4) ksc[j / 4][j % 4] = gld<uint64_t>(at);
+                        else ksc[j / 4][j % 4] = gld<uint32_t>(at);
+                    }
+                }
+            };
+            auto load_v = [&](uint32_t t0) {
+                const uint32_t* of = off + (t0 - w0);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint32_t o16 = of[(j & 4) * 4 + 4 * g + (j & 3)];
+                    vr[j] = once<words<VW>>(vb + (size_t)o16 * 16);
+                    if constexpr (C == Q8_0) vs[j] = gld<uint16_t>(vsb + o16);
+                }
+            };
+            f4 s[2];
+            auto scores = [&](uint32_t t0) {
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) {
+                    s[kt] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        if constexpr (C == Q8_0) {
+                            u4 k16;
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const uint32_t x = kr[kt][c][i] ^ 0x80808080u;
+                                k16[2 * i] = bits_of(codes2(__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)));
+                                k16[2 * i + 1] = bits_of(codes2(__builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)));
+                            }
+                            const f4 acc = mfma32<F16>(k16, q[c], f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                s[kt][r] = fmaf(acc[r], (float)__builtin_bit_cast(_Float16, (uint16_t)(ksc[kt][r] >> (16 * c))),
+                                                s[kt][r]);
+                        } else {
+                            s[kt] = mfma32<C>(kr[kt][c], q[c], s[kt]);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[kt][r] *= qs;
+                }
+            };
+            auto sums = [&](uint32_t t0) {
+                if (a.score && n < nh) {  // nh is at most 8; the row holds whole steps
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++)
+                        *reinterpret_cast<f4*>(a.score + ((size_t)b * a.heads + h0 + n) * a.score_row + t0 + 16 * kt + 4 * g) = s[kt];
+                }
+                if (t0 + 32 > k1) {  // no weight, and no value, past the end
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const bool past = t0 + (j & 4) * 4 + 4 * g + (j & 3) >= k1;
+                        if (past) s[j / 4][j % 4] = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < VW; i++) vr[j][i] = past ? 0u : vr[j][i];
+                        if constexpr (C == Q8_0) vs[j] = past ? 0u : vs[j];
+                    }
+                }
+                float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                  fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+                if (__any(top > m + 15.f)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float M = fmaxf(m, top - 7.f), alpha = M == -INFINITY ? 1.f : exp2_of(m - M);
+                    m = M;
+                    l *= alpha;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) o[t][r] *= alpha;
+                }
+                const float mf = m == -INFINITY ? 0.f : m;
+                u4 p;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = exp2_of(s[i / 2][2 * (i % 2)] - mf), y = exp2_of(s[i / 2][2 * (i % 2) + 1] - mf);
+                    l += x + y;
+                    const uint32_t hi = pack2<C>(x, y);
+                    const float2 back = unpack2<C>(hi);
+                    const uint32_t lo = pack2<C>(x - back.x, y - back.y);
+                    p[i] = n < 8 ? hi : lo;
+                }
+                if constexpr (C == Q8_0) {
+                    h2 d[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(h2, vs[2 * i] | vs[2 * i + 1] << 16);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int i = 0; i < VW; i++) vr[j][i] ^= 0x80808080u;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        u4 hi, lo;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t sel = 0x0c000c00u | (uint32_t)(t % 4) | (uint32_t)(4 + t % 4) << 16;
+                            const h2 c = codes2(__builtin_amdgcn_perm(vr[2 * i + 1][t / 4], vr[2 * i][t / 4], sel) | 0x64006400u);
+                            const h2 v = c * d[i];
+                            hi[i] = bits_of(v);
+                            lo[i] = bits_of(__builtin_elementwise_fma(c, d[i], -v));
+                        }
+                        o[t] = mfma32<F16>(hi, p, o[t]);
+                        o[t] = mfma32<F16>(lo, p, o[t]);
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        u4 v;
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            v[i] = __builtin_amdgcn_perm(vr[2 * i + 1][t / 2], vr[2 * i][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
+                        o[t] = mfma32<C>(v, p, o[t]);
+                    }
+                }
+            };
+            for (uint32_t t0 = w0 + kStep * wv; t0 < end; t0 += kStep * kWaves) {
+                load_k(t0);
+                load_v(t0);
+                __builtin_amdgcn_sched_barrier(0);  // V is requested before K is waited for
+                scores(t0);
+                sums(t0);
+            }
         }
-    if (n < 8) {
+        if (bad) l = __builtin_nanf("");
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) red[wv][n][(4 * g + r) * NT + t] = o[t][r];
-        if (g == 0) {
-            rm[wv][n] = m;
-            rl[wv][n] = l;
+            for (int r = 0; r < 4; r++) {  // the lo parts' sums, from column n + 8
+                const float lo = __shfl_xor(o[t][r], 8, 64);
+                if (finite_f(o[t][r])) o[t][r] += lo;
+            }
+        __syncthreads();  // the unit before has been stored
+        if (n < 8) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) red[wv][n][(4 * g + r) * NT + t] = o[t][r];
+            if (g == 0) {
+                rm[wv][n] = m;
+                rl[wv][n] = l;
+            }
+        }
+        __syncthreads();
+        merge_waves<8, D>(a, run, h0, nh, red, rm, rl);
+    } while (run.next(a));
+}
+
+// out of the units that several workgroups hold parts of: a workgroup per `heads`
+// heads of a unit, with V dims of a head (4, or 1 where a head's width is no multiple of 4) a
+// thread and its parts dealt to `groups` threads.  The parts of a unit: the
+// second slot of the workgroup whose run it begins in, and the first slot of
+// those behind.
+constexpr uint32_t kJoinMost = 1024, kJoinAhead = 8;  // threads; parts in flight
+template <int V>
+__global__ __launch_bounds__(kJoinMost) void k_page_join(PageAttn a, uint32_t heads, uint32_t wide) {
+    __shared__ float red[kJoinMost][V + 2];
+    const uint32_t u = blockIdx.x, b = blockIdx.y, d = a.c.dim, tid = threadIdx.x, groups = blockDim.x / wide;
+    const uint32_t G = a.heads / a.c.kvheads, in = u % a.groups * a.per, nh = min(a.per, G - in), z = blockIdx.z * heads;
+    if (z >= nh) return;
+    const uint32_t items = min(heads, nh - z) * d / V;
+    const uint64_t total = gld<uint64_t>(a.begin + a.r.batch), runs = runs_of(a, total);
+    const uint32_t steps = steps_of(length_of(a.r, b));
+    const uint64_t x = gld<uint64_t>(a.begin + b) + (uint64_t)u * steps, first = run_with(total, runs, x + kUnitCost);
+    const uint32_t parts = (uint32_t)(run_with(total, runs, x + steps - 1) - first) + 1;
+    if (parts == 1) return;  // whole in its workgroup
+    const uint32_t item = min(tid % wide, items - 1), n = z + item * V / d, j = item * V % d;
+    float M = -INFINITY, L = 0.f, O[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) O[k] = 0.f;
+    for (uint32_t i0 = tid / wide; i0 < parts; i0 += kJoinAhead * groups) {
+        float2 ml[kJoinAhead];
+        float o[kJoinAhead][V];
+#pragma unroll
+        for (uint32_t k = 0; k < kJoinAhead; k++) {
+            const uint32_t i = min(i0 + k * groups, parts - 1);
+            const size_t slot = ((first + i) * 2 + (i == 0)) * a.per + n;
+            ml[k] = gld<float2>(a.ml + slot);
+            if constexpr (V == 4) {
+                const float4 t = gld<float4>(a.o + slot * d + j);
+                o[k][0] = t.x, o[k][1] = t.y, o[k][2] = t.z, o[k][3] = t.w;
+            } else {
+                o[k][0] = gld<float>(a.o + slot * d + j);
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kJoinAhead; k++) {
+            if (i0 + k * groups >= parts) break;
+            const float Mn = fmaxf(M, ml[k].x), Mf = Mn == -INFINITY ? 0.f : Mn;
+            const float f = exp2_of(M - Mf), e = exp2_of(ml[k].x - Mf);
+            M = Mn;
+            L = fmaf(ml[k].y, e, L * f);
+#pragma unroll
+            for (int c = 0; c < V; c++) O[c] = fmaf(o[k][c], e, O[c] * f);
         }
     }
+    red[tid][V] = M;
+    red[tid][V + 1] = L;
+#pragma unroll
+    for (int c = 0; c < V; c++) red[tid][c] = O[c];
     __syncthreads();
-    merge_waves<8, D>(a, b, h0, nh, part, red, rm, rl);
-}
-
-// The parts in use of a sequence of n keys (one where it has none).
-__device__ __forceinline__ uint32_t parts_of(const PageAttn& a, int32_t len) {
-    return len <= 0 ? 1u : ((uint32_t)len + a.span - 1) / a.span;
-}
-
-// (max, sum) of head h's parts, by one wave.
-__device__ __forceinline__ float2 fold_parts(const PageAttn& a, uint32_t b, uint32_t h, uint32_t parts, uint32_t lane) {
-    const float* ml = a.ml + 2 * ((size_t)b * a.heads + h) * a.splits;
-    float M = -INFINITY, L = 0.f;
-    for (uint32_t i = lane; i < parts; i += 64) M = fmaxf(M, gld<float>(ml + 2 * i));
-    M = wave_max(M);
-    if (M == -INFINITY) M = 0.f;
-    for (uint32_t i = lane; i < parts; i += 64) L += gld<float>(ml + 2 * i + 1) * exp2_of(gld<float>(ml + 2 * i) - M);
-    L = wave_sum(L);
-    return {M, L};
-}
-
-// out[b][h] from its parts: a workgroup per sequence and head.
-__global__ __launch_bounds__(kBlock) void k_page_join(PageAttn a) {
-    const uint32_t h = blockIdx.x, b = blockIdx.y, d = a.c.dim, parts = parts_of(a, length_of(a.r, b));
-    const float2 mi = fold_parts(a, b, h, parts, threadIdx.x & 63);
-    const size_t slot = ((size_t)b * a.heads + h) * a.splits;
-    for (uint32_t j = threadIdx.x; j < d; j += kBlock) {
-        float O = 0.f;
-        for (uint32_t i = 0; i < parts; i++)
-            O = fmaf(gld<float>(a.o + (slot + i) * d + j), exp2_of(gld<float>(a.ml + 2 * (slot + i)) - mi.x), O);
-        put_kind(a.out.kind, a.out.p, b * a.out.row + h * a.out.head + j, mi.y == 0.f ? 0.f : O / mi.y);
+    if (tid >= wide || tid >= items) return;
+    float Ma = M;
+    for (uint32_t i = 1; i < groups; i++) Ma = fmaxf(Ma, red[i * wide + tid][V]);
+    const float Mf = Ma == -INFINITY ? 0.f : Ma, f0 = exp2_of(M - Mf);
+    L *= f0;
+#pragma unroll
+    for (int c = 0; c < V; c++) O[c] *= f0;
+    for (uint32_t i = 1; i < groups; i++) {
+        const float* t = red[i * wide + tid];
+        const float f = exp2_of(t[V] - Mf);
+        L = fmaf(t[V + 1], f, L);
+#pragma unroll
+        for (int c = 0; c < V; c++) O[c] = fmaf(t[c], f, O[c]);
     }
+    const uint32_t h = u / a.groups * G + in + n;
+#pragma unroll
+    for (int c = 0; c < V; c++)
+        put_kind(a.out.kind, a.out.p, b * a.out.row + h * a.out.head + j + c, L == 0.f ? 0.f : O[c] / L);
+    if (a.sum && j == 0) a.sum[(size_t)b * a.heads + h] = make_float2(Ma, L);
 }
 
-// wout[b][g][t] = win[b][g][t] + sum over g's query heads of exp(s - m) / l:
-// a workgroup per kBlock keys of a sequence and KV head.  In the heads' order,
-// so the same bits on every call.
+// wout[b][g][t] = win[b][g][t] + sum over g's query heads of 2^(s - m) / l: four
+// keys a thread.  In the heads' order, so the same bits on every call.
 __global__ __launch_bounds__(kBlock) void k_page_weights(PageAttn a) {
-    const uint32_t g = blockIdx.y, b = blockIdx.z, G = a.heads / a.c.kvheads;
+    const uint32_t g = blockIdx.y, b = blockIdx.z, G = a.heads / a.c.kvheads, t = (blockIdx.x * kBlock + threadIdx.x) * 4;
     const int32_t len = length_of(a.r, b);
-    if ((int32_t)(blockIdx.x * kBlock) >= len) return;
-    const uint32_t t = blockIdx.x * kBlock + threadIdx.x, parts = parts_of(a, len);
-    float w = 0.f;
+    if ((int64_t)t >= len) return;
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (uint32_t i = 0; i < G; i++) {
-        const uint32_t h = g * G + i;
-        const float2 mi = fold_parts(a, b, h, parts, threadIdx.x & 63);
-        if ((int32_t)t < len && mi.y != 0.f)
-            w += exp2_of(gld<float>(a.score + ((size_t)b * a.heads + h) * a.score_row + t) - mi.x) / mi.y;
+        const size_t h = (size_t)b * a.heads + g * G + i;
+        const float2 ml = gld<float2>(a.sum + h);
+        const float4 s = gld<float4>(a.score + h * a.score_row + t);
+        const float Mf = ml.x == -INFINITY ? 0.f : ml.x, inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+        w[0] = fmaf(exp2_of(s.x - Mf), inv, w[0]);
+        w[1] = fmaf(exp2_of(s.y - Mf), inv, w[1]);
+        w[2] = fmaf(exp2_of(s.z - Mf), inv, w[2]);
+        w[3] = fmaf(exp2_of(s.w - Mf), inv, w[3]);
     }
-    if ((int32_t)t >= len) return;
-    if (a.win) w += gld<float>(a.win + b * a.win_row + g * a.win_head + t);
-    a.wout[b * a.wout_row + g * a.wout_head + t] = w;
+    const float* in = a.win ? a.win + b * a.win_row + g * a.win_head + t : nullptr;
+    float* out = a.wout + b * a.wout_row + g * a.wout_head + t;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++)
+        if ((int64_t)t + i < len) out[i] = in ? w[i] + gld<float>(in + i) : w[i];
 }
 
 // Whether k_page_attn16 takes the call: 16-bit queries of the cache's type (or
@@ -652,61 +823,76 @@ static bool fits16(const PageAttn& a) {
     return ((a.c.count - 1) * a.c.ps + (a.c.page - 1) * a.c.ts) * es < (uint64_t)1 << 36;
 }
 
-// Parts of at least 128 keys, and as many as give the chip about 1,024
-// workgroups of eight query heads.
-size_t page_attn_plan(PageAttn& a, bool weights) {
+// At most kPageMaxRuns workgroups, and no more than there may be runs of work.
+bool page_attn_fast(const PageAttn& a) { return fits16(a); }
+void page_attn_plan(PageAttn& a, bool fast, uint32_t cus) {
     const uint32_t G = a.heads / a.c.kvheads;
-    a.groups = (G + 7) / 8;
+    a.fast = fast;
+    a.groups = fast ? (G + 7) / 8 : G;
     a.per = (G + a.groups - 1) / a.groups;
-    const uint64_t most = std::max<uint32_t>(a.r.most, 1), blocks = (uint64_t)a.r.batch * a.c.kvheads * a.groups;
-    const uint64_t units = (uint64_t)a.r.batch * a.heads;
-    uint64_t span = (most * blocks / 1024 + 127) / 128 * 128;
-    span = std::max<uint64_t>(span, ((most + kPageMaxSplits - 1) / kPageMaxSplits + 127) / 128 * 128);
-    span = std::min<uint64_t>(std::max<uint64_t>(span, 128), (most + 127) / 128 * 128);
-    a.span = (uint32_t)span;
-    a.splits = (uint32_t)((most + span - 1) / span);
-    a.score_row = (most + 63) / 64 * 64;
-    if (a.splits == 1 && !weights) return 0;
-    const uint64_t slots = units * a.splits;
-    return (slots * (2 + a.c.dim) + (weights ? units * a.score_row : 0)) * 4 + 64;
+    a.units = a.c.kvheads * a.groups;
+    const uint64_t steps = std::max<uint64_t>(1, ((uint64_t)a.r.most + kStep - 1) / kStep) + kUnitCost;
+    // as many as are resident at a time (k_page_attn16 at 48 ragged histories:
+    // 512 workgroups 55 us, 768 62, 1,024 56)
+    const uint64_t fill = std::min<uint64_t>((uint64_t)cus * (fast ? 2 : 4), kPageMaxRuns);
+    a.runs = (uint32_t)std::min<uint64_t>(fill, (a.units * steps * a.r.batch + kRunMin - 1) / kRunMin);
+    a.score_row = ((uint64_t)a.r.most + 63) / 64 * 64;
 }
 
+// The slots, and with weights every score and every head's (m, l).
+static size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+size_t page_attn_bytes(const PageAttn& a, bool weights) {
+    const size_t slots = (size_t)a.runs * 2 * a.per, heads = (size_t)a.r.batch * a.heads;
+    return round16(slots * a.c.dim * 4) + round16(slots * 8) + round16((a.r.batch + 1) * 8) + (weights ? heads * a.score_row * 4 + heads * 8 : 0);
+}
 void page_attn_place(PageAttn& a, void* work, bool weights) {
-    a.ml = a.o = a.score = nullptr;
-    if (a.splits == 1 && !weights) return;
-    const uint64_t units = (uint64_t)a.r.batch * a.heads, slots = units * a.splits;
-    a.o = static_cast<float*>(work);
-    if (weights) a.score = a.o + (slots * a.c.dim + 3) / 4 * 4;
-    a.ml = weights ? a.score + units * a.score_row : a.o + (slots * a.c.dim + 3) / 4 * 4;
+    const size_t slots = (size_t)a.runs * 2 * a.per, heads = (size_t)a.r.batch * a.heads;
+    uint8_t* p = static_cast<uint8_t*>(work);
+    a.o = reinterpret_cast<float*>(p);
+    p += round16(slots * a.c.dim * 4);
+    a.ml = reinterpret_cast<float2*>(p);
+    p += round16(slots * 8);
+    a.begin = reinterpret_cast<uint64_t*>(p);
+    p += round16((a.r.batch + 1) * 8);
+    a.score = weights ? reinterpret_cast<float*>(p) : nullptr;
+    a.sum = weights ? reinterpret_cast<float2*>(p + heads * a.score_row * 4) : nullptr;
 }
 
 template <uint32_t K> static void launch_any(const PageAttn& a, hipStream_t s) {
-    const dim3 grid(a.heads, a.splits, a.r.batch), block(kBlock);
+    const dim3 grid(a.runs), block(kBlock);
     if (a.c.dim <= 64) hipLaunchKernelGGL((k_page_attn_any<K, 8>), grid, block, 0, s, a);
     else if (a.c.dim <= 128) hipLaunchKernelGGL((k_page_attn_any<K, 16>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((k_page_attn_any<K, 32>), grid, block, 0, s, a);
 }
-
 template <uint32_t C> static void launch16(const PageAttn& a, hipStream_t s) {
-    const dim3 grid(a.c.kvheads * a.groups, a.splits, a.r.batch), block(kBlock);
-    if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn16<C, 64>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_page_attn16<C, 128>), grid, block, 0, s, a);
+    if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn16<C, 64>), dim3(a.runs), dim3(kBlock), 0, s, a);
+    else hipLaunchKernelGGL((k_page_attn16<C, 128>), dim3(a.runs), dim3(kBlock), 0, s, a);
 }
 
 void launch_page_attn(const PageAttn& a, hipStream_t s) {
-    if (fits16(a)) {
-        if (a.c.kind == F16) launch16<F16>(a, s);
-        else if (a.c.kind == BF16) launch16<BF16>(a, s);
-        else launch16<Q8_0>(a, s);
-    } else if (a.c.kind == F32) launch_any<F32>(a, s);
+    const bool fast = a.fast;
+    if (fast && a.c.kind == F16) launch16<F16>(a, s);
+    else if (fast && a.c.kind == BF16) launch16<BF16>(a, s);
+    else if (fast) launch16<Q8_0>(a, s);
+    else if (a.c.kind == F32) launch_any<F32>(a, s);
     else if (a.c.kind == F16) launch_any<F16>(a, s);
     else if (a.c.kind == BF16) launch_any<BF16>(a, s);
     else launch_any<Q8_0>(a, s);
-    if (!a.ml) return;
-    hipLaunchKernelGGL(k_page_join, dim3(a.heads, a.r.batch), dim3(kBlock), 0, s, a);
+    if (a.runs > 1) {
+        const uint32_t v = a.c.dim % 4 ? 1 : 4;
+        // few units hold many parts each (65,537 keys: 64), and a workgroup of
+        // 1,024 threads takes one of their heads, else 512 threads a unit's
+        const bool few = (uint64_t)a.units * a.r.batch < 128;
+        const uint32_t heads = few ? 1 : a.per;
+        uint32_t wide = 16;
+        while (wide < heads * a.c.dim / v) wide *= 2;  // at most 256
+        const dim3 grid(a.units, a.r.batch, few ? a.per : 1), block(few ? kJoinMost : kJoinMost / 2);
+        if (v == 4) hipLaunchKernelGGL(k_page_join<4>, grid, block, 0, s, a, heads, wide);
+        else hipLaunchKernelGGL(k_page_join<1>, grid, block, 0, s, a, heads, wide);
+    }
     if (a.score && a.r.most)
-        hipLaunchKernelGGL(k_page_weights, dim3((a.r.most + kBlock - 1) / kBlock, a.c.kvheads, a.r.batch), dim3(kBlock),
-                           0, s, a);
+        hipLaunchKernelGGL(k_page_weights, dim3((a.r.most + 4 * kBlock - 1) / (4 * kBlock), a.c.kvheads, a.r.batch),
+                           dim3(kBlock), 0, s, a);
 }
 
 }  // namespace qh

@@ -15,7 +15,7 @@ namespace qh {
 // a cache, Q8_0.
 constexpr uint32_t BF16 = 30;
 constexpr uint32_t kPageMaxDim = 256;      // widest head of the paged operators
-constexpr uint32_t kPageMaxSplits = 256;   // most parts of one sequence's keys
+constexpr uint32_t kPageMaxRuns = 1024;    // most workgroups of the attention
 constexpr uint32_t kMoveKeys = 16;         // keys per workgroup of k_page_move
 constexpr uint32_t kLogprobMaxTop = 128;   // most alternatives of a row
 
@@ -62,28 +62,33 @@ struct PageAppend {
 };
 void launch_page_append(const PageAppend& a, hipStream_t s);
 
-// Attention of one token per sequence.  A sequence's keys are cut into parts of
-// `span` keys; a part of a head leaves its running maximum and sum in ml
-// [batch][heads][splits][2] and its weighted values in o
-// [batch][heads][splits][dim]; k_page_join folds them.
+// Attention of one token per sequence (paged.hip: runs of work, their slots).
 struct PageAttn {
     Pages c;
     Rows r;
     Heads q, out;
     uint32_t heads;
     float scale;
-    uint32_t span, splits;
-    uint32_t groups, per;  // a KV head's query heads, `per` to a workgroup
-    float *ml, *o;          // null: one part, written to out
-    float* score;           // [batch][heads][score_row] scaled scores, or null
+    bool fast;              // k_page_attn16, not k_page_attn_any
+    uint32_t groups, per;   // a KV head's query heads, `per` to a unit of work
+    uint32_t units;         // of a sequence
+    uint32_t runs;          // workgroups
+    float* o;               // [runs][2][per][dim] weighted values of parts of units
+    float2* ml;             // [runs][2][per] and their (max, sum)
+    uint64_t* begin;        // [batch + 1] steps of work before each sequence, and in all
+    float* score;           // [batch][heads][score_row] scores, or null
+    float2* sum;            // [batch][heads] (max, sum), with score
     size_t score_row;
     const float* win;       // softmax weights so far, or null
     float* wout;            // and with this call's added
     size_t win_row, win_head, wout_row, wout_head;
 };
-// Chooses the parts and head groups, whatever the queries' kind; bytes of
-// workspace.
-size_t page_attn_plan(PageAttn& a, bool weights);
+// Whether the matrix-core kernel takes the call (q set).
+bool page_attn_fast(const PageAttn& a);
+// The units and runs of a kernel on a GPU of `cus` compute units, then the bytes
+// of its workspace and its pointers.
+void page_attn_plan(PageAttn& a, bool fast, uint32_t cus);
+size_t page_attn_bytes(const PageAttn& a, bool weights);
 void page_attn_place(PageAttn& a, void* work, bool weights);
 void launch_page_attn(const PageAttn& a, hipStream_t s);
 
