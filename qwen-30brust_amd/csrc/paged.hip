@@ -7,6 +7,7 @@
 // of range gets NaN from the attention, and an append to such a page is left
 // out.
 #include <algorithm>
+#include <type_traits>
 
 #include "qh_block.hpp"
 #include "serving_device.hpp"
@@ -150,8 +151,8 @@ void launch_page_append(const PageAppend& a, hipStream_t s) {
 // the device only, so every workgroup finds its run from them (a wave per 64
 // lengths and pass).
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kStep = 32, kRunMin = 4;  // keys; steps of a run at least
-constexpr uint32_t kUnitCost = 4;            // steps in front of a unit's own that are not work
+constexpr uint32_t kStep = 32, kRunMin = 2;  // keys; steps of a run at least
+constexpr uint32_t kUnitCost = 2;            // steps in front of a unit's own that are not work
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32
 
 __device__ __forceinline__ uint32_t steps_of(int32_t len) {
@@ -361,27 +362,6 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
     } while (w.next(a));
 }
 
-// The waves' (m, l, o) of a unit's heads h0 .. h0 + nh - 1, folded and stored.
-// After a barrier.
-template <int H, int D>
-__device__ __forceinline__ void merge_waves(const PageAttn& a, const Run& w, uint32_t h0, uint32_t nh,
-                                            const float (*red)[H][D + 4], const float (*rm)[H], const float (*rl)[H]) {
-    for (uint32_t i = threadIdx.x; i < nh * D; i += kBlock) {
-        const uint32_t n = i / D, j = i % D;
-        float M = -INFINITY, L = 0.f, O = 0.f;
-#pragma unroll
-        for (int x = 0; x < kWaves; x++) M = fmaxf(M, rm[x][n]);
-        const float Mf = M == -INFINITY ? 0.f : M;
-#pragma unroll
-        for (int x = 0; x < kWaves; x++) {
-            const float f = exp2_of(rm[x][n] - Mf);
-            L = fmaf(rl[x][n], f, L);
-            O = fmaf(red[x][n][j], f, O);
-        }
-        store_part(a, w, h0 + n, n, j, M, L, O);
-    }
-}
-
 // -------------------------------------------- attention on the matrix cores --
 // A wave takes 32 keys a step and up to eight query heads of one KV head, and
 // keeps K, V, scores, weights and sums in its registers:
@@ -427,7 +407,7 @@ template <typename T> __device__ __forceinline__ T once(const uint8_t* p) {
 #endif
 }
 
-constexpr uint32_t kWindow = 2048;
+constexpr uint32_t kWindow = 512;
 
 template <uint32_t C> __device__ __forceinline__ f4 mfma32(u4 a, u4 b, f4 c) {
     if constexpr (C == BF16)
@@ -456,30 +436,56 @@ __device__ __forceinline__ h2 codes2(uint32_t w) {
 __device__ __forceinline__ uint32_t bits_of(h2 h) { return __builtin_bit_cast(uint32_t, h); }
 
 // Offsets (16 bytes) of keys [t0, t0 + kWindow) into off, keys past k1 as the
-// last; a barrier.  True where a page id is out of range.
+// last, by a wave.  True where a page id is out of range.
 __device__ __forceinline__ bool window_offsets(const PageAttn& a, uint32_t b, uint32_t t0, uint32_t k1, uint32_t bytes,
                                                uint32_t* off) {
-    int bad = 0;
-    for (uint32_t i = threadIdx.x; i < kWindow && t0 + i < (k1 + 31) / 32 * 32; i += kBlock) {
+    const uint32_t end = min(kWindow, (k1 - t0 + kStep - 1) / kStep * kStep);
+    bool bad = false;
+    __syncthreads();  // off is still read (one wave: an order for the compiler)
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < end; i += 64) {
         const uint32_t t = min(t0 + i, k1 - 1), at = t / a.c.page;
         uint32_t page = (uint32_t)gld<int32_t>(a.r.table + b * a.r.stride + at);
         if (page >= a.c.count) {
-            bad = 1;
+            bad = true;
             page = 0;
         }
         off[i] = (uint32_t)((page * a.c.ps + (t - at * a.c.page) * a.c.ts) * bytes / 16);
     }
-    return __syncthreads_or(bad);
+    __syncthreads();
+    return __any(bad);
+}
+
+// store_part for head n, of which the lane has dims (4 g + r) D / 16 + t.
+template <int D>
+__device__ __forceinline__ void store_head(const PageAttn& a, const Run& w, uint32_t h, uint32_t n, uint32_t g, float M,
+                                           float L, const f4 (&o)[D / 16]) {
+    constexpr int NT = D / 16;
+    if (!w.whole()) {
+        const size_t slot = ((size_t)blockIdx.x * 2 + w.head()) * a.per + n;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int t = 0; t < NT; t += 4)
+                *reinterpret_cast<f4*>(a.o + slot * D + (4 * g + r) * NT + t) = f4{o[t][r], o[t + 1][r], o[t + 2][r], o[t + 3][r]};
+        if (g == 0) a.ml[slot] = make_float2(M, L);
+        return;
+    }
+    const size_t at = w.b * a.out.row + h * a.out.head + 4 * g * NT;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) put_kind(a.out.kind, a.out.p, at + r * NT + t, L == 0.f ? 0.f : o[t][r] / L);
+    if (a.sum && g == 0) a.sum[(size_t)w.b * a.heads + h] = make_float2(M, L);
 }
 
 template <uint32_t C, int D>
-__global__ __launch_bounds__(kBlock, 2) void k_page_attn16(PageAttn a) {
+__global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
     constexpr int NC = D / 32, NT = D / 16;             // 32-dim steps of S, 16-dim tiles of O
     constexpr uint32_t ES = C == Q8_0 ? 1 : 2;
     constexpr int KW = 2 * ES, VW = D / 64 * ES;         // words of a K load (8 dims) and of a V load (D / 16 dims)
     __shared__ uint32_t off[kWindow];
-    __shared__ float red[kWaves][8][D + 4], rm[kWaves][8], rl[kWaves][8];
-    const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+    const uint32_t lane = threadIdx.x, g = lane >> 4, n = lane & 15;
     const uint32_t G = a.heads / a.c.kvheads;
     Run run;
     if (!run.start(a)) return;
@@ -541,7 +547,6 @@ __global__ __launch_bounds__(kBlock, 2) void k_page_attn16(PageAttn a) {
         const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.c.ks) + kv * a.c.hs / 16;
         const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.c.vs) + kv * a.c.hs / 16 + (D / 16 * n / 32) * 2;
         for (uint32_t w0 = k0; w0 < k1; w0 += kWindow) {
-            __syncthreads();  // off is still read
             if (window_offsets(a, b, w0, k1, ES, off)) {
                 bad = true;
                 break;
@@ -605,13 +610,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_page_attn16(PageAttn a) {
                     for (int r = 0; r < 4; r++) s[kt][r] *= qs;
                 }
             };
-            auto sums = [&](uint32_t t0) {
-                if (a.score && n < nh) {  // nh is at most 8; the row holds whole steps
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++)
-                        *reinterpret_cast<f4*>(a.score + ((size_t)b * a.heads + h0 + n) * a.score_row + t0 + 16 * kt + 4 * g) = s[kt];
-                }
-                if (t0 + 32 > k1) {  // no weight, and no value, past the end
+            auto sums = [&](uint32_t t0, auto last) {
+                if constexpr (last) {  // no weight, and no value, past the end
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const bool past = t0 + (j & 4) * 4 + 4 * g + (j & 3) >= k1;
@@ -678,13 +678,21 @@ __global__ __launch_bounds__(kBlock, 2) void k_page_attn16(PageAttn a) {
                     }
                 }
             };
-            for (uint32_t t0 = w0 + kStep * wv; t0 < end; t0 += kStep * kWaves) {
+            auto step = [&](uint32_t t0, auto last) {
                 load_k(t0);
                 load_v(t0);
                 __builtin_amdgcn_sched_barrier(0);  // V is requested before K is waited for
                 scores(t0);
-                sums(t0);
-            }
+                sums(t0, last);
+                if (a.score && n < nh) {  // behind the products: a store waits for the loads of other waves
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++)  // the row holds whole steps
+                        *reinterpret_cast<f4*>(a.score + ((size_t)b * a.heads + h0 + n) * a.score_row + t0 + 16 * kt + 4 * g) = s[kt];
+                }
+            };
+            uint32_t t0 = w0;
+            for (; t0 + kStep <= end; t0 += kStep) step(t0, std::false_type());
+            if (t0 < end) step(t0, std::true_type());
         }
         if (bad) l = __builtin_nanf("");
         l += __shfl_xor(l, 16, 64);
@@ -696,19 +704,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_page_attn16(PageAttn a) {
                 const float lo = __shfl_xor(o[t][r], 8, 64);
                 if (finite_f(o[t][r])) o[t][r] += lo;
             }
-        __syncthreads();  // the unit before has been stored
-        if (n < 8) {
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) red[wv][n][(4 * g + r) * NT + t] = o[t][r];
-            if (g == 0) {
-                rm[wv][n] = m;
-                rl[wv][n] = l;
-            }
-        }
-        __syncthreads();
-        merge_waves<8, D>(a, run, h0, nh, red, rm, rl);
+        if (n < nh) store_head<D>(a, run, h0 + n, n, g, m, l, o);
     } while (run.next(a));
 }
 
@@ -832,9 +828,9 @@ void page_attn_plan(PageAttn& a, bool fast, uint32_t cus) {
     a.per = (G + a.groups - 1) / a.groups;
     a.units = a.c.kvheads * a.groups;
     const uint64_t steps = std::max<uint64_t>(1, ((uint64_t)a.r.most + kStep - 1) / kStep) + kUnitCost;
-    // as many as are resident at a time (k_page_attn16 at 48 ragged histories:
-    // 512 workgroups 55 us, 768 62, 1,024 56)
-    const uint64_t fill = std::min<uint64_t>((uint64_t)cus * (fast ? 2 : 4), kPageMaxRuns);
+    // k_page_attn16 over 48 ragged histories of bf16 keys: 1,024 waves 52.6 us,
+    // 1,536 and 2,048 54.3; over 96 of Q8_0 keys 85, 77 and 74
+    const uint64_t fill = std::min<uint64_t>((uint64_t)cus * (fast && a.c.kind == Q8_0 ? 8 : 4), kPageMaxRuns);
     a.runs = (uint32_t)std::min<uint64_t>(fill, (a.units * steps * a.r.batch + kRunMin - 1) / kRunMin);
     a.score_row = ((uint64_t)a.r.most + 63) / 64 * 64;
 }
@@ -865,8 +861,8 @@ template <uint32_t K> static void launch_any(const PageAttn& a, hipStream_t s) {
     else hipLaunchKernelGGL((k_page_attn_any<K, 32>), grid, block, 0, s, a);
 }
 template <uint32_t C> static void launch16(const PageAttn& a, hipStream_t s) {
-    if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn16<C, 64>), dim3(a.runs), dim3(kBlock), 0, s, a);
-    else hipLaunchKernelGGL((k_page_attn16<C, 128>), dim3(a.runs), dim3(kBlock), 0, s, a);
+    if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn16<C, 64>), dim3(a.runs), dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((k_page_attn16<C, 128>), dim3(a.runs), dim3(64), 0, s, a);
 }
 
 void launch_page_attn(const PageAttn& a, hipStream_t s) {

@@ -15,7 +15,7 @@ namespace qh {
 // a cache, Q8_0.
 constexpr uint32_t BF16 = 30;
 constexpr uint32_t kPageMaxDim = 256;      // widest head of the paged operators
-constexpr uint32_t kPageMaxRuns = 1024;    // most workgroups of the attention
+constexpr uint32_t kPageMaxRuns = 2048;    // most workgroups of the attention
 constexpr uint32_t kMoveKeys = 16;         // keys per workgroup of k_page_move
 constexpr uint32_t kLogprobMaxTop = 128;   // most alternatives of a row
 
