@@ -433,6 +433,11 @@ template <uint32_t C> __device__ __forceinline__ float2 unpack2(uint32_t w) {
 __device__ __forceinline__ h2 codes2(uint32_t w) {
     return __builtin_bit_cast(h2, w) - h2{(_Float16)1152, (_Float16)1152};
 }
+// Value i of 16.
+__device__ __forceinline__ float scale_of(const u4 (&w)[2], int i) {
+    const uint32_t pair = w[i / 8][i % 8 / 2];
+    return (float)__builtin_bit_cast(h2, pair)[i % 2];
+}
 __device__ __forceinline__ uint32_t bits_of(h2 h) { return __builtin_bit_cast(uint32_t, h); }
 
 // Offsets (16 bytes) of keys [t0, t0 + kWindow) into off, keys past k1 as the
@@ -485,6 +490,7 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
     constexpr uint32_t ES = C == Q8_0 ? 1 : 2;
     constexpr int KW = 2 * ES, VW = D / 64 * ES;         // words of a K load (8 dims) and of a V load (D / 16 dims)
     __shared__ uint32_t off[kWindow];
+    __shared__ __align__(16) uint16_t ksl[kStep][NC], vsl[NC][kStep];  // the step's scales (Q8_0)
     const uint32_t lane = threadIdx.x, g = lane >> 4, n = lane & 15;
     const uint32_t G = a.heads / a.c.kvheads;
     Run run;
@@ -544,8 +550,9 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
         bool bad = run.len < 0;
         const uint8_t* kb = a.c.k + kv * a.c.hs * ES + 8 * ES * g;
         const uint8_t* vb = a.c.v + kv * a.c.hs * ES + (D / 16) * ES * n;
-        const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.c.ks) + kv * a.c.hs / 16;
-        const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.c.vs) + kv * a.c.hs / 16 + (D / 16 * n / 32) * 2;
+        // lane l fetches scales l % 2 * NC / 2 .. of key l / 2
+        const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.c.ks) + kv * a.c.hs / 16 + (lane & 1) * NC;
+        const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.c.vs) + kv * a.c.hs / 16 + (lane & 1) * NC;
         for (uint32_t w0 = k0; w0 < k1; w0 += kWindow) {
             if (window_offsets(a, b, w0, k1, ES, off)) {
                 bad = true;
@@ -554,8 +561,7 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
             const uint32_t end = min(k1, w0 + kWindow);
             words<KW> kr[2][NC];
             words<VW> vr[8];
-            uint32_t vs[8];
-            uint64_t ksc[2][4];
+            typename std::conditional<NC == 4, uint32_t, uint16_t>::type ksr, vsr;  // half a key's scales
             auto load_k = [&](uint32_t t0) {
                 const uint32_t* of = off + (t0 - w0);
 #pragma unroll
@@ -564,26 +570,27 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
 #pragma unroll
                     for (int c = 0; c < NC; c++) kr[kt][c] = once<words<KW>>(row + 16 * KW * c);
                 }
-                if constexpr (C == Q8_0) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {  // of the keys that the lane's scores belong to
-                        const uint8_t* at = ksb + of[(j & 4) * 4 + 4 * g + (j & 3)];
-                        if constexpr (NC == 4) ksc[j / 4][j % 4] = gld<uint64_t>(at);
-                        else ksc[j / 4][j % 4] = gld<uint32_t>(at);
-                    }
-                }
+                if constexpr (C == Q8_0) ksr = gld<decltype(ksr)>(ksb + of[lane / 2]);
             };
             auto load_v = [&](uint32_t t0) {
                 const uint32_t* of = off + (t0 - w0);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const uint32_t o16 = of[(j & 4) * 4 + 4 * g + (j & 3)];
-                    vr[j] = once<words<VW>>(vb + (size_t)o16 * 16);
-                    if constexpr (C == Q8_0) vs[j] = gld<uint16_t>(vsb + o16);
+                    vr[j] = once<words<VW>>(vb + (size_t)of[(j & 4) * 4 + 4 * g + (j & 3)] * 16);
                 }
+                if constexpr (C == Q8_0) vsr = gld<decltype(vsr)>(vsb + of[lane / 2]);
             };
             f4 s[2];
             auto scores = [&](uint32_t t0) {
+                u4 kq[2][2];  // scales of keys 16 kt + 4 g .. + 3
+                if constexpr (C == Q8_0) {
+                    __syncthreads();  // those of the step before are still read
+                    __builtin_memcpy(&ksl[lane / 2][(lane & 1) * NC / 2], &ksr, NC);
+                    __syncthreads();
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++)
+                        __builtin_memcpy(&kq[kt], __builtin_assume_aligned(&ksl[16 * kt + 4 * g][0], 16), 8 * NC);
+                }
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++) {
                     s[kt] = f4{0.f, 0.f, 0.f, 0.f};
@@ -600,8 +607,7 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
                             const f4 acc = mfma32<F16>(k16, q[c], f4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
                             for (int r = 0; r < 4; r++)
-                                s[kt][r] = fmaf(acc[r], (float)__builtin_bit_cast(_Float16, (uint16_t)(ksc[kt][r] >> (16 * c))),
-                                                s[kt][r]);
+                                s[kt][r] = fmaf(acc[r], scale_of(kq[kt], r * NC + c), s[kt][r]);
                         } else {
                             s[kt] = mfma32<C>(kr[kt][c], q[c], s[kt]);
                         }
@@ -618,8 +624,8 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
                         if (past) s[j / 4][j % 4] = -INFINITY;
 #pragma unroll
                         for (int i = 0; i < VW; i++) vr[j][i] = past ? 0u : vr[j][i];
-                        if constexpr (C == Q8_0) vs[j] = past ? 0u : vs[j];
                     }
+                    if constexpr (C == Q8_0) vsr = t0 + lane / 2 >= k1 ? 0 : vsr;
                 }
                 float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                   fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -646,9 +652,16 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
                     p[i] = n < 8 ? hi : lo;
                 }
                 if constexpr (C == Q8_0) {
-                    h2 d[4];
+                    // scales of the lane's block and keys, in pairs
+                    __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(h2, vs[2 * i] | vs[2 * i + 1] << 16);
+                    for (int i = 0; i < NC / 2; i++)
+                        vsl[(lane & 1) * NC / 2 + i][lane / 2] = (uint16_t)((uint32_t)vsr >> (16 * i));
+                    __syncthreads();
+                    const uint16_t* vl = vsl[D / 16 * n / 32];
+                    h2 d[4];
+                    __builtin_memcpy(d, __builtin_assume_aligned(vl + 4 * g, 8), 8);
+                    __builtin_memcpy(d + 2, __builtin_assume_aligned(vl + 16 + 4 * g, 8), 8);
 #pragma unroll
                     for (int j = 0; j < 8; j++)
 #pragma unroll
