@@ -2686,8 +2686,8 @@ int qh_paged_attention_bytes(qh_ctx* c, const qh_pages_t* cache, const qh_sequen
         if (!out) throw Error("null output buffer");
         PageAttn a = attn_of(cache, seqs, heads);
         *out = 0;
-        for (const bool fast : {false, true}) {  // the queries' kind decides
-            page_attn_plan(a, fast, cus_of(c));
+        for (const uint32_t kernel : {0u, 16u}) {  // the queries' kind decides
+            page_attn_plan(a, kernel, cus_of(c));
             if (a.r.batch) *out = std::max(*out, page_attn_bytes(a, with_weights));
         }
     });
@@ -2714,7 +2714,7 @@ int qh_paged_attention(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t*
             a.wout_row = weights->out_row;
             a.wout_head = weights->out_head;
         }
-        page_attn_plan(a, page_attn_fast(a), cus_of(c));
+        page_attn_plan(a, page_attn_kernel(a), cus_of(c));
         need_workspace(workspace, workspace_bytes, page_attn_bytes(a, weights));
         page_attn_place(a, workspace, weights);
         need_ctx(c);

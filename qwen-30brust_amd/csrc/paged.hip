@@ -461,6 +461,57 @@ __device__ __forceinline__ bool window_offsets(const PageAttn& a, uint32_t b, ui
     return __any(bad);
 }
 
+template <uint32_t K> struct Four;  // four elements as they lie, and as floats
+template <> struct Four<F32> {
+    typedef words<4> type;
+    static __device__ __forceinline__ f4 widen(type w) { return __builtin_bit_cast(f4, w); }
+};
+template <> struct Four<F16> {
+    typedef words<2> type;
+    static __device__ __forceinline__ f4 widen(type w) {
+        const float2 a = unpack2<F16>(w.x), b = unpack2<F16>(w.y);
+        return f4{a.x, a.y, b.x, b.y};
+    }
+};
+template <> struct Four<BF16> {
+    typedef words<2> type;
+    static __device__ __forceinline__ f4 widen(type w) {
+        const float2 a = unpack2<BF16>(w.x), b = unpack2<BF16>(w.y);
+        return f4{a.x, a.y, b.x, b.y};
+    }
+};
+template <> struct Four<Q8_0> {
+    typedef uint32_t type;
+    static __device__ __forceinline__ f4 widen(type w) {
+        return f4{(float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)((int32_t)w >> 24)};
+    }
+};
+
+// f(integral constant of the kind): the code of one branch.
+template <class F> __device__ __forceinline__ void with_kind(uint32_t kind, F f) {
+    if (kind == F32) f(std::integral_constant<uint32_t, F32>());
+    else if (kind == F16) f(std::integral_constant<uint32_t, F16>());
+    else f(std::integral_constant<uint32_t, BF16>());
+}
+// Whether four elements at a multiple of four are one access.
+__device__ __forceinline__ bool fours(const Heads& h) {
+    const size_t es = h.kind == F32 ? 4 : 2;
+    return (((uintptr_t)h.p | h.row * es | h.head * es) & (4 * es - 1)) == 0;
+}
+template <uint32_t K> __device__ __forceinline__ f4 load4(const uint8_t* p, size_t i, bool one) {
+    if (one) return Four<K>::widen(gld<typename Four<K>::type>(p + i * (K == F32 ? 4 : 2)));
+    return f4{elem<K>(p, i), elem<K>(p, i + 1), elem<K>(p, i + 2), elem<K>(p, i + 3)};
+}
+template <uint32_t K> __device__ __forceinline__ void put4(uint8_t* p, size_t i, f4 x, bool one) {
+    if (one) {
+        if constexpr (K == F32) *reinterpret_cast<f4*>(p + 4 * i) = x;
+        else *reinterpret_cast<words<2>*>(p + 2 * i) = words<2>{pack2<K>(x[0], x[1]), pack2<K>(x[2], x[3])};
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) put<K>(p, i + k, x[k]);
+}
+
 // store_part for head n, of which the lane has dims (4 g + r) D / 16 + t.
 template <int D>
 __device__ __forceinline__ void store_head(const PageAttn& a, const Run& w, uint32_t h, uint32_t n, uint32_t g, float M,
@@ -477,10 +528,16 @@ __device__ __forceinline__ void store_head(const PageAttn& a, const Run& w, uint
         return;
     }
     const size_t at = w.b * a.out.row + h * a.out.head + 4 * g * NT;
+    const bool one = fours(a.out);
+    with_kind(a.out.kind, [&](auto k) {
 #pragma unroll
-    for (int r = 0; r < 4; r++)
+        for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) put_kind(a.out.kind, a.out.p, at + r * NT + t, L == 0.f ? 0.f : o[t][r] / L);
+            for (int t = 0; t < NT; t += 4) {
+                const f4 x = {o[t][r], o[t + 1][r], o[t + 2][r], o[t + 3][r]};
+                put4<k>(a.out.p, at + r * NT + t, L == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : x / L, one);
+            }
+    });
     if (a.sum && g == 0) a.sum[(size_t)w.b * a.heads + h] = make_float2(M, L);
 }
 
@@ -721,6 +778,154 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
     } while (run.next(a));
 }
 
+// The same for 32-bit queries, or queries and caches of different types: every
+// product in 32 bits on v_mfma_f32_16x16x4_f32, K and V widened as they arrive.
+// Sixteen keys a round; k slot g of step (c, i) of the first product is dim 16 c
+// + 4 g + i, of step r of the second key 4 g + r, so that the scores again are
+// the weights' operand as they come.  An eighth of the 16-bit products' rate, and
+// half of each instruction idle with eight heads or fewer: still under the time
+// that memory takes for the rows (2,048 matrix-core cycles for 16 KB of f32 rows,
+// which take a compute unit's share of the bandwidth about 8,000).
+template <uint32_t K, int D>
+__global__ __launch_bounds__(64, 2) void k_page_attn32(PageAttn a) {
+    constexpr int NC = D / 16, NV = D / 64;  // 16-dim loads of a key, 64-dim loads of a value
+    constexpr uint32_t ES = K == F32 ? 4 : K == Q8_0 ? 1 : 2;
+    typedef typename Four<K>::type four;
+    __shared__ uint32_t off[kWindow];
+    const uint32_t lane = threadIdx.x, g = lane >> 4, n = lane & 15;
+    const uint32_t G = a.heads / a.c.kvheads;
+    Run run;
+    if (!run.start(a)) return;
+    do {
+        const uint32_t kv = run.u / a.groups, in = run.u % a.groups * a.per, h0 = kv * G + in, nh = min(a.per, G - in);
+        const uint32_t b = run.b, k0 = run.key(), k1 = run.end();
+        if (run.none()) continue;
+        f4 q[NC];  // dims 16 c + 4 g .. + 3 of head n
+        {
+            const size_t row = b * a.q.row + (h0 + min(n, nh - 1)) * a.q.head + 4 * g;
+            const float scale = a.scale * kLog2e;
+            const bool one = fours(a.q);
+            with_kind(a.q.kind, [&](auto k) {
+#pragma unroll
+                for (int c = 0; c < NC; c++) q[c] = load4<k>(a.q.p, row + 16 * c, one);
+            });
+#pragma unroll
+            for (int c = 0; c < NC; c++) q[c] = n < nh ? q[c] * scale : f4{0.f, 0.f, 0.f, 0.f};
+        }
+        f4 o[4 * NV];  // tile 4 c + i: dims 64 c + 4 (4 g + r) + i
+#pragma unroll
+        for (int t = 0; t < 4 * NV; t++) o[t] = f4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        bool bad = run.len < 0;
+        const uint8_t* kb = a.c.k + kv * a.c.hs * ES + 4 * ES * g;
+        const uint8_t* vb = a.c.v + kv * a.c.hs * ES + 4 * ES * n;
+        const uint8_t* ksb = reinterpret_cast<const uint8_t*>(a.c.ks) + kv * a.c.hs / 16;
+        const uint8_t* vsb = reinterpret_cast<const uint8_t*>(a.c.vs) + kv * a.c.hs / 16 + n / 8 * 2;
+        for (uint32_t w0 = k0; w0 < k1; w0 += kWindow) {
+            if (window_offsets(a, b, w0, k1, ES, off)) {
+                bad = true;
+                break;
+            }
+            const uint32_t end = min(k1, w0 + kWindow);
+            auto round = [&](uint32_t t0, auto last) {
+                const uint32_t* of = off + (t0 - w0);
+                four kr[NC], vr[4][NV];
+                _Float16 ks[NC / 2], vs[4][NV];
+                const uint32_t ok = of[n];
+#pragma unroll
+                for (int c = 0; c < NC; c++) kr[c] = once<four>(kb + (size_t)ok * 16 + 16 * ES * c);
+                if constexpr (K == Q8_0) {
+#pragma unroll
+                    for (int c = 0; c < NC / 2; c++) ks[c] = gld<_Float16>(ksb + ok + 2 * c);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t ov = of[4 * g + r];
+#pragma unroll
+                    for (int c = 0; c < NV; c++) {
+                        vr[r][c] = once<four>(vb + (size_t)ov * 16 + 64 * ES * c);
+                        if constexpr (K == Q8_0) vs[r][c] = gld<_Float16>(vsb + ov + 4 * c);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);  // V is requested before K is waited for
+                f4 s2[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    f4 k = Four<K>::widen(kr[c]);
+                    if constexpr (K == Q8_0) k *= (float)ks[c / 2];
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        s2[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i], q[c][i], s2[i & 1], 0, 0, 0);
+                }
+                f4 s = s2[0] + s2[1];
+                const f4 all = s;
+                if constexpr (last) {  // no weight past the end
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (t0 + 4 * g + r >= k1) s[r] = -INFINITY;
+                }
+                float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+                if (__any(top > m + 15.f)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float M = fmaxf(m, top - 7.f), alpha = M == -INFINITY ? 1.f : exp2_of(m - M);
+                    m = M;
+                    l *= alpha;
+#pragma unroll
+                    for (int t = 0; t < 4 * NV; t++) o[t] *= alpha;
+                }
+                const float mf = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float p = exp2_of(s[r] - mf);
+                    l += p;
+#pragma unroll
+                    for (int c = 0; c < NV; c++) {
+                        f4 v = Four<K>::widen(vr[r][c]);
+                        if constexpr (K == Q8_0) v *= (float)vs[r][c];
+                        if constexpr (last) {  // and no value
+                            if (t0 + 4 * g + r >= k1) v = f4{0.f, 0.f, 0.f, 0.f};
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            o[4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i], p, o[4 * c + i], 0, 0, 0);
+                    }
+                }
+                if (a.score && n < nh)  // the row holds whole steps
+                    *reinterpret_cast<f4*>(a.score + ((size_t)b * a.heads + h0 + n) * a.score_row + t0 + 4 * g) = all;
+            };
+            uint32_t t0 = w0;
+            for (; t0 + 16 <= end; t0 += 16) round(t0, std::false_type());
+            if (t0 < end) round(t0, std::true_type());
+        }
+        if (bad) l = __builtin_nanf("");
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (n >= nh) continue;
+        const bool whole = run.whole(), one = fours(a.out);
+        const size_t slot = ((size_t)blockIdx.x * 2 + run.head()) * a.per + n;
+        auto each = [&](auto f) {  // f(dim, its four values)
+#pragma unroll
+            for (int c = 0; c < NV; c++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    f(64 * c + 16 * g + 4 * r, f4{o[4 * c][r], o[4 * c + 1][r], o[4 * c + 2][r], o[4 * c + 3][r]});
+        };
+        if (!whole) {
+            each([&](uint32_t j, f4 x) { *reinterpret_cast<f4*>(a.o + slot * D + j) = x; });
+        } else {
+            const size_t at = b * a.out.row + (h0 + n) * a.out.head;
+            with_kind(a.out.kind, [&](auto k) {
+                each([&](uint32_t j, f4 x) { put4<k>(a.out.p, at + j, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : x / l, one); });
+            });
+        }
+        if (g == 0) {
+            if (!whole) a.ml[slot] = make_float2(m, l);
+            else if (a.sum) a.sum[(size_t)b * a.heads + h0 + n] = make_float2(m, l);
+        }
+    } while (run.next(a));
+}
+
 // out of the units that several workgroups hold parts of: a workgroup per `heads`
 // heads of a unit, with V dims of a head (4, or 1 where a head's width is no multiple of 4) a
 // thread and its parts dealt to `groups` threads.  The parts of a unit: the
@@ -820,30 +1025,31 @@ __global__ __launch_bounds__(kBlock) void k_page_weights(PageAttn a) {
         if ((int64_t)t + i < len) out[i] = in ? w[i] + gld<float>(in + i) : w[i];
 }
 
-// Whether k_page_attn16 takes the call: 16-bit queries of the cache's type (or
-// over Q8_0), heads of 64 or 128, rows aligned to 16 bytes within 64 GiB.
-static bool fits16(const PageAttn& a) {
+// The kernel of a call.  Both matrix-core kernels want heads of 64 or 128 and
+// rows aligned to 16 bytes within 64 GiB; k_page_attn16 takes 16-bit queries of
+// the cache's type (or over Q8_0).
+uint32_t page_attn_kernel(const PageAttn& a) {
     const bool q8 = a.c.kind == Q8_0;
-    if (a.q.kind == F32 || (!q8 && a.c.kind != a.q.kind) || (a.c.dim != 64 && a.c.dim != 128)) return false;
-    const uint64_t es = q8 ? 1 : 2, all = a.c.ps | a.c.ts | a.c.hs;
-    if (((uintptr_t)a.c.k | (uintptr_t)a.c.v | all * es) % 16) return false;
-    // a key's scales are one load
-    if (q8 && (all % a.c.dim || ((uintptr_t)a.c.ks | (uintptr_t)a.c.vs) % (a.c.dim / 16))) return false;
-    return ((a.c.count - 1) * a.c.ps + (a.c.page - 1) * a.c.ts) * es < (uint64_t)1 << 36;
+    if (a.c.dim != 64 && a.c.dim != 128) return 0;
+    const uint64_t es = q8 ? 1 : a.c.kind == F32 ? 4 : 2, all = a.c.ps | a.c.ts | a.c.hs;
+    if (((uintptr_t)a.c.k | (uintptr_t)a.c.v | all * es) % 16) return 0;
+    // a key's scales lie together
+    if (q8 && (all % a.c.dim || ((uintptr_t)a.c.ks | (uintptr_t)a.c.vs) % (a.c.dim / 16))) return 0;
+    if (((a.c.count - 1) * a.c.ps + (a.c.page - 1) * a.c.ts) * es >= (uint64_t)1 << 36) return 0;
+    return a.q.kind != F32 && (q8 || a.c.kind == a.q.kind) ? 16 : 32;
 }
 
 // At most kPageMaxRuns workgroups, and no more than there may be runs of work.
-bool page_attn_fast(const PageAttn& a) { return fits16(a); }
-void page_attn_plan(PageAttn& a, bool fast, uint32_t cus) {
+void page_attn_plan(PageAttn& a, uint32_t kernel, uint32_t cus) {
     const uint32_t G = a.heads / a.c.kvheads;
-    a.fast = fast;
-    a.groups = fast ? (G + 7) / 8 : G;
+    a.kernel = kernel;
+    a.groups = kernel ? (G + 7) / 8 : G;
     a.per = (G + a.groups - 1) / a.groups;
     a.units = a.c.kvheads * a.groups;
     const uint64_t steps = std::max<uint64_t>(1, ((uint64_t)a.r.most + kStep - 1) / kStep) + kUnitCost;
     // k_page_attn16 over 48 ragged histories of bf16 keys: 1,024 waves 52.6 us,
     // 1,536 and 2,048 54.3; over 96 of Q8_0 keys 85, 77 and 74
-    const uint64_t fill = std::min<uint64_t>((uint64_t)cus * (fast && a.c.kind == Q8_0 ? 8 : 4), kPageMaxRuns);
+    const uint64_t fill = std::min<uint64_t>((uint64_t)cus * (kernel && a.c.kind == Q8_0 ? 8 : 4), kPageMaxRuns);
     a.runs = (uint32_t)std::min<uint64_t>(fill, (a.units * steps * a.r.batch + kRunMin - 1) / kRunMin);
     a.score_row = ((uint64_t)a.r.most + 63) / 64 * 64;
 }
@@ -873,20 +1079,25 @@ template <uint32_t K> static void launch_any(const PageAttn& a, hipStream_t s) {
     else if (a.c.dim <= 128) hipLaunchKernelGGL((k_page_attn_any<K, 16>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((k_page_attn_any<K, 32>), grid, block, 0, s, a);
 }
-template <uint32_t C> static void launch16(const PageAttn& a, hipStream_t s) {
-    if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn16<C, 64>), dim3(a.runs), dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((k_page_attn16<C, 128>), dim3(a.runs), dim3(64), 0, s, a);
+template <uint32_t C> static void launch_matrix(const PageAttn& a, hipStream_t s) {
+    if constexpr (C != F32) {
+        if (a.kernel == 16 && a.c.dim == 64) hipLaunchKernelGGL((k_page_attn16<C, 64>), dim3(a.runs), dim3(64), 0, s, a);
+        else if (a.kernel == 16) hipLaunchKernelGGL((k_page_attn16<C, 128>), dim3(a.runs), dim3(64), 0, s, a);
+        if (a.kernel == 16) return;
+    }
+    if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn32<C, 64>), dim3(a.runs), dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((k_page_attn32<C, 128>), dim3(a.runs), dim3(64), 0, s, a);
+}
+template <uint32_t C> static void launch_attn(const PageAttn& a, hipStream_t s) {
+    if (a.kernel) launch_matrix<C>(a, s);
+    else launch_any<C>(a, s);
 }
 
 void launch_page_attn(const PageAttn& a, hipStream_t s) {
-    const bool fast = a.fast;
-    if (fast && a.c.kind == F16) launch16<F16>(a, s);
-    else if (fast && a.c.kind == BF16) launch16<BF16>(a, s);
-    else if (fast) launch16<Q8_0>(a, s);
-    else if (a.c.kind == F32) launch_any<F32>(a, s);
-    else if (a.c.kind == F16) launch_any<F16>(a, s);
-    else if (a.c.kind == BF16) launch_any<BF16>(a, s);
-    else launch_any<Q8_0>(a, s);
+    if (a.c.kind == F32) launch_attn<F32>(a, s);
+    else if (a.c.kind == F16) launch_attn<F16>(a, s);
+    else if (a.c.kind == BF16) launch_attn<BF16>(a, s);
+    else launch_attn<Q8_0>(a, s);
     if (a.runs > 1) {
         const uint32_t v = a.c.dim % 4 ? 1 : 4;
         // few units hold many parts each (65,537 keys: 64), and a workgroup of

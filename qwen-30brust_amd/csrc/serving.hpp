@@ -69,7 +69,7 @@ struct PageAttn {
     Heads q, out;
     uint32_t heads;
     float scale;
-    bool fast;              // k_page_attn16, not k_page_attn_any
+    uint32_t kernel;        // 16: k_page_attn16, 32: k_page_attn32, 0: k_page_attn_any
     uint32_t groups, per;   // a KV head's query heads, `per` to a unit of work
     uint32_t units;         // of a sequence
     uint32_t runs;          // workgroups
@@ -83,11 +83,10 @@ struct PageAttn {
     float* wout;            // and with this call's added
     size_t win_row, win_head, wout_row, wout_head;
 };
-// Whether the matrix-core kernel takes the call (q set).
-bool page_attn_fast(const PageAttn& a);
+uint32_t page_attn_kernel(const PageAttn& a);  // (q set)
 // The units and runs of a kernel on a GPU of `cus` compute units, then the bytes
 // of its workspace and its pointers.
-void page_attn_plan(PageAttn& a, bool fast, uint32_t cus);
+void page_attn_plan(PageAttn& a, uint32_t kernel, uint32_t cus);
 size_t page_attn_bytes(const PageAttn& a, bool weights);
 void page_attn_place(PageAttn& a, void* work, bool weights);
 void launch_page_attn(const PageAttn& a, hipStream_t s);
