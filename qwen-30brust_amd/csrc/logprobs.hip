@@ -7,7 +7,7 @@
 // ties.  A row that holds NaN or +inf gives NaN; one of -inf alone gives -inf
 // and no entropy; a target outside the vocabulary gives NaN.
 //
-// One pass over the logits, in batches of 2,048 of a row.  All rows' batches, one
+// One pass over the logits, in batches of 1,024 of a row.  All rows' batches, one
 // behind the other, are dealt to waves in equal runs, as many as fill the chip: a
 // single row and hundreds of them both do.  A row that one wave holds whole is
 // done there; of others every wave that holds a part leaves its (m, S, U) and its
@@ -15,13 +15,14 @@
 // that starts with it), and k_logprobs_join folds them.  Every lane keeps the (m,
 // S, U) of its own logits; a new maximum m' takes S to a S and U to a (U + (m -
 // m') S), a = exp(m - m').
-// The alternatives: of the first batch's 256 maxima of eight logits the top-th is
+// The alternatives: of the first batch's 256 or 128 maxima of a load the top-th is
 // a bound that top logits of the part reach, so only logits that reach it (of
 // later batches: that are above it, since ties go to the lower id) can be among
-// them.  They go to a list in LDS, a few more than top in a batch of random logits;
-// it is cut back (cut) at the part's end, or before it could overflow, as rising
-// rows make it.  The n-th largest of the lanes' numbers is found bit by bit, by
+// them.  They go to a list in LDS, which is cut back to its top ones whenever it
+// holds some more than twice that, and the bound rises with it: 777 rows of f32
+// with 20 alternatives took 158 us with the first bound alone.  The n-th largest of the lanes' numbers is found bit by bit, by
 // counting lanes (nth_of).
+#include <algorithm>
 #include <cfloat>
 
 #include "qh_block.hpp"
@@ -29,22 +30,24 @@
 
 namespace qh {
 
-constexpr uint32_t kLpLanes = 8;                     // logits of a load
-constexpr uint32_t kLpStep = 64 * kLpLanes;          // of a wave's load
-constexpr uint32_t kLpSteps = 4;                     // loads of a batch
-constexpr uint32_t kLpBatch = kLpStep * kLpSteps;
-constexpr uint32_t kLpList = 1536;                   // keys of a part's list
+constexpr uint32_t kLpLane = 16;                     // logits of a lane and batch
+constexpr uint32_t kLpBatch = 64 * kLpLane;
+constexpr uint32_t kLpList = 1024;                   // keys of a part's list
 constexpr uint32_t kLpJoin = 4096;                   // and of a row's
-constexpr uint32_t kLpRuns = 2048;                   // waves that fill the chip
+constexpr uint32_t kLpRuns = 4096;                   // waves that fill the chip
 
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)order_key(x) << 32 | (uint32_t)~i; }
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32
 
-// (m, S, U) of some logits.
+// (m, S, U) of some logits, m in units of log 2 and U with it: t = x log2(e) - m
+// is one fused multiply-add, of which a large x loses nothing, S = sum 2^t, U =
+// sum t 2^t, log p = (t - log2 S) ln 2.  A row's maximum past 2e38 either way has
+// no such m: far, and m is the maximum itself (slow_sums).
 struct Sums {
     float m = -INFINITY, S = 0.f, U = 0.f;
     __device__ __forceinline__ void move(float M) {  // to a maximum M >= m
-        const float a = m == -INFINITY ? 0.f : exp_of(m - M);
+        const float a = m == -INFINITY ? 0.f : exp2_of(m - M);
         U = a > 0.f ? a * fmaf(m - M, S, U) : 0.f;
         S *= a;
         m = M;
@@ -85,8 +88,11 @@ template <uint32_t N> struct List {
     }
     // To at least its top keys, and few more: keys below the top-th largest of 256
     // columns' maxima go.  At most top columns keep some (keys differ), so that a
-    // pass halves the list or leaves one key a column.
-    __device__ __forceinline__ void cut(uint32_t top) {
+    // pass halves the list or leaves one key a column.  First by the logits alone,
+    // which takes half as long, then, where that leaves too many alike, by whole
+    // keys.  A number that at least top keys reach, or 0.
+    __device__ __forceinline__ uint64_t cut(uint32_t top) {
+        uint64_t bound = 0;
         while (count > 64 && count > top) {
             __syncthreads();  // (one wave: an order for the compiler)
             const uint32_t n = count, lane = threadIdx.x;
@@ -97,7 +103,13 @@ template <uint32_t N> struct List {
                     const uint32_t j = i + lane + 64 * k;
                     if (j < n) most[k] = max(most[k], key[j]);
                 }
-            const uint64_t bound = max(nth_of(most, top), (uint64_t)1);  // 0: no key
+            const uint32_t high[4] = {(uint32_t)(most[0] >> 32), (uint32_t)(most[1] >> 32), (uint32_t)(most[2] >> 32),
+                                      (uint32_t)(most[3] >> 32)};
+            bound = (uint64_t)nth_of(high, top) << 32;
+            uint32_t reach = 0;
+            for (uint32_t i = 0; i < n; i += 64) reach += __popcll(__ballot(i + lane < n && key[i + lane] >= bound));
+            if (reach > n / 2 + 32) bound = nth_of(most, top);
+            bound = max(bound, (uint64_t)1);  // 0: no key
             count = 0;
             for (uint32_t i = 0; i < n; i += 64) {  // a key moves forward, never past those still to be read
                 const uint64_t k = i + lane < n ? key[i + lane] : 0;
@@ -105,7 +117,9 @@ template <uint32_t N> struct List {
                 append(k >= bound, k);
                 __syncthreads();
             }
+            if (count == n) break;  // (not by whole keys)
         }
+        return bound;
     }
     // f(rank, key) for the top largest keys, each by some lane.
     template <class F> __device__ __forceinline__ void ranked(uint32_t top, F f) {
@@ -129,164 +143,254 @@ __device__ __forceinline__ Sums fold(Sums s) {
     return s;
 }
 
-__device__ __forceinline__ float logp_of(float x, const Sums& s, bool bad) {
-    return bad ? __builtin_nanf("") : x == -INFINITY ? x : x - s.m - logf(s.S);
+// What a row's logits hold, besides.
+enum : uint32_t { kLpBad = 1, kLpHigh = 2, kLpLow = 4 };  // NaN or +inf; finite maxima past 2e38
+constexpr float kLpFar = 2e38f;
+__device__ __forceinline__ uint32_t any_of(uint32_t flags) {
+    uint32_t r = 0;
+#pragma unroll
+    for (uint32_t f = 1; f <= kLpLow; f *= 2) r |= __any(flags & f) ? f : 0;
+    return r;
 }
 
-// A row's numbers from its Sums and its list.
-template <uint32_t K, uint32_t N>
-__device__ __forceinline__ void finish_row(const Logprobs& a, List<N>& L, uint32_t r, const Sums& s, bool bad) {
-    if (threadIdx.x == 0) {
+__device__ __forceinline__ float logp_of(float x, const Sums& s, bool far, bool bad) {
+    if (bad) return __builtin_nanf("");
+    if (x == -INFINITY) return x;
+    const float t = far ? (x - s.m) * kLog2e : fmaf(x, kLog2e, -s.m);
+    if (t == -INFINITY) return far ? x - s.m : x - s.m * kLn2;  // f32::MIN among other logits
+    return (t - log2f(s.S)) * kLn2;
+}
+
+// The Sums of row r about its maximum, by a wave.
+template <uint32_t K> __device__ __forceinline__ Sums slow_sums(const Logprobs& a, uint32_t r) {
+    auto logit = [&](uint32_t i) {
+        const bool masked = a.valid && !gld<uint8_t>(a.valid + i);
+        return masked ? -FLT_MAX : elem<K>(static_cast<const uint8_t*>(a.x), r * a.stride + i);
+    };
+    Sums s;
+    float m = -INFINITY;
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < a.vocab; i += 64) m = fmaxf(m, logit(i));
+    s.m = wave_max(m);
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < a.vocab; i += 64) {
+        const float t = (logit(i) - s.m) * kLog2e, e = exp2_of(t);
+        s.S += e;
+        s.U = fmaf(fmaxf(t, -200.f), e, s.U);
+    }
+    s.S = wave_sum(s.S);
+    s.U = wave_sum(s.U);
+    return s;
+}
+
+// A row whose Sums and flags are known: writes its log probability and entropy,
+// and gives that of others.
+template <uint32_t K> struct Row {
+    Sums s;
+    bool bad, far;
+    __device__ __forceinline__ Row(const Logprobs& a, uint32_t r, Sums sums, uint32_t flags) : s(sums) {
+        bad = flags & kLpBad;
+        far = !bad && ((flags & kLpHigh) || (flags & kLpLow && s.m == -INFINITY));
+        if (far) s = slow_sums<K>(a, r);
+        if (threadIdx.x) return;
         if (a.logp) {
             const uint32_t t = (uint32_t)gld<int32_t>(a.target + r);
             float p = __builtin_nanf("");
-            if (t < a.vocab)
-                p = logp_of(a.valid && !gld<uint8_t>(a.valid + t) ? -FLT_MAX
-                                                                   : elem<K>(static_cast<const uint8_t*>(a.x), r * a.stride + t),
-                            s, bad);
+            if (t < a.vocab) {
+                const bool masked = a.valid && !gld<uint8_t>(a.valid + t);
+                p = logp(masked ? -FLT_MAX : elem<K>(static_cast<const uint8_t*>(a.x), r * a.stride + t));
+            }
             a.logp[r] = p;
         }
-        if (a.entropy) a.entropy[r] = bad ? __builtin_nanf("") : s.S > 0.f ? logf(s.S) - s.U / s.S : 0.f;
+        if (a.entropy) a.entropy[r] = bad ? __builtin_nanf("") : s.S > 0.f ? (log2f(s.S) - s.U / s.S) * kLn2 : 0.f;
     }
-    if (!a.top) return;
-    L.ranked(a.top, [&](uint32_t rank, uint64_t k) {
+    __device__ __forceinline__ float logp(float x) const { return logp_of(x, s, far, bad); }
+    __device__ __forceinline__ void put(const Logprobs& a, uint32_t r, uint32_t rank, uint64_t k) const {
         a.ids[(size_t)r * a.top + rank] = (int32_t) ~(uint32_t)k;
-        a.alt[(size_t)r * a.top + rank] = logp_of(key_value((uint32_t)(k >> 32)), s, bad);
-    });
-}
-
-// Run i holds batches [total i / runs, total (i + 1) / runs) of `all` a row.
-struct Runs {
-    uint32_t all, runs;
-    uint64_t total;
-    __host__ __device__ uint64_t begin(uint64_t i) const { return total * i / runs; }
-    __host__ __device__ uint64_t with(uint64_t x) const { return ((x + 1) * runs + total - 1) / total - 1; }  // the run of batch x
+        a.alt[(size_t)r * a.top + rank] = logp(key_value((uint32_t)(k >> 32)));
+    }
 };
 
-// Eight logits from p, whatever its alignment.
-template <uint32_t K> struct Eight {
-    typedef uint32_t words __attribute__((ext_vector_type(K == F32 ? 8 : 4), aligned(K == F32 ? 4 : 2)));
+// Of the batches, `all` a row, the first `more` runs hold len + 1 each, the others
+// len.
+struct Runs {
+    uint32_t all, runs, more;
+    uint64_t len;
+    static __host__ __device__ uint64_t div(uint64_t a, uint64_t b) {
+        return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+    }
+    __host__ __device__ uint64_t begin(uint32_t i) const { return i * len + (i < more ? i : more); }
+    __host__ __device__ uint64_t with(uint64_t x) const {  // the run of batch x
+        const uint64_t head = more * (len + 1);
+        return x < head ? div(x, len + 1) : more + div(x - head, len);
+    }
+};
+
+// The logits and mask bytes of one load: 16 bytes of a row, whatever their
+// alignment, so that a wave's loads are whole lines.
+template <uint32_t K> struct Load {
+    static constexpr uint32_t E = K == F32 ? 4 : 8, kSteps = kLpLane / E, kStep = 64 * E;
+    typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t masks __attribute__((ext_vector_type(E / 4), aligned(1)));
     words w;
-    __device__ __forceinline__ void load(const uint8_t* p) {
+    masks valid;
+    __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* v) {
 #if defined(__HIP_DEVICE_COMPILE__)
         w = __builtin_nontemporal_load((gptr<words>)p);  // read once
-#else
-        w = *reinterpret_cast<const words*>(p);  // host pass: never executed
 #endif
+        if (v) valid = gld<masks>(v);
     }
-    __device__ __forceinline__ float at(uint32_t i) const {
+    // Of a row of fewer than E logits.
+    __device__ __forceinline__ void few(const uint8_t* p, const uint8_t* v, uint32_t n) {
+        w = words(0u);
+        valid = masks(0u);
+#pragma unroll
+        for (uint32_t j = 0; j < E; j++) {
+            const uint32_t i = min(j, n - 1);
+            if constexpr (K == F32) w[j] = gld<uint32_t>(p + 4 * i);
+            else w[j / 2] |= (uint32_t)gld<uint16_t>(p + 2 * i) << 16 * (j % 2);
+            if (v) valid[j / 4] |= (uint32_t)gld<uint8_t>(v + i) << 8 * (j % 4);
+        }
+    }
+    // Not 0 where a byte is not 1.
+    __device__ __forceinline__ uint32_t masked() const {
+        uint32_t off = valid[0] ^ 0x01010101u;
+        if constexpr (E == 8) off |= valid[1] ^ 0x01010101u;
+        return off;
+    }
+    __device__ __forceinline__ bool on(uint32_t j) const {
+        const uint32_t word = valid[j / 4];
+        return word >> (8 * (j % 4)) & 255;
+    }
+    __device__ __forceinline__ float at(uint32_t j) const {
         if constexpr (K == F32) {
-            return __uint_as_float(w[i]);
+            return __uint_as_float(w[j]);
         } else {
-            const uint32_t pair = w[i / 2];
-            if constexpr (K == BF16) return __uint_as_float(i % 2 ? pair & 0xffff0000u : pair << 16);
-            return (float)__builtin_bit_cast(_Float16, (uint16_t)(i % 2 ? pair >> 16 : pair));
+            const uint32_t pair = w[j / 2];
+            if constexpr (K == BF16) return __uint_as_float(j % 2 ? pair & 0xffff0000u : pair << 16);
+            const uint16_t half = (uint16_t)(j % 2 ? pair >> 16 : pair);
+            return (float)__builtin_bit_cast(_Float16, half);
         }
     }
 };
 
-// Eight mask bytes, whatever their alignment.
-__device__ __forceinline__ uint64_t eight_bytes(const uint8_t* p) {
-    typedef uint32_t words __attribute__((ext_vector_type(2), aligned(1)));
-    const words w = gld<words>(p);
-    return (uint64_t)w.y << 32 | w.x;
-}
-
-// Work: [runs][2] (m, S, U, bad), then [runs][2][top] keys.
+// Work: [runs][2] (m, S, U, flags), then [runs][2][top] keys.
 __device__ __forceinline__ float4* sums_of(const Logprobs& a) { return static_cast<float4*>(a.work); }
 __device__ __forceinline__ uint64_t* keys_of(const Logprobs& a, uint32_t runs) {
     return reinterpret_cast<uint64_t*>(sums_of(a) + 2 * (size_t)runs);
 }
 
-template <uint32_t K> __global__ __launch_bounds__(64) void k_logprobs(Logprobs a, Runs w) {
+template <uint32_t K> __global__ __launch_bounds__(64, 4) void k_logprobs(Logprobs a, Runs w) {
     __shared__ uint64_t keys[kLpList];
     const uint32_t lane = threadIdx.x, top = a.top;
     uint64_t at = w.begin(blockIdx.x);
     const uint64_t end = w.begin(blockIdx.x + 1);
     while (at < end) {
-        const uint32_t r = (uint32_t)(at / w.all), b0 = (uint32_t)(at % w.all);
+        const uint32_t r = (uint32_t)Runs::div(at, w.all), b0 = (uint32_t)(at - (uint64_t)r * w.all);
         const uint32_t b1 = (uint32_t)min((uint64_t)w.all, b0 + (end - at));
         at += b1 - b0;
         const uint8_t* row = static_cast<const uint8_t*>(a.x) + r * a.stride * (K == F32 ? 4 : 2);
         const uint32_t lo = b0 * kLpBatch, hi = min(a.vocab, b1 * kLpBatch);
         List<kLpList> L{keys};
         Sums s;
-        bool bad = false;
+        uint32_t flags = 0;
         float bound = -INFINITY;
-        Eight<K> next[kLpSteps];
-        uint64_t mask[kLpSteps];
-        auto load = [&](uint32_t k, uint32_t i) {  // logits i .. i + 7, where all are there
-            mask[k] = ~(uint64_t)0;
-            if (i + kLpLanes > hi) return;
-            next[k].load(row + (size_t)i * (K == F32 ? 4 : 2));
-            if (a.valid) mask[k] = eight_bytes(a.valid + i);
-        };
-#pragma unroll
-        for (uint32_t k = 0; k < kLpSteps; k++) load(k, lo + kLpStep * k + lane * kLpLanes);
+        uint32_t first = 0;  // its order
+        constexpr uint32_t E = Load<K>::E, kSteps = Load<K>::kSteps, kStep = Load<K>::kStep;
         for (uint32_t b = lo; b < hi; b += kLpBatch) {
-            float x[kLpSteps][kLpLanes], M[kLpSteps];
+            // Lane's loads k: logits i .. i + E - 1, i = b + kStep k + lane E; the last
+            // ones of a row end with it, and hold some again that other loads hold
+            const bool whole = b + kLpBatch <= hi;
+            auto at_of = [&](uint32_t k) { return b + kStep * k + lane * E; };
+            auto from_of = [&](uint32_t k) { return whole ? at_of(k) : min(at_of(k), hi - min(hi, E)); };
+            Load<K> raw[kSteps];
 #pragma unroll
-            for (uint32_t k = 0; k < kLpSteps; k++) {
-                const uint32_t i = b + kLpStep * k + lane * kLpLanes;
-                if (i + kLpLanes <= hi) {
+            for (uint32_t k = 0; k < kSteps; k++) {
+                const uint32_t i = from_of(k);
+                if (hi >= E) raw[k].load(row + (size_t)i * (K == F32 ? 4 : 2), a.valid ? a.valid + i : nullptr);
+                else raw[k].few(row, a.valid, hi);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // every load is requested before one is waited for
+            float x[kSteps][E], M[kSteps], most = -INFINITY;
 #pragma unroll
-                    for (uint32_t j = 0; j < kLpLanes; j++) x[k][j] = mask[k] >> (8 * j) & 255 ? next[k].at(j) : -FLT_MAX;
-                } else {
+            for (uint32_t k = 0; k < kSteps; k++)
 #pragma unroll
-                    for (uint32_t j = 0; j < kLpLanes; j++)
-                        x[k][j] = i + j >= hi ? -INFINITY : a.valid && !gld<uint8_t>(a.valid + i + j) ? -FLT_MAX : elem<K>(row, i + j);
+                for (uint32_t j = 0; j < E; j++) x[k][j] = raw[k].at(j);
+            if (a.valid) {
+                uint32_t off = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < kSteps; k++) off |= raw[k].masked();
+                if (__any(off)) {
+#pragma unroll
+                    for (uint32_t k = 0; k < kSteps; k++)
+#pragma unroll
+                        for (uint32_t j = 0; j < E; j++) x[k][j] = raw[k].on(j) ? x[k][j] : -FLT_MAX;
                 }
-                load(k, i + kLpBatch);
+            }
+            if (!whole) {
+#pragma unroll
+                for (uint32_t k = 0; k < kSteps; k++)
+#pragma unroll
+                    for (uint32_t j = 0; j < E; j++) {
+                        const uint32_t i = from_of(k) + j;
+                        x[k][j] = i >= at_of(k) && i < hi ? x[k][j] : -INFINITY;
+                    }
             }
 #pragma unroll
-            for (uint32_t k = 0; k < kLpSteps; k++) {
+            for (uint32_t k = 0; k < kSteps; k++) {
                 M[k] = x[k][0];
 #pragma unroll
-                for (uint32_t j = 1; j < kLpLanes; j++) M[k] = fmaxf(M[k], x[k][j]);  // NaN only if all are
+                for (uint32_t j = 1; j < E; j++) M[k] = fmaxf(M[k], x[k][j]);  // NaN only if all are
+                most = fmaxf(most, M[k]);
             }
-            const float most = fmaxf(fmaxf(M[0], M[1]), fmaxf(M[2], M[3]));
-            if (most > s.m) s.move(most);
+            if (most * kLog2e > s.m) s.move(most * kLog2e);
             const float m = s.m == -INFINITY ? 0.f : s.m;
             float S = 0.f, U = 0.f;
 #pragma unroll
-            for (uint32_t k = 0; k < kLpSteps; k++)
+            for (uint32_t k = 0; k < kSteps; k++)
 #pragma unroll
-                for (uint32_t j = 0; j < kLpLanes; j++) {
-                    const float d = x[k][j] - m, e = exp_of(d);
+                for (uint32_t j = 0; j < E; j++) {
+                    const float t = fmaf(x[k][j], kLog2e, -m), e = exp2_of(t);
                     S += e;
-                    U = fmaf(fmaxf(d, -1e4f), e, U);  // 0, not NaN, for -inf
+                    U = fmaf(fmaxf(t, -200.f), e, U);  // 0, not NaN, for -inf
                 }
             s.S += S;
             s.U += U;
-            bad |= most == INFINITY || S != S;
+            if (fabsf(most) > kLpFar && most != -INFINITY) flags |= most == INFINITY ? kLpBad : most > 0.f ? kLpHigh : kLpLow;
+            if (S != S && most <= kLpFar) flags |= kLpBad;
             if (!top) continue;
-            const bool first = b == lo;
-            if (first) {
-                uint32_t mine[kLpSteps];
+            if (b == lo) {
+                uint32_t mine[kSteps];
 #pragma unroll
-                for (uint32_t k = 0; k < kLpSteps; k++)
-                    mine[k] = b + kLpStep * k + lane * kLpLanes < hi ? order_key(M[k]) : 0;
-                const uint32_t t = nth_of(mine, top);
-                bound = t ? key_value(t) : -INFINITY;
+                for (uint32_t k = 0; k < kSteps; k++) mine[k] = at_of(k) < hi ? order_key(M[k]) : 0;
+                first = nth_of(mine, top);
+                bound = first ? key_value(first) : -INFINITY;
             }
+            if (!__any(!(most < bound) || flags & kLpBad)) continue;
 #pragma unroll
-            for (uint32_t k = 0; k < kLpSteps; k++) {
-                if (!__any(bad || (first ? !(M[k] < bound) : M[k] > bound))) continue;
-                if (L.count > kLpList - kLpStep) L.cut(top);
-                const uint32_t i = b + kLpStep * k + lane * kLpLanes;
+            for (uint32_t k = 0; k < kSteps; k++) {
+                if (!__any(!(M[k] < bound) || flags & kLpBad)) continue;
+                if (L.count > kLpList - kStep) L.cut(top);
+                const uint32_t at = at_of(k), i = from_of(k);
 #pragma unroll
-                for (uint32_t j = 0; j < kLpLanes; j++)
-                    L.append(i + j < hi && (first ? !(x[k][j] < bound) : !(x[k][j] <= bound)), key_of(x[k][j], i + j));
+                for (uint32_t j = 0; j < E; j++)
+                    L.append(!(x[k][j] < bound) && (whole || (i + j >= at && i + j < hi)), key_of(x[k][j], i + j));
             }
+            // from here on only what is above what top keys reach
+            if (L.count > 2 * top + 32) first = (uint32_t)(L.cut(top) >> 32);
+            else if (b != lo) continue;
+            bound = key_value(first);
+            if (bound < INFINITY) bound = key_value(first + 1);
         }
-        const bool any = __any(bad);
+        flags = any_of(flags);
         s = fold(s);
+        const size_t slot = (size_t)blockIdx.x * 2 + (b0 == 0);
+        uint64_t* out = keys_of(a, w.runs) + slot * top;
         if (b1 - b0 == w.all) {
-            finish_row<K>(a, L, r, s, any);
+            const Row<K> done(a, r, s, flags);
+            if (top) L.ranked(top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
         } else {
-            const size_t slot = (size_t)blockIdx.x * 2 + (b0 == 0);
-            if (lane == 0) sums_of(a)[slot] = make_float4(s.m, s.S, s.U, any ? 1.f : 0.f);
-            uint64_t* out = keys_of(a, w.runs) + slot * top;
+            if (lane == 0) sums_of(a)[slot] = make_float4(s.m, s.S, s.U, __uint_as_float(flags));
             for (uint32_t i = hi - lo + lane; i < top; i += 64) out[i] = 0;  // a part may hold fewer
             if (top) L.ranked(top, [&](uint32_t rank, uint64_t k) { out[rank] = k; });
         }
@@ -300,19 +404,20 @@ template <uint32_t K> __global__ __launch_bounds__(64) void k_logprobs(Logprobs 
 // reach the largest such bound go to the list.
 template <uint32_t K> __global__ __launch_bounds__(64) void k_logprobs_join(Logprobs a, Runs w) {
     __shared__ uint64_t listed[kLpJoin];
+    constexpr uint32_t kAhead = 16;  // keys of a lane in flight
     const uint32_t r = blockIdx.x, lane = threadIdx.x, top = a.top;
     const uint64_t x = (uint64_t)r * w.all, first = w.with(x);
     const uint32_t parts = (uint32_t)(w.with(x + w.all - 1) - first) + 1;
     if (parts == 1) return;  // done in its wave
     auto slot = [&](uint32_t i) { return (first + i) * 2 + (i == 0); };
     Sums s;
-    bool bad = false;
+    uint32_t flags = 0;
     for (uint32_t i = lane; i < parts; i += 64) {
         const float4 v = gld<float4>(sums_of(a) + slot(i));
         Sums o;
         o.m = v.x, o.S = v.y, o.U = v.z;
         s.add(o);
-        bad |= v.w != 0.f;
+        flags |= __float_as_uint(v.w);
     }
     List<kLpJoin> L{listed};
     if (top) {
@@ -327,27 +432,31 @@ template <uint32_t K> __global__ __launch_bounds__(64) void k_logprobs_join(Logp
             bound = max(nth_of(nth, (top + n - 1) / n), (uint64_t)1);  // 0: a part of fewer keys
         }
         const uint32_t all = parts * top;
-#pragma unroll 8
-        for (uint32_t i0 = 0; i0 < all; i0 += 64) {
-            const uint32_t i = min(i0 + lane, all - 1);
-            const uint64_t k = gld<uint64_t>(keys + slot(i / top) * top + i % top);
-            L.append(i0 + lane < all && k >= bound, k);
+        for (uint32_t i0 = 0; i0 < all; i0 += 64 * kAhead) {
+            uint64_t k[kAhead];
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; j++) {
+                const uint32_t i = min(i0 + 64 * j + lane, all - 1), part = i / top;
+                k[j] = gld<uint64_t>(keys + slot(part) * top + (i - part * top));
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; j++) L.append(i0 + 64 * j + lane < all && k[j] >= bound, k[j]);
         }
     }
-    finish_row<K>(a, L, r, fold(s), __any(bad));
+    const Row<K> done(a, r, fold(s), any_of(flags));
+    if (top) L.ranked(top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
 }
 
 static Runs lp_runs(uint32_t rows, uint32_t vocab, uint32_t top) {
     Runs w{};
     w.all = (vocab + kLpBatch - 1) / kLpBatch;
-    w.total = (uint64_t)rows * w.all;
-    w.runs = (uint32_t)(w.total < kLpRuns ? w.total : kLpRuns);
-    // the list of k_logprobs_join holds the keys of a row's parts: one more may
-    // begin in the row than runs fit it
-    if (top && kLpJoin / top < w.all + 2) {
-        const uint64_t most = (uint64_t)rows * (kLpJoin / top - 2);
-        if (w.runs > most) w.runs = (uint32_t)most;
-    }
+    const uint64_t total = (uint64_t)rows * w.all;
+    // the list of k_logprobs_join holds the keys of a row's parts: ceil(all / len)
+    // and one more
+    const uint64_t fit = top ? kLpJoin / top - 1 : w.all, least = (w.all + fit - 1) / fit;
+    w.runs = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(total / least, kLpRuns));
+    w.len = total / w.runs;
+    w.more = (uint32_t)(total % w.runs);
     return w;
 }
 
