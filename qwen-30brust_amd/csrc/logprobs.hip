@@ -15,13 +15,13 @@
 // that starts with it), and k_logprobs_join folds them.  Every lane keeps the (m,
 // S, U) of its own logits; a new maximum m' takes S to a S and U to a (U + (m -
 // m') S), a = exp(m - m').
-// The alternatives: of the first batch's 256 or 128 maxima of a load the top-th is
-// a bound that top logits of the part reach, so only logits that reach it (of
-// later batches: that are above it, since ties go to the lower id) can be among
-// them.  They go to a list in LDS, which is cut back to its top ones whenever it
-// holds some more than twice that, and the bound rises with it: 777 rows of f32
-// with 20 alternatives took 158 us with the first bound alone.  The n-th largest of the lanes' numbers is found bit by bit, by
-// counting lanes (nth_of).
+// The alternatives: a wave keeps its part's top keys (a logit's order and its id,
+// so that no two are alike) in its lanes' registers, in descending order.  Only
+// logits above the top-th of them can get in (one that equals it has a higher id);
+// of a batch with many such, as the first, only those that the top-th largest of
+// its loads' maxima lets through.  A key is put in its place by counting the keys
+// above it and moving the others up a lane: about a hundred cycles, and a part of
+// n batches of random logits has some top (1 + ln n) of them.
 #include <algorithm>
 #include <cfloat>
 
@@ -32,8 +32,7 @@ namespace qh {
 
 constexpr uint32_t kLpLane = 16;                     // logits of a lane and batch
 constexpr uint32_t kLpBatch = 64 * kLpLane;
-constexpr uint32_t kLpList = 1024;                   // keys of a part's list
-constexpr uint32_t kLpJoin = 4096;                   // and of a row's
+constexpr uint32_t kLpMany = 32;                     // loads of a batch that hold logits above the bound
 constexpr uint32_t kLpRuns = 4096;                   // waves that fill the chip
 
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)order_key(x) << 32 | (uint32_t)~i; }
@@ -76,61 +75,37 @@ template <typename T, uint32_t R> __device__ __forceinline__ T nth_of(const T (&
     return found;
 }
 
-// Keys of one wave in LDS; the count is the same in every lane.
-template <uint32_t N> struct List {
-    uint64_t* key;
-    uint32_t count = 0;
-    __device__ __forceinline__ void append(bool on, uint64_t k) {
-        const uint64_t who = __ballot(on);
-        if (who == 0) return;
-        if (on) key[count + __popcll(who & (((uint64_t)1 << (threadIdx.x & 63)) - 1))] = k;
-        count += __popcll(who);
+// The largest 64 R keys that came, in descending order: the i-th in lane i % 64 of
+// key[i / 64]; 0: none.
+template <uint32_t R> struct Best {
+    uint64_t key[R] = {};
+    __device__ __forceinline__ static uint64_t up(uint64_t v, uint64_t in) {  // a lane up, `in` into lane 0
+        const uint32_t lo = __builtin_amdgcn_update_dpp((uint32_t)in, (uint32_t)v, 0x138, 0xf, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp((uint32_t)(in >> 32), (uint32_t)(v >> 32), 0x138, 0xf, 0xf, false);
+        return (uint64_t)hi << 32 | lo;
     }
-    // To at least its top keys, and few more: keys below the top-th largest of 256
-    // columns' maxima go.  At most top columns keep some (keys differ), so that a
-    // pass halves the list or leaves one key a column.  First by the logits alone,
-    // which takes half as long, then, where that leaves too many alike, by whole
-    // keys.  A number that at least top keys reach, or 0.
-    __device__ __forceinline__ uint64_t cut(uint32_t top) {
-        uint64_t bound = 0;
-        while (count > 64 && count > top) {
-            __syncthreads();  // (one wave: an order for the compiler)
-            const uint32_t n = count, lane = threadIdx.x;
-            uint64_t most[4] = {0, 0, 0, 0};
-            for (uint32_t i = 0; i < n; i += 256)
+    __device__ __forceinline__ static uint64_t of_lane(uint64_t v, uint32_t l) {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), l) << 32 |
+               (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, l);
+    }
+    __device__ __forceinline__ uint64_t at(uint32_t i) const {
+        uint64_t v = of_lane(key[0], i & 63);
+        if constexpr (R == 2) v = i < 64 ? v : of_lane(key[1], i & 63);
+        return v;
+    }
+    // c, the same in every lane.
+    __device__ __forceinline__ void put(uint64_t c) {
+        const uint32_t lane = threadIdx.x;
+        uint64_t spill = 0;  // what leaves lane 63 of a row
 #pragma unroll
-                for (uint32_t k = 0; k < 4; k++) {
-                    const uint32_t j = i + lane + 64 * k;
-                    if (j < n) most[k] = max(most[k], key[j]);
-                }
-            const uint32_t high[4] = {(uint32_t)(most[0] >> 32), (uint32_t)(most[1] >> 32), (uint32_t)(most[2] >> 32),
-                                      (uint32_t)(most[3] >> 32)};
-            bound = (uint64_t)nth_of(high, top) << 32;
-            uint32_t reach = 0;
-            for (uint32_t i = 0; i < n; i += 64) reach += __popcll(__ballot(i + lane < n && key[i + lane] >= bound));
-            if (reach > n / 2 + 32) bound = nth_of(most, top);
-            bound = max(bound, (uint64_t)1);  // 0: no key
-            count = 0;
-            for (uint32_t i = 0; i < n; i += 64) {  // a key moves forward, never past those still to be read
-                const uint64_t k = i + lane < n ? key[i + lane] : 0;
-                __syncthreads();
-                append(k >= bound, k);
-                __syncthreads();
-            }
-            if (count == n) break;  // (not by whole keys)
-        }
-        return bound;
-    }
-    // f(rank, key) for the top largest keys, each by some lane.
-    template <class F> __device__ __forceinline__ void ranked(uint32_t top, F f) {
-        cut(top);
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < count; i += 64) {
-            const uint64_t k = key[i];
-            uint32_t above = 0;
-#pragma unroll 8
-            for (uint32_t j = 0; j < count; j++) above += key[j] > k;
-            if (above < top) f(above, k);
+        for (uint32_t r = 0; r < R; r++) {
+            const uint32_t above = __popcll(__ballot(key[r] > c));  // a row of larger keys stays
+            const uint64_t last = of_lane(key[r], 63), moved = up(key[r], spill);
+            const uint64_t in = r && spill ? spill : c;
+            const uint32_t place = r && spill ? 0 : above;
+            key[r] = lane < place ? key[r] : lane == place ? in : moved;
+            spill = place < 64 ? last : 0;
+            if (place < 64 && last == 0) break;
         }
     }
 };
@@ -211,6 +186,13 @@ template <uint32_t K> struct Row {
     }
 };
 
+// f(rank, key) for the first `top` keys.
+template <uint32_t R, class F> __device__ __forceinline__ void each(const Best<R>& best, uint32_t top, F f) {
+#pragma unroll
+    for (uint32_t r = 0; r < R; r++)
+        if (threadIdx.x + 64 * r < top) f(threadIdx.x + 64 * r, best.key[r]);
+}
+
 // Of the batches, `all` a row, the first `more` runs hold len + 1 each, the others
 // len.
 struct Runs {
@@ -280,8 +262,7 @@ __device__ __forceinline__ uint64_t* keys_of(const Logprobs& a, uint32_t runs) {
     return reinterpret_cast<uint64_t*>(sums_of(a) + 2 * (size_t)runs);
 }
 
-template <uint32_t K> __global__ __launch_bounds__(64, 4) void k_logprobs(Logprobs a, Runs w) {
-    __shared__ uint64_t keys[kLpList];
+template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_logprobs(Logprobs a, Runs w) {
     const uint32_t lane = threadIdx.x, top = a.top;
     uint64_t at = w.begin(blockIdx.x);
     const uint64_t end = w.begin(blockIdx.x + 1);
@@ -291,11 +272,10 @@ template <uint32_t K> __global__ __launch_bounds__(64, 4) void k_logprobs(Logpro
         at += b1 - b0;
         const uint8_t* row = static_cast<const uint8_t*>(a.x) + r * a.stride * (K == F32 ? 4 : 2);
         const uint32_t lo = b0 * kLpBatch, hi = min(a.vocab, b1 * kLpBatch);
-        List<kLpList> L{keys};
+        Best<R> best;
         Sums s;
         uint32_t flags = 0;
-        float bound = -INFINITY;
-        uint32_t first = 0;  // its order
+        float bound = -INFINITY;  // logits below it do not get in
         constexpr uint32_t E = Load<K>::E, kSteps = Load<K>::kSteps, kStep = Load<K>::kStep;
         for (uint32_t b = lo; b < hi; b += kLpBatch) {
             // Lane's loads k: logits i .. i + E - 1, i = b + kStep k + lane E; the last
@@ -359,51 +339,57 @@ template <uint32_t K> __global__ __launch_bounds__(64, 4) void k_logprobs(Logpro
             if (fabsf(most) > kLpFar && most != -INFINITY) flags |= most == INFINITY ? kLpBad : most > 0.f ? kLpHigh : kLpLow;
             if (S != S && most <= kLpFar) flags |= kLpBad;
             if (!top) continue;
-            if (b == lo) {
+            if (!__any(!(most < bound) || flags & kLpBad)) continue;
+            uint32_t loads = 0;  // that hold such logits
+#pragma unroll
+            for (uint32_t k = 0; k < kSteps; k++) loads += __popcll(__ballot(!(M[k] < bound)));
+            float low = bound;
+            if (loads > kLpMany) {
                 uint32_t mine[kSteps];
 #pragma unroll
                 for (uint32_t k = 0; k < kSteps; k++) mine[k] = at_of(k) < hi ? order_key(M[k]) : 0;
-                first = nth_of(mine, top);
-                bound = first ? key_value(first) : -INFINITY;
+                const uint32_t t = nth_of(mine, top);
+                if (t && key_value(t) > low) low = key_value(t);
             }
-            if (!__any(!(most < bound) || flags & kLpBad)) continue;
 #pragma unroll
             for (uint32_t k = 0; k < kSteps; k++) {
-                if (!__any(!(M[k] < bound) || flags & kLpBad)) continue;
-                if (L.count > kLpList - kStep) L.cut(top);
+                if (!__any(!(M[k] < low) || flags & kLpBad)) continue;
                 const uint32_t at = at_of(k), i = from_of(k);
 #pragma unroll
-                for (uint32_t j = 0; j < E; j++)
-                    L.append(!(x[k][j] < bound) && (whole || (i + j >= at && i + j < hi)), key_of(x[k][j], i + j));
+                for (uint32_t j = 0; j < E; j++) {
+                    uint64_t who = __ballot(!(x[k][j] < low) && (whole || (i + j >= at && i + j < hi)));
+                    for (; who; who &= who - 1) {
+                        const uint32_t l = __ffsll((unsigned long long)who) - 1;
+                        const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[k][j]), l));
+                        best.put(key_of(v, __builtin_amdgcn_readlane(i + j, l)));
+                    }
+                }
             }
-            // from here on only what is above what top keys reach
-            if (L.count > 2 * top + 32) first = (uint32_t)(L.cut(top) >> 32);
-            else if (b != lo) continue;
-            bound = key_value(first);
-            if (bound < INFINITY) bound = key_value(first + 1);
+            const uint32_t last = (uint32_t)(best.at(top - 1) >> 32);
+            if (last) {
+                bound = key_value(last);
+                if (bound < INFINITY) bound = key_value(last + 1);
+            }
         }
         flags = any_of(flags);
         s = fold(s);
         const size_t slot = (size_t)blockIdx.x * 2 + (b0 == 0);
-        uint64_t* out = keys_of(a, w.runs) + slot * top;
         if (b1 - b0 == w.all) {
             const Row<K> done(a, r, s, flags);
-            if (top) L.ranked(top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
+            each(best, top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
         } else {
             if (lane == 0) sums_of(a)[slot] = make_float4(s.m, s.S, s.U, __uint_as_float(flags));
-            for (uint32_t i = hi - lo + lane; i < top; i += 64) out[i] = 0;  // a part may hold fewer
-            if (top) L.ranked(top, [&](uint32_t rank, uint64_t k) { out[rank] = k; });
+            uint64_t* out = keys_of(a, w.runs) + slot * top;
+            each(best, top, [&](uint32_t rank, uint64_t k) { out[rank] = k; });
         }
-        __syncthreads();
     }
 }
 
-// A row that several waves hold parts of, at most kLpJoin / top of them.  Their
-// keys lie in descending order.  With n = ceil(top / parts), ceil(top / n) parts'
-// n-th keys that reach a bound stand for top keys that do, so that only keys that
-// reach the largest such bound go to the list.
-template <uint32_t K> __global__ __launch_bounds__(64) void k_logprobs_join(Logprobs a, Runs w) {
-    __shared__ uint64_t listed[kLpJoin];
+// A row that several waves hold parts of.  Their keys lie in descending order.
+// With n = ceil(top / parts), ceil(top / n) parts' n-th keys that reach a bound
+// stand for top keys that do, so that only keys that reach the largest such bound
+// are looked at.
+template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64) void k_logprobs_join(Logprobs a, Runs w) {
     constexpr uint32_t kAhead = 16;  // keys of a lane in flight
     const uint32_t r = blockIdx.x, lane = threadIdx.x, top = a.top;
     const uint64_t x = (uint64_t)r * w.all, first = w.with(x);
@@ -419,63 +405,70 @@ template <uint32_t K> __global__ __launch_bounds__(64) void k_logprobs_join(Logp
         s.add(o);
         flags |= __float_as_uint(v.w);
     }
-    List<kLpJoin> L{listed};
+    Best<R> best;
     if (top) {
         const uint64_t* keys = keys_of(a, w.runs);
-        const uint32_t n = (top + parts - 1) / parts;
-        uint64_t bound = 1;
+        const uint32_t n = (top + parts - 1) / parts, all = parts * top;
+        uint64_t bound = 1;  // 0: a part of fewer keys
         if (parts <= 256) {
-            uint64_t nth[4];
+            uint32_t nth[4];
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++)
-                nth[k] = lane + 64 * k < parts ? gld<uint64_t>(keys + slot(lane + 64 * k) * top + n - 1) : 0;
-            bound = max(nth_of(nth, (top + n - 1) / n), (uint64_t)1);  // 0: a part of fewer keys
+                nth[k] = lane + 64 * k < parts ? (uint32_t)(gld<uint64_t>(keys + slot(lane + 64 * k) * top + n - 1) >> 32) : 0;
+            bound = max((uint64_t)nth_of(nth, (top + n - 1) / n) << 32, (uint64_t)1);
         }
-        const uint32_t all = parts * top;
         for (uint32_t i0 = 0; i0 < all; i0 += 64 * kAhead) {
             uint64_t k[kAhead];
 #pragma unroll
             for (uint32_t j = 0; j < kAhead; j++) {
-                const uint32_t i = min(i0 + 64 * j + lane, all - 1), part = i / top;
-                k[j] = gld<uint64_t>(keys + slot(part) * top + (i - part * top));
+                const uint32_t i = i0 + 64 * j + lane, rank = min(i, all - 1) / parts, part = min(i, all - 1) - rank * parts;
+                k[j] = gld<uint64_t>(keys + slot(part) * top + rank);  // the parts' first keys first
+                if (i >= all) k[j] = 0;
             }
 #pragma unroll
-            for (uint32_t j = 0; j < kAhead; j++) L.append(i0 + 64 * j + lane < all && k[j] >= bound, k[j]);
+            for (uint32_t j = 0; j < kAhead; j++) {
+                for (uint64_t who = __ballot(k[j] >= bound); who; who &= who - 1) {
+                    const uint64_t c = Best<R>::of_lane(k[j], __ffsll((unsigned long long)who) - 1);
+                    if (c >= bound) best.put(c);
+                }
+                bound = max(bound, best.at(top - 1));
+            }
         }
     }
     const Row<K> done(a, r, fold(s), any_of(flags));
-    if (top) L.ranked(top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
+    each(best, top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
 }
 
-static Runs lp_runs(uint32_t rows, uint32_t vocab, uint32_t top) {
+static Runs lp_runs(uint32_t rows, uint32_t vocab) {
     Runs w{};
     w.all = (vocab + kLpBatch - 1) / kLpBatch;
     const uint64_t total = (uint64_t)rows * w.all;
-    // the list of k_logprobs_join holds the keys of a row's parts: ceil(all / len)
-    // and one more
-    const uint64_t fit = top ? kLpJoin / top - 1 : w.all, least = (w.all + fit - 1) / fit;
-    w.runs = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(total / least, kLpRuns));
+    w.runs = (uint32_t)std::min<uint64_t>(total, kLpRuns);
     w.len = total / w.runs;
     w.more = (uint32_t)(total % w.runs);
     return w;
 }
 
 size_t logprobs_bytes(uint32_t rows, uint32_t vocab, uint32_t top) {
-    const Runs w = lp_runs(rows, vocab, top);
+    const Runs w = lp_runs(rows, vocab);
     return (size_t)w.runs * 2 * (16 + 8 * (size_t)top);
 }
 
-template <uint32_t K> static void launch(const Logprobs& a, hipStream_t s) {
-    const Runs w = lp_runs(a.rows, a.vocab, a.top);
-    hipLaunchKernelGGL(k_logprobs<K>, dim3(w.runs), dim3(64), 0, s, a, w);
+template <uint32_t K, uint32_t R> static void launch(const Logprobs& a, hipStream_t s) {
+    const Runs w = lp_runs(a.rows, a.vocab);
+    hipLaunchKernelGGL((k_logprobs<K, R>), dim3(w.runs), dim3(64), 0, s, a, w);
     if (a.rows % w.runs)  // else every run holds whole rows
-        hipLaunchKernelGGL(k_logprobs_join<K>, dim3(a.rows), dim3(64), 0, s, a, w);
+        hipLaunchKernelGGL((k_logprobs_join<K, R>), dim3(a.rows), dim3(64), 0, s, a, w);
+}
+template <uint32_t K> static void launch_kind(const Logprobs& a, hipStream_t s) {
+    if (a.top <= 64) launch<K, 1>(a, s);
+    else launch<K, 2>(a, s);
 }
 
 void launch_logprobs(const Logprobs& a, hipStream_t s) {
-    if (a.kind == F32) launch<F32>(a, s);
-    else if (a.kind == F16) launch<F16>(a, s);
-    else launch<BF16>(a, s);
+    if (a.kind == F32) launch_kind<F32>(a, s);
+    else if (a.kind == F16) launch_kind<F16>(a, s);
+    else launch_kind<BF16>(a, s);
 }
 
 }  // namespace qh
