@@ -16,7 +16,7 @@ namespace qh {
 constexpr uint32_t BF16 = 30;
 constexpr uint32_t kPageMaxDim = 256;      // widest head of the paged operators
 constexpr uint32_t kPageMaxRuns = 2048;    // most workgroups of the attention
-constexpr uint32_t kMoveKeys = 16;         // keys per workgroup of k_page_move
+constexpr uint32_t kMoveKeys = 64;         // keys per workgroup of k_page_move
 constexpr uint32_t kLogprobMaxTop = 128;   // most alternatives of a row
 
 // A cache: element j of head g of slot s of page p is at p * ps + s * ts +
