@@ -15,14 +15,157 @@
 namespace qh {
 
 // ------------------------------------------------------------------ append --
-// A wave per token and head (q's heads, then k's, then v's):
+// For every token and head (q's heads, then k's, then v's):
 //   y = x / sqrt(sum x^2 / dim + eps) * w              (q and k, with weights)
 //   (y_i, y_j) = (y_i cos - y_j sin, y_j cos + y_i sin), j = i + dim / 2
 // in 32 bits, rounded once to the type it is stored in.  Q8_0: per 32 values
 // d = f16(max |y| / 127) and codes round(y / d), as GGML lays them out, but
 // codes and scales each in an array of their own.
 // A token outside the table of angles becomes NaN.
-__global__ __launch_bounds__(kBlock) void k_page_append(PageAppend a) {
+
+// Where token i goes: into place t of sequence b, or nowhere.  By a wave.
+struct Place {
+    uint32_t b;
+    int32_t t;
+    bool live;
+};
+__device__ __forceinline__ Place place_of(const PageAppend& a, uint32_t i) {
+    const uint32_t lane = threadIdx.x & 63;
+    Place p{i, 0, true};
+    int32_t at = 0, count = 1;  // the token's number in its sequence, and of how many
+    if (a.first) {
+        // the last sequence whose first token is not behind it
+        uint32_t before = 0;
+        for (uint32_t j = 0; j <= a.r.batch; j += 64) {
+            const bool le = j + lane <= a.r.batch && gld<int32_t>(a.first + min(j + lane, a.r.batch)) <= (int32_t)i;
+            before += __popcll(__ballot(le));
+        }
+        p.live = before > 0 && before <= a.r.batch;
+        p.b = p.live ? before - 1 : 0;
+        const int32_t f = gld<int32_t>(a.first + p.b);
+        at = (int32_t)i - f;
+        count = gld<int32_t>(a.first + p.b + 1) - f;
+    }
+    const int32_t len = p.live ? length_of(a.r, p.b) : -1;
+    p.t = len - count + at;
+    p.live = p.live && p.t >= 0 && p.t < len;
+    return p;
+}
+// The cache's page of a place, or -1.
+__device__ __forceinline__ int32_t page_of(const PageAppend& a, const Place& p) {
+    const int32_t page = gld<int32_t>(a.r.table + p.b * a.r.stride + (uint32_t)p.t / a.c.page);
+    return page < 0 || (uint32_t)page >= a.c.count ? -1 : page;
+}
+__device__ __forceinline__ size_t slot_of(const PageAppend& a, const Place& p, int32_t page, uint32_t g) {
+    return (size_t)page * a.c.ps + (size_t)((uint32_t)p.t % a.c.page) * a.c.ts + g * a.c.hs;
+}
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef bf16_t b4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u4h __attribute__((ext_vector_type(4)));
+
+// Elements i .. i + 3 of p, aligned so.
+__device__ __forceinline__ f4 four(uint32_t kind, const uint8_t* p, size_t i) {
+    if (kind == F32) return gld<f4>(p + 4 * i);
+    if (kind == F16) return __builtin_convertvector(gld<h4>(p + 2 * i), f4);
+    const u4h u = gld<u4h>(p + 2 * i);
+    f4 x;
+    for (int j = 0; j < 4; j++) x[j] = __uint_as_float((uint32_t)u[j] << 16);
+    return x;
+}
+__device__ __forceinline__ void put_four(uint32_t kind, uint8_t* p, size_t i, f4 x) {
+    if (kind == F32) *reinterpret_cast<f4*>(p + 4 * i) = x;
+    else if (kind == F16) *reinterpret_cast<h4*>(p + 2 * i) = __builtin_convertvector(x, h4);
+    else *reinterpret_cast<b4*>(p + 2 * i) = __builtin_convertvector(x, b4);
+}
+// Q8_0 codes of a value: fine, whether its block is finite, f the block's scale.
+__device__ __forceinline__ int32_t code_of(float x, bool fine, float f) {
+    return fine && f > 0.f ? (int32_t)fminf(fmaxf(rintf(x / f), -127.f), 127.f) : 0;
+}
+
+// Heads of 8 L values, all rows aligned to four elements: a wave takes 64 / L
+// heads of a token, a lane four values of the first half and the four they turn
+// with, so nothing is exchanged but the norm's sum and, in Q8_0, a block's maximum
+// (8 lanes).  Bound by memory where there are many tokens: 2,001 tokens of 32 + 2 x 4
+// heads of 128 from f32 into f16 take 16 us (79 MB, 4.9 TB/s), 48 with a wave a head; 64
+// tokens of a decode step 4.5 us, the four dependent look-ups of a place.
+template <uint32_t L> __global__ __launch_bounds__(kBlock) void k_page_append(PageAppend a, uint32_t groups) {
+    constexpr uint32_t D = 8 * L;
+    const uint32_t lane = threadIdx.x & 63, l = lane % L;
+    const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+    const uint32_t i = unit / groups, h = unit % groups * (64 / L) + lane / L;
+    if (i >= a.n) return;
+    const bool mine = h < a.heads + 2 * a.c.kvheads;
+    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.c.kvheads;
+    const uint32_t g = !mine ? 0 : is_q ? h : is_k ? h - a.heads : h - a.heads - a.c.kvheads;
+    const Heads& src = is_q ? a.q : is_k ? a.k : a.v;
+    const size_t from = i * src.row + g * src.head + 4 * l;
+    f4 x = four(src.kind, src.p, from), y = four(src.kind, src.p, from + D / 2);
+    const Place p = place_of(a, i);
+    if (!p.live || !mine) return;
+    const float* w = is_q ? a.qw : is_k ? a.kw : nullptr;
+    if (w) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) ss = fmaf(x[j], x[j], fmaf(y[j], y[j], ss));
+#pragma unroll
+        for (uint32_t s = 1; s < L; s <<= 1) ss += __shfl_xor(ss, s, 64);
+        const float s = 1.f / sqrtf(ss / (float)D + a.eps);
+        x = x * s * gld<f4>(w + 4 * l);
+        y = y * s * gld<f4>(w + D / 2 + 4 * l);
+    }
+    if (a.rope && (is_q || is_k)) {
+        const int32_t at = a.pos ? gld<int32_t>(a.pos + i) : p.t;
+        const bool in = at >= 0 && (uint32_t)at < a.rope_rows;
+        const float* row = reinterpret_cast<const float*>(a.rope + (size_t)(in ? at : 0) * (D / 2)) + 8 * l;
+        const f4 c0 = gld<f4>(row), c1 = gld<f4>(row + 4);
+        const f4 c = {c0.x, c0.z, c1.x, c1.z}, s = {c0.y, c0.w, c1.y, c1.w};
+        const f4 turned = x * c - y * s;
+        y = y * c + x * s;
+        x = turned;
+        if (!in) x = y = __builtin_nanf("");
+    }
+    if (is_q) {
+        const size_t o = i * a.qo.row + g * a.qo.head + 4 * l;
+        put_four(a.qo.kind, a.qo.p, o, x);
+        put_four(a.qo.kind, a.qo.p, o + D / 2, y);
+        return;
+    }
+    const int32_t page = page_of(a, p);
+    if (page < 0) return;
+    const size_t o = slot_of(a, p, page, g) + 4 * l;
+    uint8_t* to = is_k ? a.c.k : a.c.v;
+    if (a.c.kind != Q8_0) {
+        put_four(a.c.kind, to, o, x);
+        put_four(a.c.kind, to, o + D / 2, y);
+        return;
+    }
+    _Float16* scale = is_k ? a.c.ks : a.c.vs;
+#pragma unroll
+    for (uint32_t half = 0; half < 2; half++) {
+        const f4 z = half ? y : x;
+        float m = 0.f;
+        bool fine = true;
+#pragma unroll
+        for (int j = 0; j < 4; j++) m = fmaxf(m, fabsf(z[j])), fine &= finite_f(z[j]);
+        m = fine ? m : __builtin_inff();  // one that is not finite gives its block a scale of NaN
+#pragma unroll
+        for (uint32_t s = 1; s < 8; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+        fine = finite_f(m);
+        const _Float16 dq = fine ? (_Float16)(m / 127.f) : (_Float16)__builtin_nanf("");
+        uint32_t codes = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) codes |= (uint32_t)(code_of(z[j], fine, (float)dq) & 255) << 8 * j;
+        const size_t e = o + half * (D / 2);
+        *reinterpret_cast<uint32_t*>(to + e) = codes;
+        if (l % 8 == 0) scale[e / 32] = dq;
+    }
+}
+
+// Any other width up to 256 and alignment: a wave per token and head, every 64th
+// value to a lane.
+__global__ __launch_bounds__(kBlock) void k_page_append_any(PageAppend a) {
     constexpr uint32_t E = kPageMaxDim / 64;
     __shared__ float turn[kWaves][kPageMaxDim];
     const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, d = a.c.dim;
@@ -30,25 +173,8 @@ __global__ __launch_bounds__(kBlock) void k_page_append(PageAppend a) {
     const uint64_t unit = (uint64_t)blockIdx.x * kWaves + wv;
     const uint32_t i = (uint32_t)min(unit / slots, (uint64_t)a.n - 1);
     const uint32_t h = (uint32_t)(unit % slots);
-    // the token's sequence: the last whose first token is not behind it
-    uint32_t b = i;
-    int32_t at = 0, count = 1;  // the token's number in its sequence, and of how many
-    bool live = unit / slots < a.n;
-    if (a.first) {
-        uint32_t before = 0;
-        for (uint32_t j = 0; j <= a.r.batch; j += 64) {
-            const bool le = j + lane <= a.r.batch && gld<int32_t>(a.first + min(j + lane, a.r.batch)) <= (int32_t)i;
-            before += __popcll(__ballot(le));
-        }
-        live = live && before > 0 && before <= a.r.batch;
-        b = live ? before - 1 : 0;
-        const int32_t f = gld<int32_t>(a.first + b);
-        at = (int32_t)i - f;
-        count = gld<int32_t>(a.first + b + 1) - f;
-    }
-    const int32_t len = live ? length_of(a.r, b) : -1;
-    const int32_t t = len - count + at;
-    live = live && t >= 0 && t < len;
+    const Place p = place_of(a, i);
+    const bool live = p.live && unit / slots < a.n;
     const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.c.kvheads;
     const uint32_t g = is_q ? h : is_k ? h - a.heads : h - a.heads - a.c.kvheads;
     const Heads& src = is_q ? a.q : is_k ? a.k : a.v;
@@ -71,9 +197,9 @@ __global__ __launch_bounds__(kBlock) void k_page_append(PageAppend a) {
         }
     }
     if (a.rope && (is_q || is_k)) {
-        const int32_t p = live ? (a.pos ? gld<int32_t>(a.pos + i) : t) : 0;
-        const bool in = p >= 0 && (uint32_t)p < a.rope_rows;
-        const float2* row = a.rope + (size_t)(in ? p : 0) * (d / 2);
+        const int32_t at = live ? (a.pos ? gld<int32_t>(a.pos + i) : p.t) : 0;
+        const bool in = at >= 0 && (uint32_t)at < a.rope_rows;
+        const float2* row = a.rope + (size_t)(in ? at : 0) * (d / 2);
 #pragma unroll
         for (uint32_t j = 0; j < E; j++) turn[wv][lane + 64 * j] = x[j];
         // the row is this wave's own
@@ -99,9 +225,9 @@ __global__ __launch_bounds__(kBlock) void k_page_append(PageAppend a) {
             if (lane + 64 * j < d) put_kind(a.qo.kind, a.qo.p, i * a.qo.row + g * a.qo.head + lane + 64 * j, x[j]);
         return;
     }
-    const int32_t page = gld<int32_t>(a.r.table + b * a.r.stride + (uint32_t)t / a.c.page);
-    if (page < 0 || (uint32_t)page >= a.c.count) return;
-    const size_t o = (size_t)page * a.c.ps + (size_t)((uint32_t)t % a.c.page) * a.c.ts + g * a.c.hs;
+    const int32_t page = page_of(a, p);
+    if (page < 0) return;
+    const size_t o = slot_of(a, p, page, g);
     uint8_t* to = is_k ? a.c.k : a.c.v;
     if (a.c.kind != Q8_0) {
 #pragma unroll
@@ -123,16 +249,32 @@ __global__ __launch_bounds__(kBlock) void k_page_append(PageAppend a) {
         const uint32_t e = lane + 64 * j;
         if (e >= d) continue;
         const _Float16 dq = fine ? (_Float16)(m / 127.f) : (_Float16)__builtin_nanf("");
-        const float f = (float)dq;
-        const float code = fine && f > 0.f ? fminf(fmaxf(rintf(x[j] / f), -127.f), 127.f) : 0.f;
-        reinterpret_cast<int8_t*>(to)[o + e] = (int8_t)code;
+        reinterpret_cast<int8_t*>(to)[o + e] = (int8_t)code_of(x[j], fine, (float)dq);
         if (lane % 32 == 0) scale[(o + e) / 32] = dq;
     }
 }
 
+// Whether a run of heads, or the cache, is aligned to four elements in every row.
+static bool by_four(const void* p, size_t row, size_t head, size_t es) {
+    return ((uintptr_t)p % (4 * es) | row % 4 | head % 4) == 0;
+}
+static bool by_four(const Heads& h) { return !h.p || by_four(h.p, h.row, h.head, h.kind == F32 ? 4 : 2); }
+
 void launch_page_append(const PageAppend& a, hipStream_t s) {
-    const uint64_t units = (uint64_t)a.n * (a.heads + 2 * a.c.kvheads);
-    hipLaunchKernelGGL(k_page_append, dim3((uint32_t)((units + kWaves - 1) / kWaves)), dim3(kBlock), 0, s, a);
+    const uint32_t slots = a.heads + 2 * a.c.kvheads, d = a.c.dim;
+    const size_t es = a.c.kind == F32 ? 4 : a.c.kind == Q8_0 ? 1 : 2;
+    const uintptr_t floats = (uintptr_t)a.qw | (uintptr_t)a.kw | (uintptr_t)a.rope;
+    if ((d == 64 || d == 128 || d == 256) && by_four(a.q) && by_four(a.qo) && by_four(a.k) && by_four(a.v) &&
+        by_four(a.c.k, a.c.ts, a.c.hs, es) && by_four(a.c.v, a.c.ps, 0, es) && floats % 16 == 0) {
+        const uint32_t per = 512 / d, groups = (slots + per - 1) / per;
+        const dim3 grid((uint32_t)(((uint64_t)a.n * groups + kWaves - 1) / kWaves)), block(kBlock);
+        if (d == 64) hipLaunchKernelGGL(k_page_append<8>, grid, block, 0, s, a, groups);
+        else if (d == 128) hipLaunchKernelGGL(k_page_append<16>, grid, block, 0, s, a, groups);
+        else hipLaunchKernelGGL(k_page_append<32>, grid, block, 0, s, a, groups);
+        return;
+    }
+    const uint64_t units = (uint64_t)a.n * slots;
+    hipLaunchKernelGGL(k_page_append_any, dim3((uint32_t)((units + kWaves - 1) / kWaves)), dim3(kBlock), 0, s, a);
 }
 
 // --------------------------------------------------------------- attention --

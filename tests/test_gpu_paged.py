@@ -264,16 +264,17 @@ def angles(n, d):
 @pytest.mark.parametrize("heads,kvheads,dim", [(32, 4, 128), (4, 4, 64), (3, 1, 256), (2, 2, 34), (0, 2, 128), (1, 1, 2),
                                                (6, 2, 96)])
 @pytest.mark.parametrize("norm", [True, False])
-def test_append(dev, x, kv, heads, kvheads, dim, norm):
+@pytest.mark.parametrize("skip", [1, 8])
+def test_append(dev, x, kv, heads, kvheads, dim, norm, skip):
     """Ragged prompts with norm and RoPE (every second pattern: neither), rows in front of and behind
-    the sequences left out."""
+    the sequences left out; rows aligned to one element and to eight."""
     g = torch.Generator().manual_seed(dim + heads)
     page, counts, lengths = 16, [5, 1, 0, 19, 3], [37, 1, 8, 19, 3 + 2 * 16]
     table, pool, _ = make_table(g, lengths, page)
     k, v, _, _ = make_cache(g, pool, page, kvheads, dim, kv)
     lead, n = 2, 2 + sum(counts) + 3
     first = torch.tensor([lead] + [lead + sum(counts[:i + 1]) for i in range(len(counts))], dtype=torch.int32)
-    rows = torch.randn(n, (heads + 2 * kvheads) * dim + 1, generator=g).to(TYPES[x]).cuda()[:, 1:]
+    rows = torch.randn(n, (heads + 2 * kvheads) * dim + skip, generator=g).to(TYPES[x]).cuda()[:, skip:]
     q_new = rows[:, :heads * dim].unflatten(1, (heads, dim)) if heads else None
     k_new, v_new = (m.unflatten(1, (kvheads, dim)) for m in rows[:, heads * dim:].chunk(2, 1))
     qw, kw = (1 + 0.3 * torch.randn(dim, generator=g) for _ in range(2))
