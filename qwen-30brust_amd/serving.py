@@ -30,23 +30,25 @@ def _need(ok, message):
 
 
 def _on(dev, t, what, dtypes, ndim):
-    """Checks a tensor's place, type and rank, and that its last dimension is contiguous."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == dev.index):
+    """Checks a tensor's place, type and rank, and that its last dimension is contiguous; its shape and strides."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == dev.index):  # -1 on the host
         raise EngineError(f"{what}: not a tensor on the engine's device")
     if t.dtype not in dtypes:
         raise EngineError(f"{what}: type {t.dtype} is not supported")
-    if t.dim() != ndim:
+    shape, strides = t.shape, t.stride()
+    if len(strides) != ndim:
         raise EngineError(f"{what}: {ndim} dimensions are needed, {t.dim()} given")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if strides[-1] != 1 and shape[-1] > 1:
         raise EngineError(f"{what}: the last dimension is not contiguous")
-    return t
+    return shape, strides
 
 
 _I32, _F32 = (torch.int32,), (torch.float32,)
 
 
 def _stream(dev):
-    return torch.cuda.current_stream(dev.index).cuda_stream or engine.NULL_STREAM
+    # the handle alone: a Stream object would take a microsecond more
+    return torch._C._cuda_getCurrentRawStream(dev.index) or engine.NULL_STREAM
 
 
 def _live(dev):
@@ -56,10 +58,10 @@ def _live(dev):
 
 
 def _heads(dev, t, what, rows, heads, dim):
-    _on(dev, t, what, KIND, 3)
-    if tuple(t.shape) != (rows, heads, dim):
-        raise EngineError(f"{what}: shape {tuple(t.shape)}, not {(rows, heads, dim)}")
-    return engine._Heads(t.data_ptr(), KIND[t.dtype], t.stride(0), t.stride(1))
+    shape, strides = _on(dev, t, what, KIND, 3)
+    if shape != (rows, heads, dim):
+        raise EngineError(f"{what}: shape {tuple(shape)}, not {(rows, heads, dim)}")
+    return engine._Heads(t.data_ptr(), KIND[t.dtype], strides[0], strides[1])
 
 
 class PagedCache:
@@ -92,16 +94,15 @@ class PagedCache:
 
     def _sequences(self, table, lengths, most):
         dev = self.device
-        _on(dev, table, "page table", _I32, 2)
-        _on(dev, lengths, "lengths", _I32, 1)
-        if table.shape[0] != lengths.shape[0]:
+        (rows, pages), strides = _on(dev, table, "page table", _I32, 2)
+        (batch,), _ = _on(dev, lengths, "lengths", _I32, 1)
+        if rows != batch:
             raise EngineError("the page table has other sequences than the lengths")
         if most is None:
-            most = min(table.shape[1] * self.page, 0x7fffffff - (1 << 20))
+            most = min(pages * self.page, 0x7fffffff - (1 << 20))
         if not 0 <= most <= 0x7fffffff:
             raise EngineError("longest length out of range")
-        return engine._Sequences(table.data_ptr(), lengths.data_ptr(), table.stride(0), table.shape[1],
-                                 lengths.shape[0], most)
+        return engine._Sequences(table.data_ptr(), lengths.data_ptr(), strides[0], pages, batch, most)
 
     def append(self, k, v, table, lengths, first=None, *, q=None, q_out=None, q_norm=None, k_norm=None, eps=1e-6,
                rope=None, positions=None):
@@ -121,18 +122,17 @@ class PagedCache:
             _need(first.shape[0] == lengths.shape[0] + 1, "first tokens: one more than sequences is needed")
         more = engine._Append(eps=eps)
         if q is not None:
-            _on(dev, q, "queries", KIND, 3)
-            more.heads = q.shape[1]
-            more.q = _heads(dev, q, "queries", n, q.shape[1], d)
+            more.heads = heads = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
+            more.q = _heads(dev, q, "queries", n, heads, d)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            more.q_out = _heads(dev, q_out, "query outputs", n, q.shape[1], d)
+                q_out = q.new_empty((n, heads, d))
+            more.q_out = _heads(dev, q_out, "query outputs", n, heads, d)
         else:
             _need(q_out is None and q_norm is None, "query outputs and weights go with queries")
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
             if w is not None:
-                _on(dev, w, name, _F32, 1)
-                _need(w.shape[0] == d, f"{name}: {d} weights are needed")
+                if _on(dev, w, name, _F32, 1)[0][0] != d:
+                    raise EngineError(f"{name}: {d} weights are needed")
                 setattr(more, name, w.data_ptr())
         if rope is not None:
             _on(dev, rope, "table of angles", _F32, 3)
@@ -159,11 +159,10 @@ class PagedCache:
         weights_out (weights itself if not given); returns (out, weights_out)."""
         dev, (batch, d) = self.device, (lengths.shape[0], self.dim)
         seqs = self._sequences(table, lengths, most)
-        _on(dev, q, "queries", KIND, 3)
-        heads = q.shape[1]
+        heads = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
         qh = _heads(dev, q, "queries", batch, heads, d)
         if out is None:
-            out = torch.empty((batch, heads, d), dtype=q.dtype, device=q.device)
+            out = q.new_empty((batch, heads, d))
         oh = _heads(dev, out, "attention outputs", batch, heads, d)
         w = None
         if weights_out is None:
