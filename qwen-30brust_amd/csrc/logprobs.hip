@@ -22,6 +22,12 @@
 // its loads' maxima lets through.  A key is put in its place by counting the keys
 // above it and moving the others up a lane: about a hundred cycles, and a part of
 // n batches of random logits has some top (1 + ln n) of them.
+//
+// 777 rows of 151,936 f32 logits (472 MB): 88 us for the sums alone, memory's rate
+// (5.4 TB/s); with 20 alternatives 134 us and 11 for the join, of which the keys'
+// placing is the difference; with 128 alternatives, two keys a lane, 428 and 37.
+// One such row: 9 and 8 us, latency.  A list in LDS filled with atomics took 157 us
+// for 20.
 #include <algorithm>
 #include <cfloat>
 
@@ -60,13 +66,13 @@ struct Sums {
     }
 };
 
-// The largest number that at least n of the wave's R numbers a lane reach (0
-// where there are fewer numbers).
-template <typename T, uint32_t R> __device__ __forceinline__ T nth_of(const T (&v)[R], uint32_t n) {
-    T found = 0;
+// The largest order key of the upper 20 bits (11 of a mantissa) that at least n of
+// the wave's R keys a lane reach (0 where there are fewer).
+template <uint32_t R> __device__ __forceinline__ uint32_t nth_of(const uint32_t (&v)[R], uint32_t n) {
+    uint32_t found = 0;
 #pragma unroll 4
-    for (int bit = 8 * sizeof(T) - 1; bit >= 0; bit--) {
-        const T t = found | (T)1 << bit;
+    for (int bit = 31; bit >= 12; bit--) {
+        const uint32_t t = found | 1u << bit;
         uint32_t reach = 0;
 #pragma unroll
         for (uint32_t k = 0; k < R; k++) reach += __popcll(__ballot(v[k] >= t));
@@ -158,25 +164,34 @@ template <uint32_t K> __device__ __forceinline__ Sums slow_sums(const Logprobs& 
     return s;
 }
 
+// The target's logit of row r, on its way while the sums are folded.
+struct Target {
+    bool in = false;
+    float x = 0.f;
+    template <uint32_t K> static __device__ __forceinline__ Target load(const Logprobs& a, uint32_t r) {
+        Target t;
+        if (!a.logp) return t;
+        const uint32_t id = (uint32_t)gld<int32_t>(a.target + r);
+        t.in = id < a.vocab;
+        if (t.in) {
+            t.x = elem<K>(static_cast<const uint8_t*>(a.x), r * a.stride + id);
+            if (a.valid && !gld<uint8_t>(a.valid + id)) t.x = -FLT_MAX;
+        }
+        return t;
+    }
+};
+
 // A row whose Sums and flags are known: writes its log probability and entropy,
 // and gives that of others.
 template <uint32_t K> struct Row {
     Sums s;
     bool bad, far;
-    __device__ __forceinline__ Row(const Logprobs& a, uint32_t r, Sums sums, uint32_t flags) : s(sums) {
+    __device__ __forceinline__ Row(const Logprobs& a, uint32_t r, const Target& t, Sums sums, uint32_t flags) : s(sums) {
         bad = flags & kLpBad;
         far = !bad && ((flags & kLpHigh) || (flags & kLpLow && s.m == -INFINITY));
         if (far) s = slow_sums<K>(a, r);
         if (threadIdx.x) return;
-        if (a.logp) {
-            const uint32_t t = (uint32_t)gld<int32_t>(a.target + r);
-            float p = __builtin_nanf("");
-            if (t < a.vocab) {
-                const bool masked = a.valid && !gld<uint8_t>(a.valid + t);
-                p = logp(masked ? -FLT_MAX : elem<K>(static_cast<const uint8_t*>(a.x), r * a.stride + t));
-            }
-            a.logp[r] = p;
-        }
+        if (a.logp) a.logp[r] = t.in ? logp(t.x) : __builtin_nanf("");
         if (a.entropy) a.entropy[r] = bad ? __builtin_nanf("") : s.S > 0.f ? (log2f(s.S) - s.U / s.S) * kLn2 : 0.f;
     }
     __device__ __forceinline__ float logp(float x) const { return logp_of(x, s, far, bad); }
@@ -375,7 +390,7 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
         s = fold(s);
         const size_t slot = (size_t)blockIdx.x * 2 + (b0 == 0);
         if (b1 - b0 == w.all) {
-            const Row<K> done(a, r, s, flags);
+            const Row<K> done(a, r, Target::load<K>(a, r), s, flags);
             each(best, top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
         } else {
             if (lane == 0) sums_of(a)[slot] = make_float4(s.m, s.S, s.U, __uint_as_float(flags));
@@ -388,35 +403,46 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
 // A row that several waves hold parts of.  Their keys lie in descending order.
 // With n = ceil(top / parts), ceil(top / n) parts' n-th keys that reach a bound
 // stand for top keys that do, so that only keys that reach the largest such bound
-// are looked at.
+// are looked at, and none of a rank behind one where no part has any.  Bound by
+// the look-ups' latency: what does not depend on another is loaded first (11 us
+// for a row of 149 parts and 20 alternatives without, 8 with).
 template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64) void k_logprobs_join(Logprobs a, Runs w) {
-    constexpr uint32_t kAhead = 16;  // keys of a lane in flight
+    constexpr uint32_t kAhead = 8;  // keys of a lane in flight
     const uint32_t r = blockIdx.x, lane = threadIdx.x, top = a.top;
     const uint64_t x = (uint64_t)r * w.all, first = w.with(x);
     const uint32_t parts = (uint32_t)(w.with(x + w.all - 1) - first) + 1;
     if (parts == 1) return;  // done in its wave
     auto slot = [&](uint32_t i) { return (first + i) * 2 + (i == 0); };
+    const uint64_t* keys = keys_of(a, w.runs);
+    const uint32_t n = (top + parts - 1) / parts, all = parts * top;
+    // what the first 256 parts left and the target, all under way at once
+    uint32_t nth[4] = {};
+    float4 sums[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+        const uint32_t i = min(lane + 64 * k, parts - 1);
+        sums[k] = gld<float4>(sums_of(a) + slot(i));
+        if (top) nth[k] = (uint32_t)(gld<uint64_t>(keys + slot(i) * top + n - 1) >> 32);
+    }
+    const Target target = Target::load<K>(a, r);
     Sums s;
     uint32_t flags = 0;
-    for (uint32_t i = lane; i < parts; i += 64) {
-        const float4 v = gld<float4>(sums_of(a) + slot(i));
+    auto add = [&](float4 v) {
         Sums o;
         o.m = v.x, o.S = v.y, o.U = v.z;
         s.add(o);
         flags |= __float_as_uint(v.w);
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+        if (lane + 64 * k < parts) add(sums[k]);
+        else nth[k] = 0;
     }
+    for (uint32_t i = lane + 256; i < parts; i += 64) add(gld<float4>(sums_of(a) + slot(i)));
     Best<R> best;
     if (top) {
-        const uint64_t* keys = keys_of(a, w.runs);
-        const uint32_t n = (top + parts - 1) / parts, all = parts * top;
         uint64_t bound = 1;  // 0: a part of fewer keys
-        if (parts <= 256) {
-            uint32_t nth[4];
-#pragma unroll
-            for (uint32_t k = 0; k < 4; k++)
-                nth[k] = lane + 64 * k < parts ? (uint32_t)(gld<uint64_t>(keys + slot(lane + 64 * k) * top + n - 1) >> 32) : 0;
-            bound = max((uint64_t)nth_of(nth, (top + n - 1) / n) << 32, (uint64_t)1);
-        }
+        if (parts <= 256) bound = max((uint64_t)nth_of(nth, (top + n - 1) / n) << 32, (uint64_t)1);
         for (uint32_t i0 = 0; i0 < all; i0 += 64 * kAhead) {
             uint64_t k[kAhead];
 #pragma unroll
@@ -425,17 +451,20 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64) void k_logpro
                 k[j] = gld<uint64_t>(keys + slot(part) * top + rank);  // the parts' first keys first
                 if (i >= all) k[j] = 0;
             }
+            bool some = parts > 64 * kAhead;
 #pragma unroll
             for (uint32_t j = 0; j < kAhead; j++) {
+                some |= __any(k[j] >= bound);
                 for (uint64_t who = __ballot(k[j] >= bound); who; who &= who - 1) {
                     const uint64_t c = Best<R>::of_lane(k[j], __ffsll((unsigned long long)who) - 1);
                     if (c >= bound) best.put(c);
                 }
                 bound = max(bound, best.at(top - 1));
             }
+            if (!some) break;  // of every part a key, and none reached the bound
         }
     }
-    const Row<K> done(a, r, fold(s), any_of(flags));
+    const Row<K> done(a, r, target, fold(s), any_of(flags));
     each(best, top, [&](uint32_t rank, uint64_t k) { done.put(a, r, rank, k); });
 }
 
