@@ -436,7 +436,9 @@ typedef struct {
  * Sums in 32 bits, out rounded once to its kind.  A sequence without keys, or
  * whose scores are all -inf, gives zeros; one with a length or a page id out of
  * range NaN.  weights nullable; the weights of a sequence whose length is out of
- * range are left as they were. */
+ * range are left as they were.  A Q8_0 cache's values (code times scale) past
+ * f16's range, 65504, come out not finite with F16 or BF16 queries; with F32 ones
+ * they are read in 32 bits.  q and out may be the same. */
 int qh_paged_attention(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const qh_heads_t *q,
                        uint32_t heads, float scale, const qh_heads_t *out, const qh_key_weights_t *weights,
                        void *workspace, size_t workspace_bytes, void *stream);

@@ -47,8 +47,9 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 
 // (m, S, U) of some logits, m in units of log 2 and U with it: t = x log2(e) - m
 // is one fused multiply-add, of which a large x loses nothing, S = sum 2^t, U =
-// sum t 2^t, log p = (t - log2 S) ln 2.  A row's maximum past 2e38 either way has
-// no such m: far, and m is the maximum itself (slow_sums).
+// sum t 2^t, log p = (t - log2 S) ln 2.  m is rounded and the product in t is
+// not, so that t reaches half a step of m, 1 for an x of 2^24: a row whose maximum
+// lies past that either way is far, and m is the maximum itself (slow_sums).
 struct Sums {
     float m = -INFINITY, S = 0.f, U = 0.f;
     __device__ __forceinline__ void move(float M) {  // to a maximum M >= m
@@ -124,9 +125,10 @@ __device__ __forceinline__ Sums fold(Sums s) {
     return s;
 }
 
-// What a row's logits hold, besides.
-enum : uint32_t { kLpBad = 1, kLpHigh = 2, kLpLow = 4 };  // NaN or +inf; finite maxima past 2e38
-constexpr float kLpFar = 2e38f;
+// What a row's logits hold, besides: NaN or +inf; finite maxima past 2^24.  Of a
+// lane's logits below -2^24 the sums hold nothing, and m is -inf.
+enum : uint32_t { kLpBad = 1, kLpHigh = 2, kLpLow = 4 };
+constexpr float kLpFar = 16777216.f;
 __device__ __forceinline__ uint32_t any_of(uint32_t flags) {
     uint32_t r = 0;
 #pragma unroll
@@ -189,7 +191,10 @@ template <uint32_t K> struct Row {
     __device__ __forceinline__ Row(const Logprobs& a, uint32_t r, const Target& t, Sums sums, uint32_t flags) : s(sums) {
         bad = flags & kLpBad;
         far = !bad && ((flags & kLpHigh) || (flags & kLpLow && s.m == -INFINITY));
-        if (far) s = slow_sums<K>(a, r);
+        if (far) {
+            s = slow_sums<K>(a, r);
+            bad = s.S != s.S;
+        }
         if (threadIdx.x) return;
         if (a.logp) a.logp[r] = t.in ? logp(t.x) : __builtin_nanf("");
         if (a.entropy) a.entropy[r] = bad ? __builtin_nanf("") : s.S > 0.f ? (log2f(s.S) - s.U / s.S) * kLn2 : 0.f;
@@ -338,7 +343,7 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
                 for (uint32_t j = 1; j < E; j++) M[k] = fmaxf(M[k], x[k][j]);  // NaN only if all are
                 most = fmaxf(most, M[k]);
             }
-            if (most * kLog2e > s.m) s.move(most * kLog2e);
+            if (most >= -kLpFar && most * kLog2e > s.m) s.move(most * kLog2e);
             const float m = s.m == -INFINITY ? 0.f : s.m;
             float S = 0.f, U = 0.f;
 #pragma unroll
@@ -352,7 +357,7 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
             s.S += S;
             s.U += U;
             if (fabsf(most) > kLpFar && most != -INFINITY) flags |= most == INFINITY ? kLpBad : most > 0.f ? kLpHigh : kLpLow;
-            if (S != S && most <= kLpFar) flags |= kLpBad;
+            if (S != S) flags |= kLpBad;  // of finite logits, however large, no term is NaN
             if (!top) continue;
             if (!__any(!(most < bound) || flags & kLpBad)) continue;
             uint32_t loads = 0;  // that hold such logits

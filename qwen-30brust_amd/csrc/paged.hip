@@ -527,7 +527,7 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 // Q8_0: codes are exact in f16 (byte | 0x6400 is 1024 + byte), a block's scale
 // multiplies its 32-dim product in 32 bits, and code * scale of V goes in as two
 // f16 parts (the product and its rounding error, by a fused multiply-add);
-// values past f16's range become infinite.  Queries then are f16, scaled by a
+// values past f16's range come out not finite.  Queries then are f16, scaled by a
 // power of two of their own.
 // The keys' rows come through LDS: every window of kWindow keys is looked up in
 // the page table once (any page size), as 32-bit offsets of 16 bytes.

@@ -132,6 +132,33 @@ def test_patterns(dev, kind, vocab):
             check(got, want, x, vocab)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [7, 1000, 151936])
+def test_ends_of_the_range(dev, kind, vocab):
+    """Rows whose maximum lies near either end of the type, with ties there, one batch of such logits
+    among ordinary ones, ordinary ones with the lowest value among them; a log probability past the
+    type's range is -inf."""
+    g = torch.Generator().manual_seed(vocab)
+    t, big = torch.arange(vocab), torch.finfo(TYPES[kind]).max
+    noise = torch.randn(vocab, generator=g)
+    rows = [torch.where(t % 5 == 0, big, 0.9 * big), torch.where(t == vocab - 1, big, -big), torch.where(t % 3 == 0, -0.7 * big, -big),
+            torch.full((vocab,), -big), torch.where(t == vocab // 2, 0.99 * big, noise), torch.where(t < 3, -big, noise),
+            torch.where(t < 1100, -big, noise), torch.where(t >= 5, -math.inf, -0.8 * big),
+            torch.where(t == 4, 1.9e38, torch.where(t == 6, -1.9e38, 0.0)), torch.where(t == vocab - 1, 2.1e38, -2.1e38),
+            # between: past 2^24 half a step of the maximum is more than 1
+            torch.where(t % 7 == 0, 1.01e9, noise), 1e4 * noise + 3e7, 1e4 * noise - 3e7, 1e3 * noise + 2 ** 24, 1e3 * noise - 2 ** 24,
+            1e6 * noise, 1e12 * noise, torch.where(t % 64 < 9, -1e10, noise), torch.where(t < 2000, -1e10, noise),
+            torch.where(t == 3, math.nan, 1e12 * noise), torch.where(t == 2, math.nan, -1e12)]
+    x = torch.stack([r.float() for r in rows]).to(TYPES[kind])
+    targets = torch.randint(0, vocab, (len(rows),), generator=g).int()
+    for v in (None, (torch.rand(vocab, generator=g) < 0.9).to(torch.uint8)):
+        for top in (0, min(vocab, 5), min(vocab, 100)):
+            want = exact(x.float(), targets, top, v)
+            want = [None if w is None else w if w.dtype == torch.int32 else w.float().double() for w in want]
+            got = serving.logprobs(dev, x.cuda(), targets.cuda(), top=top, valid=None if v is None else v.cuda())
+            check(got, want, x, vocab)
+
+
 def test_views(dev):
     """Rows with a stride, at an odd element; without targets."""
     g = torch.Generator().manual_seed(1)
