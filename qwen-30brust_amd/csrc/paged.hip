@@ -79,7 +79,9 @@ __device__ __forceinline__ void put_four(uint32_t kind, uint8_t* p, size_t i, f4
     else if (kind == F16) *reinterpret_cast<h4*>(p + 2 * i) = __builtin_convertvector(x, h4);
     else *reinterpret_cast<b4*>(p + 2 * i) = __builtin_convertvector(x, b4);
 }
-// Q8_0 codes of a value: fine, whether its block is finite, f the block's scale.
+// The Q8_0 code of a value: fine, whether its block is finite, f the block's scale.
+// Of 11 bits of f the middle between two codes is an f32 value, and the quotient
+// of any other, rounded to the nearest, stays on its side of the middle.
 __device__ __forceinline__ int32_t code_of(float x, bool fine, float f) {
     return fine && f > 0.f ? (int32_t)fminf(fmaxf(rintf(x / f), -127.f), 127.f) : 0;
 }

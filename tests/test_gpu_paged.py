@@ -351,6 +351,37 @@ def test_append_8bit(dev, x, kvheads, dim):
                                w.nan_to_num(77.0) if w.dtype == torch.float16 else w)
 
 
+def test_append_8bit_next_to_ties(dev):
+    """Values on, and one and two steps of f32 beside, the middle between two codes: the code of the
+    exact quotient."""
+    top = 0.987  # a scale of 1.99 * 2^-8: a step of a value is down to half a step of its quotient
+    f = (torch.tensor(top) / 127).half().float()
+    mid = (torch.arange(126) + 0.5).repeat_interleave(5).reshape(126, 5) * f  # exact: 7 + 11 bits
+    near = [mid[:, 0]]
+    for way in (-math.inf, math.inf):
+        x = mid[:, 0]
+        for _ in range(2):
+            x = torch.nextafter(x, torch.tensor(way))
+            near.append(x)
+    x = torch.stack(near, 1).reshape(-1)
+    x = torch.cat([x, -x])
+    x = torch.cat([x, torch.zeros(-len(x) % 31)]).reshape(-1, 31)
+    x = torch.cat([x, torch.full((len(x), 1), top)], 1)  # every block has the same scale
+    want = (x.double() / f.double()).round().clamp(-127, 127).to(torch.int8)
+    n, g = -(-len(x) // 8), torch.Generator().manual_seed(1)
+    rows = torch.zeros(n * 8, 32)
+    rows[:len(x)] = x
+    for kvheads, dim in ((2, 128), (1, 256), (8, 32)):
+        c = make_cache(g, 4, 64, kvheads, dim, "q8_0")
+        k_new = rows.reshape(n, kvheads, dim)
+        serving.PagedCache(dev, *c).append(k_new.cuda(), k_new.cuda(), torch.tensor([[2, 0, 3]], dtype=torch.int32).cuda(),
+                                           torch.tensor([n], dtype=torch.int32).cuda(),
+                                           torch.tensor([0, n], dtype=torch.int32).cuda())
+        for held in c[:2]:
+            got = held[[2, 0, 3]].reshape(-1, kvheads * dim)[:n].reshape(-1, 32)[:len(x)]
+            assert torch.equal(got.cpu(), want)
+
+
 def test_append_one_token_each(dev):
     """Without `first`: a token for each sequence at its end; padded rows, lengths and pages out of
     range and a position outside the table."""
