@@ -297,20 +297,23 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
         uint32_t flags = 0;
         float bound = -INFINITY;  // logits below it do not get in
         constexpr uint32_t E = Load<K>::E, kSteps = Load<K>::kSteps, kStep = Load<K>::kStep;
-        for (uint32_t b = lo; b < hi; b += kLpBatch) {
-            // Lane's loads k: logits i .. i + E - 1, i = b + kStep k + lane E; the last
-            // ones of a row end with it, and hold some again that other loads hold
-            const bool whole = b + kLpBatch <= hi;
-            auto at_of = [&](uint32_t k) { return b + kStep * k + lane * E; };
-            auto from_of = [&](uint32_t k) { return whole ? at_of(k) : min(at_of(k), hi - min(hi, E)); };
-            Load<K> raw[kSteps];
+        // Lane's loads k of a batch: logits i .. i + E - 1, i = b + kStep k + lane E; the
+        // last ones of a row end with it, and hold some again that other loads hold
+        Load<K> raw[kSteps];
+        auto request = [&](uint32_t b) {
+            const uint32_t last = b + kLpBatch <= hi ? ~0u : hi - min(hi, E);
 #pragma unroll
             for (uint32_t k = 0; k < kSteps; k++) {
-                const uint32_t i = from_of(k);
+                const uint32_t i = min(b + kStep * k + lane * E, last);
                 if (hi >= E) raw[k].load(row + (size_t)i * (K == F32 ? 4 : 2), a.valid ? a.valid + i : nullptr);
                 else raw[k].few(row, a.valid, hi);
             }
-            __builtin_amdgcn_sched_barrier(0);  // every load is requested before one is waited for
+        };
+        request(lo);
+        for (uint32_t b = lo; b < hi; b += kLpBatch) {
+            const bool whole = b + kLpBatch <= hi;
+            auto at_of = [&](uint32_t k) { return b + kStep * k + lane * E; };
+            auto from_of = [&](uint32_t k) { return whole ? at_of(k) : min(at_of(k), hi - min(hi, E)); };
             float x[kSteps][E], M[kSteps], most = -INFINITY;
 #pragma unroll
             for (uint32_t k = 0; k < kSteps; k++)
@@ -327,6 +330,10 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
                         for (uint32_t j = 0; j < E; j++) x[k][j] = raw[k].on(j) ? x[k][j] : -FLT_MAX;
                 }
             }
+            // the next batch is on its way while this one is worked on
+            __builtin_amdgcn_sched_barrier(0);
+            if (b + kLpBatch < hi) request(b + kLpBatch);
+            __builtin_amdgcn_sched_barrier(0);
             if (!whole) {
 #pragma unroll
                 for (uint32_t k = 0; k < kSteps; k++)
