@@ -23,11 +23,12 @@
 // above it and moving the others up a lane: about a hundred cycles, and a part of
 // n batches of random logits has some top (1 + ln n) of them.
 //
-// 777 rows of 151,936 f32 logits (472 MB): 88 us for the sums alone, memory's rate
-// (5.4 TB/s); with 20 alternatives 134 us and 11 for the join, of which the keys'
-// placing is the difference; with 128 alternatives, two keys a lane, 428 and 37.
-// One such row: 9 and 8 us, latency.  A list in LDS filled with atomics took 157 us
-// for 20.
+// 777 rows of 151,936 f32 logits (472 MB): 81 us for the sums alone, memory's rate
+// (5.9 TB/s; 88 without the next batch under way); with 20 alternatives 129 us and
+// 11 for the join: placing some 90 keys a wave, 80 operations each, of which half
+// hides behind the loads (a list in LDS filled with atomics took 157 us).  With 128
+// alternatives, two keys a lane, about 420 and 37.  One such row: 9 and 8 us,
+// latency.
 #include <algorithm>
 #include <cfloat>
 
