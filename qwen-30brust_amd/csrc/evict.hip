@@ -4,6 +4,8 @@
 // the lower index on ties); they move, in their order, to new pages.  Other
 // sequences move whole.  Attention does not depend on the keys' order or
 // places, so each KV head keeps keys of its own in the same pages.
+#include <type_traits>
+
 #include "qh_block.hpp"
 #include "serving_device.hpp"
 
@@ -75,20 +77,29 @@ __global__ __launch_bounds__(kSelBlock) void k_page_select(PageEvict a) {
     const uint32_t lo = longer ? a.first : 0, hi = longer ? n - a.recent : 0;  // the keys to choose from
     uint32_t need = longer ? a.keep - a.first - a.recent : 0, cut = 0, known = 0;  // known: bits of cut
     const bool choose = need != 0;
+    // f(whether all of round r's keys lie in [lo, hi)): most rounds', whose keys need no look at their place
+    auto by_place = [&](uint32_t t0, uint32_t r, auto f) {
+        const uint32_t from = t0 + r * kSelRound;
+        if (from >= lo && from + kSelRound <= hi) f(std::true_type());
+        else if (from < n) f(std::false_type());
+    };
     for (uint32_t pass = 0; choose && pass < 3; pass++) {
-        const uint32_t bits = pass < 2 ? 11 : 10, shift = 32 - known - bits;
+        const uint32_t bits = pass < 2 ? 11 : 10, shift = 32 - known - bits, mask = (1u << bits) - 1;
+        const uint32_t above = known ? ~0u << (32 - known) : 0;
         for (uint32_t i = tid; i < kBins * kCopies / 4; i += kSelBlock) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         for (uint32_t t0 = 0; t0 < n; t0 += kSelSpan) {
             if (n > kSelSpan && (pass || t0)) load(t0);
 #pragma unroll
             for (uint32_t r = 0; r < kSelRounds; r++)
+                by_place(t0, r, [&](auto inside) {
 #pragma unroll
-                for (uint32_t k = 0; k < kSelPer; k++) {
-                    const uint32_t t = t0 + r * kSelRound + tid * kSelPer + k, key = order_key(x[r][k]);
-                    if (t >= lo && t < hi && (known == 0 || (key ^ cut) >> (32 - known) == 0))
-                        atomicAdd(&hist[(key >> shift & ((1u << bits) - 1)) * kCopies + lane % kCopies], 1u);
-                }
+                    for (uint32_t k = 0; k < kSelPer; k++) {
+                        const uint32_t t = t0 + r * kSelRound + tid * kSelPer + k, key = order_key(x[r][k]);
+                        if ((key & above) == cut && (inside || (t >= lo && t < hi)))
+                            atomicAdd(&hist[(key >> shift & mask) * kCopies + lane % kCopies], 1u);
+                    }
+                });
         }
         __syncthreads();
         // the digit that holds the need-th largest: two digits a thread, the largest first
@@ -116,25 +127,28 @@ __global__ __launch_bounds__(kSelBlock) void k_page_select(PageEvict a) {
         __syncthreads();
     }
     // need: how many of the keys equal to cut stay
+    const uint32_t above = choose ? cut : ~0u;  // no key is larger than the latter
     uint32_t sure0 = 0, equal0 = 0;  // of the spans before
     for (uint32_t t0 = 0; t0 < n; t0 += kSelSpan) {
         if (n > kSelSpan) load(t0);
-        auto sort_of = [&](uint32_t r, uint32_t k, bool& is_sure, bool& is_equal) {
+        auto sort_of = [&](auto inside, uint32_t r, uint32_t k, bool& is_sure, bool& is_equal) {
             const uint32_t t = t0 + r * kSelRound + tid * kSelPer + k, key = order_key(x[r][k]);
-            const bool mid = t >= lo && t < hi;
-            is_sure = t < n && (!mid || (choose && key > cut));
+            const bool mid = inside || (t >= lo && t < hi);
+            is_sure = inside ? key > above : t < n && (!mid || key > above);
             is_equal = mid && choose && key == cut;
         };
         uint32_t upto[kSelRounds];  // of the wave: equal ones in the low half, sure ones in the high half
 #pragma unroll
         for (uint32_t r = 0; r < kSelRounds; r++) {
             uint32_t mine = 0;
+            by_place(t0, r, [&](auto inside) {
 #pragma unroll
-            for (uint32_t k = 0; k < kSelPer; k++) {
-                bool is_sure, is_equal;
-                sort_of(r, k, is_sure, is_equal);
-                mine += (is_sure ? 1u << 16 : 0u) + is_equal;
-            }
+                for (uint32_t k = 0; k < kSelPer; k++) {
+                    bool is_sure, is_equal;
+                    sort_of(inside, r, k, is_sure, is_equal);
+                    mine += (is_sure ? 1u << 16 : 0u) + is_equal;
+                }
+            });
             upto[r] = scan_wave(mine);
             if (lane == 63) part[r * kSelWaves + wv] = upto[r];
             upto[r] -= mine;
@@ -147,18 +161,20 @@ __global__ __launch_bounds__(kSelBlock) void k_page_select(PageEvict a) {
         for (uint32_t r = 0; r < kSelRounds; r++) {
             const uint32_t base = __shfl(sum - mine, r * kSelWaves + wv, 64) + upto[r];
             uint32_t ps = sure0 + (base >> 16), pe = equal0 + (base & 0xffff);
+            by_place(t0, r, [&](auto inside) {
 #pragma unroll
-            for (uint32_t k = 0; k < kSelPer; k++) {
-                bool is_sure, is_equal;
-                sort_of(r, k, is_sure, is_equal);
-                if (is_sure || (is_equal && pe < need)) {
-                    const uint32_t j = ps + min(pe, need);
-                    a.kept[row + j] = (int32_t)(t0 + r * kSelRound + tid * kSelPer + k);
-                    a.wout[row + j] = x[r][k];
+                for (uint32_t k = 0; k < kSelPer; k++) {
+                    bool is_sure, is_equal;
+                    sort_of(inside, r, k, is_sure, is_equal);
+                    if (is_sure || (is_equal && pe < need)) {
+                        const uint32_t j = ps + min(pe, need);
+                        a.kept[row + j] = (int32_t)(t0 + r * kSelRound + tid * kSelPer + k);
+                        a.wout[row + j] = x[r][k];
+                    }
+                    ps += is_sure;
+                    pe += is_equal;
                 }
-                ps += is_sure;
-                pe += is_equal;
-            }
+            });
         }
         sure0 += all >> 16;
         equal0 += all & 0xffff;
