@@ -20,11 +20,11 @@ constexpr uint32_t kSelBlock = 1024, kSelWaves = kSelBlock / 64;
 // bits (11, 11 and 10), then the keys above it and the first of those equal to it,
 // by a running count in index order: no atomics but the counts' own, so the same
 // keys on every call.  A sequence with a length or page out of range keeps nothing.
-// Bound by one compute unit's issue rate, 20 to 30 operations a key, and by the
-// steps between the passes: 62 us for 8,192 of 65,537 keys (4 heads), 17 us for
-// 1,024 of up to 4,096 (16 sequences).  With one copy of the counts and 8 rounds,
-// whose weights do not fit the registers, 91 and 30; with the next span's weights
-// read ahead 65 and 17.6.
+// Bound by one compute unit's issue rate, some 20 operations a key, and by the
+// steps between the passes: 50 us for 8,192 of 65,537 keys (4 heads), 15 us for
+// 1,024 of up to 4,096 (16 sequences).  Reading the next span ahead changes nothing;
+// with every key's place looked at 62 and 17, with one copy of the counts and 8
+// rounds, whose weights do not fit the registers, 91 and 30.
 constexpr uint32_t kSelPer = 4, kSelRound = kSelBlock * kSelPer, kSelRounds = 4, kSelSpan = kSelRound * kSelRounds;
 constexpr uint32_t kBins = 2048, kCopies = 8;  // copies of a count, for lanes that hit the same one
 
