@@ -573,7 +573,7 @@ template <uint32_t C> __device__ __forceinline__ float2 unpack2(uint32_t w) {
     const h2 h = __builtin_bit_cast(h2, w);
     return {(float)h.x, (float)h.y};
 }
-// Two f16 codes from the words whose bytes 0 and 2 are code + 128.
+// Two f16 codes from a word of 0x6400 | code + 128 each.
 __device__ __forceinline__ h2 codes2(uint32_t w) {
     return __builtin_bit_cast(h2, w) - h2{(_Float16)1152, (_Float16)1152};
 }
@@ -864,16 +864,12 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
                     __builtin_memcpy(d, __builtin_assume_aligned(vl + 4 * g, 8), 8);
                     __builtin_memcpy(d + 2, __builtin_assume_aligned(vl + 16 + 4 * g, 8), 8);
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-#pragma unroll
-                        for (int i = 0; i < VW; i++) vr[j][i] ^= 0x80808080u;
-#pragma unroll
                     for (int t = 0; t < NT; t++) {
                         u4 hi, lo;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const uint32_t sel = 0x0c000c00u | (uint32_t)(t % 4) | (uint32_t)(4 + t % 4) << 16;
-                            const h2 c = codes2(__builtin_amdgcn_perm(vr[2 * i + 1][t / 4], vr[2 * i][t / 4], sel) | 0x64006400u);
+                            const h2 c = codes2(__builtin_amdgcn_perm(vr[2 * i + 1][t / 4], vr[2 * i][t / 4], sel) ^ 0x64806480u);
                             const h2 v = c * d[i];
                             hi[i] = bits_of(v);
                             lo[i] = bits_of(__builtin_elementwise_fma(c, d[i], -v));
