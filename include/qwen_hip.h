@@ -452,7 +452,8 @@ int qh_paged_attention_bytes(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequ
  * between by weights ([batch][kvheads][most], strides weight_row and
  * weight_head; total order as f32::total_cmp, the lower index on ties).  Kept
  * keys move in ascending order to the slots 0.. of the pages to[b * to_stride +
- * i] (to_pages of them a row), which no sequence of the call may read.  Outputs:
+ * i] (to_pages of them a row; those that kept keys need are all different), which
+ * no sequence of the call may read.  Outputs:
  * kept[batch][kvheads][keep] their indexes (-1 behind them), kept_weights
  * [batch][kvheads][keep] their weights (0 behind them), new_length[batch].  A
  * sequence with a length or a page id out of range keeps nothing (length 0). */

@@ -523,7 +523,8 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 // to 7, the lo parts in columns 8 to 15, so that the second part costs no
 // instruction; their sums are added at the end.  (Where a value is not finite
 // the hi column alone says so.)  That leaves 2^-18 (bf16) or 2^-23 (f16) of a
-// weight's bits off; one part would leave 2^-9.
+// weight's bits off; one part would leave 2^-9.  f16 has no weights below 2^-32 of
+// the largest: n keys lose at most n 2^-32 of the largest value.
 // The running maximum moves only when a score is 15 above it (2^15 fits f16),
 // to 7 below the new one: nearly never, so the sums are rarely rescaled.
 // Q8_0: codes are exact in f16 (byte | 0x6400 is 1024 + byte), a block's scale

@@ -188,7 +188,7 @@ class PagedCache:
         """Brings sequences to at most `keep` keys: each KV head keeps its first
         `first` keys, its last `recent` and the heaviest between by `weights`
         ([batch][kvheads][most or more]), moved in order to the pages `to`
-        [batch][pages], which no sequence of the call reads.  Returns (kept
+        [batch][pages], all different, which no sequence of the call reads.  Returns (kept
         indexes [batch][kvheads][keep] with -1 behind them, their weights, new
         lengths)."""
         dev = self.device
