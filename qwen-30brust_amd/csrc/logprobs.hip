@@ -24,10 +24,10 @@
 // n batches of random logits has some top (1 + ln n) of them.
 //
 // 777 rows of 151,936 f32 logits (472 MB): 81 us for the sums alone, memory's rate
-// (5.9 TB/s; 88 without the next batch under way); with 20 alternatives 129 us and
-// 11 for the join: placing some 90 keys a wave, 80 operations each, of which half
-// hides behind the loads (a list in LDS filled with atomics took 157 us).  With 128
-// alternatives, two keys a lane, about 420 and 37.  One such row: 9 and 8 us,
+// (5.9 TB/s; 88 without the next batch under way); with 20 alternatives 122 us and
+// 11 for the join: finding and placing some 90 keys a wave, half of it hidden behind
+// the loads (a list in LDS filled with atomics took 157 us).  With 128
+// alternatives, two keys a lane, 399 and 37.  One such row: 9 and 8 us,
 // latency.
 #include <algorithm>
 #include <cfloat>
@@ -39,7 +39,7 @@ namespace qh {
 
 constexpr uint32_t kLpLane = 16;                     // logits of a lane and batch
 constexpr uint32_t kLpBatch = 64 * kLpLane;
-constexpr uint32_t kLpMany = 32;                     // loads of a batch that hold logits above the bound
+constexpr uint32_t kLpMany = 32;                     // lanes that hold logits of a batch above the bound
 constexpr uint32_t kLpRuns = 4096;                   // waves that fill the chip
 
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)order_key(x) << 32 | (uint32_t)~i; }
@@ -367,12 +367,10 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
             if (fabsf(most) > kLpFar && most != -INFINITY) flags |= most == INFINITY ? kLpBad : most > 0.f ? kLpHigh : kLpLow;
             if (S != S) flags |= kLpBad;  // of finite logits, however large, no term is NaN
             if (!top) continue;
-            if (!__any(!(most < bound) || flags & kLpBad)) continue;
-            uint32_t loads = 0;  // that hold such logits
-#pragma unroll
-            for (uint32_t k = 0; k < kSteps; k++) loads += __popcll(__ballot(!(M[k] < bound)));
+            const uint64_t some = __ballot(!(most < bound)), bad = __ballot(flags & kLpBad);
+            if (!(some | bad)) continue;
             float low = bound;
-            if (loads > kLpMany) {
+            if (__popcll(some) > kLpMany) {
                 uint32_t mine[kSteps];
 #pragma unroll
                 for (uint32_t k = 0; k < kSteps; k++) mine[k] = at_of(k) < hi ? order_key(M[k]) : 0;
@@ -381,11 +379,12 @@ template <uint32_t K, uint32_t R> __global__ __launch_bounds__(64, 4) void k_log
             }
 #pragma unroll
             for (uint32_t k = 0; k < kSteps; k++) {
-                if (!__any(!(M[k] < low) || flags & kLpBad)) continue;
+                if (!(__ballot(!(M[k] < low)) | bad)) continue;
                 const uint32_t at = at_of(k), i = from_of(k);
 #pragma unroll
                 for (uint32_t j = 0; j < E; j++) {
-                    uint64_t who = __ballot(!(x[k][j] < low) && (whole || (i + j >= at && i + j < hi)));
+                    uint64_t who = __ballot(!(x[k][j] < low));
+                    if (!whole) who &= __ballot(i + j >= at && i + j < hi);
                     for (; who; who &= who - 1) {
                         const uint32_t l = __ffsll((unsigned long long)who) - 1;
                         const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[k][j]), l));
