@@ -287,9 +287,9 @@ void launch_page_append(const PageAppend& a, hipStream_t s) {
 //
 // Work is counted in steps of 32 keys of a unit (a sequence, one of its KV heads
 // and `per` of that head's query heads), a sequence without keys as one, and
-// kUnitCost more for its start and end.  All units' steps, one behind the other, are dealt to the workgroups in equal runs,
-// whatever the lengths: a ragged batch and one long sequence both fill the
-// chip.  A run may hold several units; one that it holds whole goes straight to
+// kUnitCost more for its start and end.  All units' steps, one behind the other,
+// are dealt to the workgroups in equal runs, whatever the lengths: a ragged batch
+// and one long sequence both fill the chip.  A run may hold several units; one that it holds whole goes straight to
 // out, and at most the first and the last it holds in part: their (m, l, o) go
 // to the workgroup's two slots, and k_page_join folds them.  Lengths are known on
 // the device only, so every workgroup finds its run from them (a wave per 64
@@ -411,25 +411,48 @@ __device__ __forceinline__ void store_part(const PageAttn& a, const Run& w, uint
     if (j == 0) a.ml[slot] = make_float2(M, L);
 }
 
-// One query head, any head width up to 8 E: eight lanes share a key, with E
-// elements of its row each, and keep the (m, l, o) of their own keys, so there is
-// no barrier before the merge at the end.
+// Elements e .. e + 3 of a row of d at p + at; `one`: aligned to four, d too.
+template <uint32_t K> __device__ __forceinline__ f4 row4(const uint8_t* p, size_t at, uint32_t e, uint32_t d, bool one) {
+    if (one) {
+        if constexpr (K == Q8_0) {
+            const uint32_t w = gld<uint32_t>(p + at + e);
+            return f4{(float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)((int32_t)w >> 24)};
+        } else {
+            return four(K, p, at + e);
+        }
+    }
+    f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t c = 0; c < 4; c++)
+        if (e + c < d) x[c] = elem<K>(p, at + e + c);
+    return x;
+}
+
+// One query head, any head width up to 8 E: eight lanes share a key, with every
+// eighth four elements of its row each, and keep the (m, l, o) of their own keys, so
+// there is no barrier before the merge at the end.
 template <uint32_t K, int E>
 __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
     __shared__ float red[kWaves][8 * E], rm[kWaves], rl[kWaves];
     const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, kl = lane >> 3, p = lane & 7, d = a.c.dim;
+    constexpr size_t ES = K == F32 ? 4 : K == Q8_0 ? 1 : 2;
+    const bool one = (d % 4 | ((uintptr_t)a.c.k | (uintptr_t)a.c.v) % (4 * ES) | (a.c.ps | a.c.ts | a.c.hs) % 4) == 0;
     Run w;
     if (!w.start(a)) return;
     do {
         const uint32_t h = w.u, b = w.b, g = h / (a.heads / a.c.kvheads);
         const uint32_t k0 = w.key(), k1 = w.end();
         if (w.none()) continue;
-        float q[E], o[E], m = -INFINITY, l = 0.f;
+        constexpr int N = E / 4;
+        f4 q[N], o[N];
+        float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            const uint32_t e = p + 8 * i;
-            q[i] = e < d ? elem_kind(a.q.kind, a.q.p, b * a.q.row + h * a.q.head + e) : 0.f;
-            o[i] = 0.f;
+        for (int i = 0; i < N; i++) {
+            const uint32_t e = 4 * (p + 8 * i);
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++)
+                q[i][c] = e + c < d ? elem_kind(a.q.kind, a.q.p, b * a.q.row + h * a.q.head + e + c) : 0.f;
+            o[i] = f4{0.f, 0.f, 0.f, 0.f};
         }
         bool bad = w.len < 0;
         for (uint32_t t = k0 + 8 * wv + kl; t - kl < k1; t += 8 * kWaves) {  // wave-uniform
@@ -440,14 +463,14 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
                 page = 0;
             }
             const size_t at = (size_t)page * a.c.ps + (size_t)(tt % a.c.page) * a.c.ts + g * a.c.hs;
-            float kr[E], vr[E];
+            f4 kr[N], vr[N];
 #pragma unroll
-            for (int i = 0; i < E; i++) {
-                const uint32_t e = p + 8 * i;
-                kr[i] = vr[i] = 0.f;
+            for (int i = 0; i < N; i++) {
+                const uint32_t e = 4 * (p + 8 * i);
+                kr[i] = vr[i] = f4{0.f, 0.f, 0.f, 0.f};
                 if (e < d) {
-                    kr[i] = elem<K>(a.c.k, at + e);
-                    vr[i] = elem<K>(a.c.v, at + e);
+                    kr[i] = row4<K>(a.c.k, at, e, d, one);
+                    vr[i] = row4<K>(a.c.v, at, e, d, one);
                     if constexpr (K == Q8_0) {
                         kr[i] *= (float)gld<_Float16>(a.c.ks + (at + e) / 32);
                         vr[i] *= (float)gld<_Float16>(a.c.vs + (at + e) / 32);
@@ -456,7 +479,9 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
             }
             float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; i++) s = fmaf(q[i], kr[i], s);
+            for (int i = 0; i < N; i++)
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) s = fmaf(q[i][c], kr[i][c], s);
 #pragma unroll
             for (int x = 1; x < 8; x <<= 1) s += __shfl_xor(s, x, 64);
             s *= a.scale * kLog2e;
@@ -467,7 +492,9 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
             m = M;
             l = fmaf(l, alpha, e);
 #pragma unroll
-            for (int i = 0; i < E; i++) o[i] = fmaf(e, vr[i], o[i] * alpha);
+            for (int i = 0; i < N; i++)
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) o[i][c] = fmaf(e, vr[i][c], o[i][c] * alpha);
         }
         if (bad) l = __builtin_nanf("");
         // the wave's eight lane groups, then the waves
@@ -477,17 +504,17 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
         const float e = exp2_of(m - (M == -INFINITY ? 0.f : M));
         l *= e;
 #pragma unroll
-        for (int i = 0; i < E; i++) o[i] *= e;
+        for (int i = 0; i < N; i++) o[i] *= e;
 #pragma unroll
         for (int x = 8; x < 64; x <<= 1) {
             l += __shfl_xor(l, x, 64);
 #pragma unroll
-            for (int i = 0; i < E; i++) o[i] += __shfl_xor(o[i], x, 64);
+            for (int i = 0; i < E; i++) o[i / 4][i % 4] += __shfl_xor(o[i / 4][i % 4], x, 64);
         }
         __syncthreads();  // the unit before has been stored
         if (kl == 0) {
 #pragma unroll
-            for (int i = 0; i < E; i++) red[wv][p + 8 * i] = o[i];
+            for (int i = 0; i < E; i++) red[wv][4 * (p + 8 * (i / 4)) + i % 4] = o[i / 4][i % 4];
         }
         if (lane == 0) {
             rm[wv] = M;
@@ -534,6 +561,10 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 // power of two of their own.
 // The keys' rows come through LDS: every window of kWindow keys is looked up in
 // the page table once (any page size), as 32-bit offsets of 16 bytes.
+// Bound by memory: two histories of 65,537 f16 keys (268 MB) 51 us, 5.3 TB/s; 48
+// ragged ones of up to 4,096 bf16 keys (201 MB) 41, and 52 where the scores are
+// kept.  Q8_0 by the codes' conversions, some 500 vector operations a step: 96
+// ragged histories (217 MB) 67 us.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
@@ -542,8 +573,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 template <int N> struct Words { typedef uint32_t type __attribute__((ext_vector_type(N))); };
 template <int N> using words = typename Words<N>::type;
-// A load of what no other workgroup reads (58 us for 268 MB of rows; 61 without
-// the hint).
+// A load of what no other workgroup reads (3 us of 61 less for 268 MB of rows).
 template <typename T> __device__ __forceinline__ T once(const uint8_t* p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_nontemporal_load((gptr<T>)p);
@@ -926,7 +956,8 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
 // the weights' operand as they come.  An eighth of the 16-bit products' rate, and
 // half of each instruction idle with eight heads or fewer: still under the time
 // that memory takes for the rows (2,048 matrix-core cycles for 16 KB of f32 rows,
-// which take a compute unit's share of the bandwidth about 8,000).
+// which take a compute unit's share of the bandwidth about 8,000).  One history of
+// 517 f32 keys takes 10 us, the latency of its look-ups and rows.
 template <uint32_t K, int D>
 __global__ __launch_bounds__(64, 2) void k_page_attn32(PageAttn a) {
     constexpr int NC = D / 16, NV = D / 64;  // 16-dim loads of a key, 64-dim loads of a value
@@ -1071,7 +1102,7 @@ __global__ __launch_bounds__(64, 2) void k_page_attn32(PageAttn a) {
 // heads of a unit, with V dims of a head (4, or 1 where a head's width is no multiple of 4) a
 // thread and its parts dealt to `groups` threads.  The parts of a unit: the
 // second slot of the workgroup whose run it begins in, and the first slot of
-// those behind.
+// those behind.  Bound by latency: 5 us for one unit's parts, 6 to 7 for hundreds.
 constexpr uint32_t kJoinMost = 1024, kJoinAhead = 8;  // threads; parts in flight
 template <int V>
 __global__ __launch_bounds__(kJoinMost) void k_page_join(PageAttn a, uint32_t heads, uint32_t wide) {
@@ -1142,7 +1173,8 @@ __global__ __launch_bounds__(kJoinMost) void k_page_join(PageAttn a, uint32_t he
 }
 
 // wout[b][g][t] = win[b][g][t] + sum over g's query heads of 2^(s - m) / l: four
-// keys a thread.  In the heads' order, so the same bits on every call.
+// keys a thread.  In the heads' order, so the same bits on every call.  5.6 us for
+// 48 histories of up to 4,096 keys (13 MB of scores).
 __global__ __launch_bounds__(kBlock) void k_page_weights(PageAttn a) {
     const uint32_t g = blockIdx.y, b = blockIdx.z, G = a.heads / a.c.kvheads, t = (blockIdx.x * kBlock + threadIdx.x) * 4;
     const int32_t len = length_of(a.r, b);
