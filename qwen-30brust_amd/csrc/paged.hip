@@ -430,7 +430,10 @@ template <uint32_t K> __device__ __forceinline__ f4 row4(const uint8_t* p, size_
 
 // One query head, any head width up to 8 E: eight lanes share a key, with every
 // eighth four elements of its row each, and keep the (m, l, o) of their own keys, so
-// there is no barrier before the merge at the end.
+// there is no barrier before the merge at the end.  Every query head reads its keys
+// again, from L2: 48 ragged histories of width 96, eight heads a KV head, 290 us in
+// bf16 (743 with an element a load), some seven times what k_page_attn16 takes for
+// width 128.
 template <uint32_t K, int E>
 __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
     __shared__ float red[kWaves][8 * E], rm[kWaves], rl[kWaves];
@@ -957,9 +960,12 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
 // half of each instruction idle with eight heads or fewer: still under the time
 // that memory takes for the rows (2,048 matrix-core cycles for 16 KB of f32 rows,
 // which take a compute unit's share of the bandwidth about 8,000).  One history of
-// 517 f32 keys takes 10 us, the latency of its look-ups and rows.
+// 517 f32 keys takes 10 us, the latency of its look-ups and rows; 48 ragged ones of
+// up to 4,096 keys 71 us (403 MB, 5.7 TB/s).  Heads of 256 take one wave a SIMD for
+// their registers: the same 48 histories 149 us in f32 (805 MB), 141 in bf16, where
+// the products bound it (1,263 on k_page_attn_any).
 template <uint32_t K, int D>
-__global__ __launch_bounds__(64, 2) void k_page_attn32(PageAttn a) {
+__global__ __launch_bounds__(64, D == 256 ? 1 : 2) void k_page_attn32(PageAttn a) {
     constexpr int NC = D / 16, NV = D / 64;  // 16-dim loads of a key, 64-dim loads of a value
     constexpr uint32_t ES = K == F32 ? 4 : K == Q8_0 ? 1 : 2;
     typedef typename Four<K>::type four;
@@ -1198,18 +1204,19 @@ __global__ __launch_bounds__(kBlock) void k_page_weights(PageAttn a) {
         if ((int64_t)t + i < len) out[i] = in ? w[i] + gld<float>(in + i) : w[i];
 }
 
-// The kernel of a call.  Both matrix-core kernels want heads of 64 or 128 and
-// rows aligned to 16 bytes within 64 GiB; k_page_attn16 takes 16-bit queries of
-// the cache's type (or over Q8_0).
+// The kernel of a call.  The matrix-core kernels want rows aligned to 16 bytes
+// within 64 GiB; k_page_attn16 takes heads of 64 or 128 and 16-bit queries of the
+// cache's type (or over Q8_0), k_page_attn32 those heads with other types and heads
+// of 256.
 uint32_t page_attn_kernel(const PageAttn& a) {
     const bool q8 = a.c.kind == Q8_0;
-    if (a.c.dim != 64 && a.c.dim != 128) return 0;
+    if (a.c.dim != 64 && a.c.dim != 128 && a.c.dim != 256) return 0;
     const uint64_t es = q8 ? 1 : a.c.kind == F32 ? 4 : 2, all = a.c.ps | a.c.ts | a.c.hs;
     if (((uintptr_t)a.c.k | (uintptr_t)a.c.v | all * es) % 16) return 0;
     // a key's scales lie together
     if (q8 && (all % a.c.dim || ((uintptr_t)a.c.ks | (uintptr_t)a.c.vs) % (a.c.dim / 16))) return 0;
     if (((a.c.count - 1) * a.c.ps + (a.c.page - 1) * a.c.ts) * es >= (uint64_t)1 << 36) return 0;
-    return a.q.kind != F32 && (q8 || a.c.kind == a.q.kind) ? 16 : 32;
+    return a.c.dim != 256 && a.q.kind != F32 && (q8 || a.c.kind == a.q.kind) ? 16 : 32;
 }
 
 // At most kPageMaxRuns workgroups, and no more than there may be runs of work.
@@ -1258,7 +1265,8 @@ template <uint32_t C> static void launch_matrix(const PageAttn& a, hipStream_t s
         else if (a.kernel == 16) hipLaunchKernelGGL((k_page_attn16<C, 128>), dim3(a.runs), dim3(64), 0, s, a);
         if (a.kernel == 16) return;
     }
-    if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn32<C, 64>), dim3(a.runs), dim3(64), 0, s, a);
+    if (a.c.dim == 256) hipLaunchKernelGGL((k_page_attn32<C, 256>), dim3(a.runs), dim3(64), 0, s, a);
+    else if (a.c.dim == 64) hipLaunchKernelGGL((k_page_attn32<C, 64>), dim3(a.runs), dim3(64), 0, s, a);
     else hipLaunchKernelGGL((k_page_attn32<C, 128>), dim3(a.runs), dim3(64), 0, s, a);
 }
 template <uint32_t C> static void launch_attn(const PageAttn& a, hipStream_t s) {

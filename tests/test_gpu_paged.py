@@ -109,7 +109,8 @@ def test_attend_pages(dev, q, kv, page):
 
 
 @pytest.mark.parametrize("q,kv", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "q8_0")])
-@pytest.mark.parametrize("heads,kvheads,dim", [(4, 2, 96), (3, 1, 256), (4, 4, 32), (5, 5, 160)])
+@pytest.mark.parametrize("heads,kvheads,dim", [(4, 2, 96), (3, 1, 256), (4, 4, 32), (5, 5, 160), (20, 2, 256),
+                                               (8, 4, 192)])
 def test_attend_other_widths(dev, q, kv, heads, kvheads, dim):
     run_attend(dev, [200, 1, 77], heads, kvheads, dim, 16, q, kv)
 
