@@ -571,7 +571,6 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 template <int N> struct Words { typedef uint32_t type __attribute__((ext_vector_type(N))); };
