@@ -50,7 +50,8 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 // is one fused multiply-add, of which a large x loses nothing, S = sum 2^t, U =
 // sum t 2^t, log p = (t - log2 S) ln 2.  m is rounded and the product in t is
 // not, so that t reaches half a step of m, 1 for an x of 2^24: a row whose maximum
-// lies past that either way is far, and m is the maximum itself (slow_sums).
+// lies past that either way, or just above -2^24 with logits below it, is far, and m
+// is the maximum itself (slow_sums).
 struct Sums {
     float m = -INFINITY, S = 0.f, U = 0.f;
     __device__ __forceinline__ void move(float M) {  // to a maximum M >= m
@@ -126,10 +127,12 @@ __device__ __forceinline__ Sums fold(Sums s) {
     return s;
 }
 
-// What a row's logits hold, besides: NaN or +inf; finite maxima past 2^24.  Of a
-// lane's logits below -2^24 the sums hold nothing, and m is -inf.
+// What a row's logits hold, besides: NaN or +inf; finite maxima past 2^24.  A lane
+// whose logits of a batch all lie below -2^24 leaves them out of its sums (kLpLow):
+// they have no weight where the row's maximum lies kLpClear above, e^-256, and a row
+// whose maximum does not is far too.
 enum : uint32_t { kLpBad = 1, kLpHigh = 2, kLpLow = 4 };
-constexpr float kLpFar = 16777216.f;
+constexpr float kLpFar = 16777216.f, kLpClear = 256.f;
 __device__ __forceinline__ uint32_t any_of(uint32_t flags) {
     uint32_t r = 0;
 #pragma unroll
@@ -191,7 +194,7 @@ template <uint32_t K> struct Row {
     bool bad, far;
     __device__ __forceinline__ Row(const Logprobs& a, uint32_t r, const Target& t, Sums sums, uint32_t flags) : s(sums) {
         bad = flags & kLpBad;
-        far = !bad && ((flags & kLpHigh) || (flags & kLpLow && s.m == -INFINITY));
+        far = !bad && ((flags & kLpHigh) || (flags & kLpLow && s.m < (kLpClear - kLpFar) * kLog2e));
         if (far) {
             s = slow_sums<K>(a, r);
             bad = s.S != s.S;
