@@ -357,7 +357,8 @@ int qh_bench_read(qh_ctx *ctx, size_t bytes, size_t copies, size_t iters, qh_mat
  *     each other, need one each;
  *   - arguments on the host are checked, with an error; what lies in device
  *     memory (lengths, page ids, targets) is checked by the kernels, which read
- *     and write nothing out of range: each call says what it does instead;
+ *     and write nothing out of range: each call says what it does instead.  What
+ *     a call reads must not change before it ends;
  *   - the calling thread's current HIP device is left as it was. */
 #define QH_NULL_STREAM ((void *)(intptr_t)-1)
 #define QH_BF16 30u

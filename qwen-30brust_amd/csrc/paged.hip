@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "page_runs.hpp"
 #include "qh_block.hpp"
 #include "serving_device.hpp"
 
@@ -288,22 +289,20 @@ void launch_page_append(const PageAppend& a, hipStream_t s) {
 // Work is counted in steps of 32 keys of a unit (a sequence, one of its KV heads
 // and `per` of that head's query heads), a sequence without keys as one, and
 // kUnitCost more for its start and end.  All units' steps, one behind the other,
-// are dealt to the workgroups in equal runs, whatever the lengths: a ragged batch
-// and one long sequence both fill the chip.  A run may hold several units; one that it holds whole goes straight to
-// out, and at most the first and the last it holds in part: their (m, l, o) go
-// to the workgroup's two slots, and k_page_join folds them.  Lengths are known on
-// the device only, so every workgroup finds its run from them (a wave per 64
-// lengths and pass).
+// are dealt to the workgroups in equal runs (page_runs.hpp), whatever the lengths: a
+// ragged batch and one long sequence both fill the chip.  A run may hold several
+// units; one that it holds whole goes straight to out, and at most the first and the
+// last it holds in part: their (m, l, o) go to the workgroup's two slots, and
+// k_page_join folds them.  Lengths are known on the device only, so every workgroup
+// finds its run from them (a wave per 64 lengths and pass).  It reads them more than
+// once: lengths that change meanwhile give a wrong result, but every loop ends with
+// the batch, and the join takes its slots from the noted steps, in range.
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kStep = 32, kRunMin = 2;  // keys; steps of a run at least
-constexpr uint32_t kUnitCost = 2;            // steps in front of a unit's own that are not work
+constexpr uint32_t kStep = 32;  // keys
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32
 
 __device__ __forceinline__ uint32_t steps_of(int32_t len) {
     return (len <= 0 ? 1u : ((uint32_t)len + kStep - 1) / kStep) + kUnitCost;
-}
-__device__ __forceinline__ uint64_t div64(uint64_t a, uint64_t b) {
-    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
 }
 // A value that all lanes hold, in scalar registers.
 __device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -318,17 +317,6 @@ __device__ __forceinline__ uint64_t steps_before(const PageAttn& a, uint32_t end
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor((unsigned long long)n, o, 64);
     return same64(n);
 }
-// Run i of `total` steps in all holds the steps [total i / runs, total (i + 1) /
-// runs); fewer runs where they would be too short.
-__device__ __forceinline__ uint64_t runs_of(const PageAttn& a, uint64_t total) {
-    const uint64_t n = (total + kRunMin - 1) / kRunMin;
-    return n < a.runs ? n : a.runs;
-}
-__device__ __forceinline__ uint64_t run_begin(uint64_t total, uint64_t runs, uint64_t i) { return div64(total * i, runs); }
-__device__ __forceinline__ uint64_t run_with(uint64_t total, uint64_t runs, uint64_t x) {  // the run of step x
-    return div64((x + 1) * runs + total - 1, total) - 1;
-}
-
 // A workgroup's run: unit u (of a.units) of sequence b, from step r of its
 // `steps`; `left` steps to go.  Of a unit in hand: key(), the first key, and
 // end(), behind the last.
@@ -338,13 +326,13 @@ struct Run {
     uint64_t x, left;  // the step's number
     __device__ __forceinline__ bool start(const PageAttn& a) {
         const uint32_t lane = threadIdx.x & 63;
-        const uint64_t total = a.units * steps_before(a, a.r.batch), runs = runs_of(a, total);
+        const uint64_t total = a.units * steps_before(a, a.r.batch), runs = runs_of(total, a.runs);
         if (blockIdx.x >= runs) return false;
         x = run_begin(total, runs, blockIdx.x);
         left = run_begin(total, runs, blockIdx.x + 1) - x;
         if (blockIdx.x == 0 && threadIdx.x == 0) a.begin[a.r.batch] = total;
         uint64_t base = 0;
-        for (uint32_t j = 0;; j += 64) {  // ends: x lies in a sequence
+        for (uint32_t j = 0; j < a.r.batch; j += 64) {
             const uint32_t n = j + lane < a.r.batch ? steps_of(length_of(a.r, j + lane)) : 0;
             uint64_t sum = n;
 #pragma unroll
@@ -360,13 +348,13 @@ struct Run {
                 const uint64_t rest = same64(x - a.units * (base + shfl64(sum - n, at)));
                 u = (uint32_t)div64(rest, steps);
                 r = (uint32_t)(rest - (uint64_t)u * steps);
-                break;
+                len = (int32_t)same(length_of(a.r, b));
+                note(a);
+                return true;
             }
             base += same64(shfl64(sum, 63));
         }
-        len = (int32_t)same(length_of(a.r, b));
-        note(a);
-        return true;
+        return false;  // only where lengths changed meanwhile
     }
     // for k_page_join
     __device__ __forceinline__ void note(const PageAttn& a) const {
@@ -389,7 +377,8 @@ struct Run {
         r = 0;
         if (++u == a.units) {
             u = 0;
-            len = (int32_t)same(length_of(a.r, ++b));
+            if (++b == a.r.batch) return false;  // as in start()
+            len = (int32_t)same(length_of(a.r, b));
             steps = steps_of(len);
             note(a);
         }
@@ -1116,11 +1105,11 @@ __global__ __launch_bounds__(kJoinMost) void k_page_join(PageAttn a, uint32_t he
     const uint32_t G = a.heads / a.c.kvheads, in = u % a.groups * a.per, nh = min(a.per, G - in), z = blockIdx.z * heads;
     if (z >= nh) return;
     const uint32_t items = min(heads, nh - z) * d / V;
-    const uint64_t total = gld<uint64_t>(a.begin + a.r.batch), runs = runs_of(a, total);
-    const uint32_t steps = steps_of(length_of(a.r, b));
-    const uint64_t x = gld<uint64_t>(a.begin + b) + (uint64_t)u * steps, first = run_with(total, runs, x + kUnitCost);
-    const uint32_t parts = (uint32_t)(run_with(total, runs, x + steps - 1) - first) + 1;
-    if (parts == 1) return;  // whole in its workgroup
+    const uint64_t total = gld<uint64_t>(a.begin + a.r.batch);
+    const Parts held = parts_of(total, a.runs, gld<uint64_t>(a.begin + b), gld<uint64_t>(a.begin + b + 1), a.units, u);
+    const uint64_t first = held.first;
+    const uint32_t parts = held.count;
+    if (parts <= 1) return;  // whole in its workgroup
     const uint32_t item = min(tid % wide, items - 1), n = z + item * V / d, j = item * V % d;
     float M = -INFINITY, L = 0.f, O[V];
 #pragma unroll
