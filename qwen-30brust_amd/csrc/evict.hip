@@ -20,6 +20,8 @@ constexpr uint32_t kSelBlock = 1024, kSelWaves = kSelBlock / 64;
 // bits (11, 11 and 10), then the keys above it and the first of those equal to it,
 // by a running count in index order: no atomics but the counts' own, so the same
 // keys on every call.  A sequence with a length or page out of range keeps nothing.
+// The length is read once a workgroup, and a place is compared with `keep` before it
+// is written: weights or lengths that change meanwhile choose wrong keys, no more.
 // Bound by one compute unit's issue rate, some 20 operations a key, and by the
 // steps between the passes: 50 us for 8,192 of 65,537 keys (4 heads), 15 us for
 // 1,024 of up to 4,096 (16 sequences).  Reading the next span ahead changes nothing;
@@ -41,8 +43,11 @@ template <typename T> __device__ __forceinline__ T scan_wave(T v) {
 __global__ __launch_bounds__(kSelBlock) void k_page_select(PageEvict a) {
     __shared__ __align__(16) uint32_t hist[kBins * kCopies];
     __shared__ uint32_t pick[2], part[kSelRounds * kSelWaves];
+    __shared__ int32_t held;
     const uint32_t g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int32_t len = length_of(a.r, b);
+    if (tid == 0) held = length_of(a.r, b);
+    __syncthreads();
+    const int32_t len = held;
     uint32_t n = len < 0 ? 0u : (uint32_t)len, m = min(n, a.keep);
     const float* w = a.w + b * a.w_row + g * a.w_head;
     float x[kSelRounds][kSelPer];  // weights t0 + r kSelRound + 4 tid .. + 3
@@ -168,8 +173,10 @@ __global__ __launch_bounds__(kSelBlock) void k_page_select(PageEvict a) {
                     sort_of(inside, r, k, is_sure, is_equal);
                     if (is_sure || (is_equal && pe < need)) {
                         const uint32_t j = ps + min(pe, need);
-                        a.kept[row + j] = (int32_t)(t0 + r * kSelRound + tid * kSelPer + k);
-                        a.wout[row + j] = x[r][k];
+                        if (j < m) {
+                            a.kept[row + j] = (int32_t)(t0 + r * kSelRound + tid * kSelPer + k);
+                            a.wout[row + j] = x[r][k];
+                        }
                     }
                     ps += is_sure;
                     pe += is_equal;
@@ -185,7 +192,7 @@ __global__ __launch_bounds__(kSelBlock) void k_page_select(PageEvict a) {
 // Moves the kept keys' rows: a workgroup per kMoveKeys of them, `lanes` lanes (a
 // power of two) with B bytes each a row, K and V of several rows in flight.  B is
 // 16 where rows are aligned so, else an element; the work is two dependent
-// look-ups (kept, then the page) and a copy, 7.6 us for 8,192 keys of four heads
+// look-ups (kept, then the page; both compared with their ranges once more) and a copy, 7.6 us for 8,192 keys of four heads
 // of 128 in bf16 (33.5 MB moved, 4.4 TB/s) and 12.5 us for 16 sequences' 1,024;
 // 13.8 and 27.6 with an element a lane.
 template <uint32_t B> struct Bytes;
@@ -199,18 +206,20 @@ template <uint32_t B> __global__ __launch_bounds__(kBlock) void k_page_move(Page
     constexpr uint32_t kAhead = 4;  // rows of a thread in flight
     __shared__ uint64_t src[kMoveKeys], dst[kMoveKeys];
     const uint32_t g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, j0 = blockIdx.x * kMoveKeys;
-    const uint32_t m = (uint32_t)gld<int32_t>(a.length + b), es = a.c.kind == F32 ? 4 : a.c.kind == Q8_0 ? 1 : 2;
+    const uint32_t m = min((uint32_t)gld<int32_t>(a.length + b), a.keep), es = a.c.kind == F32 ? 4 : a.c.kind == Q8_0 ? 1 : 2;
     if (j0 >= m) return;
     const uint32_t n = min(kMoveKeys, m - j0);
+    int bad = 0;
     if (tid < n) {
         const uint32_t j = j0 + tid, t = (uint32_t)gld<int32_t>(a.kept + ((size_t)b * a.c.kvheads + g) * a.keep + j);
         const uint32_t pt = t / a.c.page, pj = j / a.c.page;
-        const uint32_t from = (uint32_t)gld<int32_t>(a.r.table + b * a.r.stride + pt);
         const uint32_t into = (uint32_t)gld<int32_t>(a.to + b * a.to_stride + pj);
+        const uint32_t from = t < a.r.most ? (uint32_t)gld<int32_t>(a.r.table + b * a.r.stride + pt) : ~0u;
+        bad = from >= a.c.count || into >= a.c.count;
         src[tid] = from * a.c.ps + (t - pt * a.c.page) * a.c.ts + g * a.c.hs;
         dst[tid] = into * a.c.ps + (j - pj * a.c.page) * a.c.ts + g * a.c.hs;
     }
-    __syncthreads();
+    if (__syncthreads_or(bad)) return;  // only where what the choice was made from changed meanwhile
     const uint32_t c = tid % lanes, per = kBlock / lanes;
     for (uint32_t o = c * B; o < row; o += lanes * B)
         for (uint32_t i0 = tid / lanes; i0 < n; i0 += per * kAhead) {
