@@ -358,7 +358,8 @@ int qh_bench_read(qh_ctx *ctx, size_t bytes, size_t copies, size_t iters, qh_mat
  *   - arguments on the host are checked, with an error; what lies in device
  *     memory (lengths, page ids, targets) is checked by the kernels, which read
  *     and write nothing out of range: each call says what it does instead.  What
- *     a call reads must not change before it ends;
+ *     a call reads must not change before it ends, nor be one of its outputs
+ *     where it does not say so;
  *   - the calling thread's current HIP device is left as it was. */
 #define QH_NULL_STREAM ((void *)(intptr_t)-1)
 #define QH_BF16 30u
@@ -454,10 +455,12 @@ int qh_paged_attention_bytes(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequ
  * weight_head; total order as f32::total_cmp, the lower index on ties).  Kept
  * keys move in ascending order to the slots 0.. of the pages to[b * to_stride +
  * i] (to_pages of them a row; those that kept keys need are all different), which
- * no sequence of the call may read.  Outputs:
- * kept[batch][kvheads][keep] their indexes (-1 behind them), kept_weights
- * [batch][kvheads][keep] their weights (0 behind them), new_length[batch].  A
- * sequence with a length or a page id out of range keeps nothing (length 0). */
+ * no sequence of the call may read.  Outputs: kept[batch][kvheads][keep] their
+ * indexes (-1 behind them), kept_weights [batch][kvheads][keep] their weights (0
+ * behind them), new_length[batch]; none may lie where the call reads (lengths,
+ * page tables, weights, from their first element to their last) or another
+ * output lies.  A sequence with a length or a page id out of range keeps nothing
+ * (length 0). */
 int qh_paged_evict(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const float *weights,
                    size_t weight_row, size_t weight_head, size_t keep, size_t first, size_t recent, const int32_t *to,
                    size_t to_stride, size_t to_pages, int32_t *kept, float *kept_weights, int32_t *new_length,

@@ -2611,6 +2611,25 @@ void need_workspace(const void* p, size_t have, size_t need) {
     need_ptr(p, 16, "workspace");
 }
 
+// Memory of a call, from its first byte to its last.
+struct Span {
+    const void* p;
+    uint64_t bytes;
+    const char* what;
+};
+// Outputs that overlap neither each other nor what the call reads: its workgroups
+// read while others write.
+void need_apart(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+    auto apart = [](const Span& a, const Span& b) {
+        const uint64_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+        if (x < y + b.bytes && y < x + a.bytes) throw Error(std::string(a.what) + " overlap the " + b.what);
+    };
+    for (auto a = outputs.begin(); a != outputs.end(); ++a) {
+        for (const Span& b : inputs) apart(*a, b);
+        for (auto b = a + 1; b != outputs.end(); ++b) apart(*a, *b);
+    }
+}
+
 // The call's kernels are launched; without a stream of the caller's, waits.
 void launched(const qh_ctx* c, void* stream) {
     HIP_OK(hipGetLastError());
@@ -2758,6 +2777,13 @@ int qh_paged_evict(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seq
         a.wout = kept_weights;
         a.length = new_length;
         need_ctx(c);
+        const uint64_t rows = a.r.batch, all = rows * a.c.kvheads * a.keep * 4;
+        const uint64_t heavy = ((rows - 1) * weight_row + (a.c.kvheads - 1) * weight_head + a.r.most) * 4;
+        need_apart({{kept, all, "kept indexes"}, {kept_weights, all, "kept weights"}, {new_length, rows * 4, "new lengths"}},
+                   {{a.r.length, rows * 4, "lengths"},
+                    {a.r.table, ((rows - 1) * a.r.stride + seqs->table_pages) * 4, "page table"},
+                    {weights, a.r.most ? heavy : 0, "weights"},
+                    {to, ((rows - 1) * to_stride + to_pages) * 4, "new pages"}});
         const OnDevice on(c->device);
         launch_page_evict(a, stream_of(c, stream));
         launched(c, stream);
