@@ -541,8 +541,9 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 // Weights go in as two parts of 16 bits, p = hi + lo: the hi parts in columns 0
 // to 7, the lo parts in columns 8 to 15, so that the second part costs no
 // instruction; their sums are added at the end.  (Where a value is not finite
-// the hi column alone says so.)  That leaves 2^-18 (bf16) or 2^-23 (f16) of a
-// weight's bits off; one part would leave 2^-9.  f16 has no weights below 2^-32 of
+// the hi column alone says so.)  That leaves 2^-17 (bf16) or 2^-23 (f16) of a
+// weight off; one part would leave 2^-8 or 2^-11.  Outputs of 16 bits are rounded by
+// more; those of 32 bits take k_page_attn32.  f16 has no weights below 2^-32 of
 // the largest: n keys lose at most n 2^-32 of the largest value.
 // The running maximum moves only when a score is 15 above it (2^15 fits f16),
 // to 7 below the new one: nearly never, so the sums are rarely rescaled.
@@ -940,7 +941,7 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
     } while (run.next(a));
 }
 
-// The same for 32-bit queries, or queries and caches of different types: every
+// The same for 32-bit queries or outputs, or queries and caches of different types: every
 // product in 32 bits on v_mfma_f32_16x16x4_f32, K and V widened as they arrive.
 // Sixteen keys a round; k slot g of step (c, i) of the first product is dim 16 c
 // + 4 g + i, of step r of the second key 4 g + r, so that the scores again are
@@ -949,7 +950,8 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
 // that memory takes for the rows (2,048 matrix-core cycles for 16 KB of f32 rows,
 // which take a compute unit's share of the bandwidth about 8,000).  One history of
 // 517 f32 keys takes 10 us, the latency of its look-ups and rows; 48 ragged ones of
-// up to 4,096 keys 71 us (403 MB, 5.7 TB/s).  Heads of 256 take one wave a SIMD for
+// up to 4,096 keys 71 us (403 MB, 5.7 TB/s); the same in bf16 or f16 with a 32-bit
+// output 70 us where k_page_attn16 takes 46, 75 over Q8_0 against 48.  Heads of 256 take one wave a SIMD for
 // their registers: the same 48 histories 149 us in f32 (805 MB), 141 in bf16, where
 // the products bound it (1,263 on k_page_attn_any).
 template <uint32_t K, int D>
@@ -1193,9 +1195,9 @@ __global__ __launch_bounds__(kBlock) void k_page_weights(PageAttn a) {
 }
 
 // The kernel of a call.  The matrix-core kernels want rows aligned to 16 bytes
-// within 64 GiB; k_page_attn16 takes heads of 64 or 128 and 16-bit queries of the
-// cache's type (or over Q8_0), k_page_attn32 those heads with other types and heads
-// of 256.
+// within 64 GiB; k_page_attn16 takes heads of 64 or 128, 16-bit queries of the
+// cache's type (or over Q8_0) and a 16-bit output, whose rounding hides that of the
+// weights; k_page_attn32 those heads with other types and heads of 256.
 uint32_t page_attn_kernel(const PageAttn& a) {
     const bool q8 = a.c.kind == Q8_0;
     if (a.c.dim != 64 && a.c.dim != 128 && a.c.dim != 256) return 0;
@@ -1204,7 +1206,7 @@ uint32_t page_attn_kernel(const PageAttn& a) {
     // a key's scales lie together
     if (q8 && (all % a.c.dim || ((uintptr_t)a.c.ks | (uintptr_t)a.c.vs) % (a.c.dim / 16))) return 0;
     if (((a.c.count - 1) * a.c.ps + (a.c.page - 1) * a.c.ts) * es >= (uint64_t)1 << 36) return 0;
-    return a.c.dim != 256 && a.q.kind != F32 && (q8 || a.c.kind == a.q.kind) ? 16 : 32;
+    return a.c.dim != 256 && a.q.kind != F32 && a.out.kind != F32 && (q8 || a.c.kind == a.q.kind) ? 16 : 32;
 }
 
 // At most kPageMaxRuns workgroups, and no more than there may be runs of work.

@@ -83,7 +83,7 @@ struct PageAttn {
     float* wout;            // and with this call's added
     size_t win_row, win_head, wout_row, wout_head;
 };
-uint32_t page_attn_kernel(const PageAttn& a);  // (q set)
+uint32_t page_attn_kernel(const PageAttn& a);  // (q and out set)
 // The units and runs of a kernel on a GPU of `cus` compute units, then the bytes
 // of its workspace and its pointers.
 void page_attn_plan(PageAttn& a, uint32_t kernel, uint32_t cus);

@@ -1,0 +1,142 @@
+"""What attention over the paged cache keeps of its scores, weights and values: weights in two parts
+of 16 bits, queries over 8-bit codes, the ends of the types' ranges, outputs of another type than the
+queries'."""
+import importlib
+import math
+
+import pytest
+import torch
+
+from serving_reference import HALF, TINY, TYPES, attend, make_cache, make_table, values
+
+engine = importlib.import_module("qwen-30brust_amd")
+serving = importlib.import_module("qwen-30brust_amd.serving")
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24  # half a step of 32 bits
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = engine.Device(0)
+    yield d
+    d.close()
+
+
+def close(got, want, bound):
+    g = got.cpu().double()
+    assert torch.isfinite(g).all()
+    tol = bound + HALF[got.dtype] * (want.abs() + bound) + TINY[got.dtype]
+    off = (g - want).abs()
+    assert (off <= tol).all(), (off / tol).max()
+
+
+# Relative error of a weight that enters a product of 16 bits in two parts: the second part is off by
+# half its step, and it is at most half a step of the first.
+SPLIT = {"bf16": 2.0 ** -17, "f16": 2.0 ** -23, "q8_0": 2.0 ** -23}
+
+
+def pairs(kv, dim, n, heads, g):
+    """A cache of one sequence of n keys in pages of 16 and queries whose scores are exact: q = (a, 2^-13,
+    0 ..), k = (s, 0 or 1, 0 ..) with s of few bits.  Key i's value is +1 or -1 (every second key) in
+    column i / 2 alone, so that an output column is the difference of two weights, or (where heads'
+    second element is 0 and values are not negated) a weight."""
+    s = torch.randint(-60, 61, (n // 2,), generator=g).repeat_interleave(2)
+    k, v = torch.zeros(n, dim), torch.zeros(n, dim)
+    k[:, 0], k[1::2, 1] = s / 64, 1.0
+    i = torch.arange(n)
+    v[i, i // 2] = 1.0 - 2.0 * (i % 2)
+    q = torch.zeros(1, heads, dim)
+    q[0, :, 0] = 1 - torch.arange(heads) / 32
+    q[0, :, 1] = 2.0 ** -13
+    page = 16
+    shape = (n // page, page, 1, dim)
+    if kv == "q8_0":
+        d = torch.full((n, dim // 32), 1.0)
+        d[:, 0] = 1 / 64
+        codes = k.clone()
+        codes[:, :32] *= 64
+        cache = (codes, v, d, torch.ones(n, dim // 32))
+        cache = (cache[0].to(torch.int8).reshape(shape).cuda(), cache[1].to(torch.int8).reshape(shape).cuda(),
+                 cache[2].half().reshape(*shape[:3], -1).cuda(), cache[3].half().reshape(*shape[:3], -1).cuda())
+    else:
+        cache = (k.to(TYPES[kv]).reshape(shape).cuda(), v.to(TYPES[kv]).reshape(shape).cuda(), None, None)
+    return cache, q
+
+
+# A weight in 32 bits of such a case (|s| <= 1): s off by 3 half steps, s - m by |s - m| <= 12 of them
+# (m at most 8 from the top), the exponential by 2, all times ln 2 but the last; the sum by as much and
+# its n / 4 + 8 additions; the division by 2
+def weight_error(n):
+    return (2 * (3 + 12 + 2) + n / 4 + 8 + 2) * U
+
+
+@pytest.mark.parametrize("q,kv,dim", [("bf16", "bf16", 128), ("bf16", "bf16", 64), ("f16", "f16", 128), ("f16", "f16", 64),
+                                      ("bf16", "q8_0", 128), ("f16", "q8_0", 64)])
+@pytest.mark.parametrize("n", [16, 64, 128])
+def test_differences_of_weights(dev, q, kv, dim, n):
+    """Outputs that are a difference of two nearly equal weights show the weights' own error, not the
+    output's rounding."""
+    cache, query = pairs(kv, dim, n, 8, torch.Generator().manual_seed(n))
+    query = query.to(TYPES[q]).cuda()
+    table = torch.arange(n // 16, dtype=torch.int32)[None]
+    k, v = values(cache[0], cache[2]), values(cache[1], cache[3])
+    want, p, _ = attend(query, k, v, table, [n], 1.0)
+    size = attend(query, k, v.abs(), table, [n], 1.0)[0]  # both weights
+    c = serving.PagedCache(dev, *cache)
+    lengths = torch.tensor([n], dtype=torch.int32).cuda()
+    got = c.attend(query, table.cuda(), lengths, scale=1.0)
+    close(got, want, (SPLIT[kv] + weight_error(n)) * size)
+    # a 32-bit output keeps 32 bits
+    out = torch.empty(1, 8, dim, device="cuda")
+    c.attend(query, table.cuda(), lengths, scale=1.0, out=out)
+    close(out, want, weight_error(n) * size)
+
+
+@pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "q8_0"), ("f32", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,kvheads", [(128, 32, 4), (64, 6, 2), (256, 4, 2), (96, 4, 2)])
+def test_output_types(dev, q, kv, out, dim, heads, kvheads):
+    """Outputs of every type, ragged lengths, the same with and without key weights."""
+    g = torch.Generator().manual_seed(dim)
+    lengths = [129, 1, 0, 700]
+    table, pool, _ = make_table(g, lengths, 16)
+    cache = make_cache(g, pool, 16, kvheads, dim, kv)
+    query = (2 * torch.randn(4, heads, dim, generator=g)).to(TYPES[q]).cuda()
+    k, v = values(cache[0], cache[2]), values(cache[1], cache[3])
+    want, _, bound = attend(query, k, v, table, lengths, 0.9 / math.sqrt(dim))
+    narrow = out != "f32" and dim in (64, 128) and q != "f32" and (kv == "q8_0" or q == kv)
+    bound = bound + (SPLIT[kv] if narrow else 0.0) * v.abs().max()
+    c = serving.PagedCache(dev, *cache)
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    held = torch.full((4, heads, dim), 7.0, dtype=TYPES[out], device="cuda")
+    assert c.attend(query, table.cuda(), n, scale=0.9 / math.sqrt(dim), out=held) is held
+    close(held, want, bound)
+    again = torch.full_like(held, 5.0)
+    w = torch.zeros(4, kvheads, 704, device="cuda")
+    c.attend(query, table.cuda(), n, 704, scale=0.9 / math.sqrt(dim), out=again, weights=w)
+    assert torch.equal(held, again)
+
+
+@pytest.mark.parametrize("x,to", [("f32", "bf16"), ("bf16", "f32"), ("f16", "bf16"), ("bf16", "f16")])
+@pytest.mark.parametrize("dim", [128, 34])
+def test_append_queries_of_another_type(dev, x, to, dim):
+    """Queries rounded to the type of q_out, beside keys in a cache of another type."""
+    g = torch.Generator().manual_seed(dim)
+    H, G, n, page = 6, 2, 21, 16
+    table = torch.tensor([[2, 0]], dtype=torch.int32)
+    k, v, _, _ = make_cache(g, 3, page, G, dim, to)
+    q_new = torch.randn(n, H, dim, generator=g).to(TYPES[x])
+    kv_new = torch.randn(2, n, G, dim, generator=g).to(TYPES[x])
+    w = 1 + 0.3 * torch.randn(dim, generator=g)
+    out = torch.full((n, H, dim), 9.0, dtype=TYPES[to], device="cuda")
+    c = serving.PagedCache(dev, k, v)
+    got = c.append(kv_new[0].cuda(), kv_new[1].cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(),
+                   torch.tensor([0, n], dtype=torch.int32).cuda(), q=q_new.cuda(), q_out=out, q_norm=w.cuda(), eps=1e-5)
+    assert got is out
+    y = q_new.double()
+    want = y / torch.sqrt((y * y).mean(-1, keepdim=True) + 1e-5) * w.double()
+    close(out, want, (dim + 12) * U * want.abs())
+    at = torch.arange(n)
+    assert torch.equal(k.cpu()[table[0].long()[at // page], at % page], kv_new[0].to(TYPES[to]))
+    assert torch.equal(v.cpu()[table[0].long()[at // page], at % page], kv_new[1].to(TYPES[to]))
