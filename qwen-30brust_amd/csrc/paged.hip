@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 // multiplies its 32-dim product in 32 bits, and code * scale of V goes in as two
 // f16 parts (the product and its rounding error, by a fused multiply-add);
 // values past f16's range come out not finite.  Queries then are f16, scaled by a
-// power of two of their own.
+// power of two of each head's own so that its largest element is just in range.
 // The keys' rows come through LDS: every window of kWindow keys is looked up in
 // the page table once (any page size), as 32-bit offsets of 16 bytes.
 // Bound by memory: two histories of 65,537 f16 keys (268 MB) 51 us, 5.3 TB/s; 48
@@ -756,11 +756,12 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
                     }
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
-                // 2^-exponent of the largest; its inverse goes to the scores
-                const uint32_t e = __float_as_uint(top) >> 23;
-                const bool scaled = e > 1 && e < 253;
-                const float f = scaled ? __uint_as_float((254 - e) << 23) : 1.f;
-                qs *= scaled ? __uint_as_float(e << 23) : 1.f;
+                // The largest goes to [2^14, 2^15), and the power's inverse to the scores: f16
+                // queries keep all their bits, bf16 ones down to 2^-31 of the largest, and what
+                // is smaller is off by 2^-39 of it at most
+                const uint32_t f23 = min(268 - (__float_as_uint(top) >> 23), 253u);
+                const float f = __uint_as_float(f23 << 23);
+                qs *= __uint_as_float((254 - f23) << 23);
 #pragma unroll
                 for (int c = 0; c < NC; c++)
 #pragma unroll

@@ -118,6 +118,57 @@ def test_output_types(dev, q, kv, out, dim, heads, kvheads):
     assert torch.equal(held, again)
 
 
+@pytest.mark.parametrize("q", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("small", [-12, -20, -24])
+def test_small_query_elements_over_codes(dev, q, dim, small):
+    """A query whose largest element meets keys of 0 there: the others, 2^small of it, keep their bits."""
+    g = torch.Generator().manual_seed(dim - small)
+    lengths, page = [5, 40, 333], 16
+    table, pool, _ = make_table(g, lengths, page)
+    cache = make_cache(g, pool, page, 2, dim, "q8_0")
+    cache[0][..., 0] = 0
+    # f16's own smallest values bound what it can hold
+    top = 1.0 if q == "bf16" else 1024.0
+    query = torch.randn(3, 8, dim, generator=g) * 2.0 ** small * top
+    query[..., 0] = top
+    query = query.to(TYPES[q]).cuda()
+    scale = 2.0 ** -small / top / math.sqrt(dim)
+    want, p, bound = attend(query, values(cache[0], cache[2]), values(cache[1], cache[3]), table, lengths, scale)
+    w = torch.zeros(3, 2, 336, device="cuda")
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    got, _ = serving.PagedCache(dev, *cache).attend(query, table.cuda(), n, 336, scale=scale, weights=w)
+    close(got, want, bound + SPLIT["q8_0"] * 5)
+    for b, t in enumerate(lengths):
+        # as the outputs' bound: a score's error is at most (d + 3) half steps of its terms' sum
+        qq = query[b].cpu().double().reshape(2, 4, dim)
+        kk = values(cache[0], cache[2])[table[b].long()[torch.arange(t) // page], torch.arange(t) % page].transpose(0, 1)
+        size = scale * (qq.abs()[:, :, None] * kk.abs()[:, None]).sum(-1).amax()
+        rel = (4 * (dim + 3) * size + 16 * size + 2 * (t + 8) + 64 + 4) * U
+        assert ((w[b, :, :t].cpu().double() - p[b]).abs() <= rel * p[b] + 2.0 ** -23 * p[b]).all()
+
+
+@pytest.mark.parametrize("kv,power", [("q8_0", p) for p in (-125, -112, -60, 0, 60, 112, 125)] +
+                         [("bf16", p) for p in (-100, -60, 60, 112, 125)])
+def test_queries_of_any_size(dev, kv, power):
+    """bf16 queries near both ends of their range, with the scale that brings the scores back."""
+    g = torch.Generator().manual_seed(200 + power)
+    lengths, dim = [70, 3], 128
+    table, pool, _ = make_table(g, lengths, 16)
+    cache = make_cache(g, pool, 16, 1, dim, kv)
+    # the largest lies at 3.9 x 2^power
+    query = torch.randn(2, 4, dim, generator=g).clamp(-3.9, 3.9)
+    query[0, 0, 0], query[1, 1, 5] = 3.9, -3.9
+    query = (query * 2.0 ** power).bfloat16().cuda()
+    scale = 2.0 ** -power / math.sqrt(dim)
+    if power > 100:  # a scale, and scores, in 32 bits' normal range
+        cache[0 if kv == "bf16" else 2].mul_(2.0 ** -10)
+        scale *= 2.0 ** 10
+    want, _, bound = attend(query, values(cache[0], cache[2]), values(cache[1], cache[3]), table, lengths, scale)
+    got = serving.PagedCache(dev, *cache).attend(query, table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), scale=scale)
+    close(got, want, bound + SPLIT[kv] * 5)
+
+
 @pytest.mark.parametrize("x,to", [("f32", "bf16"), ("bf16", "f32"), ("f16", "bf16"), ("bf16", "f16")])
 @pytest.mark.parametrize("dim", [128, 34])
 def test_append_queries_of_another_type(dev, x, to, dim):
