@@ -332,7 +332,8 @@ struct Run {
         left = run_begin(total, runs, blockIdx.x + 1) - x;
         if (blockIdx.x == 0 && threadIdx.x == 0) a.begin[a.r.batch] = total;
         uint64_t base = 0;
-        for (uint32_t j = 0; j < a.r.batch; j += 64) {
+        for (uint32_t j = 0;; j += 64) {
+            if (j >= a.r.batch) return false;  // only where lengths changed meanwhile
             const uint32_t n = j + lane < a.r.batch ? steps_of(length_of(a.r, j + lane)) : 0;
             uint64_t sum = n;
 #pragma unroll
@@ -348,13 +349,13 @@ struct Run {
                 const uint64_t rest = same64(x - a.units * (base + shfl64(sum - n, at)));
                 u = (uint32_t)div64(rest, steps);
                 r = (uint32_t)(rest - (uint64_t)u * steps);
-                len = (int32_t)same(length_of(a.r, b));
-                note(a);
-                return true;
+                break;
             }
             base += same64(shfl64(sum, 63));
         }
-        return false;  // only where lengths changed meanwhile
+        len = (int32_t)same(length_of(a.r, b));
+        note(a);
+        return true;
     }
     // for k_page_join
     __device__ __forceinline__ void note(const PageAttn& a) const {
@@ -543,8 +544,10 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 // instruction; their sums are added at the end.  (Where a value is not finite
 // the hi column alone says so.)  That leaves 2^-17 (bf16) or 2^-23 (f16) of a
 // weight off; one part would leave 2^-8 or 2^-11.  Outputs of 16 bits are rounded by
-// more; those of 32 bits take k_page_attn32.  f16 has no weights below 2^-32 of
-// the largest: n keys lose at most n 2^-32 of the largest value.
+// more; those of 32 bits take k_page_attn32.  f16's lo part is 2^11 times the rest, so
+// that it is as large as the hi part and holds weights down to 2^-43 of the largest (the
+// rest as it is would end at 2^-32, and keys that together count beside one that much
+// heavier would be lost: one whose value is 0 above 8,191 others).
 // The running maximum moves only when a score is 15 above it (2^15 fits f16),
 // to 7 below the new one: nearly never, so the sums are rarely rescaled.
 // Q8_0: codes are exact in f16 (byte | 0x6400 is 1024 + byte), a block's scale
@@ -713,9 +716,11 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
     constexpr int NC = D / 32, NT = D / 16;             // 32-dim steps of S, 16-dim tiles of O
     constexpr uint32_t ES = C == Q8_0 ? 1 : 2;
     constexpr int KW = 2 * ES, VW = D / 64 * ES;         // words of a K load (8 dims) and of a V load (D / 16 dims)
+    constexpr float kLo = C == BF16 ? 1.f : 2048.f;      // of a weight's lo part
     __shared__ uint32_t off[kWindow];
     __shared__ __align__(16) uint16_t ksl[kStep][NC], vsl[NC][kStep];  // the step's scales (Q8_0)
     const uint32_t lane = threadIdx.x, g = lane >> 4, n = lane & 15;
+    const float part = n < 8 ? 1.f : kLo, rest = n < 8 ? 0.f : -kLo;  // x part + hi rest: x, or its lo part
     const uint32_t G = a.heads / a.c.kvheads;
     Run run;
     if (!run.start(a)) return;
@@ -871,10 +876,8 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
                 for (int i = 0; i < 4; i++) {
                     const float x = exp2_of(s[i / 2][2 * (i % 2)] - mf), y = exp2_of(s[i / 2][2 * (i % 2) + 1] - mf);
                     l += x + y;
-                    const uint32_t hi = pack2<C>(x, y);
-                    const float2 back = unpack2<C>(hi);
-                    const uint32_t lo = pack2<C>(x - back.x, y - back.y);
-                    p[i] = n < 8 ? hi : lo;
+                    const float2 hi = unpack2<C>(pack2<C>(x, y));
+                    p[i] = pack2<C>(fmaf(hi.x, rest, x * part), fmaf(hi.y, rest, y * part));
                 }
                 if constexpr (C == Q8_0) {
                     // scales of the lane's block and keys, in pairs
@@ -936,7 +939,7 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {  // the lo parts' sums, from column n + 8
                 const float lo = __shfl_xor(o[t][r], 8, 64);
-                if (finite_f(o[t][r])) o[t][r] += lo;
+                if (finite_f(o[t][r])) o[t][r] = fmaf(lo, 1.f / kLo, o[t][r]);
             }
         if (n < nh) store_head<D>(a, run, h0 + n, n, g, m, l, o);
     } while (run.next(a));

@@ -169,6 +169,36 @@ def test_queries_of_any_size(dev, kv, power):
     close(got, want, bound + SPLIT[kv] * 5)
 
 
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("f16", "q8_0"), ("bf16", "q8_0"), ("bf16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("gap", [12, 23, 25])
+def test_one_key_far_above_the_others(dev, q, kv, gap):
+    """A first key `gap` above all others whose value is 0: the output is the many others' alone, each
+    weight e^-gap.  1,024 sequences and KV heads of 8,192 keys, so that no split over the keys gives the
+    others a wave without the first one."""
+    dim, n, page, G, B = 64, 8192, 16, 16, 64
+    k, v = torch.zeros(2, page, G, dim), torch.zeros(2, page, G, dim)
+    k[0, 0, :, 0] = gap
+    v[:] = 96.0 + torch.arange(G)[:, None]
+    v[0, 0] = 0.0
+    if kv == "q8_0":
+        ones = torch.ones(2, page, G, dim // 32, dtype=torch.float16)
+        cache = (k.to(torch.int8).cuda(), v.to(torch.int8).cuda(), ones.cuda(), ones.clone().cuda())
+    else:
+        cache = (k.to(TYPES[kv]).cuda(), v.to(TYPES[kv]).cuda(), None, None)
+    query = torch.zeros(B, G, dim)
+    query[..., 0] = 1.0
+    table = torch.ones(B, n // page, dtype=torch.int32)
+    table[:, 0] = 0
+    got = serving.PagedCache(dev, *cache).attend(query.to(TYPES[q]).cuda(), table.cuda(),
+                                                 torch.full((B,), n, dtype=torch.int32).cuda(), scale=1.0)
+    others = (n - 1) * math.exp(-gap)
+    want = (others / (1 + others) * (96.0 + torch.arange(G, dtype=torch.float64)))[None, :, None].expand(B, G, dim)
+    # scores are whole numbers: off by 3 |s| half steps, s - m by |s - m| < 64, the exponential by 2; sums
+    # of n weights in runs, at most n additions; below 2^-43 of the largest weight nothing counts
+    bound = (2 * (3 * gap + 64 + 2) + n + 64) * U * want + 2.0 ** -17 * want * (kv == "bf16") + n * 2.0 ** -43 * 112
+    close(got, want, bound)
+
+
 @pytest.mark.parametrize("x,to", [("f32", "bf16"), ("bf16", "f32"), ("f16", "bf16"), ("bf16", "f16")])
 @pytest.mark.parametrize("dim", [128, 34])
 def test_append_queries_of_another_type(dev, x, to, dim):
