@@ -435,10 +435,11 @@ typedef struct {
 /* Attention of one token per sequence over its cached keys (qh_attention's
  * formula with a scale of the caller's): q and out [batch][heads][dim], heads a
  * multiple of kvheads, query head h reading KV head h / (heads / kvheads).
- * Sums in 32 bits, out rounded once to its kind.  With an out of F16 or BF16 and
- * queries of the cache's own 16-bit kind, or 16-bit ones over Q8_0, a key's softmax
- * weight enters the products with 17 bits (BF16) or 23 (F16, Q8_0); with an F32 out
- * everything is in 32 bits and takes half as long again.  A sequence without keys, or
+ * Sums in 32 bits, out rounded once to its kind; values whose sum over a
+ * sequence's keys is past 32 bits' range (from 2^128 / keys on) may come out not
+ * finite.  With an out of F16 or BF16 and queries of the cache's own 16-bit kind, or
+ * 16-bit ones over Q8_0, a key's softmax weight enters the products with 17 bits
+ * (BF16) or 23 (F16, Q8_0); with an F32 out everything is in 32 bits and takes half as long again.  A sequence without keys, or
  * whose scores are all -inf, gives zeros; one with a length or a page id out of
  * range NaN.  weights nullable; the weights of a sequence whose length is out of
  * range are left as they were.  A Q8_0 cache's values (code times scale) past

@@ -548,8 +548,11 @@ __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
 // that it is as large as the hi part and holds weights down to 2^-43 of the largest (the
 // rest as it is would end at 2^-32, and keys that together count beside one that much
 // heavier would be lost: one whose value is 0 above 8,191 others).
-// The running maximum moves only when a score is 15 above it (2^15 fits f16),
-// to 7 below the new one: nearly never, so the sums are rarely rescaled.
+// The running reference m moves only when a score is kRoom above it, to 8 - kRoom
+// above that score: nearly never, so the sums are rarely rescaled.  Weights of f16
+// reach 2^15 (kRoom 15; a sum of 2^31 f16 values is far from 32 bits' end), those of
+// bf16 and of 32-bit products 1 (kRoom 0): a value near the end of its range comes
+// out as it is as long as the values' sum is in range.
 // Q8_0: codes are exact in f16 (byte | 0x6400 is 1024 + byte), a block's scale
 // multiplies its 32-dim product in 32 bits, and code * scale of V goes in as two
 // f16 parts (the product and its rounding error, by a fused multiply-add);
@@ -717,6 +720,7 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
     constexpr uint32_t ES = C == Q8_0 ? 1 : 2;
     constexpr int KW = 2 * ES, VW = D / 64 * ES;         // words of a K load (8 dims) and of a V load (D / 16 dims)
     constexpr float kLo = C == BF16 ? 1.f : 2048.f;      // of a weight's lo part
+    constexpr float kRoom = C == BF16 ? 0.f : 15.f;
     __shared__ uint32_t off[kWindow];
     __shared__ __align__(16) uint16_t ksl[kStep][NC], vsl[NC][kStep];  // the step's scales (Q8_0)
     const uint32_t lane = threadIdx.x, g = lane >> 4, n = lane & 15;
@@ -859,10 +863,10 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
                 }
                 float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                   fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-                if (__any(top > m + 15.f)) {
+                if (__any(top > m + kRoom)) {
                     top = fmaxf(top, __shfl_xor(top, 16, 64));
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float M = fmaxf(m, top - 7.f), alpha = M == -INFINITY ? 1.f : exp2_of(m - M);
+                    const float M = fmaxf(m, top + (8.f - kRoom)), alpha = M == -INFINITY ? 1.f : exp2_of(m - M);
                     m = M;
                     l *= alpha;
 #pragma unroll
@@ -1037,10 +1041,10 @@ __global__ __launch_bounds__(64, D == 256 ? 1 : 2) void k_page_attn32(PageAttn a
                         if (t0 + 4 * g + r >= k1) s[r] = -INFINITY;
                 }
                 float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-                if (__any(top > m + 15.f)) {
+                if (__any(top > m)) {  // no weight above 1, as in bf16 above
                     top = fmaxf(top, __shfl_xor(top, 16, 64));
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float M = fmaxf(m, top - 7.f), alpha = M == -INFINITY ? 1.f : exp2_of(m - M);
+                    const float M = fmaxf(m, top + 8.f), alpha = M == -INFINITY ? 1.f : exp2_of(m - M);
                     m = M;
                     l *= alpha;
 #pragma unroll

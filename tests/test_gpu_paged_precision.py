@@ -199,6 +199,21 @@ def test_one_key_far_above_the_others(dev, q, kv, gap):
     close(got, want, bound)
 
 
+@pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("dim", [64, 128, 256, 96])
+def test_large_values(dev, q, kv, dim):
+    """Values whose sum over the keys is still in 32 bits' range."""
+    g = torch.Generator().manual_seed(dim)
+    lengths = [8, 1, 5, 0]
+    table, pool, _ = make_table(g, lengths, 16)
+    k, v, _, _ = make_cache(g, pool, 16, 2, dim, kv)
+    v.clamp_(-2, 2).mul_(2e37)
+    query = (2 * torch.randn(4, 8, dim, generator=g)).to(TYPES[q]).cuda()
+    want, _, bound = attend(query, values(k, None), values(v, None), table, lengths, 1 / math.sqrt(dim))
+    got = serving.PagedCache(dev, k, v).attend(query, table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda())
+    close(got, want, bound + (SPLIT["bf16"] * 4e37 if q == kv == "bf16" else 0.0))
+
+
 @pytest.mark.parametrize("x,to", [("f32", "bf16"), ("bf16", "f32"), ("f16", "bf16"), ("bf16", "f16")])
 @pytest.mark.parametrize("dim", [128, 34])
 def test_append_queries_of_another_type(dev, x, to, dim):
