@@ -439,10 +439,11 @@ typedef struct {
  * sequence's keys is past 32 bits' range (from 2^128 / keys on) may come out not
  * finite.  With an out of F16 or BF16 and queries of the cache's own 16-bit kind, or
  * 16-bit ones over Q8_0, a key's softmax weight enters the products with 17 bits
- * (BF16) or 23 (F16, Q8_0); with an F32 out everything is in 32 bits and takes half as long again.  A sequence without keys, or
- * whose scores are all -inf, gives zeros; one with a length or a page id out of
- * range NaN.  weights nullable; the weights of a sequence whose length is out of
- * range are left as they were.  A Q8_0 cache's values (code times scale) past
+ * (BF16) or 23 (F16, Q8_0); with an F32 out everything is in 32 bits and takes half
+ * as long again.  A sequence without keys, or whose scores are all -inf, gives
+ * zeros; one with a length or a page id out of range NaN.  weights nullable; the
+ * weights of a sequence whose length is out of range are left as they were, those
+ * of one with such a page become NaN.  A Q8_0 cache's values (code times scale) past
  * f16's range, 65504, come out not finite with F16 or BF16 queries and outputs; with
  * F32 ones they are read in 32 bits.  q and out may be the same. */
 int qh_paged_attention(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const qh_heads_t *q,

@@ -97,7 +97,7 @@ template <uint32_t L> __global__ __launch_bounds__(kBlock) void k_page_append(Pa
     constexpr uint32_t D = 8 * L;
     const uint32_t lane = threadIdx.x & 63, l = lane % L;
     const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-    const uint32_t i = unit / groups, h = unit % groups * (64 / L) + lane / L;
+    const uint32_t i = a.from + unit / groups, h = unit % groups * (64 / L) + lane / L;
     if (i >= a.n) return;
     const bool mine = h < a.heads + 2 * a.c.kvheads;
     const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.c.kvheads;
@@ -173,11 +173,11 @@ __global__ __launch_bounds__(kBlock) void k_page_append_any(PageAppend a) {
     __shared__ float turn[kWaves][kPageMaxDim];
     const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6, d = a.c.dim;
     const uint32_t slots = a.heads + 2 * a.c.kvheads;
-    const uint64_t unit = (uint64_t)blockIdx.x * kWaves + wv;
-    const uint32_t i = (uint32_t)min(unit / slots, (uint64_t)a.n - 1);
-    const uint32_t h = (uint32_t)(unit % slots);
+    const uint32_t unit = blockIdx.x * kWaves + wv;
+    const uint32_t i = min(a.from + unit / slots, a.n - 1);
+    const uint32_t h = unit % slots;
     const Place p = place_of(a, i);
-    const bool live = p.live && unit / slots < a.n;
+    const bool live = p.live && a.from + unit / slots < a.n;
     const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.c.kvheads;
     const uint32_t g = is_q ? h : is_k ? h - a.heads : h - a.heads - a.c.kvheads;
     const Heads& src = is_q ? a.q : is_k ? a.k : a.v;
@@ -263,21 +263,34 @@ static bool by_four(const void* p, size_t row, size_t head, size_t es) {
 }
 static bool by_four(const Heads& h) { return !h.p || by_four(h.p, h.row, h.head, h.kind == F32 ? 4 : 2); }
 
-void launch_page_append(const PageAppend& a, hipStream_t s) {
-    const uint32_t slots = a.heads + 2 * a.c.kvheads, d = a.c.dim;
-    const size_t es = a.c.kind == F32 ? 4 : a.c.kind == Q8_0 ? 1 : 2;
-    const uintptr_t floats = (uintptr_t)a.qw | (uintptr_t)a.kw | (uintptr_t)a.rope;
-    if ((d == 64 || d == 128 || d == 256) && by_four(a.q) && by_four(a.qo) && by_four(a.k) && by_four(a.v) &&
-        by_four(a.c.k, a.c.ts, a.c.hs, es) && by_four(a.c.v, a.c.ps, 0, es) && floats % 16 == 0) {
+// f(args, waves) for ranges of tokens, `each` waves a token: a launch has fewer than
+// 2^32 threads.
+constexpr uint32_t kAppendWaves = 1u << 25;
+template <class F> static void by_tokens(PageAppend a, uint32_t each, F f) {
+    const uint32_t n = a.n, most = kAppendWaves / each;  // heads <= 65535 and as many KV heads twice
+    for (uint32_t done = 0; done < n; done = a.n) {
+        a.from = done;
+        a.n = std::min(n, done + most);
+        f(a, dim3(((a.n - done) * each + kWaves - 1) / kWaves));
+    }
+}
+
+void launch_page_append(const PageAppend& args, hipStream_t s) {
+    const uint32_t slots = args.heads + 2 * args.c.kvheads, d = args.c.dim;
+    const size_t es = args.c.kind == F32 ? 4 : args.c.kind == Q8_0 ? 1 : 2;
+    const uintptr_t floats = (uintptr_t)args.qw | (uintptr_t)args.kw | (uintptr_t)args.rope;
+    const dim3 block(kBlock);
+    if ((d == 64 || d == 128 || d == 256) && by_four(args.q) && by_four(args.qo) && by_four(args.k) && by_four(args.v) &&
+        by_four(args.c.k, args.c.ts, args.c.hs, es) && by_four(args.c.v, args.c.ps, 0, es) && floats % 16 == 0) {
         const uint32_t per = 512 / d, groups = (slots + per - 1) / per;
-        const dim3 grid((uint32_t)(((uint64_t)a.n * groups + kWaves - 1) / kWaves)), block(kBlock);
-        if (d == 64) hipLaunchKernelGGL(k_page_append<8>, grid, block, 0, s, a, groups);
-        else if (d == 128) hipLaunchKernelGGL(k_page_append<16>, grid, block, 0, s, a, groups);
-        else hipLaunchKernelGGL(k_page_append<32>, grid, block, 0, s, a, groups);
+        by_tokens(args, groups, [&](const PageAppend& a, dim3 grid) {
+            if (d == 64) hipLaunchKernelGGL(k_page_append<8>, grid, block, 0, s, a, groups);
+            else if (d == 128) hipLaunchKernelGGL(k_page_append<16>, grid, block, 0, s, a, groups);
+            else hipLaunchKernelGGL(k_page_append<32>, grid, block, 0, s, a, groups);
+        });
         return;
     }
-    const uint64_t units = (uint64_t)a.n * slots;
-    hipLaunchKernelGGL(k_page_append_any, dim3((uint32_t)((units + kWaves - 1) / kWaves)), dim3(kBlock), 0, s, a);
+    by_tokens(args, slots, [&](const PageAppend& a, dim3 grid) { hipLaunchKernelGGL(k_page_append_any, grid, block, 0, s, a); });
 }
 
 // --------------------------------------------------------------- attention --

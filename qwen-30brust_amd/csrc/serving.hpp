@@ -51,7 +51,7 @@ struct PageAppend {
     Pages c;
     Rows r;
     const int32_t* first;  // [batch + 1] tokens before each sequence's, or null: one each
-    uint32_t n;            // tokens
+    uint32_t from, n;      // tokens [from, n)
     Heads k, v, q, qo;     // q.p null: no queries
     uint32_t heads;
     const float *qw, *kw;  // RMSNorm weights [dim], or null
