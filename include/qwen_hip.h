@@ -454,8 +454,9 @@ int qh_paged_attention(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_
 int qh_paged_attention_bytes(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, uint32_t heads,
                              int with_weights, size_t *out);
 
-/* Brings every sequence to at most keep keys: of a longer one every KV head
- * keeps its first `first` keys, its last `recent` and the heaviest of those
+/* Brings every sequence to at most keep keys (fewer than 2^30 - 63 to move): of a
+ * longer one every KV head keeps its first `first` keys, its last `recent` and the
+ * heaviest of those
  * between by weights ([batch][kvheads][most], strides weight_row and
  * weight_head; total order as f32::total_cmp, the lower index on ties).  Kept
  * keys move in ascending order to the slots 0.. of the pages to[b * to_stride +

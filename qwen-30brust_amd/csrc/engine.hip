@@ -2755,6 +2755,7 @@ int qh_paged_evict(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seq
         if (first > keep || recent > keep - first) throw Error("the first and recent keys are more than those kept");
         if (!a.r.batch) return;
         const uint64_t most = std::min<uint64_t>(keep, a.r.most);
+        if (most > (1u << 30) - kMoveKeys) throw Error("keys to keep out of range");  // a launch has fewer than 2^32 threads
         if ((uint64_t)to_pages * a.c.page < most) throw Error("the new pages hold fewer keys than those kept");
         if (a.r.most) {
             need_ptr(weights, 4, "weights");
