@@ -8,7 +8,8 @@ given engine Device's, returns at once, and may be captured into a graph.  What
 it allocates (outputs that are not given, workspaces) comes from torch's
 allocator.  Arguments on the host are checked (EngineError); lengths, page ids
 and targets lie on the device and are checked there: the header says what a call
-does with those out of range.
+does with those out of range.  Nothing here has a gradient: a tensor that requires
+one is refused where torch records gradients (call under torch.no_grad()).
 
     serving = importlib.import_module("qwen-30brust_amd.serving")
 """
@@ -31,7 +32,11 @@ def _need(ok, message):
 
 def _on(dev, t, what, dtypes, ndim):
     """Checks a tensor's place, type and rank, and that its last dimension is contiguous; its shape and strides."""
-    if not (isinstance(t, torch.Tensor) and t.get_device() == dev.index):  # -1 on the host
+    if not isinstance(t, torch.Tensor):
+        raise EngineError(f"{what}: not a tensor on the engine's device")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise EngineError(f"{what}: no gradient is recorded here; call under torch.no_grad()")
+    if t.get_device() != dev.index:  # -1 on the host
         raise EngineError(f"{what}: not a tensor on the engine's device")
     if t.dtype not in dtypes:
         raise EngineError(f"{what}: type {t.dtype} is not supported")
