@@ -359,7 +359,7 @@ int qh_bench_read(qh_ctx *ctx, size_t bytes, size_t copies, size_t iters, qh_mat
  *     memory (lengths, page ids, targets) is checked by the kernels, which read
  *     and write nothing out of range: each call says what it does instead.  What
  *     a call reads must not change before it ends, nor be one of its outputs
- *     where it does not say so;
+ *     where it does not say so, and an output's elements share no memory;
  *   - the calling thread's current HIP device is left as it was. */
 #define QH_NULL_STREAM ((void *)(intptr_t)-1)
 #define QH_BF16 30u

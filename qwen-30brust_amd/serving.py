@@ -62,6 +62,16 @@ def _live(dev):
     return dev.h
 
 
+def _shared(t):
+    """Whether elements share memory (an expanded dimension)."""
+    return any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+
+
+def _apart(t, what):
+    if _shared(t):
+        raise EngineError(f"{what}: elements of an output share memory")
+
+
 def _heads(dev, t, what, rows, heads, dim):
     shape, strides = _on(dev, t, what, KIND, 3)
     if shape != (rows, heads, dim):
@@ -90,6 +100,7 @@ class PagedCache:
         else:
             _need(k_scale is None and v_scale is None, "scales go with a cache of 8-bit codes")
         self.device, self.k, self.v, self.k_scale, self.v_scale = device, k, v, k_scale, v_scale
+        self._writable = not (_shared(k) or _shared(v))
         pages, self.page, self.kvheads, self.dim = k.shape
         # a dimension of one has no stride of its own
         st = [s if n > 1 else 32 * -(-s // 32) for n, s in zip(k.shape[:3], k.stride())]
@@ -119,6 +130,7 @@ class PagedCache:
         [n] (None: their places).  Returns q_out (allocated if not given), or
         None without q."""
         dev, (n, d) = self.device, (k.shape[0], self.dim)
+        _need(self._writable, "a cache whose elements share memory is read only")
         seqs = self._sequences(table, lengths, None)
         kh = _heads(dev, k, "keys", n, self.kvheads, d)
         vh = _heads(dev, v, "values", n, self.kvheads, d)
@@ -129,9 +141,12 @@ class PagedCache:
         if q is not None:
             more.heads = heads = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
             more.q = _heads(dev, q, "queries", n, heads, d)
-            if q_out is None:
+            given = q_out is not None
+            if not given:
                 q_out = q.new_empty((n, heads, d))
             more.q_out = _heads(dev, q_out, "query outputs", n, heads, d)
+            if given:
+                _apart(q_out, "query outputs")
         else:
             _need(q_out is None and q_norm is None, "query outputs and weights go with queries")
         for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
@@ -166,9 +181,12 @@ class PagedCache:
         seqs = self._sequences(table, lengths, most)
         heads = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
         qh = _heads(dev, q, "queries", batch, heads, d)
-        if out is None:
+        given = out is not None
+        if not given:
             out = q.new_empty((batch, heads, d))
         oh = _heads(dev, out, "attention outputs", batch, heads, d)
+        if given:
+            _apart(out, "attention outputs")
         w = None
         if weights_out is None:
             weights_out = weights
@@ -178,6 +196,7 @@ class PagedCache:
                     _on(dev, t, what, _F32, 3)
                     _need(t.shape[0] == batch and t.shape[1] == self.kvheads and t.shape[2] >= seqs.most,
                           f"{what}: [sequences][KV heads][longest length] is needed")
+            _apart(weights_out, "weight outputs")
             i = (None, 0, 0) if weights is None else (weights.data_ptr(), weights.stride(0), weights.stride(1))
             w = engine._KeyWeights(i[0], weights_out.data_ptr(), i[1], i[2], weights_out.stride(0),
                                    weights_out.stride(1))
@@ -197,6 +216,7 @@ class PagedCache:
         indexes [batch][kvheads][keep] with -1 behind them, their weights, new
         lengths)."""
         dev = self.device
+        _need(self._writable, "a cache whose elements share memory is read only")
         _on(dev, weights, "weights", _F32, 3)
         if most is None:
             most = min(weights.shape[2], table.shape[-1] * self.page)
