@@ -414,11 +414,12 @@ typedef struct {
  * sequence b's tokens are first[b] .. first[b + 1] - 1 of k and v (first:
  * batch + 1 ascending numbers; NULL: one token each, n = batch), the last of
  * them at length[b] - 1.  Values are rounded once to the cache's kind (Q8_0:
- * scale max |x| / 127 of each 32, rounded to f16; a block with a value that is
- * not finite becomes NaN).  Tokens without a place (in front of first[0] or
- * behind first[batch], a length of 0 or out of range) leave every output as it
- * was, those of a page id outside the cache leave the cache as it was.  Two
- * sequences must not append to the same slot.  more: nullable. */
+ * scale max |x| / 127 of each 32, rounded to f16, and the code nearest to x / that
+ * scale, which can be one off from GGML's own quantiser; a block with a value that
+ * is not finite, or past 127 x 65504, becomes NaN).  Tokens without a place (in
+ * front of first[0] or behind first[batch], a length of 0 or out of range) leave
+ * every output as it was, those of a page id outside the cache leave the cache as it
+ * was.  Two sequences must not append to the same slot.  more: nullable. */
 int qh_paged_append(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,
                     const qh_heads_t *k, const qh_heads_t *v, const qh_append_t *more, void *stream);
 
@@ -450,7 +451,9 @@ int qh_paged_attention(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_
                        uint32_t heads, float scale, const qh_heads_t *out, const qh_key_weights_t *weights,
                        void *workspace, size_t workspace_bytes, void *stream);
 /* Bytes of workspace that a call of these shapes needs (0: none; its pointer
- * may then be NULL, else it is aligned to 16 bytes). */
+ * may then be NULL, else it is aligned to 16 bytes).  With weights it holds every
+ * score, batch x heads x most x 4 bytes whatever the lengths are (1 GiB for 64
+ * sequences of up to 131,072 keys and 32 heads); without, at most some 34 MB. */
 int qh_paged_attention_bytes(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, uint32_t heads,
                              int with_weights, size_t *out);
 

@@ -20,8 +20,10 @@ namespace qh {
 //   y = x / sqrt(sum x^2 / dim + eps) * w              (q and k, with weights)
 //   (y_i, y_j) = (y_i cos - y_j sin, y_j cos + y_i sin), j = i + dim / 2
 // in 32 bits, rounded once to the type it is stored in.  Q8_0: per 32 values
-// d = f16(max |y| / 127) and codes round(y / d), as GGML lays them out, but
-// codes and scales each in an array of their own.
+// d = f16(max |y| / 127) and codes round(y / d), the blocks of GGML's format with
+// codes and scales each in an array of their own.  GGML's own quantiser multiplies
+// by the inverse of the unrounded scale and takes ties away from 0: its codes can be
+// one off from these, which are the nearest to y in the scale that is stored.
 // A token outside the table of angles becomes NaN.
 
 // Where token i goes: into place t of sequence b, or nowhere.  By a wave.
@@ -311,7 +313,8 @@ void launch_page_append(const PageAppend& args, hipStream_t s) {
 // once: lengths that change meanwhile give a wrong result, but every loop ends with
 // the batch, and the join takes its slots from the noted steps, in range.
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kStep = 32;  // keys
+constexpr uint32_t kStep = 32;     // keys
+constexpr uint32_t kPerMost = 8;   // query heads of a unit
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32
 
 __device__ __forceinline__ uint32_t steps_of(int32_t len) {
@@ -972,9 +975,10 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
 // which take a compute unit's share of the bandwidth about 8,000).  One history of
 // 517 f32 keys takes 10 us, the latency of its look-ups and rows; 48 ragged ones of
 // up to 4,096 keys 71 us (403 MB, 5.7 TB/s); the same in bf16 or f16 with a 32-bit
-// output 70 us where k_page_attn16 takes 46, 75 over Q8_0 against 48.  Heads of 256 take one wave a SIMD for
-// their registers: the same 48 histories 149 us in f32 (805 MB), 141 in bf16, where
-// the products bound it (1,263 on k_page_attn_any).
+// output 70 us where k_page_attn16 takes 46, 75 over Q8_0 against 48 (whole calls).
+// Heads of 256 take one wave a SIMD for their registers: the same 48 histories 149 us
+// in f32 (805 MB), 141 in bf16, where the products bound it (1,263 on
+// k_page_attn_any).
 template <uint32_t K, int D>
 __global__ __launch_bounds__(64, D == 256 ? 1 : 2) void k_page_attn32(PageAttn a) {
     constexpr int NC = D / 16, NV = D / 64;  // 16-dim loads of a key, 64-dim loads of a value
@@ -1121,6 +1125,7 @@ __global__ __launch_bounds__(64, D == 256 ? 1 : 2) void k_page_attn32(PageAttn a
 // second slot of the workgroup whose run it begins in, and the first slot of
 // those behind.  Bound by latency: 5 us for one unit's parts, 6 to 7 for hundreds.
 constexpr uint32_t kJoinMost = 1024, kJoinAhead = 8;  // threads; parts in flight
+static_assert(kPerMost * kPageMaxDim / 4 <= kJoinMost / 2 && kPageMaxDim <= kJoinMost / 2, "a thread each, whatever V");
 template <int V>
 __global__ __launch_bounds__(kJoinMost) void k_page_join(PageAttn a, uint32_t heads, uint32_t wide) {
     __shared__ float red[kJoinMost][V + 2];
@@ -1234,12 +1239,13 @@ uint32_t page_attn_kernel(const PageAttn& a) {
 void page_attn_plan(PageAttn& a, uint32_t kernel, uint32_t cus) {
     const uint32_t G = a.heads / a.c.kvheads;
     a.kernel = kernel;
-    a.groups = kernel ? (G + 7) / 8 : G;
+    a.groups = kernel ? (G + kPerMost - 1) / kPerMost : G;
     a.per = (G + a.groups - 1) / a.groups;
     a.units = a.c.kvheads * a.groups;
     const uint64_t steps = std::max<uint64_t>(1, ((uint64_t)a.r.most + kStep - 1) / kStep) + kUnitCost;
-    // k_page_attn16 over 48 ragged histories of bf16 keys: 1,024 waves 52.6 us,
-    // 1,536 and 2,048 54.3; over 96 of Q8_0 keys 85, 77 and 74
+    // k_page_attn16 over 48 ragged histories of bf16 keys: 1,024 waves 52.5 us, 1,536 and
+    // 2,048 53.5 and 54.4, and the join 2 more.  Over 96 of Q8_0 keys whole calls of 1,024
+    // and 2,048 waves: 128 wide 74 and 76, 64 wide 52.5 and 50, f32 queries 143 and 128
     const uint64_t fill = std::min<uint64_t>((uint64_t)cus * (kernel && a.c.kind == Q8_0 ? 8 : 4), kPageMaxRuns);
     a.runs = (uint32_t)std::min<uint64_t>(fill, (a.units * steps * a.r.batch + kRunMin - 1) / kRunMin);
     a.score_row = ((uint64_t)a.r.most + 63) / 64 * 64;
@@ -1297,7 +1303,7 @@ void launch_page_attn(const PageAttn& a, hipStream_t s) {
         const bool few = (uint64_t)a.units * a.r.batch < 128;
         const uint32_t heads = few ? 1 : a.per;
         uint32_t wide = 16;
-        while (wide < heads * a.c.dim / v) wide *= 2;  // at most 256
+        while (wide < heads * a.c.dim / v) wide *= 2;  // at most 512: eight heads of 256, or one in single dims
         const dim3 grid(a.units, a.r.batch, few ? a.per : 1), block(few ? kJoinMost : kJoinMost / 2);
         if (v == 4) hipLaunchKernelGGL(k_page_join<4>, grid, block, 0, s, a, heads, wide);
         else hipLaunchKernelGGL(k_page_join<1>, grid, block, 0, s, a, heads, wide);

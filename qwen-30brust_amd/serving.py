@@ -176,7 +176,9 @@ class PagedCache:
         given.  With weights and / or weights_out ([batch][kvheads][most or
         more] in f32) every key's softmax weight, summed over its KV head's query
         heads, is added to weights (zeros if not given) and written to
-        weights_out (weights itself if not given); returns (out, weights_out)."""
+        weights_out (weights itself if not given); returns (out, weights_out).
+        The call's workspace then holds every score: batch x heads x most x 4
+        bytes."""
         dev, (batch, d) = self.device, (lengths.shape[0], self.dim)
         seqs = self._sequences(table, lengths, most)
         heads = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0

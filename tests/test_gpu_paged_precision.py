@@ -236,3 +236,36 @@ def test_append_queries_of_another_type(dev, x, to, dim):
     at = torch.arange(n)
     assert torch.equal(k.cpu()[table[0].long()[at // page], at % page], kv_new[0].to(TYPES[to]))
     assert torch.equal(v.cpu()[table[0].long()[at // page], at % page], kv_new[1].to(TYPES[to]))
+
+
+@pytest.mark.parametrize("q,kv,size", [("f16", "f16", -14), ("bf16", "q8_0", -14), ("f32", "q8_0", -14), ("f32", "f16", -14),
+                                       ("bf16", "bf16", -90), ("f32", "f32", -90), ("f32", "bf16", -90)])
+@pytest.mark.parametrize("dim", [128, 64])
+def test_small_values(dev, q, kv, size, dim):
+    """Values of 2^size, in f16 below its normal range (a step of 2^-24 there)."""
+    g = torch.Generator().manual_seed(dim)
+    lengths = [70, 1, 333]
+    table, pool, _ = make_table(g, lengths, 16)
+    cache = make_cache(g, pool, 16, 2, dim, kv)
+    cache[3 if kv == "q8_0" else 1].mul_(2.0 ** size)
+    query = (2 * torch.randn(3, 8, dim, generator=g)).to(TYPES[q]).cuda()
+    out = torch.empty(3, 8, dim, dtype=torch.bfloat16 if q == "f16" else TYPES[q], device="cuda")
+    v = values(cache[1], cache[3])
+    want, _, bound = attend(query, values(cache[0], cache[2]), v, table, lengths, 1 / math.sqrt(dim))
+    serving.PagedCache(dev, *cache).attend(query, table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), out=out)
+    close(out, want, bound + (SPLIT[kv] if q != "f32" else 0.0) * v.abs().max())
+
+
+def test_blocks_past_the_scale(dev):
+    """An 8-bit block whose scale is past f16's range reads as NaN, its neighbours as they are."""
+    g = torch.Generator().manual_seed(1)
+    cache = make_cache(g, 2, 16, 1, 64, "q8_0")
+    c = serving.PagedCache(dev, *cache)
+    table, n = torch.tensor([[1]], dtype=torch.int32).cuda(), torch.tensor([3], dtype=torch.int32).cuda()
+    new = torch.randn(2, 3, 1, 64, generator=g)
+    new[1, 1, 0, 40] = 9e6
+    new[1, 2, 0, 41] = -8.3e6  # 65,354 x 127
+    c.append(new[0].cuda(), new[1].cuda(), table, n, torch.tensor([0, 3], dtype=torch.int32).cuda())
+    for q in (torch.zeros(1, 2, 64, device="cuda"), torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")):
+        out = c.attend(q, table, n).cpu()
+        assert torch.isfinite(out[..., :32]).all() and out[..., 32:].isnan().all()
