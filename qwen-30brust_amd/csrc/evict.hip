@@ -22,11 +22,12 @@ constexpr uint32_t kSelBlock = 1024, kSelWaves = kSelBlock / 64;
 // keys on every call.  A sequence with a length or page out of range keeps nothing.
 // The length is read once a workgroup, and a place is compared with `keep` before it
 // is written: weights or lengths that change meanwhile choose wrong keys, no more.
-// Bound by one compute unit's issue rate, some 20 operations a key, and by the
-// steps between the passes: 50 us for 8,192 of 65,537 keys (4 heads), 15 us for
-// 1,024 of up to 4,096 (16 sequences).  Reading the next span ahead changes nothing;
-// with every key's place looked at 62 and 17, with one copy of the counts and 8
-// rounds, whose weights do not fit the registers, 91 and 30.
+// One workgroup a head is simple and needs no workspace; a long history pays for it
+// with all but a few compute units idle, and is bound by one unit's issue rate, some
+// 20 operations a key, and by the steps between the passes: 51 us for 8,192 of 65,537
+// keys (4 heads), 15 us for 1,024 of up to 4,096 (16 sequences).  Reading the next
+// span ahead changes nothing; with every key's place looked at 62 and 17, with one
+// copy of the counts and 8 rounds, whose weights do not fit the registers, 91 and 30.
 constexpr uint32_t kSelPer = 4, kSelRound = kSelBlock * kSelPer, kSelRounds = 4, kSelSpan = kSelRound * kSelRounds;
 constexpr uint32_t kBins = 2048, kCopies = 8;  // copies of a count, for lanes that hit the same one
 
@@ -192,8 +193,8 @@ __global__ __launch_bounds__(kSelBlock) void k_page_select(PageEvict a) {
 // Moves the kept keys' rows: a workgroup per kMoveKeys of them, `lanes` lanes (a
 // power of two) with B bytes each a row, K and V of several rows in flight.  B is
 // 16 where rows are aligned so, else an element; the work is two dependent
-// look-ups (kept, then the page; both compared with their ranges once more) and a copy, 7.6 us for 8,192 keys of four heads
-// of 128 in bf16 (33.5 MB moved, 4.4 TB/s) and 12.5 us for 16 sequences' 1,024;
+// look-ups (kept, then the page; both compared with their ranges once more) and a copy, 8.0 us for 8,192 keys of four heads
+// of 128 in f16 (33.5 MB moved, 4.2 TB/s) and 13.1 us for 16 sequences' 1,024;
 // 13.8 and 27.6 with an element a lane.
 template <uint32_t B> struct Bytes;
 template <> struct Bytes<16> { typedef uint4 type; };

@@ -169,7 +169,7 @@ template <uint32_t L> __global__ __launch_bounds__(kBlock) void k_page_append(Pa
 }
 
 // Any other width up to 256 and alignment: a wave per token and head, every 64th
-// value to a lane.
+// value to a lane.  2,001 tokens of 32 + 2 x 4 heads of 96 take 47 us.
 __global__ __launch_bounds__(kBlock) void k_page_append_any(PageAppend a) {
     constexpr uint32_t E = kPageMaxDim / 64;
     __shared__ float turn[kWaves][kPageMaxDim];
@@ -437,9 +437,9 @@ template <uint32_t K> __device__ __forceinline__ f4 row4(const uint8_t* p, size_
 // One query head, any head width up to 8 E: eight lanes share a key, with every
 // eighth four elements of its row each, and keep the (m, l, o) of their own keys, so
 // there is no barrier before the merge at the end.  Every query head reads its keys
-// again, from L2: 48 ragged histories of width 96, eight heads a KV head, 290 us in
-// bf16 (743 with an element a load), some seven times what k_page_attn16 takes for
-// width 128.
+// again, from L2: 48 ragged histories of up to 4,096 keys of width 96, eight heads a KV
+// head, 316 us in bf16 (2.5 times that with an element a load), some seven times what
+// k_page_attn16 takes for width 128.
 template <uint32_t K, int E>
 __global__ __launch_bounds__(kBlock) void k_page_attn_any(PageAttn a) {
     __shared__ float red[kWaves][8 * E], rm[kWaves], rl[kWaves];
@@ -974,11 +974,11 @@ __global__ __launch_bounds__(64, 2) void k_page_attn16(PageAttn a) {
 // that memory takes for the rows (2,048 matrix-core cycles for 16 KB of f32 rows,
 // which take a compute unit's share of the bandwidth about 8,000).  One history of
 // 517 f32 keys takes 10 us, the latency of its look-ups and rows; 48 ragged ones of
-// up to 4,096 keys 71 us (403 MB, 5.7 TB/s); the same in bf16 or f16 with a 32-bit
-// output 70 us where k_page_attn16 takes 46, 75 over Q8_0 against 48 (whole calls).
-// Heads of 256 take one wave a SIMD for their registers: the same 48 histories 149 us
-// in f32 (805 MB), 141 in bf16, where the products bound it (1,263 on
-// k_page_attn_any).
+// up to 4,096 keys 72 us (403 MB, 5.6 TB/s), f32 queries over f16 or bf16 65, over
+// Q8_0 67.  16-bit queries with a 32-bit output 70 us where k_page_attn16 takes 46, 75
+// over Q8_0 against 48 (whole calls).  Heads of 256 take one wave a SIMD for their
+// registers: the same 48 histories 155 us in f32 (805 MB), 138 in bf16, where the
+// products bound it (nine times that on k_page_attn_any).
 template <uint32_t K, int D>
 __global__ __launch_bounds__(64, D == 256 ? 1 : 2) void k_page_attn32(PageAttn a) {
     constexpr int NC = D / 16, NV = D / 64;  // 16-dim loads of a key, 64-dim loads of a value
