@@ -5,7 +5,7 @@ import importlib
 import pytest
 import torch
 
-from test_serving import A, cache, evict, message, seqs
+from test_serving import evict, message, seqs
 
 engine = importlib.import_module("qwen-30brust_amd")
 serving = importlib.import_module("qwen-30brust_amd.serving")
