@@ -341,8 +341,9 @@ int qh_bench_read(qh_ctx *ctx, size_t bytes, size_t copies, size_t iters, qh_mat
 /* ---- operators on device tensors --------------------------------------- *
  * For a program that serves several sequences from device memory of its own
  * (no counterpart in the reference, which holds one sequence): a key-value
- * cache in pages (append, attention of one new token per sequence, eviction)
- * and the log probabilities of tokens.  They allocate nothing and keep nothing;
+ * cache in pages (append, attention of new tokens, eviction; pages given out and
+ * taken back; drafted tokens attended and accepted) and the log probabilities of
+ * tokens.  They allocate nothing and keep nothing;
  * what they read and write is device memory of the context's device.
  *
  *   - element kinds: 0 F32, 1 F16, 30 BF16 (GGML's ids), and in a cache 8 Q8_0;
@@ -474,6 +475,88 @@ int qh_paged_evict(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *s
                    size_t weight_row, size_t weight_head, size_t keep, size_t first, size_t recent, const int32_t *to,
                    size_t to_stride, size_t to_pages, int32_t *kept, float *kept_weights, int32_t *new_length,
                    void *stream);
+
+/* Attention of several new tokens per sequence, packed: sequence b's are rows
+ * first[b] .. first[b + 1] - 1 of q and out ([n][heads][dim]), and their keys are
+ * the last of its length[b] keys (appended before).  Token i of m new ones sees the
+ * keys up to its own, length - m + i: a whole prompt, the next piece of one, or a
+ * single token.  Formula, types, sums and what is out of range as in
+ * qh_paged_attention, but: a row gives NaN where one of the keys that it sees is in a
+ * page out of range; the rows of a sequence whose length is out of range or below its
+ * new tokens give NaN; rows of no sequence (in front of first[0], behind first[batch],
+ * or of a sequence whose bounds do not ascend within 0 .. n) are left as they were.
+ * Keys and values that a row does not see take no part in it, whatever they hold. */
+int qh_paged_prompts(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,
+                     const qh_heads_t *q, uint32_t heads, float scale, const qh_heads_t *out, void *workspace,
+                     size_t workspace_bytes, void *stream);
+/* The same for drafted tokens: a sequence's new tokens are the nodes of a tree, at
+ * most 64 (more give NaN), and node i sees every key in front of them and the key of
+ * node j where bit j of ancestors[i] ([n]) is set (its own bit, too, is the caller's;
+ * bits at or past the number of nodes are ignored).  A row that sees no key gives
+ * zeros; one page out of range gives NaN in all of its sequence's rows. */
+int qh_paged_tree(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,
+                  const uint64_t *ancestors, const qh_heads_t *q, uint32_t heads, float scale, const qh_heads_t *out,
+                  void *workspace, size_t workspace_bytes, void *stream);
+/* Bytes of workspace that either call needs for these shapes. */
+int qh_paged_prompts_bytes(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, size_t n, uint32_t heads,
+                           size_t *out);
+
+/* Pages of `page` slots each: the ids free[0 .. count[0]) are in no table, the last
+ * of them is the next to go.  Both lie in device memory and are the caller's; free
+ * has room for `pages` ids. */
+typedef struct {
+    int32_t *free, *count;
+    uint64_t pages;
+    uint32_t page;
+} qh_pool_t;
+
+/* What a plan gives out; first and length are needed.  The others are [n], a row for
+ * each new token, packed as first says, and may be NULL; -1 (ancestors: 0) behind the
+ * last token. */
+typedef struct {
+    int32_t *length;     /* [batch] new lengths; may be the lengths read */
+    int32_t *first;      /* [batch + 1] new tokens in front of each sequence's, and in all */
+    int64_t *slot;       /* page id * page + slot within it */
+    int32_t *position;   /* the token's place; with parents its depth behind the context */
+    int32_t *sequence;
+    uint64_t *ancestors; /* with parents: the token's own bit and its ancestors' */
+} qh_plan_t;
+
+/* Grows sequences by grow[b] tokens (shrinks them where it is negative): table rows
+ * ([batch][table_pages], table_stride apart) of which held[b] entries are in use get
+ * pages from the pool, or give those back that the new length does not need, all in
+ * place.  Pages that are given back may go to a sequence that grows in the same call.
+ * Growth is served in the sequences' order, and from the first on that asks for more
+ * pages than are left, or brings the new tokens past n, no sequence grows: it keeps
+ * its length and gets no tokens (first tells).  So does one whose length, held pages or
+ * new length are out of range (of 0 .. table_pages * page).  Pages go out from the
+ * stack's end, in order of sequence and place, and come back in the opposite order,
+ * so that what is claimed and given back leaves the stack as it was.
+ * parents (nullable, [n], packed as the tokens are): each sequence's new tokens are a
+ * tree, parents[i] the number (within its sequence) of i's parent, -1 for a root; what
+ * is no earlier node counts as -1, and nodes from the 64th on get no ancestors and
+ * their place as position. */
+int qh_paged_plan(qh_ctx *ctx, const qh_pool_t *pool, int32_t *table, size_t table_stride, size_t table_pages,
+                  int32_t *held, const int32_t *length, const int32_t *grow, uint32_t batch, size_t n,
+                  const int32_t *parents, const qh_plan_t *out, void *stream);
+
+/* Accepts drafted tokens: sequence b's new tokens (the last keys of its length[b], as
+ * in qh_paged_tree) are a tree with its root in front (node 0, a token that is
+ * certain), parents and tokens ([n]) as drafted, chosen[i] the model's choice after
+ * node i.  From the root on the walk goes to the first later node whose parent is the
+ * node reached and whose token is the one chosen there.  The nodes reached are
+ * accepted: their keys and values move, in all `layers` caches (of one shape, kind and
+ * strides, with the same tables), to the slots behind the context, in order.
+ * Outputs: new_length[batch] = length - nodes + accepted; accepted[batch] (root
+ * included); path[n]: the accepted nodes' numbers from the sequence's first row on, -1
+ * in all other rows; next[batch] = chosen at the last of them.  A sequence without
+ * nodes, with more than 64, or whose length, bounds or pages (those of its nodes) are
+ * out of range: length as it was, 0 accepted, next -1, nothing moves.  No output may
+ * lie where the call reads, and no two sequences hold the same page. */
+int qh_paged_accept(qh_ctx *ctx, const qh_pages_t *caches, size_t layers, const qh_sequences_t *seqs,
+                    const int32_t *first, size_t n, const int32_t *parents, const int32_t *tokens,
+                    const int32_t *chosen, int32_t *new_length, int32_t *accepted, int32_t *path, int32_t *next,
+                    void *stream);
 
 /* Rows of logits ([rows][vocab], row_stride) of F32, F16 or BF16: logp[rows] =
  * log softmax at target[rows] (both nullable), entropy[rows] (nullable), and the

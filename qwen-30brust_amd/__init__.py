@@ -79,6 +79,14 @@ class _KeyWeights(C.Structure):
                 ("before_head", C.c_size_t), ("after_row", C.c_size_t), ("after_head", C.c_size_t)]
 
 
+class _Pool(C.Structure):
+    _fields_ = [("free", C.c_void_p), ("count", C.c_void_p), ("pages", C.c_uint64), ("page", C.c_uint32)]
+
+
+class _Plan(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("length", "first", "slot", "position", "sequence", "ancestors")]
+
+
 NULL_STREAM = C.c_void_p(-1).value  # QH_NULL_STREAM
 
 _SIGS = {
@@ -154,6 +162,20 @@ _SIGS = {
     "qh_paged_evict": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.c_void_p, C.c_size_t,
                                  C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t,
                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "qh_paged_prompts": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.c_void_p, C.c_size_t,
+                                   C.POINTER(_Heads), C.c_uint32, C.c_float, C.POINTER(_Heads), C.c_void_p,
+                                   C.c_size_t, C.c_void_p]),
+    "qh_paged_tree": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.c_void_p, C.c_size_t,
+                                C.c_void_p, C.POINTER(_Heads), C.c_uint32, C.c_float, C.POINTER(_Heads), C.c_void_p,
+                                C.c_size_t, C.c_void_p]),
+    "qh_paged_prompts_bytes": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.POINTER(_Sequences), C.c_size_t, C.c_uint32,
+                                         C.POINTER(C.c_size_t)]),
+    "qh_paged_plan": (C.c_int, [C.c_void_p, C.POINTER(_Pool), C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p,
+                                C.c_void_p, C.c_void_p, C.c_uint32, C.c_size_t, C.c_void_p, C.POINTER(_Plan),
+                                C.c_void_p]),
+    "qh_paged_accept": (C.c_int, [C.c_void_p, C.POINTER(_Pages), C.c_size_t, C.POINTER(_Sequences), C.c_void_p,
+                                  C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                  C.c_void_p, C.c_void_p]),
     "qh_logprobs": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p,
                               C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                               C.c_size_t, C.c_void_p]),

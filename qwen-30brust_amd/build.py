@@ -28,7 +28,7 @@ HIP_FLAGS = [
     "-I", os.path.join(ROOT, "include"),
 ]
 ENGINE_SOURCES = ["kernels.hip", "matvec.hip", "step.hip", "decode.hip", "prefill.hip", "sample.hip", "paged.hip",
-                  "evict.hip", "logprobs.hip", "engine.hip", "gguf.cpp"]
+                  "evict.hip", "prompts.hip", "pool.hip", "accept.hip", "logprobs.hip", "engine.hip", "gguf.cpp"]
 
 
 def _run(cmd):

@@ -2791,6 +2791,198 @@ int qh_paged_evict(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seq
     });
 }
 
+namespace {
+
+// `first` NULL only without rows
+PageMany many_of(const qh_pages_t* cache, const qh_sequences_t* seqs, size_t n, uint32_t heads) {
+    PageMany a{};
+    a.c = pages_of(cache);
+    a.r = rows_of(seqs, a.c);
+    need_heads(heads, a.c.kvheads);
+    if (n > (1u << 24)) throw Error("at most 16777216 tokens");
+    if ((uint64_t)n * heads > 0x7fffffffu) throw Error("too many tokens and heads");
+    a.n = (uint32_t)n;
+    a.heads = heads;
+    return a;
+}
+
+int attend_many(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, const int32_t* first, size_t n,
+                const uint64_t* ancestors, bool tree, const qh_heads_t* q, uint32_t heads, float scale,
+                const qh_heads_t* out, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded(c, [&] {
+        PageMany a = many_of(cache, seqs, n, heads);
+        a.q = heads_of(q, n, heads, "queries");
+        a.out = heads_of(out, n, heads, "attention outputs");
+        a.scale = scale;
+        if (!n || !a.r.batch) return;
+        need_ptr(first, 4, "first tokens");
+        a.first = first;
+        if (tree) need_ptr(ancestors, 8, "ancestors");
+        a.seen = ancestors;
+        need_ctx(c);
+        const OnDevice on(c->device);
+        launch_page_many(a, stream_of(c, stream));
+        launched(c, stream);
+    });
+}
+
+}  // namespace
+
+int qh_paged_prompts_bytes(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, size_t n, uint32_t heads,
+                           size_t* out) {
+    return guarded(c, [&] {
+        if (!out) throw Error("null output buffer");
+        many_of(cache, seqs, n, heads);
+        *out = 0;
+    });
+}
+
+int qh_paged_prompts(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, const int32_t* first, size_t n,
+                     const qh_heads_t* q, uint32_t heads, float scale, const qh_heads_t* out, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    return attend_many(c, cache, seqs, first, n, nullptr, false, q, heads, scale, out, workspace, workspace_bytes, stream);
+}
+
+int qh_paged_tree(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, const int32_t* first, size_t n,
+                  const uint64_t* ancestors, const qh_heads_t* q, uint32_t heads, float scale, const qh_heads_t* out,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+    return attend_many(c, cache, seqs, first, n, ancestors, true, q, heads, scale, out, workspace, workspace_bytes, stream);
+}
+
+int qh_paged_plan(qh_ctx* c, const qh_pool_t* pool, int32_t* table, size_t table_stride, size_t table_pages,
+                  int32_t* held, const int32_t* length, const int32_t* grow, uint32_t batch, size_t n,
+                  const int32_t* parents, const qh_plan_t* out, void* stream) {
+    return guarded(c, [&] {
+        if (!pool) throw Error("null pool");
+        if (!out) throw Error("null plan");
+        if (!pool->pages || !pool->page) throw Error("empty pool");
+        if (pool->pages > 0x7fffffffu) throw Error("too many pages");
+        if (pool->page > (1u << 30)) throw Error("page size out of range");
+        if (batch > 65535) throw Error("at most 65535 sequences");
+        if (n > (1u << 24)) throw Error("at most 16777216 tokens");
+        need_ptr(pool->free, 4, "free pages");
+        need_ptr(pool->count, 4, "count of free pages");
+        need_ptr(out->first, 4, "first tokens");
+        if (batch) {
+            if (!table_pages) throw Error("empty page table");
+            need_ptr(table, 4, "page table");
+            need_ptr(held, 4, "held pages");
+            need_ptr(length, 4, "lengths");
+            need_ptr(grow, 4, "growth");
+            need_ptr(out->length, 4, "new lengths");
+            need_extent({{batch, table_stride}, {table_pages, 1}}, "page table");
+            if (batch > 1 && table_stride < table_pages) throw Error("the page table's rows overlap");
+            if (table_pages > 0x7fffffffu / batch) throw Error("page table out of range");
+            if ((unsigned __int128)table_pages * pool->page > 0x7fffffffu - (1u << 20)) throw Error("the page table's rows hold too many keys");
+        }
+        if (n) {
+            if (out->slot) need_ptr(out->slot, 8, "slots");
+            if (out->position) need_ptr(out->position, 4, "positions");
+            if (out->sequence) need_ptr(out->sequence, 4, "token sequences");
+            if (parents) need_ptr(parents, 4, "parents");
+            if (out->ancestors) need_ptr(out->ancestors, 8, "ancestors");
+            if (out->ancestors && !parents) throw Error("ancestors go with parents");
+        }
+        const uint64_t rows = batch, in_table = rows ? ((rows - 1) * table_stride + table_pages) * 4 : 0;
+        auto bytes = [](const void* p, uint64_t each) { return p ? each : 0; };
+        const bool in_place = out->length == length;
+        need_apart({{out->length, rows * 4, "new lengths"},
+                    {out->first, rows * 4 + 4, "first tokens"},
+                    {out->slot, bytes(out->slot, n * 8), "slots"},
+                    {out->position, bytes(out->position, n * 4), "positions"},
+                    {out->sequence, bytes(out->sequence, n * 4), "token sequences"},
+                    {out->ancestors, bytes(out->ancestors, n * 8), "ancestors"},
+                    {table, in_table, "page table"},
+                    {held, rows * 4, "held pages"},
+                    {pool->free, pool->pages * 4, "free pages"},
+                    {pool->count, 4, "count of free pages"}},
+                   {{length, in_place ? 0 : rows * 4, "lengths"},
+                    {grow, rows * 4, "growth"},
+                    {parents, bytes(parents, n * 4), "parents"}});
+        need_ctx(c);
+        PagePlan a{};
+        a.free = pool->free;
+        a.count = pool->count;
+        a.pages = (uint32_t)pool->pages;
+        a.page = pool->page;
+        a.table = table;
+        a.stride = table_stride;
+        a.table_pages = (uint32_t)table_pages;
+        a.batch = batch;
+        a.held = held;
+        a.length = length;
+        a.grow = grow;
+        a.new_length = out->length;
+        a.first = out->first;
+        a.n = (uint32_t)n;
+        a.slot = out->slot;
+        a.position = out->position;
+        a.sequence = out->sequence;
+        a.parent = n ? parents : nullptr;
+        a.seen = out->ancestors;
+        const OnDevice on(c->device);
+        launch_page_plan(a, stream_of(c, stream));
+        launched(c, stream);
+    });
+}
+
+int qh_paged_accept(qh_ctx* c, const qh_pages_t* caches, size_t layers, const qh_sequences_t* seqs,
+                    const int32_t* first, size_t n, const int32_t* parents, const int32_t* tokens,
+                    const int32_t* chosen, int32_t* new_length, int32_t* accepted, int32_t* path, int32_t* next,
+                    void* stream) {
+    return guarded(c, [&] {
+        if (!layers) throw Error("no caches");
+        PageAccept a{};
+        a.c = pages_of(caches);
+        a.r = rows_of(seqs, a.c);
+        for (size_t i = 1; i < layers; i++) {
+            const Pages p = pages_of(caches + i);
+            if (p.kind != a.c.kind || p.page != a.c.page || p.kvheads != a.c.kvheads || p.dim != a.c.dim ||
+                p.count != a.c.count || p.ps != a.c.ps || p.ts != a.c.ts || p.hs != a.c.hs)
+                throw Error("caches differ in shape, kind or strides");
+        }
+        if (n > (1u << 24)) throw Error("at most 16777216 tokens");
+        if (!a.r.batch) return;
+        need_ptr(first, 4, "first tokens");
+        if (n) {
+            need_ptr(parents, 4, "parents");
+            need_ptr(tokens, 4, "drafted tokens");
+            need_ptr(chosen, 4, "chosen tokens");
+            need_ptr(path, 4, "path");
+        }
+        need_ptr(new_length, 4, "new lengths");
+        need_ptr(accepted, 4, "accepted counts");
+        need_ptr(next, 4, "next tokens");
+        const uint64_t rows = a.r.batch;
+        need_apart({{new_length, rows * 4, "new lengths"}, {accepted, rows * 4, "accepted counts"},
+                    {path, n * 4, "path"}, {next, rows * 4, "next tokens"}},
+                   {{a.r.length, rows * 4, "lengths"},
+                    {a.r.table, a.r.most ? ((rows - 1) * a.r.stride + seqs->table_pages) * 4 : 0, "page table"},
+                    {first, rows * 4 + 4, "first tokens"},
+                    {parents, n * 4, "parents"}, {tokens, n * 4, "drafted tokens"}, {chosen, n * 4, "chosen tokens"}});
+        need_ctx(c);
+        a.first = first;
+        a.n = (uint32_t)n;
+        a.parent = parents;
+        a.token = tokens;
+        a.chosen = chosen;
+        a.new_length = new_length;
+        a.accepted = accepted;
+        a.path = path;
+        a.next = next;
+        const OnDevice on(c->device);
+        for (size_t done = 0; done < layers; done += a.layers) {
+            a.layers = (uint32_t)std::min<size_t>(layers - done, kAcceptLayers);
+            for (uint32_t i = 0; i < a.layers; i++) {
+                const Pages p = pages_of(caches + done + i);
+                a.layer[i] = {p.k, p.v, p.ks, p.vs};
+            }
+            launch_page_accept(a, stream_of(c, stream));
+        }
+        launched(c, stream);
+    });
+}
+
 int qh_logprobs_bytes(qh_ctx* c, size_t rows, size_t vocab, size_t top, size_t* out) {
     return guarded(c, [&] {
         if (!out) throw Error("null output buffer");

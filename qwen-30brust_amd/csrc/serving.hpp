@@ -1,6 +1,6 @@
 // Argument blocks and launch helpers of the operators on device tensors
-// (paged.hip, evict.hip, logprobs.hip): a key-value cache held in pages and the
-// log probabilities of tokens.
+// (paged.hip, evict.hip, prompts.hip, pool.hip, accept.hip, logprobs.hip): a
+// key-value cache held in pages and the log probabilities of tokens.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -104,6 +104,56 @@ struct PageEvict {
     int32_t* length;       // [batch] keys kept
 };
 void launch_page_evict(const PageEvict& a, hipStream_t s);
+
+// Attention of several tokens per sequence, packed: sequence b's are rows
+// first[b] .. first[b + 1] - 1 of q and out, the last of its keys their own.
+struct PageMany {
+    Pages c;
+    Rows r;
+    const int32_t* first;  // [batch + 1]
+    uint32_t n;            // rows of q and out
+    const uint64_t* seen;  // [n] bit j: the sequence's new token j is seen; null: those up to the token's own
+    Heads q, out;
+    uint32_t heads;
+    float scale;
+};
+void launch_page_many(const PageMany& a, hipStream_t s);
+
+// Pages from and to a stack of free ones, and what the new tokens need.
+struct PagePlan {
+    int32_t *free, *count;  // [pages] ids, the first count[0] of them free
+    uint32_t pages, page;
+    int32_t* table;
+    size_t stride;
+    uint32_t table_pages, batch;
+    int32_t* held;          // [batch] pages of each table row
+    const int32_t *length, *grow;
+    int32_t *new_length, *first;
+    uint32_t n;             // rows of what follows
+    int64_t* slot;          // page * `page` + slot, or null
+    int32_t *position, *sequence;  // or null
+    const int32_t* parent;  // [n], or null
+    uint64_t* seen;         // [n], with parent
+};
+void launch_page_plan(const PagePlan& a, hipStream_t s);
+
+// The walk down trees of drafted tokens, and the accepted ones' move.
+constexpr uint32_t kTreeMost = 64;         // nodes of a tree
+constexpr uint32_t kAcceptLayers = 64;     // caches of a launch
+struct PageAccept {
+    Pages c;  // of every cache, but the pointers
+    Rows r;
+    const int32_t* first;
+    uint32_t n;
+    const int32_t *parent, *token, *chosen;
+    int32_t *new_length, *accepted, *path, *next;
+    uint32_t layers;
+    struct {
+        uint8_t *k, *v;
+        _Float16 *ks, *vs;
+    } layer[kAcceptLayers];
+};
+void launch_page_accept(const PageAccept& a, hipStream_t s);
 
 struct Logprobs {
     const void* x;

@@ -1,7 +1,9 @@
 """Operators on torch tensors of the GPU, for a program that serves several
-sequences: a key-value cache held in pages (`PagedCache`: append, attend, evict)
-and the log probabilities of tokens (`logprobs`), over the C ABI's entry points
-for device tensors (include/qwen_hip.h: qh_paged_*, qh_logprobs).
+sequences: a key-value cache held in pages (`PagedCache`: append, attend,
+attend_prompts, attend_tree, evict), pages given out and taken back (`PagePool`),
+drafted tokens accepted (`accept`) and the log probabilities of tokens
+(`logprobs`), over the C ABI's entry points for device tensors
+(include/qwen_hip.h: qh_paged_*, qh_logprobs).
 
 Every call runs on torch's current stream of the tensors' device, which is the
 given engine Device's, returns at once, and may be captured into a graph.  What
@@ -13,6 +15,7 @@ one is refused where torch records gradients (call under torch.no_grad()).
 
     serving = importlib.import_module("qwen-30brust_amd.serving")
 """
+import collections
 import ctypes as C
 import importlib
 
@@ -210,6 +213,48 @@ class PagedCache:
                                           w, None if work is None else work.data_ptr(), need.value, _stream(dev)))
         return out if w is None else (out, weights_out)
 
+    def attend_prompts(self, q, table, lengths, first, most=None, *, scale=None, out=None):
+        """Causal attention of several new tokens per sequence, q
+        [n][heads][dim]: sequence b's are rows first[b] .. first[b + 1] - 1, the
+        last of its `lengths[b]` keys (appended before) their own, and each sees
+        the keys up to its own.  A whole prompt, the next piece of one, or a single
+        token.  out like q (allocated if not given); rows of no sequence are left as
+        they were.  most and scale as in attend."""
+        return self._many(q, table, lengths, first, None, most, scale, out)
+
+    def attend_tree(self, q, table, lengths, first, ancestors, most=None, *, scale=None, out=None):
+        """attend_prompts for drafted tokens: a sequence's new tokens are the nodes
+        of a tree (at most 64), and node i sees every key in front of them and
+        the key of node j where bit j of ancestors[i] ([n], int64) is set."""
+        _on(self.device, ancestors, "ancestors", (torch.int64,), 1)
+        return self._many(q, table, lengths, first, ancestors, most, scale, out)
+
+    def _many(self, q, table, lengths, first, ancestors, most, scale, out):
+        dev, d = self.device, self.dim
+        seqs = self._sequences(table, lengths, most)
+        n, heads = q.shape[:2] if isinstance(q, torch.Tensor) and q.dim() == 3 else (0, 0)
+        qh = _heads(dev, q, "queries", n, heads, d)
+        _on(dev, first, "first tokens", _I32, 1)
+        _need(first.shape[0] == lengths.shape[0] + 1, "first tokens: one more than sequences is needed")
+        _need(ancestors is None or ancestors.shape[0] == n, "ancestors: one for each token")
+        given = out is not None
+        if not given:
+            out = q.new_empty((n, heads, d))
+        oh = _heads(dev, out, "attention outputs", n, heads, d)
+        if given:
+            _apart(out, "attention outputs")
+        lib, h = engine.lib(), _live(dev)
+        need = _BYTES()
+        dev._check(lib.qh_paged_prompts_bytes(h, self._pages, seqs, n, heads, need))
+        work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        more = (qh, heads, d ** -0.5 if scale is None else scale, oh, None if work is None else work.data_ptr(),
+                need.value, _stream(dev))
+        if ancestors is None:
+            dev._check(lib.qh_paged_prompts(h, self._pages, seqs, first.data_ptr(), n, *more))
+        else:
+            dev._check(lib.qh_paged_tree(h, self._pages, seqs, first.data_ptr(), n, ancestors.data_ptr(), *more))
+        return out
+
     def evict(self, weights, table, lengths, keep, to, *, first=0, recent=0, most=None):
         """Brings sequences to at most `keep` keys: each KV head keeps its first
         `first` keys, its last `recent` and the heaviest between by `weights`
@@ -237,6 +282,96 @@ class PagedCache:
                                                to.shape[1], kept.data_ptr(), kept_weights.data_ptr(), new.data_ptr(),
                                                _stream(dev)))
         return kept, kept_weights, new
+
+
+Plan = collections.namedtuple("Plan", "lengths first slots positions sequences ancestors")
+
+
+class PagePool:
+    """The free pages of caches whose sequences share tables: a stack of page ids
+    on the GPU, free [pages] of which the first count[0] are free (both int32;
+    None: all pages, the lowest goes first).  They stay the caller's."""
+
+    def __init__(self, device, pages, page, *, free=None, count=None):
+        where = torch.device("cuda", device.index)
+        _need(0 < pages < 1 << 31 and 0 < page <= 1 << 30, "pages out of range")
+        _need((free is None) == (count is None), "free pages and their count go together")
+        if free is None:
+            free = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=where)
+            count = torch.full((1,), pages, dtype=torch.int32, device=where)
+        for t, what, n in ((free, "free pages", pages), (count, "count of free pages", 1)):
+            _on(device, t, what, _I32, 1)
+            _need(t.shape[0] == n, f"{what}: {n} are needed")
+            _apart(t, what)
+        self.device, self.pages, self.page, self.free, self.count = device, pages, page, free, count
+        self._pool = engine._Pool(free.data_ptr(), count.data_ptr(), pages, page)
+
+    def plan(self, table, held, lengths, grow, n, *, parents=None, out=None):
+        """Grows sequences by `grow` tokens (shrinks them where it is negative):
+        table [batch][pages] and held [batch], the entries of its rows in use, get pages
+        or give them back in place.  n: room for new tokens; growth ends with the
+        first sequence that does not fit into n or the free pages.  Returns a Plan:
+        lengths [batch] (out, which may be lengths; allocated if not given), first
+        [batch + 1], and for each of n rows, packed by first, slots (int64: page id * page
+        + slot), positions, sequences (-1 behind the last token) and, with parents
+        ([n], a tree per sequence: numbers within it, -1 for a root), ancestors
+        (int64) for attend_tree, positions then counting a node's depth."""
+        dev = self.device
+        (batch, pages), strides = _on(dev, table, "page table", _I32, 2)
+        for t, what in ((held, "held pages"), (lengths, "lengths"), (grow, "growth")):
+            _on(dev, t, what, _I32, 1)
+            _need(t.shape[0] == batch, f"{what}: one for each row of the page table")
+        for t, what in ((table, "page table"), (held, "held pages")):
+            _apart(t, what)
+        _need(0 <= n <= 1 << 24, "new tokens out of range")
+        if parents is not None:
+            _on(dev, parents, "parents", _I32, 1)
+            _need(parents.shape[0] == n, "parents: one for each new token")
+        if out is None:
+            out = torch.empty_like(lengths, memory_format=torch.contiguous_format)
+        else:
+            _on(dev, out, "new lengths", _I32, 1)
+            _need(out.shape[0] == batch, "new lengths: one for each row of the page table")
+            _apart(out, "new lengths")
+        # one allocation: slots, ancestors, first, positions, sequences
+        wide = n * (2 if parents is not None else 1)
+        ints = torch.empty(2 * wide + batch + 1 + 2 * n, dtype=torch.int32, device=table.device)
+        longs, rest = ints[:2 * wide].view(torch.int64), ints[2 * wide:]
+        plan = Plan(out, rest[:batch + 1], longs[:n], rest[batch + 1:batch + 1 + n], rest[batch + 1 + n:],
+                    longs[n:] if parents is not None else None)
+        places = engine._Plan(*(None if t is None else t.data_ptr() for t in plan))
+        dev._check(engine.lib().qh_paged_plan(_live(dev), self._pool, table.data_ptr(), strides[0], pages, held.data_ptr(),
+                                              lengths.data_ptr(), grow.data_ptr(), batch, n,
+                                              None if parents is None else parents.data_ptr(), places, _stream(dev)))
+        return plan
+
+
+def accept(caches, parents, tokens, chosen, table, lengths, first):
+    """Accepts drafted tokens after attend_tree: walks each sequence's tree from its
+    root (its first new token) to the child whose token ([n]) is the one that the model
+    chose ([n]) after the node reached, and moves the accepted nodes' keys and values,
+    in all `caches` (PagedCaches of one shape: a model's layers), to the slots behind
+    the context.  Returns (new lengths, accepted counts, path [n]: accepted nodes'
+    numbers from each sequence's first row on and -1, next tokens)."""
+    caches = list(caches)
+    _need(caches and all(isinstance(c, PagedCache) for c in caches), "a list of caches is needed")
+    dev, cache = caches[0].device, caches[0]
+    _need(all(c.device is dev for c in caches), "caches of several devices")
+    _need(all(c._writable for c in caches), "a cache whose elements share memory is read only")
+    seqs = cache._sequences(table, lengths, None)
+    batch = lengths.shape[0]
+    for t, what in ((parents, "parents"), (tokens, "drafted tokens"), (chosen, "chosen tokens"), (first, "first tokens")):
+        _on(dev, t, what, _I32, 1)
+    n = parents.shape[0]
+    _need(tokens.shape[0] == n and chosen.shape[0] == n, "a drafted and a chosen token for each node")
+    _need(first.shape[0] == batch + 1, "first tokens: one more than sequences is needed")
+    ints = torch.empty(3 * batch + n, dtype=torch.int32, device=table.device)
+    new, accepted, following, path = ints[:batch], ints[batch:2 * batch], ints[2 * batch:3 * batch], ints[3 * batch:]
+    pages = (engine._Pages * len(caches))(*(c._pages for c in caches))
+    dev._check(engine.lib().qh_paged_accept(_live(dev), pages, len(caches), seqs, first.data_ptr(), n, parents.data_ptr(),
+                                            tokens.data_ptr(), chosen.data_ptr(), new.data_ptr(), accepted.data_ptr(),
+                                            path.data_ptr(), following.data_ptr(), _stream(dev)))
+    return new, accepted, path, following
 
 
 def logprobs(device, logits, targets=None, *, top=0, valid=None):
