@@ -2801,6 +2801,9 @@ PageMany many_of(const qh_pages_t* cache, const qh_sequences_t* seqs, size_t n, 
     need_heads(heads, a.c.kvheads);
     if (n > (1u << 24)) throw Error("at most 16777216 tokens");
     if ((uint64_t)n * heads > 0x7fffffffu) throw Error("too many tokens and heads");
+    // the work, in keys times heads, is counted in 64 bits
+    const unsigned __int128 tiles = (unsigned __int128)n * heads / 128 + (uint64_t)a.r.batch * a.c.kvheads;
+    if (tiles * (a.r.most + 1ull) * (heads / a.c.kvheads) * 2 + tiles * 256 >> 62) throw Error("too many tokens, heads and keys");
     a.n = (uint32_t)n;
     a.heads = heads;
     return a;
@@ -2819,6 +2822,9 @@ int attend_many(qh_ctx* c, const qh_pages_t* cache, const qh_sequences_t* seqs, 
         a.first = first;
         if (tree) need_ptr(ancestors, 8, "ancestors");
         a.seen = ancestors;
+        page_many_plan(a, cus_of(c));
+        need_workspace(workspace, workspace_bytes, page_many_bytes(a));
+        a.work = workspace;
         need_ctx(c);
         const OnDevice on(c->device);
         launch_page_many(a, stream_of(c, stream));
@@ -2832,8 +2838,9 @@ int qh_paged_prompts_bytes(qh_ctx* c, const qh_pages_t* cache, const qh_sequence
                            size_t* out) {
     return guarded(c, [&] {
         if (!out) throw Error("null output buffer");
-        many_of(cache, seqs, n, heads);
-        *out = 0;
+        PageMany a = many_of(cache, seqs, n, heads);
+        page_many_plan(a, cus_of(c));
+        *out = a.n && a.r.batch ? page_many_bytes(a) : 0;
     });
 }
 

@@ -116,7 +116,16 @@ struct PageMany {
     Heads q, out;
     uint32_t heads;
     float scale;
+    // by page_many_plan
+    uint32_t group, wide, runs;     // query heads of a KV head, width of the tiles, workgroups
+    bool narrow;                    // products of the cache's own 16-bit type, else of 32 bits
+    bool q_wide, out_wide, kv_wide; // rows aligned to what is read and written at a time
+    uint32_t page_mul, page_shift;  // t / page
+    float sign, c2;                 // scale * log2 e = sign * c2
+    void* work;
 };
+void page_many_plan(PageMany& a, uint32_t cus);
+size_t page_many_bytes(const PageMany& a);  // (aligned to 16)
 void launch_page_many(const PageMany& a, hipStream_t s);
 
 // Pages from and to a stack of free ones, and what the new tokens need.
