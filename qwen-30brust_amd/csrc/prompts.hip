@@ -31,8 +31,10 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef bf16_t b2 __attribute__((ext_vector_type(2)));
+typedef bf16_t b4 __attribute__((ext_vector_type(4)));
 typedef bf16_t b8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32
@@ -218,18 +220,17 @@ struct Run {
 };
 
 // --------------------------------------------------------------- the tiles --
-// Four consecutive values of a row of out.
-__device__ __forceinline__ void put_row(const PageMany& a, uint32_t dim, uint32_t row, uint32_t h, uint32_t d, f4 x) {
-    const size_t at = (size_t)row * a.out.row + (size_t)h * a.out.head + d;
+// Values d .. d + 3 of the row of out at `at`.
+__device__ __forceinline__ void put_row(const PageMany& a, uint32_t dim, size_t at, uint32_t d, f4 x) {
     if (a.out_wide && d + 4 <= dim) {
-        if (a.out.kind == F32) *reinterpret_cast<f4*>(a.out.p + 4 * at) = x;
-        else if (a.out.kind == F16) *reinterpret_cast<__attribute__((ext_vector_type(4))) _Float16*>(a.out.p + 2 * at) = __builtin_convertvector(x, __attribute__((ext_vector_type(4))) _Float16);
-        else *reinterpret_cast<__attribute__((ext_vector_type(4))) bf16_t*>(a.out.p + 2 * at) = __builtin_convertvector(x, __attribute__((ext_vector_type(4))) bf16_t);
+        if (a.out.kind == F32) *reinterpret_cast<f4*>(a.out.p + 4 * (at + d)) = x;
+        else if (a.out.kind == F16) *reinterpret_cast<h4*>(a.out.p + 2 * (at + d)) = __builtin_convertvector(x, h4);
+        else *reinterpret_cast<b4*>(a.out.p + 2 * (at + d)) = __builtin_convertvector(x, b4);
         return;
     }
 #pragma unroll
     for (uint32_t j = 0; j < 4; j++)
-        if (d + j < dim) put_kind(a.out.kind, a.out.p, at + j, x[j]);
+        if (d + j < dim) put_kind(a.out.kind, a.out.p, at + d + j, x[j]);
 }
 
 // The 16-byte chunk of a tile's row that chunk c lies in: rows that are read together
@@ -239,27 +240,40 @@ template <uint32_t CH> __device__ __forceinline__ constexpr uint32_t turn(uint32
     return CH >= 16 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
 
-// T: type of the products; D: width of the tiles, at least the heads'; DIRECT: the
-// cache's rows are T, D wide and aligned to 16 bytes, and go to LDS by themselves.
+// Where a kernel's tiles come from: the cache's rows as they are, by loads that go to LDS
+// by themselves (kDirect: rows of T, D wide, aligned to 16 bytes), or through registers, rows
+// of that kind aligned to 8 values, or of any kind and alignment (kAny; 16 bits: of T).
+constexpr uint32_t kDirect = 100, kAny = 101;
+
+// T: type of the products; D: width of the tiles, at least the heads'.
 //
 // A wave has 32 query rows.  It takes the scores as K Q^T, so that a lane has one
 // row's scores (of the keys 8 i + 4 (lane / 32) + j), its maximum and sum need one
 // exchange, and the weights lie where O^T = V^T P^T wants its second operand: for 16-bit
 // types keys 16 c + 8 (e / 4) + 4 (lane / 32) + e % 4 are element e, for V^T read by the
 // transposing LDS read.  K and V of the next step come in while one is worked on.
-template <class T, uint32_t D, bool DIRECT>
+template <class T, uint32_t D, uint32_t SRC>
 __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany a) {
     constexpr bool F = std::is_same<T, float>::value, H = std::is_same<T, _Float16>::value;
+    constexpr bool DIRECT = SRC == kDirect, Q8 = SRC == Q8_0 && !F;
     constexpr uint32_t KT = F || D == 256 ? 32 : 64;  // keys of a step
-    constexpr uint32_t NS = KT / 32, ND = D / 32, CH = D * sizeof(T) / 16;
+    constexpr uint32_t NS = KT / 32, ND = D / 32, CH = D * sizeof(T) / 16, TILE = KT * D * sizeof(T);
     constexpr uint32_t NQ = F ? D / 2 : D / 16;
+    constexpr uint32_t QKIND = F ? F32 : H && !Q8 ? F16 : BF16;  // of queries that are loaded as they are
     // weights are at most 2^(kAhead + kUp), so that f16 holds them and small ones too
     constexpr float kAhead = 8.f, kUp = H ? 7.f : 0.f;
     typedef typename std::conditional<H, h8, b8>::type T8;
     typedef typename std::conditional<F, float, T8>::type Q;
-    __shared__ __align__(16) uint8_t ks[2][KT * D * sizeof(T)], vs[2][KT * D * sizeof(T)];
+    __shared__ __align__(16) uint8_t lds[4][TILE];  // K, K, V, V; in front and behind a part for each wave
+    __shared__ __align__(16) float scales[Q8 ? 2 : 1][Q8 ? ND : 1][Q8 ? KT : 1];  // of K's blocks
     __shared__ uint32_t bad_at;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wv = same(tid >> 6), n = lane & 31, half = lane >> 5;
+    auto settle = [] {  // what the wave wrote to its own part of LDS can be read
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto shfl64 = [](size_t v, uint32_t from) { return (size_t)__shfl((unsigned long long)v, from, 64); };
     Run run;
     if (!run.start(a)) return;
     do {
@@ -269,64 +283,78 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         const bool whole = run.off == 0 && run.here() == s.cost(run.i);
         const uint32_t hi = same(run.off + run.here() == s.cost(run.i) ? end : key_at(a, run.off + run.here(), end, KT));
         const uint32_t r0 = run.i * kTileRows + wv * 32, r = r0 + n;  // rows of the sequence and KV head
-        const bool mine = r < R;
-        // hidden from the optimiser, that it keeps no comparison with it over the whole loop
-        uint32_t dim = a.c.dim;
-        asm volatile("" : "+s"(dim));
+        const uint32_t rows = r0 >= R ? 0 : min(32u, R - r0);        // of the wave
+        const bool mine = n < rows;
+        const uint32_t dim = a.c.dim;
         const uint32_t token = mine ? r / a.group : 0, row = s.f0 + token, h = run.kv * a.group + (mine ? r % a.group : 0);
+        const size_t to = (size_t)row * a.out.row + (size_t)h * a.out.head;
         if (s.bad) {
             if (run.off == 0 && mine)
-                for (uint32_t d = half * 4; d < dim; d += 8) put_row(a, dim, row, h, d, f4(__builtin_nanf("")));
+                for (uint32_t d = half * 4; d < dim; d += 8) put_row(a, dim, to, d, f4(__builtin_nanf("")));
             continue;
         }
         if (lo >= hi) continue;
-        // keys that all of the wave's rows see, and behind the last that one sees
-        const uint32_t all = r0 >= R ? 0 : a.seen ? s.c0 : s.c0 + r0 / a.group + 1;
-        const uint32_t most = r0 >= R ? 0 : a.seen ? end : s.c0 + min(r0 + 31, R - 1) / a.group + 1;
+        // behind the last key that one of the wave's rows sees
+        const uint32_t most = !rows ? 0 : a.seen ? end : s.c0 + (r0 + rows - 1) / a.group + 1;
         const uint32_t own = a.seen ? end : s.c0 + token + 1;  // behind this row's last
         uint64_t bits = 0;
         if (a.seen && mine) bits = gld<uint64_t>(a.seen + row) & (s.count == 64 ? ~0ull : (1ull << s.count) - 1);
 
         Q q[NQ];
+        float c2 = a.c2;
         {
             const size_t at = (size_t)row * a.q.row + (size_t)h * a.q.head;
-            if constexpr (F) {
-                auto load = [&](auto kind) {
+            constexpr uint32_t each = F ? 4 : 8;  // values of a load: 2 each g + each half + ..
+            u4 x[D / 2 / each];
+            if (a.q_wide && a.q.kind == QKIND) {
 #pragma unroll
-                    for (uint32_t g = 0; g < D / 8; g++)
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) {
-                            const uint32_t d = 8 * g + 4 * half + j;
-                            q[4 * g + j] = mine && d < dim ? elem<kind()>(a.q.p, at + d) * a.sign : 0.f;
-                        }
-                };
-                if (a.q.kind == F16) load(std::integral_constant<uint32_t, F16>());
-                else if (a.q.kind == BF16) load(std::integral_constant<uint32_t, BF16>());
-                else if (!a.q_wide) load(std::integral_constant<uint32_t, F32>());
-                else {
-#pragma unroll
-                    for (uint32_t g = 0; g < D / 8; g++) {
-                        const uint32_t d = 8 * g + 4 * half;
-                        f4 x = {0.f, 0.f, 0.f, 0.f};
-                        if (mine && d < dim) x = gld<f4>(a.q.p + 4 * (at + d)) * a.sign;
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) q[4 * g + j] = x[j];
-                    }
+                for (uint32_t g = 0; g < D / 2 / each; g++) {
+                    const uint32_t d = (2 * g + half) * each;
+                    x[g] = u4{0, 0, 0, 0};
+                    if (mine && d < dim) x[g] = gld<u4>(a.q.p + (F ? 4 : 2) * (at + d));
                 }
+            } else {  // through the wave's part of LDS, a value at a time; 16 bits: of the type of the product
+                uint8_t* part = lds[wv];
+#pragma nounroll
+                for (uint32_t i = lane; i < 32 * D; i += 64) {
+                    const uint32_t d = i % D;
+                    const size_t from = shfl64(at, i / D) + d;
+                    const bool in = i / D < rows && d < dim;
+                    if constexpr (F) reinterpret_cast<float*>(part)[i] = in ? elem_kind(a.q.kind, a.q.p, from) : 0.f;
+                    else reinterpret_cast<uint16_t*>(part)[i] = in ? gld<uint16_t>(a.q.p + 2 * from) : (uint16_t)0;
+                }
+                settle();
+#pragma unroll
+                for (uint32_t g = 0; g < D / 2 / each; g++)
+                    x[g] = *reinterpret_cast<const u4*>(part + (n * D + (2 * g + half) * each) * (F ? 4 : 2));
+                __syncthreads();  // before K and V go there
+            }
+            if constexpr (F) {
+#pragma unroll
+                for (uint32_t i = 0; i < NQ; i++) q[i] = __uint_as_float(x[i / 4][i % 4]) * a.sign;
             } else {
                 const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u, keep = a.sign == 0.f ? 0u : ~0u;
 #pragma unroll
-                for (uint32_t g = 0; g < D / 16; g++) {
-                    const uint32_t d = 16 * g + 8 * half;
-                    u4 x = {0, 0, 0, 0};
-                    if (a.q_wide) {
-                        if (mine && d < dim) x = gld<u4>(a.q.p + 2 * (at + d));
-                    } else {
+                for (uint32_t g = 0; g < NQ; g++) x[g] = (x[g] ^ flip) & keep;
+                if constexpr (Q8) {
+                    // bf16 queries as f16, the row's largest value in [2^14, 2^15): what lies below 2^-38
+                    // of it is lost, what is not finite stays so
+                    uint32_t top = 0;
 #pragma unroll
-                        for (uint32_t j = 0; j < 8; j++)
-                            if (mine && d + j < dim) x[j / 2] |= (uint32_t)gld<uint16_t>(a.q.p + 2 * (at + d + j)) << 16 * (j & 1);
-                    }
-                    q[g] = __builtin_bit_cast(T8, (x ^ flip) & keep);
+                    for (uint32_t g = 0; g < NQ; g++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) top = max(top, max(x[g][j] << 16 & 0x7fff0000u, x[g][j] & 0x7fff0000u));
+                    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64)) >> 23;
+                    const int up = top == 0 || top == 255 ? 0 : 141 - (int)top;
+                    c2 = ldexpf(c2, -up);
+#pragma unroll
+                    for (uint32_t g = 0; g < NQ; g++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            q[g][j] = (T)ldexpf(__uint_as_float(j & 1 ? x[g][j / 2] & 0xffff0000u : x[g][j / 2] << 16), up);
+                } else {
+#pragma unroll
+                    for (uint32_t g = 0; g < NQ; g++) q[g] = __builtin_bit_cast(T8, x[g]);
                 }
             }
         }
@@ -344,86 +372,121 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         // ---- a step's K and V
         const int32_t* table = a.r.table + run.b * a.r.stride;
         const size_t base = run.kv * a.c.hs;
+        auto page_number = [&](uint32_t t) { return (uint32_t)(((uint64_t)t * a.page_mul) >> a.page_shift); };
+        auto page_of = [&](uint32_t t) { return gld<int32_t>(table + page_number(t)); };
         auto place = [&](uint32_t t, int32_t page) {  // of key t; a page out of range is read as page 0
-            const uint32_t in = t - (uint32_t)(((uint64_t)t * a.page_mul) >> a.page_shift) * a.c.page;
             if ((uint32_t)page >= a.c.count) bad = min(bad, t), page = 0;
-            return (size_t)page * a.c.ps + (size_t)in * a.c.ts + base;
+            return (size_t)page * a.c.ps + (size_t)(t - page_number(t) * a.c.page) * a.c.ts + base;
         };
-        auto page_of = [&](uint32_t t) { return gld<int32_t>(table + (uint32_t)(((uint64_t)t * a.page_mul) >> a.page_shift)); };
         // keys behind the tile's last are read as that one: none of them is seen
-        auto key = [&](uint32_t k0, uint32_t row) { return min(k0 + row, end - 1); };
         constexpr uint32_t ROUNDS = KT * D / 8 / kBlock;  // groups of 8 values a thread
-        constexpr uint32_t PER = D / 8;                   // of a row
+        constexpr uint32_t PER = D / 8, LINES = 64 / PER; // of a row; rows of a wave's load
         int32_t pages[ROUNDS];
-        auto group_row = [&](uint32_t r) { return DIRECT ? (r * kWaves + wv) * (64 / PER) + lane / PER : (r * kBlock + tid) / PER; };
+        auto group_row = [&](uint32_t r) { return DIRECT ? (r * kWaves + wv) * LINES + lane / PER : (r * kBlock + tid) / PER; };
+        // the rows of a wave's load lie in one page: its place is computed once for all lanes
+        const bool one_page = DIRECT && a.one_page;
+        auto first_row = [&](uint32_t k0, uint32_t r) { return min(k0 + (r * kWaves + wv) * LINES, (end - 1) / LINES * LINES); };
         auto look = [&](uint32_t k0) {
 #pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; r++) pages[r] = page_of(key(k0, group_row(r)));
+            for (uint32_t r = 0; r < ROUNDS; r++) pages[r] = page_of(one_page ? first_row(k0, r) : min(k0 + group_row(r), end - 1));
         };
         typedef typename std::conditional<F, f4, u4>::type Word;
         constexpr uint32_t WORDS = F ? 2 : 1;
         Word kw[DIRECT ? 1 : ROUNDS][WORDS], vw[DIRECT ? 1 : ROUNDS][WORDS];
-        auto fetch = [&](uint32_t k0, uint32_t buf) {
-#pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; r++) {
-                const uint32_t line = group_row(r);
-                const size_t at = place(key(k0, line), pages[r]);
-                if constexpr (DIRECT) {
+        float kf[Q8 ? ROUNDS : 1];
+        auto to_lds = [&](const uint8_t* k, const uint8_t* v, uint32_t off, uint32_t buf, uint32_t r) {
 #if defined(__HIP_DEVICE_COMPILE__)
-                    const uint32_t c = lane % PER ^ turn<CH>(line);
-                    const uint32_t to = (r * kWaves + wv) * 1024;
-                    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(a.c.k + 2 * at + 16 * c),
-                                                     (__attribute__((address_space(3))) void*)(ks[buf] + to), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(a.c.v + 2 * at + 16 * c),
-                                                     (__attribute__((address_space(3))) void*)(vs[buf] + to), 16, 0, 0);
+            const uint32_t at = (r * kWaves + wv) * 1024;
+            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(k + off),
+                                             (__attribute__((address_space(3))) void*)(lds[buf] + at), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(v + off),
+                                             (__attribute__((address_space(3))) void*)(lds[2 + buf] + at), 16, 0, 0);
 #endif
+        };
+        auto fetch = [&](uint32_t k0, uint32_t buf) {
+            if constexpr (DIRECT) {
+                const uint32_t line = lane / PER;
+                if (one_page) {
+                    constexpr bool SAME = turn<CH>(kWaves * LINES) == 0;  // a row's turn in every round
+#pragma unroll
+                    for (uint32_t r = 0; r < ROUNDS; r++) {
+                        const uint32_t t = same(first_row(k0, r));
+                        const size_t at = place(t, (int32_t)same((uint32_t)pages[r]));
+                        const uint32_t chunk = 16 * (lane % PER ^ turn<CH>((SAME ? wv : r * kWaves + wv) * LINES + line));
+                        const uint32_t in = k0 + KT > end ? min(line, end - 1 - t) : line;
+                        to_lds(a.c.k + 2 * at, a.c.v + 2 * at, in * (uint32_t)a.c.ts * 2 + chunk, buf, r);
+                    }
                 } else {
+#pragma unroll
+                    for (uint32_t r = 0; r < ROUNDS; r++) {
+                        const uint32_t g = group_row(r);
+                        const size_t at = place(min(k0 + g, end - 1), pages[r]);
+                        to_lds(a.c.k + 2 * at, a.c.v + 2 * at, 16 * (lane % PER ^ turn<CH>(g)), buf, r);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (uint32_t r = 0; r < ROUNDS; r++) {
+                    const size_t at = place(min(k0 + group_row(r), end - 1), pages[r]);
                     const uint32_t d = (r * kBlock + tid) % PER * 8;
-                    auto load = [&](const uint8_t* p, const _Float16* sc, Word* w) {
+                    auto load = [&](const uint8_t* p, const _Float16* sc, Word* w, auto is_k) {
                         if (d >= dim) {
                             for (uint32_t i = 0; i < WORDS; i++) w[i] = Word{0, 0, 0, 0};
-                            return;
-                        }
-                        if constexpr (F) {
-                            float x[8];
-                            if (a.kv_wide) {
-                                if (a.c.kind == F32) {
-                                    w[0] = gld<f4>(p + 4 * (at + d)), w[1] = gld<f4>(p + 4 * (at + d) + 16);
-                                    return;
-                                }
-                                if (a.c.kind == Q8_0) {
-                                    const uint2 u = gld<uint2>(p + at + d);
-                                    const float f = (float)gld<_Float16>(sc + (at + d) / 32);
+                            if constexpr (Q8 && is_k()) kf[r] = 0.f;
+                        } else if constexpr (SRC == F32) {
+                            w[0] = gld<f4>(p + 4 * (at + d)), w[1] = gld<f4>(p + 4 * (at + d) + 16);
+                        } else if constexpr (Q8) {
+                            // code + 128 in the low bits of 1024 + 128 + code, less 1152: the code; V's times its
+                            // scale, rounded once
+                            const uint2 u = gld<uint2>(p + at + d);
+                            const _Float16 f1 = gld<_Float16>(sc + (at + d) / 32);
+                            const h2 less = h2((_Float16)1152.f);
+                            if constexpr (is_k()) kf[r] = (float)f1;
 #pragma unroll
-                                    for (int j = 0; j < 8; j++) x[j] = (float)(int8_t)((j < 4 ? u.x : u.y) >> 8 * (j & 3)) * f;
-                                } else {
-                                    const u4 u = gld<u4>(p + 2 * (at + d));
+                            for (int j = 0; j < 4; j++) {
+                                const uint32_t c = (j < 2 ? u.x : u.y) ^ 0x80808080u;
+                                const uint32_t both = __builtin_amdgcn_perm(0x64646464u, c, j & 1 ? 0x07030702u : 0x07010700u);
+                                h2 x = __builtin_bit_cast(h2, both) - less;
+                                if constexpr (!is_k()) x *= h2(f1);
+                                w[0][j] = __builtin_bit_cast(uint32_t, x);
+                            }
+                        } else if constexpr (SRC == Q8_0) {
+                            const uint2 u = gld<uint2>(p + at + d);
+                            const float f = (float)gld<_Float16>(sc + (at + d) / 32);
 #pragma unroll
-                                    for (int j = 0; j < 8; j++) {
-                                        const uint32_t v = j & 1 ? u[j / 2] >> 16 : u[j / 2] & 0xffff;
-                                        x[j] = a.c.kind == F16 ? h2f(v) : __uint_as_float(v << 16);
-                                    }
-                                }
-                            } else {
+                            for (int j = 0; j < 8; j++) w[j / 4][j % 4] = (float)(int8_t)((j < 4 ? u.x : u.y) >> 8 * (j & 3)) * f;
+                        } else if constexpr (SRC == F16 || SRC == BF16) {
+                            const u4 u = gld<u4>(p + 2 * (at + d));
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                const uint32_t v = j & 1 ? u[j / 2] >> 16 : u[j / 2] & 0xffff;
+                                w[j / 4][j % 4] = SRC == F16 ? h2f(v) : __uint_as_float(v << 16);
+                            }
+                        } else if constexpr (F) {
+                            auto each = [&](auto kind) {
 #pragma unroll
                                 for (uint32_t j = 0; j < 8; j++) {
                                     const size_t e = at + min(d + j, dim - 1);
-                                    x[j] = a.c.kind == Q8_0 ? elem<Q8_0>(p, e) * (float)gld<_Float16>(sc + e / 32) : elem_kind(a.c.kind, p, e);
-                                    if (d + j >= dim) x[j] = 0.f;
+                                    float x = elem<kind()>(p, e);
+                                    if constexpr (kind() == Q8_0) x *= (float)gld<_Float16>(sc + e / 32);
+                                    w[j / 4][j % 4] = d + j < dim ? x : 0.f;
                                 }
-                            }
-                            w[0] = {x[0], x[1], x[2], x[3]}, w[1] = {x[4], x[5], x[6], x[7]};
+                            };
+                            if (a.c.kind == F32) each(std::integral_constant<uint32_t, F32>());
+                            else if (a.c.kind == F16) each(std::integral_constant<uint32_t, F16>());
+                            else if (a.c.kind == BF16) each(std::integral_constant<uint32_t, BF16>());
+                            else each(std::integral_constant<uint32_t, Q8_0>());
                         } else if (a.kv_wide) {
                             w[0] = gld<u4>(p + 2 * (at + d));
                         } else {
-                            uint32_t x[8];
+                            w[0] = u4{0, 0, 0, 0};
 #pragma unroll
-                            for (uint32_t j = 0; j < 8; j++) x[j] = d + j < dim ? gld<uint16_t>(p + 2 * (at + d + j)) : 0;
-                            w[0] = {x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16};
+                            for (uint32_t j = 0; j < 8; j++)
+                                if (d + j < dim) w[0][j / 2] |= (uint32_t)gld<uint16_t>(p + 2 * (at + d + j)) << 16 * (j & 1);
                         }
                     };
-                    load(a.c.k, a.c.ks, kw[r]);
-                    load(a.c.v, a.c.vs, vw[r]);
+                    load(a.c.k, a.c.ks, kw[r], std::true_type());
+                    load(a.c.v, a.c.vs, vw[r], std::false_type());
                 }
             }
         };
@@ -432,47 +495,74 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 #pragma unroll
                 for (uint32_t r = 0; r < ROUNDS; r++) {
                     const uint32_t u = r * kBlock + tid, line = u / PER;
+                    if constexpr (Q8)
+                        if (u % PER % 4 == 0) scales[buf][u % PER / 4][line] = kf[r];
 #pragma unroll
                     for (uint32_t w = 0; w < WORDS; w++) {
-                        const uint32_t to = line * D * sizeof(T) + (u % PER * WORDS + w ^ turn<CH>(line)) * 16;
-                        *reinterpret_cast<Word*>(ks[buf] + to) = kw[r][w];
-                        *reinterpret_cast<Word*>(vs[buf] + to) = vw[r][w];
+                        const uint32_t at = line * D * sizeof(T) + ((u % PER * WORDS + w) ^ turn<CH>(line)) * 16;
+                        *reinterpret_cast<Word*>(lds[buf] + at) = kw[r][w];
+                        *reinterpret_cast<Word*>(lds[2 + buf] + at) = vw[r][w];
                     }
                 }
             }
         };
 
         // ---- a step
-        auto step = [&](uint32_t k0, uint32_t buf) {
-            const uint8_t *kt = ks[buf], *vt = vs[buf];
+        // Where the lane reads: of K row n (and 32 on), chunk 2 g + half; of V, by the transposing
+        // read, row (lane % 16) / 4 of four at 16 c + 8 e + 4 half, values 4 (lane % 4) .. + 3 of 16 of
+        // chunks 4 d .. + 3.  Both chunks are turned by their row, so that g, d and e flip bits.
+        const uint32_t k_at = n * D * sizeof(T) + (half ^ turn<CH>(n)) * 16;
+        const uint32_t vrow = 4 * half + lane % 16 / 4;
+        const uint32_t v_at = F ? 4 * half * D * 4 + n % 4 * 4
+                                : vrow * D * 2 + (((lane >> 4 & 1) * 2 + (lane % 4 >> 1)) ^ turn<CH>(vrow)) * 16 + lane % 2 * 8;
+        auto step = [&](uint32_t k0, auto masked, auto buf) {
+            const uint8_t *kt = lds[buf], *vt = lds[2 + buf];
             f16v sc[NS];
 #pragma unroll
             for (uint32_t m = 0; m < NS; m++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) sc[m][j] = 0.f;
-            const uint8_t* krow = kt + n * D * sizeof(T);
-            const uint32_t kturn = turn<CH>(n);
             if constexpr (F) {
 #pragma unroll
                 for (uint32_t g = 0; g < D / 8; g++) {
-                    const f4 x = *reinterpret_cast<const f4*>(krow + ((2 * g + half) ^ opaque(kturn)) * 16);
+                    const f4 x = *reinterpret_cast<const f4*>(kt + (opaque(k_at) ^ g * 32));
 #pragma unroll
                     for (uint32_t j = 0; j < 4; j++) sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], q[4 * g + j], sc[0], 0, 0, 0);
                 }
             } else {
+                auto product = [&](const T8& x, const T8& y, const f16v& z) {
+                    if constexpr (H) return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, z, 0, 0, 0);
+                    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
+                };
+                auto k_part = [&](uint32_t g, uint32_t m) { return *reinterpret_cast<const T8*>(kt + (k_at ^ g * 32) + m * 32 * D * 2); };
+                if constexpr (Q8) {
+                    // a block's codes are exact, its scale is the score's
 #pragma unroll
-                for (uint32_t g = 0; g < D / 16; g++)
+                    for (uint32_t g = 0; g < D / 16; g += 2)
 #pragma unroll
-                    for (uint32_t m = 0; m < NS; m++) {
-                        const T8 x = *reinterpret_cast<const T8*>(krow + m * 32 * D * 2 + ((2 * g + half) ^ kturn) * 16);
-                        if constexpr (H) sc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[g], sc[m], 0, 0, 0);
-                        else sc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[g], sc[m], 0, 0, 0);
-                    }
+                        for (uint32_t m = 0; m < NS; m++) {
+                            f16v x;
+#pragma unroll
+                            for (int j = 0; j < 16; j++) x[j] = 0.f;
+                            x = product(k_part(g, m), q[g], x);
+                            x = product(k_part(g + 1, m), q[g + 1], x);
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; i++) {
+                                const f4 f = *reinterpret_cast<const f4*>(&scales[buf][g / 2][32 * m + 8 * i + 4 * half]);
+#pragma unroll
+                                for (uint32_t j = 0; j < 4; j++) sc[m][4 * i + j] = fmaf(x[4 * i + j], f[j], sc[m][4 * i + j]);
+                            }
+                        }
+                } else {
+#pragma unroll
+                    for (uint32_t g = 0; g < D / 16; g++)
+#pragma unroll
+                        for (uint32_t m = 0; m < NS; m++) sc[m] = product(k_part(g, m), q[g], sc[m]);
+                }
             }
-            // which of the step's keys the row sees, one a bit
-            const bool masked = k0 + KT > all;
-            uint64_t sees = ~0ull;
-            if (masked) {
+            if constexpr (masked()) {
+                // which of the step's keys the row sees, one a bit
+                uint64_t sees = ~0ull;
                 if (a.seen) {
                     const uint32_t d = k0 >= s.c0 ? k0 - s.c0 : s.c0 - k0;
                     if (k0 >= s.c0) sees = d < 64 ? bits >> d : 0;
@@ -487,6 +577,14 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 #pragma unroll
                     for (uint32_t j = 0; j < 16; j++) sc[m][j] = w >> (j / 4 * 8 + j % 4) & 1 ? sc[m][j] : -INFINITY;
                 }
+                uint32_t found = 0;
+                constexpr uint32_t top_bits = F ? 0x7f800000u : H ? 0x7c007c00u : 0x7f807f80u, one = F ? 0x00800000u : H ? 0x04000400u : 0x00800080u;
+                for (uint32_t i = lane; i < KT * CH; i += 64) {
+                    const u4 x = *reinterpret_cast<const u4*>(vt + i * 16);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) found |= (x[j] & top_bits) + one;
+                }
+                if (odd == ~0u && __any((found & (F ? 0x80000000u : 0x80008000u)) != 0)) odd = k0;
             }
             float top = -INFINITY;
 #pragma unroll
@@ -494,7 +592,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 #pragma unroll
                 for (int j = 0; j < 16; j++) top = fmaxf(top, sc[m][j]);
             const float2 t2 = halves(top);
-            top = fmaxf(t2.x, t2.y) * a.c2;
+            top = fmaxf(t2.x, t2.y) * c2;
             // the reference follows the maximum only where that is far above it
             if (__any(top - kUp > M + (F ? 0.f : kAhead))) {
                 const float Mn = fmaxf(M, top - kUp), f = Mn == -INFINITY ? 1.f : exp2_of(M - Mn);
@@ -506,33 +604,23 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     for (int j = 0; j < 16; j++) o[d][j] *= f;
             }
             const float Mf = M == -INFINITY ? 0.f : M;
-            if (masked && odd == ~0u) {
-                uint32_t found = 0;
-                constexpr uint32_t top_bits = F ? 0x7f800000u : H ? 0x7c007c00u : 0x7f807f80u, one = F ? 0x00800000u : H ? 0x04000400u : 0x00800080u;
-#pragma unroll 2
-                for (uint32_t i = lane; i < KT * CH; i += 64) {
-                    const u4 x = *reinterpret_cast<const u4*>(vt + i * 16);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) found |= (x[j] & top_bits) + one;
-                }
-                if (__any((found & (F ? 0x80000000u : 0x80008000u)) != 0)) odd = k0;
-            }
             if constexpr (F) {
                 float p[16];
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    p[j] = exp2_of(fmaf(sc[0][j], a.c2, -Mf));
+                    p[j] = exp2_of(fmaf(sc[0][j], c2, -Mf));
                     L += p[j];
                 }
-                if (odd != ~0u) return;
+                if (masked() && odd != ~0u) return;
 #pragma unroll
                 for (uint32_t j = 0; j < 16; j++) {
-                    const uint32_t line = j / 4 * 8 + 4 * half + j % 4;
+                    // row 8 (j / 4) + 4 half + j % 4
+                    static_assert(!F || CH >= 16, "turn's form");
+                    const uint32_t turned = j % 4 << 2 | j / 4 * 2 % 4;  // and half
                     const uint32_t l = opaque(n);  // computed here: one operation a product is free, registers are not
-                    const uint8_t* v = vt + line * D * 4 + l % 4 * 4;
 #pragma unroll
                     for (uint32_t d = 0; d < ND; d++) {
-                        const float x = *reinterpret_cast<const float*>(v + ((8 * d + l / 4) ^ turn<CH>(line)) * 16);
+                        const float x = *reinterpret_cast<const float*>(vt + v_at + ((8 * d + l / 4) ^ half ^ turned) * 16 + (j / 4 * 8 + j % 4) * D * 4);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[j], o[d], 0, 0, 0);
                     }
                 }
@@ -542,7 +630,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 for (uint32_t m = 0; m < NS; m++)
 #pragma unroll
                     for (uint32_t j = 0; j < 16; j += 2) {
-                        const float x = exp2_of(fmaf(sc[m][j], a.c2, -Mf)), y = exp2_of(fmaf(sc[m][j + 1], a.c2, -Mf));
+                        const float x = exp2_of(fmaf(sc[m][j], c2, -Mf)), y = exp2_of(fmaf(sc[m][j + 1], c2, -Mf));
                         // the sum is of the rounded weights, so that equal errors of all cancel
                         if constexpr (H) {
                             const h2 z = {(_Float16)x, (_Float16)y}, ones = {(_Float16)1.f, (_Float16)1.f};
@@ -554,11 +642,8 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                             p[2 * m + j / 8][j % 8] = z[0], p[2 * m + j / 8][j % 8 + 1] = z[1];
                         }
                     }
-                if (odd != ~0u) return;
-                // lane's part of the transposing read: row (lane % 16) / 4 of four, values
-                // 4 (lane % 4) .. + 3 of 16
+                if (masked() && odd != ~0u) return;
 #if defined(__HIP_DEVICE_COMPILE__)
-                const uint32_t vrow = lane % 16 / 4, col = (lane >> 4 & 1) * 2 + (lane % 4 >> 1);
 #pragma unroll
                 for (uint32_t c = 0; c < 2 * NS; c++)
 #pragma unroll
@@ -566,8 +651,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                         struct { s4 w[2]; } w;
 #pragma unroll
                         for (uint32_t e = 0; e < 2; e++) {
-                            const uint32_t line = 16 * c + 8 * e + 4 * half + vrow;
-                            const uint8_t* v = vt + line * D * 2 + ((4 * d + col) ^ turn<CH>(line)) * 16 + lane % 2 * 8;
+                            const uint8_t* v = vt + (v_at ^ (d * 64 ^ e * 32)) + (16 * c + 8 * e) * D * 2;
                             w.w[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)v);
                         }
                         const T8 x = __builtin_bit_cast(T8, w);
@@ -590,25 +674,29 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         store(0);
         if (lo + KT < hi) look(lo + KT);
         meet();
-        uint32_t buf = 0;
-        for (uint32_t k0 = lo; k0 < hi; k0 += KT, buf ^= 1) {
+        // A step and what comes in meanwhile.  Those that all of the workgroup's rows see whole have
+        // a loop of their own, without masks, in which a buffer's place is a constant.
+        const uint32_t clear = same(min(hi, (a.seen ? s.c0 : s.c0 + run.i * kTileRows / a.group + 1) / KT * KT));
+        auto both = [&](uint32_t k0, auto masked, auto buf) {
             const bool more = k0 + KT < hi;
             if (more) {
                 fetch(k0 + KT, buf ^ 1);
                 if (k0 + 2 * KT < hi) look(k0 + 2 * KT);
             }
-            if (k0 < most) step(k0, buf);
+            if (k0 < most) step(k0, masked, buf);
             if (more) store(buf ^ 1);
             meet();
+        };
+        uint32_t k0 = lo;
+        for (; k0 + 2 * KT <= clear; k0 += 2 * KT) {
+            both(k0, std::false_type(), std::integral_constant<uint32_t, 0>());
+            both(k0 + KT, std::false_type(), std::integral_constant<uint32_t, 1>());
         }
+#pragma nounroll
+        for (uint32_t buf = 0; k0 < hi; k0 += KT, buf ^= 1) both(k0, std::true_type(), buf);
         // the steps left out, a key at a time: its row goes through the wave's part of LDS
+        float* part = reinterpret_cast<float*>(lds[wv]);
         if (odd != ~0u) {
-            float* line = reinterpret_cast<float*>(ks) + wv * 2 * D;
-            auto settle = [] {  // the rows are this wave's own
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            };
             auto value = [&](const uint8_t* p, const _Float16* sc, size_t e) {
                 return a.c.kind == Q8_0 ? elem<Q8_0>(p, e) * (float)gld<_Float16>(sc + e / 32) : elem_kind(a.c.kind, p, e);
             };
@@ -617,8 +705,8 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 const size_t at = place(t, page_of(t));
                 settle();
                 for (uint32_t d = lane; d < D; d += 64) {
-                    line[d] = d < dim ? value(a.c.k, a.c.ks, at + d) : 0.f;
-                    line[D + d] = d < dim ? value(a.c.v, a.c.vs, at + d) : 0.f;
+                    part[d] = d < dim ? value(a.c.k, a.c.ks, at + d) : 0.f;
+                    part[D + d] = d < dim ? value(a.c.v, a.c.vs, at + d) : 0.f;
                 }
                 settle();
                 float x = 0.f;
@@ -628,42 +716,49 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     float y;
                     if constexpr (F) y = q[i];
                     else y = (float)q[i / 8][i % 8];
-                    x = fmaf(y, line[i / each * 2 * each + each * half + i % each], x);
+                    x = fmaf(y, part[i / each * 2 * each + each * half + i % each], x);
                 }
                 const float2 x2 = halves(x);
                 if (a.seen ? t >= s.c0 && !(bits >> (t - s.c0) & 1) : t >= own) continue;
-                const float w = exp2_of(fmaf(x2.x + x2.y, a.c2, M == -INFINITY ? 0.f : -M));
+                const float w = exp2_of(fmaf(x2.x + x2.y, c2, M == -INFINITY ? 0.f : -M));
 #pragma unroll
                 for (uint32_t i = 0; i < D / 2; i++)
-                    o[i / 16][i % 16] = fmaf(w, line[D + i / 16 * 32 + i % 16 / 4 * 8 + 4 * half + i % 4], o[i / 16][i % 16]);
+                    o[i / 16][i % 16] = fmaf(w, part[D + i / 16 * 32 + i % 16 / 4 * 8 + 4 * half + i % 4], o[i / 16][i % 16]);
             }
+            settle();
         }
         if (bad != ~0u) atomicMin(&bad_at, bad);
         __syncthreads();
         const float2 l2 = halves(L);
         L = bad_at < own ? __builtin_nanf("") : l2.x + l2.y;
-        __syncthreads();
-        if (mine && whole) {
-            const float f = L == 0.f ? 0.f : 1.f / L;
+        // out of the wave's part of LDS, whole rows at a time: four values of row n lie in
+        // chunk c ^ n % 16
+        const float f = !whole ? 1.f : L == 0.f ? 0.f : 1.f / L;
+        const size_t slot = (size_t)run.run * 2 + (run.off == 0);
+        constexpr uint32_t W = TILE / 128;  // dims at a time
 #pragma unroll
-            for (uint32_t d = 0; d < ND; d++)
+        for (uint32_t d0 = 0; d0 < D; d0 += W) {
+#pragma unroll
+            for (uint32_t d = d0 / 32; d < (d0 + W) / 32; d++)
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) {
                     f4 x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                    if (L == 0.f) x = f4(0.f);
-                    put_row(a, dim, row, h, 32 * d + 8 * i + 4 * half, x * f);
+                    if (whole && L == 0.f) x = f4(0.f);
+                    *reinterpret_cast<f4*>(part + n * W + ((8 * d - d0 / 4 + 2 * i + half) ^ (n & 15)) * 4) = x * f;
                 }
-        } else if (mine) {
-            const size_t slot = (size_t)run.run * 2 + (run.off == 0);
-            const uint32_t line = wv * 32 + n;
-            float* to = part_o(a, slot) + line * D;
-#pragma unroll
-            for (uint32_t d = 0; d < ND; d++)
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++)
-                    *reinterpret_cast<f4*>(to + 32 * d + 8 * i + 4 * half) = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            if (half == 0) part_ml(a, slot)[line] = make_float2(M, L);
+            settle();
+            for (uint32_t i = lane; i < 32 * W / 4; i += 64) {
+                const uint32_t line = i / (W / 4), c = i % (W / 4);
+                const f4 x = *reinterpret_cast<const f4*>(part + line * W + (c ^ (line & 15)) * 4);
+                const size_t at = shfl64(to, line);
+                if (line >= rows) continue;
+                if (whole) put_row(a, dim, at, d0 + 4 * c, x);
+                else *reinterpret_cast<f4*>(part_o(a, slot) + (wv * 32 + line) * D + d0 + 4 * c) = x;
+            }
+            settle();
         }
+        if (!whole && mine && half == 0) part_ml(a, slot)[wv * 32 + n] = make_float2(M, L);
+        __syncthreads();
     } while (run.next(a));
 }
 
@@ -697,7 +792,7 @@ __global__ __launch_bounds__(kBlock) void k_page_many_join(PageMany a, uint32_t 
     }
     const uint32_t r = m.row + line, row = r / a.group;
     if (row >= a.n) return;
-    put_row(a, a.c.dim, row, m.kv * a.group + r % a.group, d, L == 0.f ? f4(0.f) : O * (1.f / L));
+    put_row(a, a.c.dim, (size_t)row * a.out.row + (size_t)(m.kv * a.group + r % a.group) * a.out.head, d, L == 0.f ? f4(0.f) : O * (1.f / L));
 }
 
 // ---------------------------------------------------------------- launches --
@@ -706,7 +801,6 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     const uint32_t d = a.c.dim, es = a.c.kind == F32 ? 4 : a.c.kind == Q8_0 ? 1 : 2;
     a.group = a.heads / a.c.kvheads;
     a.wide = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-    a.narrow = a.q.kind != F32 && a.out.kind != F32 && a.c.kind == a.q.kind;
     auto aligned = [](const Heads& h, uint32_t bytes) {
         const uint64_t e = h.kind == F32 ? 4 : 2;
         return (((uintptr_t)h.p | h.row * e | h.head * e) % bytes) == 0;
@@ -714,6 +808,10 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.q_wide = d % 8 == 0 && aligned(a.q, 16);
     a.out_wide = aligned(a.out, a.out.kind == F32 ? 16 : 8);
     a.kv_wide = d % 8 == 0 && (((uintptr_t)a.c.k | (uintptr_t)a.c.v | (a.c.ps | a.c.ts | a.c.hs) * es) % std::min(8 * es, 16u)) == 0;
+    // products of 16 bits: of the cache's own type, or of f16 where bf16 queries read Q8_0
+    a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
+               (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && a.q.kind == BF16 && a.out.kind == BF16));
+    a.one_page = a.c.page % (512 / a.wide) == 0 && a.c.ts * 16 * es < 1u << 31;
     // t / page for t < 2^31: t * ceil(2^shift / page) >> shift
     uint32_t log = 0;
     while ((1ull << log) < a.c.page) log++;
@@ -726,25 +824,23 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.runs = (uint32_t)std::min<uint64_t>(cus * (a.wide == 256 ? 1 : 2), std::max<uint64_t>(most, 1));
 }
 
-template <class T, uint32_t D> static void launch_tiles(const PageMany& a, bool direct, hipStream_t s) {
+template <class T, uint32_t SRC> static void launch_many(const PageMany& a, hipStream_t s) {
     const dim3 grid((a.runs + kXcds - 1) / kXcds * kXcds), block(kBlock);
-    if constexpr (!std::is_same<T, float>::value)
-        if (direct) {
-            hipLaunchKernelGGL((k_page_many<T, D, true>), grid, block, 0, s, a);
-            return;
-        }
-    hipLaunchKernelGGL((k_page_many<T, D, false>), grid, block, 0, s, a);
-}
-template <class T> static void launch_many(const PageMany& a, hipStream_t s) {
-    const bool direct = a.narrow && a.kv_wide && a.c.dim == a.wide;
-    if (a.wide == 64) launch_tiles<T, 64>(a, direct, s);
-    else if (a.wide == 128) launch_tiles<T, 128>(a, direct, s);
-    else launch_tiles<T, 256>(a, direct, s);
+    if (a.wide == 64) hipLaunchKernelGGL((k_page_many<T, 64, SRC>), grid, block, 0, s, a);
+    else if (a.wide == 128) hipLaunchKernelGGL((k_page_many<T, 128, SRC>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_page_many<T, 256, SRC>), grid, block, 0, s, a);
 }
 void launch_page_many(const PageMany& a, hipStream_t s) {
-    if (!a.narrow) launch_many<float>(a, s);
-    else if (a.c.kind == F16) launch_many<_Float16>(a, s);
-    else launch_many<bf16_t>(a, s);
+    const bool direct = a.kv_wide && a.c.dim == a.wide;
+    if (a.narrow) {
+        if (a.c.kind == Q8_0) launch_many<_Float16, Q8_0>(a, s);
+        else if (a.c.kind == F16) direct ? launch_many<_Float16, kDirect>(a, s) : launch_many<_Float16, kAny>(a, s);
+        else direct ? launch_many<bf16_t, kDirect>(a, s) : launch_many<bf16_t, kAny>(a, s);
+    } else if (!a.kv_wide) launch_many<float, kAny>(a, s);
+    else if (a.c.kind == F32) launch_many<float, F32>(a, s);
+    else if (a.c.kind == F16) launch_many<float, F16>(a, s);
+    else if (a.c.kind == BF16) launch_many<float, BF16>(a, s);
+    else launch_many<float, Q8_0>(a, s);
     if (a.runs > 1)
         hipLaunchKernelGGL(k_page_many_join, dim3(a.runs - 1, kTileRows * a.wide / (4 * kBlock)), dim3(kBlock), 0, s, a,
                            !a.narrow || a.wide == 256 ? 32 : 64);

@@ -118,7 +118,8 @@ struct PageMany {
     float scale;
     // by page_many_plan
     uint32_t group, wide, runs;     // query heads of a KV head, width of the tiles, workgroups
-    bool narrow;                    // products of the cache's own 16-bit type, else of 32 bits
+    bool narrow;                    // products of 16 bits, else of 32
+    bool one_page;                  // eight rows of 64 values (or as many bytes of others) lie in one page
     bool q_wide, out_wide, kv_wide; // rows aligned to what is read and written at a time
     uint32_t page_mul, page_shift;  // t / page
     float sign, c2;                 // scale * log2 e = sign * c2

@@ -39,7 +39,10 @@ def signed(bits):
 
 
 def split_of(q, kv):
-    """A softmax weight that enters a product of 16 bits is rounded once, to the type of queries and cache."""
+    """A softmax weight that enters a product of 16 bits is rounded once, to the type of queries and cache; bf16 queries
+    over Q8_0 take f16 products, where the values (code times scale), too, are rounded to f16."""
+    if (q, kv) == ("bf16", "q8_0"):
+        return HALF[torch.float16]
     return HALF[TYPES[q]] if q == kv and q != "f32" else 0.0
 
 
@@ -50,6 +53,7 @@ def attend_many(q, k, v, table, lengths, first, scale, bits=None, split=0.0):
     heads, d = q.shape[1:]
     out, bound = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
     G = heads // k.shape[2]
+    q8 = split == HALF[torch.float16] and q.dtype == torch.bfloat16
     for b, n in enumerate(lengths):
         m = first[b + 1] - first[b]
         if not m:
@@ -87,6 +91,10 @@ def attend_many(q, k, v, table, lengths, first, scale, bits=None, split=0.0):
         low = torch.where(s == -math.inf, torch.zeros_like(s), (s - top).abs()).nan_to_num(0, 0, 0).amax(-1, keepdim=True)
         rel = (2 * ((d + 3) * size + 4 * low) + 2 * (n + 8) + 64) * 2.0 ** -24 + 2 * split
         near = rel * (p @ finite.abs()[:, None])
+        if q8:
+            # values as f16, half a step of 2^-11 or 2^-25; a query's elements below 2^-39 of its largest, in every score
+            lost = scale * 2.0 ** -39 * qq.abs().amax(-1, keepdim=True) * kk.abs().sum(-1).amax()
+            near = near + split * (p @ finite.abs()[:, None]) + 2.0 ** -25 + 2 * lost * finite.abs().amax()
         if split == HALF[torch.float16]:
             near = near + 2 * n * 2.0 ** -32 * finite.abs().amax()
         bound[rows] = near.permute(2, 0, 1, 3).reshape(m, heads, d)
