@@ -24,6 +24,7 @@ namespace qh {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kTileRows = 128;  // query rows of a tile, 32 a wave
 constexpr uint32_t kRunKeys = 128;   // keys of a run at least
+constexpr uint32_t kTileKeys = 128;  // a tile's start and end, in keys
 constexpr uint32_t kXcds = 8;
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -45,6 +46,10 @@ __device__ __forceinline__ float2 halves(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+
+// The compiler moves no instruction across: products, the LDS reads ahead of them and the
+// arithmetic between them are issued in the order that is written.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // ------------------------------------------------------------ runs of work --
 // Sequence b's new tokens are rows [f0, f0 + count) of q; c0 keys lie in front of
@@ -74,7 +79,7 @@ __device__ __forceinline__ Seq seq_of(const PageMany& a, const Bounds& q) {
     s.tiles = (uint32_t)(((uint64_t)s.count * a.group + kTileRows - 1) / kTileRows);
     s.bad = s.len < 0 || s.count > (uint32_t)s.len || (a.seen && s.count > kTreeMost);
     s.c0 = s.bad ? 0 : (uint32_t)s.len - s.count;
-    s.first = s.bad ? 1 : a.seen ? (uint64_t)(uint32_t)s.len * a.group : (uint64_t)(s.c0 + 1) * a.group + kTileRows - 1;
+    s.first = s.bad ? 1 : a.seen ? (uint64_t)(kTileKeys + s.len) * a.group : (uint64_t)(kTileKeys + s.c0 + 1) * a.group + kTileRows - 1;
     s.step = s.bad || a.seen ? 0 : kTileRows;
     return s;
 }
@@ -86,7 +91,8 @@ __device__ __forceinline__ uint32_t end_of(const PageMany& a, const Seq& s, uint
 }
 // The key at which the part from x on of a tile begins: at whole steps.
 __device__ __forceinline__ uint32_t key_at(const PageMany& a, uint64_t x, uint32_t end, uint32_t step) {
-    return (uint32_t)min((uint64_t)end, x / a.group / step * step);
+    const uint64_t k = x / a.group;
+    return k <= kTileKeys ? 0 : (uint32_t)min((uint64_t)end, (k - kTileKeys) / step * step);
 }
 
 __device__ __forceinline__ uint64_t run_begin(uint64_t total, uint32_t runs, uint32_t i) {
@@ -267,7 +273,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
     __shared__ __align__(16) uint8_t lds[4][TILE];  // K, K, V, V; in front and behind a part for each wave
     __shared__ __align__(16) float scales[Q8 ? 2 : 1][Q8 ? ND : 1][Q8 ? KT : 1];  // of K's blocks
     __shared__ uint32_t bad_at;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wv = same(tid >> 6), n = lane & 31, half = lane >> 5;
+    const uint32_t wv = same(threadIdx.x >> 6);
     auto settle = [] {  // what the wave wrote to its own part of LDS can be read
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -277,6 +283,8 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
     Run run;
     if (!run.start(a)) return;
     do {
+        // hidden, so that what follows from it is not kept in registers from one tile to the next
+        const uint32_t tid = opaque(threadIdx.x), lane = tid & 63, n = lane & 31, half = lane >> 5;
         const Seq& s = run.s;
         const uint32_t end = same(end_of(a, s, run.i)), R = s.count * a.group;
         const uint32_t lo = same(key_at(a, run.off, end, KT));
@@ -302,62 +310,6 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 
         Q q[NQ];
         float c2 = a.c2;
-        {
-            const size_t at = (size_t)row * a.q.row + (size_t)h * a.q.head;
-            constexpr uint32_t each = F ? 4 : 8;  // values of a load: 2 each g + each half + ..
-            u4 x[D / 2 / each];
-            if (a.q_wide && a.q.kind == QKIND) {
-#pragma unroll
-                for (uint32_t g = 0; g < D / 2 / each; g++) {
-                    const uint32_t d = (2 * g + half) * each;
-                    x[g] = u4{0, 0, 0, 0};
-                    if (mine && d < dim) x[g] = gld<u4>(a.q.p + (F ? 4 : 2) * (at + d));
-                }
-            } else {  // through the wave's part of LDS, a value at a time; 16 bits: of the type of the product
-                uint8_t* part = lds[wv];
-#pragma nounroll
-                for (uint32_t i = lane; i < 32 * D; i += 64) {
-                    const uint32_t d = i % D;
-                    const size_t from = shfl64(at, i / D) + d;
-                    const bool in = i / D < rows && d < dim;
-                    if constexpr (F) reinterpret_cast<float*>(part)[i] = in ? elem_kind(a.q.kind, a.q.p, from) : 0.f;
-                    else reinterpret_cast<uint16_t*>(part)[i] = in ? gld<uint16_t>(a.q.p + 2 * from) : (uint16_t)0;
-                }
-                settle();
-#pragma unroll
-                for (uint32_t g = 0; g < D / 2 / each; g++)
-                    x[g] = *reinterpret_cast<const u4*>(part + (n * D + (2 * g + half) * each) * (F ? 4 : 2));
-                __syncthreads();  // before K and V go there
-            }
-            if constexpr (F) {
-#pragma unroll
-                for (uint32_t i = 0; i < NQ; i++) q[i] = __uint_as_float(x[i / 4][i % 4]) * a.sign;
-            } else {
-                const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u, keep = a.sign == 0.f ? 0u : ~0u;
-#pragma unroll
-                for (uint32_t g = 0; g < NQ; g++) x[g] = (x[g] ^ flip) & keep;
-                if constexpr (Q8) {
-                    // bf16 queries as f16, the row's largest value in [2^14, 2^15): what lies below 2^-38
-                    // of it is lost, what is not finite stays so
-                    uint32_t top = 0;
-#pragma unroll
-                    for (uint32_t g = 0; g < NQ; g++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) top = max(top, max(x[g][j] << 16 & 0x7fff0000u, x[g][j] & 0x7fff0000u));
-                    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64)) >> 23;
-                    const int up = top == 0 || top == 255 ? 0 : 141 - (int)top;
-                    c2 = ldexpf(c2, -up);
-#pragma unroll
-                    for (uint32_t g = 0; g < NQ; g++)
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            q[g][j] = (T)ldexpf(__uint_as_float(j & 1 ? x[g][j / 2] & 0xffff0000u : x[g][j / 2] << 16), up);
-                } else {
-#pragma unroll
-                    for (uint32_t g = 0; g < NQ; g++) q[g] = __builtin_bit_cast(T8, x[g]);
-                }
-            }
-        }
         f16v o[ND];
 #pragma unroll
         for (uint32_t d = 0; d < ND; d++)
@@ -394,13 +346,18 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         constexpr uint32_t WORDS = F ? 2 : 1;
         Word kw[DIRECT ? 1 : ROUNDS][WORDS], vw[DIRECT ? 1 : ROUNDS][WORDS];
         float kf[Q8 ? ROUNDS : 1];
-        auto to_lds = [&](const uint8_t* k, const uint8_t* v, uint32_t off, uint32_t buf, uint32_t r) {
+        // 16 bytes a lane from its own address to LDS.  In assembly, as the compiler lets every later
+        // LDS read wait for such loads, of whatever buffer; meet() waits for them.
+        auto to_lds = [&](const uint8_t* p, uint32_t off, uint32_t buf, uint32_t r) {
 #if defined(__HIP_DEVICE_COMPILE__)
-            const uint32_t at = (r * kWaves + wv) * 1024;
-            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(k + off),
-                                             (__attribute__((address_space(3))) void*)(lds[buf] + at), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(v + off),
-                                             (__attribute__((address_space(3))) void*)(lds[2 + buf] + at), 16, 0, 0);
+            const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(p) : "memory");
+#endif
+        };
+        auto to_lds_far = [&](const uint8_t* p, uint32_t buf, uint32_t r) {
+#if defined(__HIP_DEVICE_COMPILE__)
+            const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
 #endif
         };
         auto fetch = [&](uint32_t k0, uint32_t buf) {
@@ -414,14 +371,18 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                         const size_t at = place(t, (int32_t)same((uint32_t)pages[r]));
                         const uint32_t chunk = 16 * (lane % PER ^ turn<CH>((SAME ? wv : r * kWaves + wv) * LINES + line));
                         const uint32_t in = k0 + KT > end ? min(line, end - 1 - t) : line;
-                        to_lds(a.c.k + 2 * at, a.c.v + 2 * at, in * (uint32_t)a.c.ts * 2 + chunk, buf, r);
+                        const uint32_t off = in * (uint32_t)a.c.ts * 2 + chunk;
+                        to_lds(a.c.k + 2 * at, off, buf, r);
+                        to_lds(a.c.v + 2 * at, off, 2 + buf, r);
                     }
                 } else {
 #pragma unroll
                     for (uint32_t r = 0; r < ROUNDS; r++) {
                         const uint32_t g = group_row(r);
                         const size_t at = place(min(k0 + g, end - 1), pages[r]);
-                        to_lds(a.c.k + 2 * at, a.c.v + 2 * at, 16 * (lane % PER ^ turn<CH>(g)), buf, r);
+                        const size_t off = 2 * at + 16 * (lane % PER ^ turn<CH>(g));
+                        to_lds_far(a.c.k + off, buf, r);
+                        to_lds_far(a.c.v + off, 2 + buf, r);
                     }
                 }
             } else {
@@ -554,11 +515,38 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                             }
                         }
                 } else {
+// four parts of K are on their way ahead of a product
+                    constexpr uint32_t N = NS * D / 16;
+                    T8 x[4];
 #pragma unroll
-                    for (uint32_t g = 0; g < D / 16; g++)
+                    for (uint32_t i = 0; i < 4; i++) x[i] = k_part(i / NS, i % NS);
+                    in_order();
 #pragma unroll
-                        for (uint32_t m = 0; m < NS; m++) sc[m] = product(k_part(g, m), q[g], sc[m]);
+                    for (uint32_t i = 0; i < N; i++) {
+                        sc[i % NS] = product(x[i % 4], q[i / NS], sc[i % NS]);
+                        if (i + 4 < N) x[i % 4] = k_part((i + 4) / NS, (i + 4) % NS);
+                        in_order();
+                    }
                 }
+            }
+            auto v_part = [&](uint32_t c, uint32_t d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+                struct { s4 w[2]; } w;
+#pragma unroll
+                for (uint32_t e = 0; e < 2; e++) {
+                    const uint8_t* v = vt + (v_at ^ (d * 64 ^ e * 32)) + (16 * c + 8 * e) * D * 2;
+                    w.w[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)v);
+                }
+                return __builtin_bit_cast(T8, w);
+#else
+                return T8{};
+#endif
+            };
+            T8 x[2][F ? 1 : ND];  // V's parts
+            if constexpr (!F) {
+#pragma unroll
+                for (uint32_t d = 0; d < ND; d++) x[0][d] = v_part(0, d);
+                in_order();
             }
             if constexpr (masked()) {
                 // which of the step's keys the row sees, one a bit
@@ -586,16 +574,16 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 }
                 if (odd == ~0u && __any((found & (F ? 0x80000000u : 0x80008000u)) != 0)) odd = k0;
             }
-            float top = -INFINITY;
+            float top[4];
 #pragma unroll
-            for (uint32_t m = 0; m < NS; m++)
+            for (int i = 0; i < 4; i++) top[i] = sc[0][i];
 #pragma unroll
-                for (int j = 0; j < 16; j++) top = fmaxf(top, sc[m][j]);
-            const float2 t2 = halves(top);
-            top = fmaxf(t2.x, t2.y) * c2;
+            for (int j = 4; j < 16 * (int)NS; j++) top[j % 4] = fmaxf(top[j % 4], sc[j / 16][j % 16]);
+            const float2 t2 = halves(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+            const float most_here = fmaxf(t2.x, t2.y) * c2 - kUp;
             // the reference follows the maximum only where that is far above it
-            if (__any(top - kUp > M + (F ? 0.f : kAhead))) {
-                const float Mn = fmaxf(M, top - kUp), f = Mn == -INFINITY ? 1.f : exp2_of(M - Mn);
+            if (__any(most_here > M + (F ? 0.f : kAhead))) {
+                const float Mn = fmaxf(M, most_here), f = Mn == -INFINITY ? 1.f : exp2_of(M - Mn);
                 M = Mn;
                 L *= f;
 #pragma unroll
@@ -625,52 +613,113 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     }
                 }
             } else {
-                T8 p[2 * NS];
-#pragma unroll
-                for (uint32_t m = 0; m < NS; m++)
-#pragma unroll
-                    for (uint32_t j = 0; j < 16; j += 2) {
-                        const float x = exp2_of(fmaf(sc[m][j], c2, -Mf)), y = exp2_of(fmaf(sc[m][j + 1], c2, -Mf));
-                        // the sum is of the rounded weights, so that equal errors of all cancel
-                        if constexpr (H) {
-                            const h2 z = {(_Float16)x, (_Float16)y}, ones = {(_Float16)1.f, (_Float16)1.f};
-                            L = __builtin_amdgcn_fdot2(z, ones, L, false);
-                            p[2 * m + j / 8][j % 8] = z[0], p[2 * m + j / 8][j % 8 + 1] = z[1];
-                        } else {
-                            const b2 z = {(bf16_t)x, (bf16_t)y}, ones = {(bf16_t)1.f, (bf16_t)1.f};
-                            L = __builtin_amdgcn_fdot2_f32_bf16(z, ones, L, false);
-                            p[2 * m + j / 8][j % 8] = z[0], p[2 * m + j / 8][j % 8 + 1] = z[1];
-                        }
+                constexpr uint32_t C = 2 * NS;
+                T8 p[C];
+                // weights 2 i and 2 i + 1 of p[c]; the sum is of the rounded ones, so that equal errors of all cancel
+                auto weights = [&](uint32_t c, uint32_t i) {
+                    const uint32_t m = c / 2, j = c % 2 * 8 + 2 * i;
+                    const float x = exp2_of(fmaf(sc[m][j], c2, -Mf)), y = exp2_of(fmaf(sc[m][j + 1], c2, -Mf));
+                    if constexpr (H) {
+                        const h2 z = {(_Float16)x, (_Float16)y}, ones = {(_Float16)1.f, (_Float16)1.f};
+                        L = __builtin_amdgcn_fdot2(z, ones, L, false);
+                        p[c][2 * i] = z[0], p[c][2 * i + 1] = z[1];
+                    } else {
+                        const b2 z = {(bf16_t)x, (bf16_t)y}, ones = {(bf16_t)1.f, (bf16_t)1.f};
+                        L = __builtin_amdgcn_fdot2_f32_bf16(z, ones, L, false);
+                        p[c][2 * i] = z[0], p[c][2 * i + 1] = z[1];
                     }
-                if (masked() && odd != ~0u) return;
-#if defined(__HIP_DEVICE_COMPILE__)
+                };
+                if (masked() && odd != ~0u) {
 #pragma unroll
-                for (uint32_t c = 0; c < 2 * NS; c++)
+                    for (uint32_t i = 0; i < 4 * C; i++) weights(i / 4, i % 4);
+                    return;
+                }
+                // a step of 16 keys: V's parts and the weights of the next between its products
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) weights(0, i);
+                in_order();
+#pragma unroll
+                for (uint32_t c = 0; c < C; c++)
 #pragma unroll
                     for (uint32_t d = 0; d < ND; d++) {
-                        struct { s4 w[2]; } w;
+                        if constexpr (H) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[c % 2][d], p[c], o[d], 0, 0, 0);
+                        else o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c % 2][d], p[c], o[d], 0, 0, 0);
+                        if (c + 1 < C) {
+                            x[(c + 1) % 2][d] = v_part(c + 1, d);
 #pragma unroll
-                        for (uint32_t e = 0; e < 2; e++) {
-                            const uint8_t* v = vt + (v_at ^ (d * 64 ^ e * 32)) + (16 * c + 8 * e) * D * 2;
-                            w.w[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)v);
+                            for (uint32_t i = d * 4 / ND; i < (d + 1) * 4 / ND; i++) weights(c + 1, i);
                         }
-                        const T8 x = __builtin_bit_cast(T8, w);
-                        if constexpr (H) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[c], o[d], 0, 0, 0);
-                        else o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, p[c], o[d], 0, 0, 0);
+                        in_order();
                     }
-#endif
             }
         };
 
-        // the loads that go to LDS by themselves are no ordinary accesses to it: the wave waits
-        // for its own before it meets the others
+        // the wave waits for its own loads to LDS before it meets the others
         auto meet = [&] {
             if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
         };
         if (tid == 0) bad_at = ~0u;
         look(lo);
+        constexpr uint32_t each = F ? 4 : 8;  // values of a load: 2 each g + each half + ..
+        u4 xq[D / 2 / each];
+        {
+            const size_t at = (size_t)row * a.q.row + (size_t)h * a.q.head;
+            if (a.q_wide && a.q.kind == QKIND) {
+#pragma unroll
+                for (uint32_t g = 0; g < D / 2 / each; g++) {
+                    const uint32_t d = (2 * g + half) * each;
+                    xq[g] = u4{0, 0, 0, 0};
+                    if (mine && d < dim) xq[g] = gld<u4>(a.q.p + (F ? 4 : 2) * (at + d));
+                }
+            } else {  // through the wave's part of LDS, a value at a time; 16 bits: of the type of the product
+                uint8_t* part = lds[wv];
+#pragma nounroll
+                for (uint32_t i = lane; i < 32 * D; i += 64) {
+                    const uint32_t d = i % D;
+                    const size_t from = shfl64(at, i / D) + d;
+                    const bool in = i / D < rows && d < dim;
+                    if constexpr (F) reinterpret_cast<float*>(part)[i] = in ? elem_kind(a.q.kind, a.q.p, from) : 0.f;
+                    else reinterpret_cast<uint16_t*>(part)[i] = in ? gld<uint16_t>(a.q.p + 2 * from) : (uint16_t)0;
+                }
+                settle();
+#pragma unroll
+                for (uint32_t g = 0; g < D / 2 / each; g++)
+                    xq[g] = *reinterpret_cast<const u4*>(part + (n * D + (2 * g + half) * each) * (F ? 4 : 2));
+                __syncthreads();  // before K and V go there
+            }
+        }
         fetch(lo, 0);
+        {
+            if constexpr (F) {
+#pragma unroll
+                for (uint32_t i = 0; i < NQ; i++) q[i] = __uint_as_float(xq[i / 4][i % 4]) * a.sign;
+            } else {
+                const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u, keep = a.sign == 0.f ? 0u : ~0u;
+#pragma unroll
+                for (uint32_t g = 0; g < NQ; g++) xq[g] = (xq[g] ^ flip) & keep;
+                if constexpr (Q8) {
+                    // bf16 queries as f16, the row's largest value in [2^14, 2^15): what lies below 2^-38
+                    // of it is lost, what is not finite stays so
+                    uint32_t top = 0;
+#pragma unroll
+                    for (uint32_t g = 0; g < NQ; g++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) top = max(top, max(xq[g][j] << 16 & 0x7fff0000u, xq[g][j] & 0x7fff0000u));
+                    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64)) >> 23;
+                    const int up = top == 0 || top == 255 ? 0 : 141 - (int)top;
+                    c2 = ldexpf(c2, -up);
+#pragma unroll
+                    for (uint32_t g = 0; g < NQ; g++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            q[g][j] = (T)ldexpf(__uint_as_float(j & 1 ? xq[g][j / 2] & 0xffff0000u : xq[g][j / 2] << 16), up);
+                } else {
+#pragma unroll
+                    for (uint32_t g = 0; g < NQ; g++) q[g] = __builtin_bit_cast(T8, xq[g]);
+                }
+            }
+        }
         store(0);
         if (lo + KT < hi) look(lo + KT);
         meet();
