@@ -24,7 +24,7 @@ namespace qh {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kTileRows = 128;  // query rows of a tile, 32 a wave
 constexpr uint32_t kRunKeys = 128;   // keys of a run at least
-constexpr uint32_t kTileKeys = 128;  // a tile's start and end, in keys
+constexpr uint32_t kTileKeys = 256;  // a tile's start and end, in keys
 constexpr uint32_t kXcds = 8;
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         // ---- a step's K and V
         const int32_t* table = a.r.table + run.b * a.r.stride;
         const size_t base = run.kv * a.c.hs;
-        auto page_number = [&](uint32_t t) { return (uint32_t)(((uint64_t)t * a.page_mul) >> a.page_shift); };
+        auto page_number = [&](uint32_t t) { return __umulhi(t << 1, a.page_mul) >> a.page_log; };
         auto page_of = [&](uint32_t t) { return gld<int32_t>(table + page_number(t)); };
         auto place = [&](uint32_t t, int32_t page) {  // of key t; a page out of range is read as page 0
             if ((uint32_t)page >= a.c.count) bad = min(bad, t), page = 0;
@@ -335,135 +335,126 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         constexpr uint32_t PER = D / 8, LINES = 64 / PER; // of a row; rows of a wave's load
         int32_t pages[ROUNDS];
         auto group_row = [&](uint32_t r) { return DIRECT ? (r * kWaves + wv) * LINES + lane / PER : (r * kBlock + tid) / PER; };
-        // the rows of a wave's load lie in one page: its place is computed once for all lanes
-        const bool one_page = DIRECT && a.one_page;
+        // (kDirect: the rows of a wave's load lie in one page, whose place is computed once for all lanes)
         auto first_row = [&](uint32_t k0, uint32_t r) { return min(k0 + (r * kWaves + wv) * LINES, (end - 1) / LINES * LINES); };
         auto look = [&](uint32_t k0) {
 #pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; r++) pages[r] = page_of(one_page ? first_row(k0, r) : min(k0 + group_row(r), end - 1));
+            for (uint32_t r = 0; r < ROUNDS; r++) pages[r] = page_of(DIRECT ? first_row(k0, r) : min(k0 + group_row(r), end - 1));
         };
-        typedef typename std::conditional<F, f4, u4>::type Word;
-        constexpr uint32_t WORDS = F ? 2 : 1;
-        Word kw[DIRECT ? 1 : ROUNDS][WORDS], vw[DIRECT ? 1 : ROUNDS][WORDS];
-        float kf[Q8 ? ROUNDS : 1];
-        // 16 bytes a lane from its own address to LDS.  In assembly, as the compiler lets every later
-        // LDS read wait for such loads, of whatever buffer; meet() waits for them.
-        auto to_lds = [&](const uint8_t* p, uint32_t off, uint32_t buf, uint32_t r) {
-#if defined(__HIP_DEVICE_COMPILE__)
-            const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(p) : "memory");
-#endif
-        };
-        auto to_lds_far = [&](const uint8_t* p, uint32_t buf, uint32_t r) {
-#if defined(__HIP_DEVICE_COMPILE__)
-            const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
-#endif
-        };
-        auto fetch = [&](uint32_t k0, uint32_t buf) {
+        // What a thread holds of a step meanwhile, as it is in the cache: eight values of K and of V each.
+        constexpr bool WIDE16 = !F || SRC == F16 || SRC == BF16;  // 16 bytes of 16-bit values
+        constexpr uint32_t WORDS = SRC == Q8_0 || DIRECT ? 0 : WIDE16 ? 1 : 2;
+        u4 kw[WORDS ? ROUNDS : 1][WORDS ? WORDS : 1], vw[WORDS ? ROUNDS : 1][WORDS ? WORDS : 1];
+        uint2 kc[SRC == Q8_0 ? ROUNDS : 1], vc[SRC == Q8_0 ? ROUNDS : 1];       // codes
+        uint32_t kf[SRC == Q8_0 ? ROUNDS : 1], vf[SRC == Q8_0 ? ROUNDS : 1];    // scales
+        auto fetch = [&](uint32_t k0, uint32_t buf, uint32_t r) {
             if constexpr (DIRECT) {
-                const uint32_t line = lane / PER;
-                if (one_page) {
-                    constexpr bool SAME = turn<CH>(kWaves * LINES) == 0;  // a row's turn in every round
-#pragma unroll
-                    for (uint32_t r = 0; r < ROUNDS; r++) {
-                        const uint32_t t = same(first_row(k0, r));
-                        const size_t at = place(t, (int32_t)same((uint32_t)pages[r]));
-                        const uint32_t chunk = 16 * (lane % PER ^ turn<CH>((SAME ? wv : r * kWaves + wv) * LINES + line));
-                        const uint32_t in = k0 + KT > end ? min(line, end - 1 - t) : line;
-                        const uint32_t off = in * (uint32_t)a.c.ts * 2 + chunk;
-                        to_lds(a.c.k + 2 * at, off, buf, r);
-                        to_lds(a.c.v + 2 * at, off, 2 + buf, r);
-                    }
-                } else {
-#pragma unroll
-                    for (uint32_t r = 0; r < ROUNDS; r++) {
-                        const uint32_t g = group_row(r);
-                        const size_t at = place(min(k0 + g, end - 1), pages[r]);
-                        const size_t off = 2 * at + 16 * (lane % PER ^ turn<CH>(g));
-                        to_lds_far(a.c.k + off, buf, r);
-                        to_lds_far(a.c.v + off, 2 + buf, r);
-                    }
-                }
+                // 16 bytes a lane from its own address to LDS.  In assembly, as the compiler lets every
+                // later LDS read wait for such loads, of whatever buffer; meet() waits for them.
+                const uint32_t t = same(first_row(k0, r)), line = lane / PER;
+                const size_t at = place(t, (int32_t)same((uint32_t)pages[r]));
+                constexpr bool SAME = turn<CH>(kWaves * LINES) == 0;  // a row's turn in every round
+                const uint32_t chunk = 16 * (lane % PER ^ turn<CH>((SAME ? wv : r * kWaves + wv) * LINES + line));
+                const uint32_t off = min(line, end - 1 - t) * (uint32_t)a.c.ts * 2 + chunk;
+#if defined(__HIP_DEVICE_COMPILE__)
+                const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(a.c.k + 2 * at) : "memory");
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + 2 * TILE), "v"(off), "s"(a.c.v + 2 * at) : "memory");
+#endif
             } else {
+                const size_t at = place(min(k0 + group_row(r), end - 1), pages[r]);
+                const uint32_t d = (r * kBlock + tid) % PER * 8;
+                auto load = [&](const uint8_t* p, u4* w) {
+                    if constexpr (F && SRC == kAny) {
+                        auto each = [&](auto kind) {
+                            const _Float16* sc = p == a.c.k ? a.c.ks : a.c.vs;
 #pragma unroll
-                for (uint32_t r = 0; r < ROUNDS; r++) {
-                    const size_t at = place(min(k0 + group_row(r), end - 1), pages[r]);
-                    const uint32_t d = (r * kBlock + tid) % PER * 8;
-                    auto load = [&](const uint8_t* p, const _Float16* sc, Word* w, auto is_k) {
-                        if (d >= dim) {
-                            for (uint32_t i = 0; i < WORDS; i++) w[i] = Word{0, 0, 0, 0};
-                            if constexpr (Q8 && is_k()) kf[r] = 0.f;
-                        } else if constexpr (SRC == F32) {
-                            w[0] = gld<f4>(p + 4 * (at + d)), w[1] = gld<f4>(p + 4 * (at + d) + 16);
-                        } else if constexpr (Q8) {
-                            // code + 128 in the low bits of 1024 + 128 + code, less 1152: the code; V's times its
-                            // scale, rounded once
-                            const uint2 u = gld<uint2>(p + at + d);
-                            const _Float16 f1 = gld<_Float16>(sc + (at + d) / 32);
-                            const h2 less = h2((_Float16)1152.f);
-                            if constexpr (is_k()) kf[r] = (float)f1;
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const uint32_t c = (j < 2 ? u.x : u.y) ^ 0x80808080u;
-                                const uint32_t both = __builtin_amdgcn_perm(0x64646464u, c, j & 1 ? 0x07030702u : 0x07010700u);
-                                h2 x = __builtin_bit_cast(h2, both) - less;
-                                if constexpr (!is_k()) x *= h2(f1);
-                                w[0][j] = __builtin_bit_cast(uint32_t, x);
+                            for (uint32_t j = 0; j < 8; j++) {
+                                const size_t e = at + min(d + j, dim - 1);
+                                float x = elem<kind()>(p, e);
+                                if constexpr (kind() == Q8_0) x *= (float)gld<_Float16>(sc + e / 32);
+                                w[j / 4][j % 4] = d + j < dim ? __float_as_uint(x) : 0u;
                             }
-                        } else if constexpr (SRC == Q8_0) {
-                            const uint2 u = gld<uint2>(p + at + d);
-                            const float f = (float)gld<_Float16>(sc + (at + d) / 32);
+                        };
+                        if (a.c.kind == F32) each(std::integral_constant<uint32_t, F32>());
+                        else if (a.c.kind == F16) each(std::integral_constant<uint32_t, F16>());
+                        else if (a.c.kind == BF16) each(std::integral_constant<uint32_t, BF16>());
+                        else each(std::integral_constant<uint32_t, Q8_0>());
+                    } else if (!F && !a.kv_wide) {
+                        w[0] = u4{0, 0, 0, 0};
 #pragma unroll
-                            for (int j = 0; j < 8; j++) w[j / 4][j % 4] = (float)(int8_t)((j < 4 ? u.x : u.y) >> 8 * (j & 3)) * f;
-                        } else if constexpr (SRC == F16 || SRC == BF16) {
-                            const u4 u = gld<u4>(p + 2 * (at + d));
-#pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                const uint32_t v = j & 1 ? u[j / 2] >> 16 : u[j / 2] & 0xffff;
-                                w[j / 4][j % 4] = SRC == F16 ? h2f(v) : __uint_as_float(v << 16);
-                            }
-                        } else if constexpr (F) {
-                            auto each = [&](auto kind) {
-#pragma unroll
-                                for (uint32_t j = 0; j < 8; j++) {
-                                    const size_t e = at + min(d + j, dim - 1);
-                                    float x = elem<kind()>(p, e);
-                                    if constexpr (kind() == Q8_0) x *= (float)gld<_Float16>(sc + e / 32);
-                                    w[j / 4][j % 4] = d + j < dim ? x : 0.f;
-                                }
-                            };
-                            if (a.c.kind == F32) each(std::integral_constant<uint32_t, F32>());
-                            else if (a.c.kind == F16) each(std::integral_constant<uint32_t, F16>());
-                            else if (a.c.kind == BF16) each(std::integral_constant<uint32_t, BF16>());
-                            else each(std::integral_constant<uint32_t, Q8_0>());
-                        } else if (a.kv_wide) {
-                            w[0] = gld<u4>(p + 2 * (at + d));
-                        } else {
-                            w[0] = u4{0, 0, 0, 0};
-#pragma unroll
-                            for (uint32_t j = 0; j < 8; j++)
-                                if (d + j < dim) w[0][j / 2] |= (uint32_t)gld<uint16_t>(p + 2 * (at + d + j)) << 16 * (j & 1);
-                        }
-                    };
-                    load(a.c.k, a.c.ks, kw[r], std::true_type());
-                    load(a.c.v, a.c.vs, vw[r], std::false_type());
+                        for (uint32_t j = 0; j < 8; j++)
+                            if (d + j < dim) w[0][j / 2] |= (uint32_t)gld<uint16_t>(p + 2 * (at + d + j)) << 16 * (j & 1);
+                    } else {
+                        for (uint32_t i = 0; i < WORDS; i++) w[i] = d < dim ? gld<u4>(p + (WIDE16 ? 2 : 4) * (at + d) + 16 * i) : u4{0, 0, 0, 0};
+                    }
+                };
+                if constexpr (SRC == Q8_0) {
+                    const size_t e = at + min(d, dim - 8);
+                    kc[r] = gld<uint2>(a.c.k + e);
+                    vc[r] = gld<uint2>(a.c.v + e);
+                    kf[r] = gld<uint16_t>(a.c.ks + e / 32);
+                    vf[r] = gld<uint16_t>(a.c.vs + e / 32);
+                    if (d >= dim) kf[r] = vf[r] = 0;
+                } else {
+                    load(a.c.k, kw[r]);
+                    load(a.c.v, vw[r]);
                 }
             }
         };
+        // To LDS, as the products take it.
         auto store = [&](uint32_t buf) {
-            if constexpr (!DIRECT) {
+            if constexpr (DIRECT) return;
 #pragma unroll
-                for (uint32_t r = 0; r < ROUNDS; r++) {
-                    const uint32_t u = r * kBlock + tid, line = u / PER;
-                    if constexpr (Q8)
-                        if (u % PER % 4 == 0) scales[buf][u % PER / 4][line] = kf[r];
+            for (uint32_t r = 0; r < ROUNDS; r++) {
+                const uint32_t u = r * kBlock + tid, line = u / PER;
+                auto put = [&](const u4* w, uint32_t b) {
 #pragma unroll
-                    for (uint32_t w = 0; w < WORDS; w++) {
-                        const uint32_t at = line * D * sizeof(T) + ((u % PER * WORDS + w) ^ turn<CH>(line)) * 16;
-                        *reinterpret_cast<Word*>(lds[buf] + at) = kw[r][w];
-                        *reinterpret_cast<Word*>(lds[2 + buf] + at) = vw[r][w];
-                    }
+                    for (uint32_t i = 0; i < (F ? 2 : 1); i++)
+                        *reinterpret_cast<u4*>(lds[b] + line * D * sizeof(T) + ((u % PER * (F ? 2 : 1) + i) ^ turn<CH>(line)) * 16) = w[i];
+                };
+                if constexpr (Q8) {
+                    // code + 128 in the low bits of 1024 + 128 + code, less 1152: the code; V's times its
+                    // scale, rounded once
+                    auto values = [&](uint2 c, auto f) {
+                        u4 w;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const uint32_t x = __builtin_amdgcn_perm(0x64646464u, (j < 2 ? c.x : c.y) ^ 0x80808080u, j & 1 ? 0x07030702u : 0x07010700u);
+                            w[j] = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(h2, x) - h2((_Float16)1152.f)));
+                        }
+                        return w;
+                    };
+                    const h2 f = h2(__builtin_bit_cast(_Float16, (uint16_t)vf[r]));
+                    const u4 k = values(kc[r], [](h2 x) { return x; }), v = values(vc[r], [&](h2 x) { return x * f; });
+                    put(&k, buf);
+                    put(&v, 2 + buf);
+                    if (u % PER % 4 == 0) scales[buf][u % PER / 4][line] = h2f(kf[r]);
+                } else if constexpr (SRC == Q8_0) {
+                    auto one = [&](uint2 c, uint32_t f16, uint32_t b) {
+                        u4 w[2];
+                        const float f = h2f(f16);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) w[j / 4][j % 4] = __float_as_uint((float)(int8_t)((j < 4 ? c.x : c.y) >> 8 * (j & 3)) * f);
+                        put(w, b);
+                    };
+                    one(kc[r], kf[r], buf);
+                    one(vc[r], vf[r], 2 + buf);
+                } else if constexpr (F && WIDE16) {
+                    auto one = [&](const u4& h, uint32_t b) {
+                        u4 w[2];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const uint32_t v = j & 1 ? h[j / 2] >> 16 : h[j / 2] & 0xffff;
+                            w[j / 4][j % 4] = SRC == F16 ? __float_as_uint(h2f(v)) : v << 16;
+                        }
+                        put(w, b);
+                    };
+                    one(kw[r][0], buf);
+                    one(vw[r][0], 2 + buf);
+                } else {
+                    put(kw[r], buf);
+                    put(vw[r], 2 + buf);
                 }
             }
         };
@@ -476,7 +467,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         const uint32_t vrow = 4 * half + lane % 16 / 4;
         const uint32_t v_at = F ? 4 * half * D * 4 + n % 4 * 4
                                 : vrow * D * 2 + (((lane >> 4 & 1) * 2 + (lane % 4 >> 1)) ^ turn<CH>(vrow)) * 16 + lane % 2 * 8;
-        auto step = [&](uint32_t k0, auto masked, auto buf) {
+        auto step = [&](uint32_t k0, auto masked, auto buf, auto between) {
             const uint8_t *kt = lds[buf], *vt = lds[2 + buf];
             f16v sc[NS];
 #pragma unroll
@@ -489,6 +480,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     const f4 x = *reinterpret_cast<const f4*>(kt + (opaque(k_at) ^ g * 32));
 #pragma unroll
                     for (uint32_t j = 0; j < 4; j++) sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], q[4 * g + j], sc[0], 0, 0, 0);
+                    between(g, D / 8);
                 }
             } else {
                 auto product = [&](const T8& x, const T8& y, const f16v& z) {
@@ -513,18 +505,20 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 #pragma unroll
                                 for (uint32_t j = 0; j < 4; j++) sc[m][4 * i + j] = fmaf(x[4 * i + j], f[j], sc[m][4 * i + j]);
                             }
+                            between(g / 2 * NS + m, NS * D / 32);
                         }
                 } else {
 // four parts of K are on their way ahead of a product
-                    constexpr uint32_t N = NS * D / 16;
-                    T8 x[4];
+                    constexpr uint32_t N = NS * D / 16, AHEAD = 4;
+                    T8 x[AHEAD];
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i++) x[i] = k_part(i / NS, i % NS);
+                    for (uint32_t i = 0; i < AHEAD; i++) x[i] = k_part(i / NS, i % NS);
                     in_order();
 #pragma unroll
                     for (uint32_t i = 0; i < N; i++) {
-                        sc[i % NS] = product(x[i % 4], q[i / NS], sc[i % NS]);
-                        if (i + 4 < N) x[i % 4] = k_part((i + 4) / NS, (i + 4) % NS);
+                        sc[i % NS] = product(x[i % AHEAD], q[i / NS], sc[i % NS]);
+                        if (i + AHEAD < N) x[i % AHEAD] = k_part((i + AHEAD) / NS, (i + AHEAD) % NS);
+                        between(i, N);
                         in_order();
                     }
                 }
@@ -689,7 +683,8 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 __syncthreads();  // before K and V go there
             }
         }
-        fetch(lo, 0);
+#pragma unroll
+        for (uint32_t r = 0; r < ROUNDS; r++) fetch(lo, 0, r);
         {
             if constexpr (F) {
 #pragma unroll
@@ -721,28 +716,38 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
             }
         }
         store(0);
-        if (lo + KT < hi) look(lo + KT);
+        look(lo + KT);
         meet();
         // A step and what comes in meanwhile.  Those that all of the workgroup's rows see whole have
         // a loop of their own, without masks, in which a buffer's place is a constant.
         const uint32_t clear = same(min(hi, (a.seen ? s.c0 : s.c0 + run.i * kTileRows / a.group + 1) / KT * KT));
-        auto both = [&](uint32_t k0, auto masked, auto buf) {
-            const bool more = k0 + KT < hi;
-            if (more) {
-                fetch(k0 + KT, buf ^ 1);
-                if (k0 + 2 * KT < hi) look(k0 + 2 * KT);
-            }
-            if (k0 < most) step(k0, masked, buf);
-            if (more) store(buf ^ 1);
+        // between the products of the scores, i of n: the loads of the next step, then the pages of that after it
+        auto loads = [&](uint32_t k0, uint32_t buf, uint32_t i, uint32_t n) {
+#pragma unroll
+            for (uint32_t r = 0; r < ROUNDS; r++)
+                if (i == r * n / ROUNDS) fetch(k0 + KT, buf ^ 1, r);
+            if (i == n - 1) look(k0 + 2 * KT);
+        };
+        auto both = [&](uint32_t k0, auto buf) {
+            step(k0, std::false_type(), buf, [&](uint32_t i, uint32_t n) { loads(k0, buf, i, n); });
+            store(buf ^ 1);
             meet();
         };
         uint32_t k0 = lo;
-        for (; k0 + 2 * KT <= clear; k0 += 2 * KT) {
-            both(k0, std::false_type(), std::integral_constant<uint32_t, 0>());
-            both(k0 + KT, std::false_type(), std::integral_constant<uint32_t, 1>());
-        }
+        if (rows)
+            for (; k0 + 2 * KT <= clear && k0 + 2 * KT < hi; k0 += 2 * KT) {
+                both(k0, std::integral_constant<uint32_t, 0>());
+                both(k0 + KT, std::integral_constant<uint32_t, 1>());
+            }
 #pragma nounroll
-        for (uint32_t buf = 0; k0 < hi; k0 += KT, buf ^= 1) both(k0, std::true_type(), buf);
+        for (uint32_t buf = 0; k0 < hi; k0 += KT, buf ^= 1) {
+            const bool more = k0 + KT < hi;
+            if (more)
+                for (uint32_t i = 0; i < ROUNDS; i++) loads(k0, buf, i, ROUNDS);
+            if (k0 < most) step(k0, std::true_type(), buf, [](uint32_t, uint32_t) {});
+            if (more) store(buf ^ 1);
+            meet();
+        }
         // the steps left out, a key at a time: its row goes through the wave's part of LDS
         float* part = reinterpret_cast<float*>(lds[wv]);
         if (odd != ~0u) {
@@ -861,11 +866,10 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
                (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && a.q.kind == BF16 && a.out.kind == BF16));
     a.one_page = a.c.page % (512 / a.wide) == 0 && a.c.ts * 16 * es < 1u << 31;
-    // t / page for t < 2^31: t * ceil(2^shift / page) >> shift
-    uint32_t log = 0;
-    while ((1ull << log) < a.c.page) log++;
-    a.page_shift = 31 + log;
-    a.page_mul = (uint32_t)(((1ull << a.page_shift) + a.c.page - 1) / a.c.page);
+    // t / page for t < 2^31: 2 t * ceil(2^(31 + log) / page) >> 32 + log
+    a.page_log = 0;
+    while ((1ull << a.page_log) < a.c.page) a.page_log++;
+    a.page_mul = (uint32_t)(((1ull << (31 + a.page_log)) + a.c.page - 1) / a.c.page);
     a.sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
     a.c2 = a.scale == 0.f ? 1.f : std::max(std::fabs(a.scale) * kLog2e, 1.17549435e-38f);
     const uint64_t tiles = ((uint64_t)a.n * a.group / kTileRows + a.r.batch) * a.c.kvheads;
@@ -880,7 +884,7 @@ template <class T, uint32_t SRC> static void launch_many(const PageMany& a, hipS
     else hipLaunchKernelGGL((k_page_many<T, 256, SRC>), grid, block, 0, s, a);
 }
 void launch_page_many(const PageMany& a, hipStream_t s) {
-    const bool direct = a.kv_wide && a.c.dim == a.wide;
+    const bool direct = a.kv_wide && a.one_page && a.c.dim == a.wide;
     if (a.narrow) {
         if (a.c.kind == Q8_0) launch_many<_Float16, Q8_0>(a, s);
         else if (a.c.kind == F16) direct ? launch_many<_Float16, kDirect>(a, s) : launch_many<_Float16, kAny>(a, s);

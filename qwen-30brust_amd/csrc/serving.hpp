@@ -119,9 +119,9 @@ struct PageMany {
     // by page_many_plan
     uint32_t group, wide, runs;     // query heads of a KV head, width of the tiles, workgroups
     bool narrow;                    // products of 16 bits, else of 32
-    bool one_page;                  // eight rows of 64 values (or as many bytes of others) lie in one page
+    bool one_page;                  // the rows that a wave loads at a time lie in one page
     bool q_wide, out_wide, kv_wide; // rows aligned to what is read and written at a time
-    uint32_t page_mul, page_shift;  // t / page
+    uint32_t page_mul, page_log;    // t / page
     float sign, c2;                 // scale * log2 e = sign * c2
     void* work;
 };
