@@ -333,14 +333,30 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         // keys behind the tile's last are read as that one: none of them is seen
         constexpr uint32_t ROUNDS = KT * D / 8 / kBlock;  // groups of 8 values a thread
         constexpr uint32_t PER = D / 8, LINES = 64 / PER; // of a row; rows of a wave's load
-        int32_t pages[ROUNDS];
-        auto group_row = [&](uint32_t r) { return DIRECT ? (r * kWaves + wv) * LINES + lane / PER : (r * kBlock + tid) / PER; };
-        // (kDirect: the rows of a wave's load lie in one page, whose place is computed once for all lanes)
-        auto first_row = [&](uint32_t k0, uint32_t r) { return min(k0 + (r * kWaves + wv) * LINES, (end - 1) / LINES * LINES); };
+        auto group_row = [&](uint32_t r) { return (r * kBlock + tid) / PER; };
+        // kDirect: the rows of a wave's load lie in one page.  Lane r (and r + ROUNDS ..) finds round r's first
+        // row and its place, which the round then has for all lanes.
+        int32_t pages[DIRECT ? 1 : ROUNDS];
+        uint32_t first = 0;    // that row
+        uint64_t first_at = 0;  // and its place, in bytes
         auto look = [&](uint32_t k0) {
+            if constexpr (DIRECT) {
+                first = min(k0 + (lane % ROUNDS * kWaves + wv) * LINES, (end - 1) / LINES * LINES);
+                pages[0] = page_of(first);
+            } else {
 #pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; r++) pages[r] = page_of(DIRECT ? first_row(k0, r) : min(k0 + group_row(r), end - 1));
+                for (uint32_t r = 0; r < ROUNDS; r++) pages[r] = page_of(min(k0 + group_row(r), end - 1));
+            }
         };
+        auto found = [&] {  // what look() was after
+            if constexpr (DIRECT) {
+                const bool fine = (uint32_t)pages[0] < a.c.count;
+                bad = fine ? bad : min(bad, first);
+                const uint32_t in = first - page_number(first) * a.c.page;
+                first_at = (uint64_t)(fine ? (uint32_t)pages[0] : 0u) * (uint32_t)(2 * a.c.ps) + in * (uint32_t)(2 * a.c.ts);
+            }
+        };
+        const uint8_t *kbase = a.c.k + 2 * base, *vbase = a.c.v + 2 * base;
         // What a thread holds of a step meanwhile, as it is in the cache: eight values of K and of V each.
         constexpr bool WIDE16 = !F || SRC == F16 || SRC == BF16;  // 16 bytes of 16-bit values
         constexpr uint32_t WORDS = SRC == Q8_0 || DIRECT ? 0 : WIDE16 ? 1 : 2;
@@ -351,15 +367,20 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
             if constexpr (DIRECT) {
                 // 16 bytes a lane from its own address to LDS.  In assembly, as the compiler lets every
                 // later LDS read wait for such loads, of whatever buffer; meet() waits for them.
-                const uint32_t t = same(first_row(k0, r)), line = lane / PER;
-                const size_t at = place(t, (int32_t)same((uint32_t)pages[r]));
+                if (r == 0) found();
+                const uint32_t line = lane / PER, t = __builtin_amdgcn_readlane(first, r);
+                const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(first_at >> 32), r) << 32 |
+                                    (uint32_t)__builtin_amdgcn_readlane((uint32_t)first_at, r);
                 constexpr bool SAME = turn<CH>(kWaves * LINES) == 0;  // a row's turn in every round
                 const uint32_t chunk = 16 * (lane % PER ^ turn<CH>((SAME ? wv : r * kWaves + wv) * LINES + line));
-                const uint32_t off = min(line, end - 1 - t) * (uint32_t)a.c.ts * 2 + chunk;
+                // rows behind the tile's last are read as that one
+                const uint32_t off = min(line, end - 1 - t) * (uint32_t)(2 * a.c.ts) + chunk;
 #if defined(__HIP_DEVICE_COMPILE__)
                 const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(a.c.k + 2 * at) : "memory");
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + 2 * TILE), "v"(off), "s"(a.c.v + 2 * at) : "memory");
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(kbase + at) : "memory");
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + 2 * TILE), "v"(off), "s"(vbase + at) : "memory");
+#else
+                (void)at, (void)off;
 #endif
             } else {
                 const size_t at = place(min(k0 + group_row(r), end - 1), pages[r]);
@@ -865,7 +886,7 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     // products of 16 bits: of the cache's own type, or of f16 where bf16 queries read Q8_0
     a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
                (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && a.q.kind == BF16 && a.out.kind == BF16));
-    a.one_page = a.c.page % (512 / a.wide) == 0 && a.c.ts * 16 * es < 1u << 31;
+    a.one_page = a.c.page % (512 / a.wide) == 0 && a.c.ps * 2 >> 32 == 0 && (unsigned __int128)a.c.page * a.c.ts * 2 >> 32 == 0;
     // t / page for t < 2^31: 2 t * ceil(2^(31 + log) / page) >> 32 + log
     a.page_log = 0;
     while ((1ull << a.page_log) < a.c.page) a.page_log++;
