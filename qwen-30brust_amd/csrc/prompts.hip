@@ -23,8 +23,6 @@ namespace qh {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kTileRows = 128;  // query rows of a tile, 32 a wave
-constexpr uint32_t kRunKeys = 128;   // keys of a run at least
-constexpr uint32_t kTileKeys = 256;  // a tile's start and end, in keys
 constexpr uint32_t kXcds = 8;
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -79,7 +77,7 @@ __device__ __forceinline__ Seq seq_of(const PageMany& a, const Bounds& q) {
     s.tiles = (uint32_t)(((uint64_t)s.count * a.group + kTileRows - 1) / kTileRows);
     s.bad = s.len < 0 || s.count > (uint32_t)s.len || (a.seen && s.count > kTreeMost);
     s.c0 = s.bad ? 0 : (uint32_t)s.len - s.count;
-    s.first = s.bad ? 1 : a.seen ? (uint64_t)(kTileKeys + s.len) * a.group : (uint64_t)(kTileKeys + s.c0 + 1) * a.group + kTileRows - 1;
+    s.first = s.bad ? 1 : a.seen ? (uint64_t)(a.tile_keys + s.len) * a.group : (uint64_t)(a.tile_keys + s.c0 + 1) * a.group + kTileRows - 1;
     s.step = s.bad || a.seen ? 0 : kTileRows;
     return s;
 }
@@ -92,32 +90,29 @@ __device__ __forceinline__ uint32_t end_of(const PageMany& a, const Seq& s, uint
 // The key at which the part from x on of a tile begins: at whole steps.
 __device__ __forceinline__ uint32_t key_at(const PageMany& a, uint64_t x, uint32_t end, uint32_t step) {
     const uint64_t k = x / a.group;
-    return k <= kTileKeys ? 0 : (uint32_t)min((uint64_t)end, (k - kTileKeys) / step * step);
+    return k <= a.tile_keys ? 0 : (uint32_t)min((uint64_t)end, (k - a.tile_keys) / step * step);
 }
 
 __device__ __forceinline__ uint64_t run_begin(uint64_t total, uint32_t runs, uint32_t i) {
     return total / runs * i + min((uint64_t)i, total % runs);
 }
 
-// What the join has to know of the tile that a run begins inside of.
+// What the join has to know of the tile that a run begins inside of, where it is the
+// first to: the tile's first row (times the group), rows and KV head, and the last run that
+// holds a part of it.  rows 0: nothing to join.
 struct ManyMark {
-    uint64_t at, cost;            // the tile's own place and cost; cost 0: the run begins with a tile
-    uint32_t row, rows, kv, end;  // its first row (times the group), rows, KV head, keys
-};
-struct ManyHead {
-    uint64_t total;
-    uint32_t runs, pad;
+    uint32_t row, rows, kv, last;
 };
 size_t page_many_bytes(const PageMany& a) {
     const size_t slots = (size_t)a.runs * 2 * kTileRows;
-    return slots * a.wide * 4 + slots * 8 + sizeof(ManyHead) + a.runs * sizeof(ManyMark);
+    return slots * a.wide * 4 + slots * 8 + 16 + a.runs * sizeof(ManyMark);
 }
 __device__ __forceinline__ float* part_o(const PageMany& a, size_t slot) { return (float*)a.work + slot * kTileRows * a.wide; }
 __device__ __forceinline__ float2* part_ml(const PageMany& a, size_t slot) {
     return (float2*)((float*)a.work + (size_t)a.runs * 2 * kTileRows * a.wide) + slot * kTileRows;
 }
-__device__ __forceinline__ ManyHead* head_of(const PageMany& a) { return (ManyHead*)part_ml(a, (size_t)a.runs * 2); }
-__device__ __forceinline__ ManyMark* mark_of(const PageMany& a, uint32_t run) { return (ManyMark*)(head_of(a) + 1) + run; }
+__device__ __forceinline__ uint32_t* runs_of(const PageMany& a) { return (uint32_t*)part_ml(a, (size_t)a.runs * 2); }
+__device__ __forceinline__ ManyMark* mark_of(const PageMany& a, uint32_t run) { return (ManyMark*)(runs_of(a) + 4) + run; }
 
 // A workgroup's run.
 struct Run {
@@ -156,15 +151,15 @@ struct Run {
         uint64_t total = 0;
         for (uint32_t w = 0; w < kWaves; w++) total += part[w];
         total = same64(total);
-        const uint32_t runs = (uint32_t)max((uint64_t)1, min((uint64_t)a.runs, total / (kRunKeys * (uint64_t)a.group)));
-        if (blockIdx.x == 0 && tid == 0) *head_of(a) = {total, total ? runs : 0, 0};
+        const uint32_t runs = (uint32_t)max((uint64_t)1, min((uint64_t)a.runs, total / ((uint64_t)a.run_keys * a.group)));
+        if (blockIdx.x == 0 && tid == 0) *runs_of(a) = total ? runs : 0;
         // runs that lie beside each other, and read the same keys, on one XCD
         const uint32_t per = (runs + kXcds - 1) / kXcds;
         run = blockIdx.x % kXcds * per + blockIdx.x / kXcds;
         if (!total || blockIdx.x / kXcds >= per || run >= runs) return false;
-        x = run_begin(total, runs, run);
-        end = run_begin(total, runs, run + 1);
-        if (tid == 0) mark_of(a, run)->cost = 0;
+        x = same64(run_begin(total, runs, run));
+        end = same64(run_begin(total, runs, run + 1));
+        if (tid == 0) mark_of(a, run)->rows = 0;
         uint64_t base = 0;
         for (uint32_t j = 0; j < a.r.batch; j += kBlock) {
             const uint64_t c = j ? cost(j + tid) : mine;
@@ -192,7 +187,7 @@ struct Run {
         read(a);
         const uint64_t each = same64(s.upto(s.tiles)), in = same64(x - found[1]);
         if (!each) return false;
-        kv = (uint32_t)(in / each);
+        kv = same((uint32_t)(in / each));
         off = in - kv * each;
         if (kv >= G) return false;
         uint32_t lo = 0, hi = s.tiles;  // the last tile whose place is not behind off
@@ -201,11 +196,17 @@ struct Run {
             if (s.upto(mid) <= off) lo = mid;
             else hi = mid;
         }
-        i = lo;
-        off -= s.upto(lo);
-        if (off && tid == 0)
-            *mark_of(a, run) = {x - off, s.cost(i), s.f0 * a.group + i * kTileRows,
-                                min(kTileRows, s.count * a.group - i * kTileRows), kv, end_of(a, s, i)};
+        i = same(lo);
+        off = same64(off - s.upto(i));
+        if (off && tid == 0 && !s.bad && run_begin(total, runs, run - 1) <= x - off) {
+            uint32_t last = run;
+            const uint64_t to = x - off + s.cost(i);
+            if (end < to) {  // the run of the tile's last place
+                const uint64_t each = total / runs, more = total % runs, wide = more * (each + 1);
+                last = (uint32_t)(to - 1 < wide ? (to - 1) / (each + 1) : more + (to - 1 - wide) / each);
+            }
+            *mark_of(a, run) = {s.f0 * a.group + i * kTileRows, min(kTileRows, s.count * a.group - i * kTileRows), kv, last};
+        }
         return true;
     }
     __device__ __forceinline__ uint64_t here() const { return min(s.cost(i) - off, end - x); }
@@ -259,10 +260,10 @@ constexpr uint32_t kDirect = 100, kAny = 101;
 // types keys 16 c + 8 (e / 4) + 4 (lane / 32) + e % 4 are element e, for V^T read by the
 // transposing LDS read.  K and V of the next step come in while one is worked on.
 template <class T, uint32_t D, uint32_t SRC>
-__global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany a) {
+__global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std::is_same<T, _Float16>::value) ? 1 : 2) void k_page_many(PageMany a) {
     constexpr bool F = std::is_same<T, float>::value, H = std::is_same<T, _Float16>::value;
     constexpr bool DIRECT = SRC == kDirect, Q8 = SRC == Q8_0 && !F;
-    constexpr uint32_t KT = F || D == 256 ? 32 : 64;  // keys of a step
+    constexpr uint32_t KT = F || Q8 || D == 256 ? 32 : 64;  // keys of a step
     constexpr uint32_t NS = KT / 32, ND = D / 32, CH = D * sizeof(T) / 16, TILE = KT * D * sizeof(T);
     constexpr uint32_t NQ = F ? D / 2 : D / 16;
     constexpr uint32_t QKIND = F ? F32 : H && !Q8 ? F16 : BF16;  // of queries that are loaded as they are
@@ -295,13 +296,21 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         const bool mine = n < rows;
         const uint32_t dim = a.c.dim;
         const uint32_t token = mine ? r / a.group : 0, row = s.f0 + token, h = run.kv * a.group + (mine ? r % a.group : 0);
-        const size_t to = (size_t)row * a.out.row + (size_t)h * a.out.head;
+        // where a row of the wave's goes; found anew where it is wanted, to hold no registers
+        auto out_at = [&](uint32_t n) {
+            const uint32_t r = min(r0 + n, R - 1);
+            return (size_t)(s.f0 + r / a.group) * a.out.row + (size_t)(run.kv * a.group + r % a.group) * a.out.head;
+        };
         if (s.bad) {
             if (run.off == 0 && mine)
-                for (uint32_t d = half * 4; d < dim; d += 8) put_row(a, dim, to, d, f4(__builtin_nanf("")));
+                for (uint32_t d = half * 4; d < dim; d += 8) put_row(a, dim, out_at(n), d, f4(__builtin_nanf("")));
             continue;
         }
-        if (lo >= hi) continue;
+        const size_t slot = (size_t)run.run * 2 + (run.off == 0);  // of a part
+        if (lo >= hi) {  // no step of its own
+            if (mine && half == 0) part_ml(a, slot)[wv * 32 + n] = make_float2(-INFINITY, 0.f);
+            continue;
+        }
         // behind the last key that one of the wave's rows sees
         const uint32_t most = !rows ? 0 : a.seen ? end : s.c0 + (r0 + rows - 1) / a.group + 1;
         const uint32_t own = a.seen ? end : s.c0 + token + 1;  // behind this row's last
@@ -331,8 +340,8 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
             return (size_t)page * a.c.ps + (size_t)(t - page_number(t) * a.c.page) * a.c.ts + base;
         };
         // keys behind the tile's last are read as that one: none of them is seen
-        constexpr uint32_t ROUNDS = KT * D / 8 / kBlock;  // groups of 8 values a thread
-        constexpr uint32_t PER = D / 8, LINES = 64 / PER; // of a row; rows of a wave's load
+        // a thread takes groups of 8 values, kDirect 16 bytes; PER of a row, LINES rows a wave
+        constexpr uint32_t PER = DIRECT ? CH : D / 8, LINES = 64 / PER, ROUNDS = KT * PER / kBlock;
         auto group_row = [&](uint32_t r) { return (r * kBlock + tid) / PER; };
         // kDirect: the rows of a wave's load lie in one page.  Lane r (and r + ROUNDS ..) finds round r's first
         // row and its place, which the round then has for all lanes.
@@ -345,7 +354,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 pages[0] = page_of(first);
             } else {
 #pragma unroll
-                for (uint32_t r = 0; r < ROUNDS; r++) pages[r] = page_of(min(k0 + group_row(r), end - 1));
+                    for (uint32_t r = 0; r < ROUNDS && SRC != kAny; r++) pages[r] = page_of(min(k0 + group_row(r), end - 1));
             }
         };
         auto found = [&] {  // what look() was after
@@ -353,16 +362,15 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 const bool fine = (uint32_t)pages[0] < a.c.count;
                 bad = fine ? bad : min(bad, first);
                 const uint32_t in = first - page_number(first) * a.c.page;
-                first_at = (uint64_t)(fine ? (uint32_t)pages[0] : 0u) * (uint32_t)(2 * a.c.ps) + in * (uint32_t)(2 * a.c.ts);
+                first_at = (uint64_t)(fine ? (uint32_t)pages[0] : 0u) * (uint32_t)(sizeof(T) * a.c.ps) + in * (uint32_t)(sizeof(T) * a.c.ts);
             }
         };
-        const uint8_t *kbase = a.c.k + 2 * base, *vbase = a.c.v + 2 * base;
+        [[maybe_unused]] const uint8_t *kbase = a.c.k + sizeof(T) * base, *vbase = a.c.v + sizeof(T) * base;
         // What a thread holds of a step meanwhile, as it is in the cache: eight values of K and of V each.
-        constexpr bool WIDE16 = !F || SRC == F16 || SRC == BF16;  // 16 bytes of 16-bit values
-        constexpr uint32_t WORDS = SRC == Q8_0 || DIRECT ? 0 : WIDE16 ? 1 : 2;
-        u4 kw[WORDS ? ROUNDS : 1][WORDS ? WORDS : 1], vw[WORDS ? ROUNDS : 1][WORDS ? WORDS : 1];
-        uint2 kc[SRC == Q8_0 ? ROUNDS : 1], vc[SRC == Q8_0 ? ROUNDS : 1];       // codes
-        uint32_t kf[SRC == Q8_0 ? ROUNDS : 1], vf[SRC == Q8_0 ? ROUNDS : 1];    // scales
+        constexpr bool HELD16 = SRC == F16 || SRC == BF16;
+        u4 kw[HELD16 ? ROUNDS : 1], vw[HELD16 ? ROUNDS : 1];
+        uint2 kc[SRC == Q8_0 ? ROUNDS : 1], vc[SRC == Q8_0 ? ROUNDS : 1];     // codes
+        uint32_t kf[SRC == Q8_0 ? ROUNDS : 1], vf[SRC == Q8_0 ? ROUNDS : 1];  // scales
         auto fetch = [&](uint32_t k0, uint32_t buf, uint32_t r) {
             if constexpr (DIRECT) {
                 // 16 bytes a lane from its own address to LDS.  In assembly, as the compiler lets every
@@ -374,7 +382,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 constexpr bool SAME = turn<CH>(kWaves * LINES) == 0;  // a row's turn in every round
                 const uint32_t chunk = 16 * (lane % PER ^ turn<CH>((SAME ? wv : r * kWaves + wv) * LINES + line));
                 // rows behind the tile's last are read as that one
-                const uint32_t off = min(line, end - 1 - t) * (uint32_t)(2 * a.c.ts) + chunk;
+                const uint32_t off = min(line, end - 1 - t) * (uint32_t)(sizeof(T) * a.c.ts) + chunk;
 #if defined(__HIP_DEVICE_COMPILE__)
                 const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(kbase + at) : "memory");
@@ -385,31 +393,6 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
             } else {
                 const size_t at = place(min(k0 + group_row(r), end - 1), pages[r]);
                 const uint32_t d = (r * kBlock + tid) % PER * 8;
-                auto load = [&](const uint8_t* p, u4* w) {
-                    if constexpr (F && SRC == kAny) {
-                        auto each = [&](auto kind) {
-                            const _Float16* sc = p == a.c.k ? a.c.ks : a.c.vs;
-#pragma unroll
-                            for (uint32_t j = 0; j < 8; j++) {
-                                const size_t e = at + min(d + j, dim - 1);
-                                float x = elem<kind()>(p, e);
-                                if constexpr (kind() == Q8_0) x *= (float)gld<_Float16>(sc + e / 32);
-                                w[j / 4][j % 4] = d + j < dim ? __float_as_uint(x) : 0u;
-                            }
-                        };
-                        if (a.c.kind == F32) each(std::integral_constant<uint32_t, F32>());
-                        else if (a.c.kind == F16) each(std::integral_constant<uint32_t, F16>());
-                        else if (a.c.kind == BF16) each(std::integral_constant<uint32_t, BF16>());
-                        else each(std::integral_constant<uint32_t, Q8_0>());
-                    } else if (!F && !a.kv_wide) {
-                        w[0] = u4{0, 0, 0, 0};
-#pragma unroll
-                        for (uint32_t j = 0; j < 8; j++)
-                            if (d + j < dim) w[0][j / 2] |= (uint32_t)gld<uint16_t>(p + 2 * (at + d + j)) << 16 * (j & 1);
-                    } else {
-                        for (uint32_t i = 0; i < WORDS; i++) w[i] = d < dim ? gld<u4>(p + (WIDE16 ? 2 : 4) * (at + d) + 16 * i) : u4{0, 0, 0, 0};
-                    }
-                };
                 if constexpr (SRC == Q8_0) {
                     const size_t e = at + min(d, dim - 8);
                     kc[r] = gld<uint2>(a.c.k + e);
@@ -417,15 +400,17 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     kf[r] = gld<uint16_t>(a.c.ks + e / 32);
                     vf[r] = gld<uint16_t>(a.c.vs + e / 32);
                     if (d >= dim) kf[r] = vf[r] = 0;
-                } else {
-                    load(a.c.k, kw[r]);
-                    load(a.c.v, vw[r]);
+                } else if constexpr (HELD16) {
+                    const size_t e = 2 * (at + min(d, dim - 8));
+                    kw[r] = gld<u4>(a.c.k + e);
+                    vw[r] = gld<u4>(a.c.v + e);
+                    if (d >= dim) kw[r] = vw[r] = u4{0, 0, 0, 0};
                 }
             }
         };
         // To LDS, as the products take it.
         auto store = [&](uint32_t buf) {
-            if constexpr (DIRECT) return;
+            if constexpr (DIRECT || SRC == kAny) return;
 #pragma unroll
             for (uint32_t r = 0; r < ROUNDS; r++) {
                 const uint32_t u = r * kBlock + tid, line = u / PER;
@@ -461,7 +446,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     };
                     one(kc[r], kf[r], buf);
                     one(vc[r], vf[r], 2 + buf);
-                } else if constexpr (F && WIDE16) {
+                } else if constexpr (HELD16) {
                     auto one = [&](const u4& h, uint32_t b) {
                         u4 w[2];
 #pragma unroll
@@ -471,11 +456,40 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                         }
                         put(w, b);
                     };
-                    one(kw[r][0], buf);
-                    one(vw[r][0], 2 + buf);
-                } else {
-                    put(kw[r], buf);
-                    put(vw[r], 2 + buf);
+                    one(kw[r], buf);
+                    one(vw[r], 2 + buf);
+                }
+            }
+        };
+        // kAny: a value at a time, straight to LDS (16-bit rows aligned to 8 values: eight)
+        auto bring = [&](uint32_t k0, uint32_t buf) {
+#pragma nounroll
+            for (uint32_t r = 0; r < ROUNDS; r++) {
+                const uint32_t line = group_row(r), t = min(k0 + line, end - 1), d = (r * kBlock + tid) % PER * 8;
+                const size_t at = place(t, page_of(t)) + d;
+                uint8_t *ko = lds[buf] + line * D * sizeof(T), *vo = lds[2 + buf] + line * D * sizeof(T);
+                auto to = [&](uint32_t j) { return ((d + j) * sizeof(T) / 16 ^ turn<CH>(line)) * 16 + (d + j) * sizeof(T) % 16; };
+                if (!F && a.kv_wide) {
+                    u4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+                    if (d < dim) k = gld<u4>(a.c.k + 2 * at), v = gld<u4>(a.c.v + 2 * at);
+                    *reinterpret_cast<u4*>(ko + to(0)) = k;
+                    *reinterpret_cast<u4*>(vo + to(0)) = v;
+                    continue;
+                }
+#pragma nounroll
+                for (uint32_t j = 0; j < 8; j++) {
+                    const bool in = d + j < dim;
+                    if constexpr (F) {
+                        auto value = [&](const uint8_t* p, const _Float16* sc) {
+                            if (!in) return 0.f;
+                            return a.c.kind == Q8_0 ? elem<Q8_0>(p, at + j) * (float)gld<_Float16>(sc + (at + j) / 32) : elem_kind(a.c.kind, p, at + j);
+                        };
+                        *reinterpret_cast<float*>(ko + to(j)) = value(a.c.k, a.c.ks);
+                        *reinterpret_cast<float*>(vo + to(j)) = value(a.c.v, a.c.vs);
+                    } else {
+                        *reinterpret_cast<uint16_t*>(ko + to(j)) = in ? gld<uint16_t>(a.c.k + 2 * (at + j)) : (uint16_t)0;
+                        *reinterpret_cast<uint16_t*>(vo + to(j)) = in ? gld<uint16_t>(a.c.v + 2 * (at + j)) : (uint16_t)0;
+                    }
                 }
             }
         };
@@ -508,7 +522,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     if constexpr (H) return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, z, 0, 0, 0);
                     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, z, 0, 0, 0);
                 };
-                auto k_part = [&](uint32_t g, uint32_t m) { return *reinterpret_cast<const T8*>(kt + (k_at ^ g * 32) + m * 32 * D * 2); };
+                auto k_part = [&](uint32_t g, uint32_t m) { return *reinterpret_cast<const T8*>(kt + ((Q8 ? opaque(k_at) : k_at) ^ g * 32) + m * 32 * D * 2); };
                 if constexpr (Q8) {
                     // a block's codes are exact, its scale is the score's
 #pragma unroll
@@ -527,9 +541,10 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                                 for (uint32_t j = 0; j < 4; j++) sc[m][4 * i + j] = fmaf(x[4 * i + j], f[j], sc[m][4 * i + j]);
                             }
                             between(g / 2 * NS + m, NS * D / 32);
+                            in_order();
                         }
                 } else {
-// four parts of K are on their way ahead of a product
+                    // four parts of K are on their way ahead of a product
                     constexpr uint32_t N = NS * D / 16, AHEAD = 4;
                     T8 x[AHEAD];
 #pragma unroll
@@ -558,7 +573,7 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 #endif
             };
             T8 x[2][F ? 1 : ND];  // V's parts
-            if constexpr (!F) {
+            if constexpr (!F && !Q8) {
 #pragma unroll
                 for (uint32_t d = 0; d < ND; d++) x[0][d] = v_part(0, d);
                 in_order();
@@ -650,6 +665,9 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     return;
                 }
                 // a step of 16 keys: V's parts and the weights of the next between its products
+                if constexpr (Q8)
+#pragma unroll
+                    for (uint32_t d = 0; d < ND; d++) x[0][d] = v_part(0, d);
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) weights(0, i);
                 in_order();
@@ -704,8 +722,11 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 __syncthreads();  // before K and V go there
             }
         }
+        if constexpr (SRC == kAny) bring(lo, 0);
+        else {
 #pragma unroll
-        for (uint32_t r = 0; r < ROUNDS; r++) fetch(lo, 0, r);
+            for (uint32_t r = 0; r < ROUNDS; r++) fetch(lo, 0, r);
+        }
         {
             if constexpr (F) {
 #pragma unroll
@@ -726,10 +747,12 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                     const int up = top == 0 || top == 255 ? 0 : 141 - (int)top;
                     c2 = ldexpf(c2, -up);
 #pragma unroll
-                    for (uint32_t g = 0; g < NQ; g++)
+                    for (uint32_t g = 0; g < NQ; g++) {
 #pragma unroll
                         for (int j = 0; j < 8; j++)
                             q[g][j] = (T)ldexpf(__uint_as_float(j & 1 ? xq[g][j / 2] & 0xffff0000u : xq[g][j / 2] << 16), up);
+                        in_order();
+                    }
                 } else {
 #pragma unroll
                     for (uint32_t g = 0; g < NQ; g++) q[g] = __builtin_bit_cast(T8, xq[g]);
@@ -749,8 +772,18 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 if (i == r * n / ROUNDS) fetch(k0 + KT, buf ^ 1, r);
             if (i == n - 1) look(k0 + 2 * KT);
         };
+        // Where registers are short (EARLY false) the next step comes in behind the products.
+        constexpr bool EARLY = SRC != kAny && !(D == 256 && !DIRECT);
+        auto late = [&](uint32_t k0, uint32_t buf) {
+            if constexpr (SRC == kAny) bring(k0 + KT, buf ^ 1);
+            else if constexpr (!EARLY)
+                for (uint32_t i = 0; i < ROUNDS; i++) loads(k0, buf, i, ROUNDS);
+        };
         auto both = [&](uint32_t k0, auto buf) {
-            step(k0, std::false_type(), buf, [&](uint32_t i, uint32_t n) { loads(k0, buf, i, n); });
+            step(k0, std::false_type(), buf, [&](uint32_t i, uint32_t n) {
+                if constexpr (EARLY) loads(k0, buf, i, n);
+            });
+            late(k0, buf);
             store(buf ^ 1);
             meet();
         };
@@ -763,15 +796,31 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 #pragma nounroll
         for (uint32_t buf = 0; k0 < hi; k0 += KT, buf ^= 1) {
             const bool more = k0 + KT < hi;
-            if (more)
+            if (EARLY && more)
                 for (uint32_t i = 0; i < ROUNDS; i++) loads(k0, buf, i, ROUNDS);
             if (k0 < most) step(k0, std::true_type(), buf, [](uint32_t, uint32_t) {});
-            if (more) store(buf ^ 1);
+            if (more) {
+                late(k0, buf);
+                store(buf ^ 1);
+            }
             meet();
         }
         // the steps left out, a key at a time: its row goes through the wave's part of LDS
         float* part = reinterpret_cast<float*>(lds[wv]);
         if (odd != ~0u) {
+            // hidden, so that nothing of this is prepared in front of the steps
+            if constexpr (F) {
+#pragma unroll
+                for (uint32_t i = 0; i < NQ; i++) q[i] = __uint_as_float(opaque(__float_as_uint(q[i])));
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < NQ; i++) {
+                    u4 w = __builtin_bit_cast(u4, q[i]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[j] = opaque(w[j]);
+                    q[i] = __builtin_bit_cast(T8, w);
+                }
+            }
             auto value = [&](const uint8_t* p, const _Float16* sc, size_t e) {
                 return a.c.kind == Q8_0 ? elem<Q8_0>(p, e) * (float)gld<_Float16>(sc + e / 32) : elem_kind(a.c.kind, p, e);
             };
@@ -806,11 +855,10 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
         __syncthreads();
         const float2 l2 = halves(L);
         L = bad_at < own ? __builtin_nanf("") : l2.x + l2.y;
-        // out of the wave's part of LDS, whole rows at a time: four values of row n lie in
-        // chunk c ^ n % 16
+        // out of the wave's part of LDS, whole rows at a time: chunk c of four values of row n lies at c ^ n % 16 (or % 8)
+        const size_t to = whole ? out_at(opaque(n)) : 0;
         const float f = !whole ? 1.f : L == 0.f ? 0.f : 1.f / L;
-        const size_t slot = (size_t)run.run * 2 + (run.off == 0);
-        constexpr uint32_t W = TILE / 128;  // dims at a time
+        constexpr uint32_t W = TILE / 128, FLIP = W / 4 < 16 ? W / 4 - 1 : 15;  // dims at a time
 #pragma unroll
         for (uint32_t d0 = 0; d0 < D; d0 += W) {
 #pragma unroll
@@ -819,12 +867,12 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
                 for (uint32_t i = 0; i < 4; i++) {
                     f4 x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
                     if (whole && L == 0.f) x = f4(0.f);
-                    *reinterpret_cast<f4*>(part + n * W + ((8 * d - d0 / 4 + 2 * i + half) ^ (n & 15)) * 4) = x * f;
+                    *reinterpret_cast<f4*>(part + n * W + ((8 * d - d0 / 4 + 2 * i + half) ^ (n & FLIP)) * 4) = x * f;
                 }
             settle();
             for (uint32_t i = lane; i < 32 * W / 4; i += 64) {
                 const uint32_t line = i / (W / 4), c = i % (W / 4);
-                const f4 x = *reinterpret_cast<const f4*>(part + line * W + (c ^ (line & 15)) * 4);
+                const f4 x = *reinterpret_cast<const f4*>(part + line * W + (c ^ (line & FLIP)) * 4);
                 const size_t at = shfl64(to, line);
                 if (line >= rows) continue;
                 if (whole) put_row(a, dim, at, d0 + 4 * c, x);
@@ -838,32 +886,40 @@ __global__ __launch_bounds__(kBlock, D == 256 ? 1 : 2) void k_page_many(PageMany
 }
 
 // out of the tiles that several workgroups hold parts of: a workgroup for the first
-// run that begins inside a tile, and 1,024 of its values; four a thread.
-__global__ __launch_bounds__(kBlock) void k_page_many_join(PageMany a, uint32_t step) {
+// run that begins inside a tile and 1,024 of its values, four a thread.  The parts: the
+// second slot of the run in front, and the first slot of those up to the last.
+__global__ __launch_bounds__(kBlock) void k_page_many_join(PageMany a) {
     const uint32_t D = a.wide, w = blockIdx.x + 1;
-    const ManyHead hd = *head_of(a);
-    const uint32_t runs = min(hd.runs, a.runs);
+    const uint32_t runs = min(*runs_of(a), a.runs);
     if (w >= runs) return;
     const ManyMark m = *mark_of(a, w);
-    if (!m.cost || m.kv >= a.c.kvheads || m.rows > kTileRows || run_begin(hd.total, runs, w - 1) > m.at) return;
-    const uint32_t at = (blockIdx.y * kBlock + threadIdx.x) * 4, line = at / D, d = at % D;
+    if (!m.rows || m.rows > kTileRows || m.kv >= a.c.kvheads) return;
+    const uint32_t at = (blockIdx.y * kBlock + threadIdx.x) * 4, line = at / D, d = at % D, last = min(m.last, runs - 1);
     if (line >= m.rows) return;
     float M = -INFINITY, L = 0.f;
     f4 O = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t p = w - 1; p < runs; p++) {
-        const uint64_t x0 = max(run_begin(hd.total, runs, p), m.at) - m.at, x1 = run_begin(hd.total, runs, p + 1) - m.at;
-        if (x0 >= m.cost) break;
-        const uint32_t lo = key_at(a, x0, m.end, step), hi = x1 >= m.cost ? m.end : key_at(a, x1, m.end, step);
-        if (lo >= hi) continue;  // no step of its own
-        const size_t slot = (size_t)p * 2 + (x0 == 0);
-        const float2 ml = part_ml(a, slot)[line];
-        const f4 o = *reinterpret_cast<const f4*>(part_o(a, slot) + line * D + d);
-        const float Mn = fmaxf(M, ml.x), Mf = Mn == -INFINITY ? 0.f : Mn;
-        const float f = exp2_of(M - Mf), e = exp2_of(ml.x - Mf);
-        M = Mn;
-        L = fmaf(ml.y, e, L * f);
+    constexpr uint32_t kAhead = 4;  // parts on their way
+    for (uint32_t p0 = w - 1; p0 <= last; p0 += kAhead) {
+        float2 ml[kAhead];
+        f4 o[kAhead];
 #pragma unroll
-        for (int j = 0; j < 4; j++) O[j] = fmaf(o[j], e, O[j] * f);
+        for (uint32_t i = 0; i < kAhead; i++) {
+            const uint32_t p = min(p0 + i, last);
+            const size_t slot = (size_t)p * 2 + (p == w - 1);
+            ml[i] = part_ml(a, slot)[line];
+            o[i] = *reinterpret_cast<const f4*>(part_o(a, slot) + line * D + d);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; i++) {
+            if (p0 + i > last) break;
+            const float Mn = fmaxf(M, ml[i].x), Mf = Mn == -INFINITY ? 0.f : Mn;
+            const float f = exp2_of(M - Mf), e = exp2_of(ml[i].x - Mf);
+            M = Mn;
+            L = fmaf(ml[i].y, e, L * f);
+            // a part without a step has no values
+#pragma unroll
+            for (int j = 0; j < 4; j++) O[j] = ml[i].x == -INFINITY ? O[j] * f : fmaf(o[i][j], e, O[j] * f);
+        }
     }
     const uint32_t r = m.row + line, row = r / a.group;
     if (row >= a.n) return;
@@ -885,8 +941,10 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.kv_wide = d % 8 == 0 && (((uintptr_t)a.c.k | (uintptr_t)a.c.v | (a.c.ps | a.c.ts | a.c.hs) * es) % std::min(8 * es, 16u)) == 0;
     // products of 16 bits: of the cache's own type, or of f16 where bf16 queries read Q8_0
     a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
-               (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && a.q.kind == BF16 && a.out.kind == BF16));
-    a.one_page = a.c.page % (512 / a.wide) == 0 && a.c.ps * 2 >> 32 == 0 && (unsigned __int128)a.c.page * a.c.ts * 2 >> 32 == 0;
+               (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && d <= 128 && a.q.kind == BF16 && a.out.kind == BF16));
+    a.tile_keys = a.narrow ? 256 : 32;
+    a.run_keys = a.narrow ? 128 : 32;
+    a.one_page = a.c.page % std::max(1024 / (a.wide * es), 1u) == 0 && a.c.ps * es >> 32 == 0 && (unsigned __int128)a.c.page * a.c.ts * es >> 32 == 0;
     // t / page for t < 2^31: 2 t * ceil(2^(31 + log) / page) >> 32 + log
     a.page_log = 0;
     while ((1ull << a.page_log) < a.c.page) a.page_log++;
@@ -894,7 +952,7 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
     a.c2 = a.scale == 0.f ? 1.f : std::max(std::fabs(a.scale) * kLog2e, 1.17549435e-38f);
     const uint64_t tiles = ((uint64_t)a.n * a.group / kTileRows + a.r.batch) * a.c.kvheads;
-    const uint64_t most = tiles * (a.r.most / kRunKeys + 2);
+    const uint64_t most = tiles * (a.r.most / a.run_keys + 2);
     a.runs = (uint32_t)std::min<uint64_t>(cus * (a.wide == 256 ? 1 : 2), std::max<uint64_t>(most, 1));
 }
 
@@ -902,7 +960,7 @@ template <class T, uint32_t SRC> static void launch_many(const PageMany& a, hipS
     const dim3 grid((a.runs + kXcds - 1) / kXcds * kXcds), block(kBlock);
     if (a.wide == 64) hipLaunchKernelGGL((k_page_many<T, 64, SRC>), grid, block, 0, s, a);
     else if (a.wide == 128) hipLaunchKernelGGL((k_page_many<T, 128, SRC>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_page_many<T, 256, SRC>), grid, block, 0, s, a);
+    else if constexpr (SRC == kDirect || SRC == kAny || (SRC == Q8_0 && std::is_same<T, float>::value)) hipLaunchKernelGGL((k_page_many<T, 256, SRC>), grid, block, 0, s, a);
 }
 void launch_page_many(const PageMany& a, hipStream_t s) {
     const bool direct = a.kv_wide && a.one_page && a.c.dim == a.wide;
@@ -910,14 +968,13 @@ void launch_page_many(const PageMany& a, hipStream_t s) {
         if (a.c.kind == Q8_0) launch_many<_Float16, Q8_0>(a, s);
         else if (a.c.kind == F16) direct ? launch_many<_Float16, kDirect>(a, s) : launch_many<_Float16, kAny>(a, s);
         else direct ? launch_many<bf16_t, kDirect>(a, s) : launch_many<bf16_t, kAny>(a, s);
-    } else if (!a.kv_wide) launch_many<float, kAny>(a, s);
-    else if (a.c.kind == F32) launch_many<float, F32>(a, s);
+    } else if (a.c.kind == F32 && direct) launch_many<float, kDirect>(a, s);
+    else if (a.c.kind == F32 || !a.kv_wide || (a.wide == 256 && a.c.kind != Q8_0)) launch_many<float, kAny>(a, s);
     else if (a.c.kind == F16) launch_many<float, F16>(a, s);
     else if (a.c.kind == BF16) launch_many<float, BF16>(a, s);
     else launch_many<float, Q8_0>(a, s);
     if (a.runs > 1)
-        hipLaunchKernelGGL(k_page_many_join, dim3(a.runs - 1, kTileRows * a.wide / (4 * kBlock)), dim3(kBlock), 0, s, a,
-                           !a.narrow || a.wide == 256 ? 32 : 64);
+        hipLaunchKernelGGL(k_page_many_join, dim3(a.runs - 1, kTileRows * a.wide / (4 * kBlock)), dim3(kBlock), 0, s, a);
 }
 
 }  // namespace qh

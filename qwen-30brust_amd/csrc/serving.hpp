@@ -121,6 +121,7 @@ struct PageMany {
     bool narrow;                    // products of 16 bits, else of 32
     bool one_page;                  // the rows that a wave loads at a time lie in one page
     bool q_wide, out_wide, kv_wide; // rows aligned to what is read and written at a time
+    uint32_t tile_keys, run_keys;   // a tile's start and end in keys, keys of a run at least
     uint32_t page_mul, page_log;    // t / page
     float sign, c2;                 // scale * log2 e = sign * c2
     void* work;
