@@ -59,29 +59,32 @@ __device__ __forceinline__ Sum scan_block(Sum v, Sum* part, Sum& all) {
     return v;
 }
 
-// The sequence of token i: the last whose first token is not behind it.
-__device__ __forceinline__ uint32_t sequence_of(const int32_t* first, uint32_t batch, uint32_t i) {
-    uint32_t lo = 0, hi = batch;  // first[lo] <= i < first[hi]
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (gld<int32_t>(first + mid) <= (int32_t)i) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
+// What the tokens are filled in from: new lengths, and first, of all sequences; in LDS
+// where they are few enough.
+struct Filled {
+    const int32_t *first, *length;
+    bool near;
+    __device__ __forceinline__ int32_t first_of(uint32_t b) const { return near ? first[b] : gld<int32_t>(first + b); }
+    __device__ __forceinline__ int32_t length_of(uint32_t b) const { return near ? length[b] : gld<int32_t>(length + b); }
+};
 
-// Token i's sequence, place and slot; position and ancestors of a tree's nodes are
-// its wave's (fill_trees).
-__device__ __forceinline__ void fill_token(const PagePlan& a, uint32_t i) {
-    const bool live = a.batch && (int32_t)i < gld<int32_t>(a.first + a.batch);
+// Token i's sequence (the last whose first token is not behind it), place and slot;
+// position and ancestors of a tree's nodes are its wave's (fill_tree).
+__device__ __forceinline__ void fill_token(const PagePlan& a, const Filled& q, uint32_t i) {
+    const bool live = a.batch && (int32_t)i < q.first_of(a.batch);
     int32_t b = -1, t = -1;
     int64_t slot = -1;
     if (live) {
-        b = (int32_t)sequence_of(a.first, a.batch, i);
-        const int32_t end = gld<int32_t>(a.first + b + 1);
-        t = gld<int32_t>(a.new_length + b) - end + (int32_t)i;
+        uint32_t lo = 0, hi = a.batch;  // first[lo] <= i < first[hi]
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (q.first_of(mid) <= (int32_t)i) lo = mid;
+            else hi = mid;
+        }
+        b = (int32_t)lo;
+        t = q.length_of(lo) - q.first_of(lo + 1) + (int32_t)i;
         const uint32_t page = (uint32_t)t / a.page;
-        slot = (int64_t)gld<int32_t>(a.table + b * a.stride + page) * a.page + ((uint32_t)t - page * a.page);
+        slot = (int64_t)gld<int32_t>(a.table + lo * a.stride + page) * a.page + ((uint32_t)t - page * a.page);
     }
     if (a.sequence) a.sequence[i] = b;
     if (a.slot) a.slot[i] = slot;
@@ -91,11 +94,11 @@ __device__ __forceinline__ void fill_token(const PagePlan& a, uint32_t i) {
 
 // A sequence's tree by a wave, a node a lane: a node's ancestors are its own bit and
 // its parent's ancestors, found by doubling (six times for a path of up to 64).
-__device__ __forceinline__ void fill_tree(const PagePlan& a, uint32_t b) {
+__device__ __forceinline__ void fill_tree(const PagePlan& a, const Filled& q, uint32_t b) {
     const uint32_t lane = threadIdx.x & 63;
-    const int32_t f = gld<int32_t>(a.first + b), e = gld<int32_t>(a.first + b + 1), count = e - f;
+    const int32_t f = q.first_of(b), count = q.first_of(b + 1) - f;
     if (count <= 0) return;
-    const int32_t context = gld<int32_t>(a.new_length + b) - count;
+    const int32_t context = q.length_of(b) - count;
     const int32_t parent = (int32_t)lane < count ? gld<int32_t>(a.parent + f + lane) : -1;
     uint64_t bits = 1ull << lane;
     int up = parent >= 0 && parent < (int32_t)lane ? parent : (int)lane;
@@ -122,14 +125,18 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
     __shared__ Sum part[kPlanWaves];
     __shared__ uint32_t upto[kPlanBlock];  // pages up to and with each sequence of the chunk
     __shared__ uint32_t from[kPlanBlock];  // the first of them in its table row
+    __shared__ int32_t firsts[kPlanBlock + 1], lengths[kPlanBlock];  // of a batch of one chunk
     const uint32_t tid = threadIdx.x;
+    const bool near = a.batch <= kPlanBlock;
+    const int32_t stored = gld<int32_t>(a.count);
+    const Ask own = ask_of(a, tid);
+    auto asked_by = [&](uint32_t b) { return b < kPlanBlock ? own : ask_of(a, b); };  // tid's sequence of a chunk
     Sum all;
     uint32_t gives = 0;  // at most what the table holds, below 2^31
     for (uint32_t b0 = 0; b0 < a.batch; b0 += kPlanBlock) {
-        scan_block({ask_of(a, b0 + tid).gives, 0}, part, all);
+        scan_block({asked_by(b0 + tid).gives, 0}, part, all);
         gives += (uint32_t)all.pages;
     }
-    const int32_t stored = gld<int32_t>(a.count);
     const uint32_t count = (uint32_t)min(max(stored, 0), (int32_t)a.pages), free = min(count + gives, a.pages);
     // f(a page's number among the chunk's, its sequence in the chunk, its place in the table row)
     auto each_page = [&](uint32_t sum, uint32_t total, uint32_t begin, auto f) {
@@ -148,7 +155,7 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
     if (gives) {
         uint32_t done = 0;
         for (uint32_t b0 = 0; b0 < a.batch; b0 += kPlanBlock) {
-            const Ask q = ask_of(a, b0 + tid);
+            const Ask q = asked_by(b0 + tid);
             const Sum sum = scan_block({q.gives, 0}, part, all);
             each_page((uint32_t)sum.pages, (uint32_t)all.pages, q.need, [&](uint32_t i, uint32_t s, uint32_t j) {
                 const uint32_t to = count + (gives - 1 - done - i);
@@ -158,11 +165,11 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
         }
         __syncthreads();
     }
-    if (tid == 0) a.first[0] = 0;
+    if (tid == 0) a.first[0] = firsts[0] = 0;
     Sum asked{0, 0}, given{0, 0};
     for (uint32_t b0 = 0; b0 < a.batch; b0 += kPlanBlock) {
         const uint32_t b = b0 + tid;
-        Ask q = ask_of(a, b);
+        Ask q = asked_by(b);
         const Sum sum = scan_block({q.claims, q.tokens}, part, all);
         // the sums only rise, so behind the first that does not fit none does
         if (q.tokens && (asked.pages + sum.pages > free || asked.tokens + sum.tokens > a.n))
@@ -173,6 +180,7 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
             a.first[b + 1] = (int32_t)(given.tokens + got.tokens);
             a.new_length[b] = q.grown;
             if (q.fine && q.need != q.held) a.held[b] = (int32_t)q.need;
+            if (near) firsts[b + 1] = (int32_t)(given.tokens + got.tokens), lengths[b] = q.grown;
         }
         const uint32_t top = free - (uint32_t)given.pages;
         each_page((uint32_t)got.pages, (uint32_t)all.pages, q.need - q.claims, [&](uint32_t i, uint32_t s, uint32_t j) {
@@ -183,16 +191,18 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
     if (tid == 0) a.count[0] = (int32_t)(free - (uint32_t)given.pages);
     if (!fill) return;
     __syncthreads();
-    for (uint32_t i = tid; i < a.n; i += kPlanBlock) fill_token(a, i);
+    const Filled q{near ? firsts : a.first, near ? lengths : a.new_length, near};
+    for (uint32_t i = tid; i < a.n; i += kPlanBlock) fill_token(a, q, i);
     if (a.parent)
-        for (uint32_t b = tid >> 6; b < a.batch; b += kPlanWaves) fill_tree(a, b);
+        for (uint32_t b = tid >> 6; b < a.batch; b += kPlanWaves) fill_tree(a, q, b);
 }
 
 __global__ __launch_bounds__(kBlock) void k_page_fill(PagePlan a) {
     const uint32_t i = blockIdx.x * kBlock + threadIdx.x;
-    if (i < a.n) fill_token(a, i);
+    const Filled q{a.first, a.new_length, false};
+    if (i < a.n) fill_token(a, q, i);
     if (a.parent)
-        for (uint32_t b = blockIdx.x * kWaves + (threadIdx.x >> 6); b < a.batch; b += gridDim.x * kWaves) fill_tree(a, b);
+        for (uint32_t b = blockIdx.x * kWaves + (threadIdx.x >> 6); b < a.batch; b += gridDim.x * kWaves) fill_tree(a, q, b);
 }
 
 void launch_page_plan(const PagePlan& a, hipStream_t s) {

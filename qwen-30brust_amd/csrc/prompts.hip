@@ -953,7 +953,7 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.c2 = a.scale == 0.f ? 1.f : std::max(std::fabs(a.scale) * kLog2e, 1.17549435e-38f);
     const uint64_t tiles = ((uint64_t)a.n * a.group / kTileRows + a.r.batch) * a.c.kvheads;
     const uint64_t most = tiles * (a.r.most / a.run_keys + 2);
-    a.runs = (uint32_t)std::min<uint64_t>(cus * (a.wide == 256 ? 1 : 2), std::max<uint64_t>(most, 1));
+    a.runs = (uint32_t)std::min<uint64_t>(cus * (a.wide == 256 || (a.narrow && a.c.kind == Q8_0 && a.wide == 128) ? 1 : 2), std::max<uint64_t>(most, 1));
 }
 
 template <class T, uint32_t SRC> static void launch_many(const PageMany& a, hipStream_t s) {

@@ -333,12 +333,11 @@ class PagePool:
             _on(dev, out, "new lengths", _I32, 1)
             _need(out.shape[0] == batch, "new lengths: one for each row of the page table")
             _apart(out, "new lengths")
-        # one allocation: slots, ancestors, first, positions, sequences
-        wide = n * (2 if parents is not None else 1)
-        ints = torch.empty(2 * wide + batch + 1 + 2 * n, dtype=torch.int32, device=table.device)
-        longs, rest = ints[:2 * wide].view(torch.int64), ints[2 * wide:]
-        plan = Plan(out, rest[:batch + 1], longs[:n], rest[batch + 1:batch + 1 + n], rest[batch + 1 + n:],
-                    longs[n:] if parents is not None else None)
+        longs = torch.empty((2 if parents is not None else 1, n), dtype=torch.int64, device=table.device).unbind()
+        slots, seen = longs if parents is not None else (longs[0], None)
+        first, positions, sequences = torch.empty(batch + 1 + 2 * n, dtype=torch.int32,
+                                                  device=table.device).split_with_sizes((batch + 1, n, n))
+        plan = Plan(out, first, slots, positions, sequences, seen)
         places = engine._Plan(*(None if t is None else t.data_ptr() for t in plan))
         dev._check(engine.lib().qh_paged_plan(_live(dev), self._pool, table.data_ptr(), strides[0], pages, held.data_ptr(),
                                               lengths.data_ptr(), grow.data_ptr(), batch, n,
@@ -365,8 +364,8 @@ def accept(caches, parents, tokens, chosen, table, lengths, first):
     n = parents.shape[0]
     _need(tokens.shape[0] == n and chosen.shape[0] == n, "a drafted and a chosen token for each node")
     _need(first.shape[0] == batch + 1, "first tokens: one more than sequences is needed")
-    ints = torch.empty(3 * batch + n, dtype=torch.int32, device=table.device)
-    new, accepted, following, path = ints[:batch], ints[batch:2 * batch], ints[2 * batch:3 * batch], ints[3 * batch:]
+    new, accepted, following, path = torch.empty(3 * batch + n, dtype=torch.int32,
+                                                 device=table.device).split_with_sizes((batch, batch, batch, n))
     pages = (engine._Pages * len(caches))(*(c._pages for c in caches))
     dev._check(engine.lib().qh_paged_accept(_live(dev), pages, len(caches), seqs, first.data_ptr(), n, parents.data_ptr(),
                                             tokens.data_ptr(), chosen.data_ptr(), new.data_ptr(), accepted.data_ptr(),
