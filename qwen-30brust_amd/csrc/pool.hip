@@ -131,10 +131,12 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
     const int32_t stored = gld<int32_t>(a.count);
     const Ask own = ask_of(a, tid);
     auto asked_by = [&](uint32_t b) { return b < kPlanBlock ? own : ask_of(a, b); };  // tid's sequence of a chunk
-    Sum all;
+    Sum all, sum;
     uint32_t gives = 0;  // at most what the table holds, below 2^31
     for (uint32_t b0 = 0; b0 < a.batch; b0 += kPlanBlock) {
-        scan_block({asked_by(b0 + tid).gives, 0}, part, all);
+        const uint32_t mine = asked_by(b0 + tid).gives;
+        if (!__syncthreads_or(mine)) continue;
+        sum = scan_block({mine, 0}, part, all);
         gives += (uint32_t)all.pages;
     }
     const uint32_t count = (uint32_t)min(max(stored, 0), (int32_t)a.pages), free = min(count + gives, a.pages);
@@ -156,7 +158,7 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
         uint32_t done = 0;
         for (uint32_t b0 = 0; b0 < a.batch; b0 += kPlanBlock) {
             const Ask q = asked_by(b0 + tid);
-            const Sum sum = scan_block({q.gives, 0}, part, all);
+            if (!near) sum = scan_block({q.gives, 0}, part, all);
             each_page((uint32_t)sum.pages, (uint32_t)all.pages, q.need, [&](uint32_t i, uint32_t s, uint32_t j) {
                 const uint32_t to = count + (gives - 1 - done - i);
                 if (to < a.pages) a.free[to] = gld<int32_t>(a.table + (size_t)(b0 + s) * a.stride + j);
@@ -170,20 +172,23 @@ __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t f
     for (uint32_t b0 = 0; b0 < a.batch; b0 += kPlanBlock) {
         const uint32_t b = b0 + tid;
         Ask q = asked_by(b);
-        const Sum sum = scan_block({q.claims, q.tokens}, part, all);
-        // the sums only rise, so behind the first that does not fit none does
-        if (q.tokens && (asked.pages + sum.pages > free || asked.tokens + sum.tokens > a.n))
-            q.claims = q.tokens = 0, q.grown = q.len, q.need = q.held;
-        asked.pages += all.pages, asked.tokens += all.tokens;
-        const Sum got = scan_block({q.claims, q.tokens}, part, all);
+        sum = all = {0, 0};
+        if (__syncthreads_or(q.tokens)) {
+            sum = scan_block({q.claims, q.tokens}, part, all);
+            // the sums only rise, so behind the first that does not fit none does
+            const bool late = q.tokens && (asked.pages + sum.pages > free || asked.tokens + sum.tokens > a.n);
+            if (late) q.claims = q.tokens = 0, q.grown = q.len, q.need = q.held;
+            asked.pages += all.pages, asked.tokens += all.tokens;
+            if (__syncthreads_or(late)) sum = scan_block({q.claims, q.tokens}, part, all);
+        }
         if (b < a.batch) {
-            a.first[b + 1] = (int32_t)(given.tokens + got.tokens);
+            a.first[b + 1] = (int32_t)(given.tokens + sum.tokens);
             a.new_length[b] = q.grown;
             if (q.fine && q.need != q.held) a.held[b] = (int32_t)q.need;
-            if (near) firsts[b + 1] = (int32_t)(given.tokens + got.tokens), lengths[b] = q.grown;
+            if (near) firsts[b + 1] = (int32_t)(given.tokens + sum.tokens), lengths[b] = q.grown;
         }
         const uint32_t top = free - (uint32_t)given.pages;
-        each_page((uint32_t)got.pages, (uint32_t)all.pages, q.need - q.claims, [&](uint32_t i, uint32_t s, uint32_t j) {
+        if (all.pages) each_page((uint32_t)sum.pages, (uint32_t)all.pages, q.need - q.claims, [&](uint32_t i, uint32_t s, uint32_t j) {
             a.table[(size_t)(b0 + s) * a.stride + j] = gld<int32_t>(a.free + top - 1 - i);
         });
         given.pages += all.pages, given.tokens += all.tokens;
