@@ -480,12 +480,21 @@ int qh_paged_evict(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *s
  * first[b] .. first[b + 1] - 1 of q and out ([n][heads][dim]), and their keys are
  * the last of its length[b] keys (appended before).  Token i of m new ones sees the
  * keys up to its own, length - m + i: a whole prompt, the next piece of one, or a
- * single token.  Formula, types, sums and what is out of range as in
+ * single token.  Formula, element kinds and what is out of range as in
  * qh_paged_attention, but: a row gives NaN where one of the keys that it sees is in a
  * page out of range; the rows of a sequence whose length is out of range or below its
  * new tokens give NaN; rows of no sequence (in front of first[0], behind first[batch],
  * or of a sequence whose bounds do not ascend within 0 .. n) are left as they were.
- * Keys and values that a row does not see take no part in it, whatever they hold. */
+ * Keys and values that a row does not see take no part in it, whatever they hold.
+ * Sums and maxima in 32 bits, out rounded once to its kind.  With queries and out of
+ * 16 bits over a cache of the queries' kind, each softmax weight is rounded once to
+ * that kind before it meets its value, and the sum it is divided by is of the rounded
+ * ones.  BF16 queries and out over Q8_0 (heads up to 128 wide, a multiple of 8, rows
+ * aligned to 8 bytes) are taken in F16 products: weights and values (code times
+ * scale) are rounded to F16, so a value past 65504 comes out not finite, and an
+ * element of a query below 2^-39 of the largest of its row is lost.  All other mixes
+ * and an F32 out are in 32 bits.  q and out may be the same.  A call whose tokens
+ * times heads pass 2^31, or with the keys 2^62, is refused. */
 int qh_paged_prompts(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,
                      const qh_heads_t *q, uint32_t heads, float scale, const qh_heads_t *out, void *workspace,
                      size_t workspace_bytes, void *stream);
@@ -497,13 +506,15 @@ int qh_paged_prompts(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t 
 int qh_paged_tree(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,
                   const uint64_t *ancestors, const qh_heads_t *q, uint32_t heads, float scale, const qh_heads_t *out,
                   void *workspace, size_t workspace_bytes, void *stream);
-/* Bytes of workspace that either call needs for these shapes. */
+/* Bytes of workspace that either call needs for these shapes, at most some 68 MB (0:
+ * none; its pointer may then be NULL, else it is aligned to 16 bytes).  Calls that may
+ * run at once have one each. */
 int qh_paged_prompts_bytes(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, size_t n, uint32_t heads,
                            size_t *out);
 
 /* Pages of `page` slots each: the ids free[0 .. count[0]) are in no table, the last
  * of them is the next to go.  Both lie in device memory and are the caller's; free
- * has room for `pages` ids. */
+ * has room for `pages` ids.  The plans of a pool run one after another. */
 typedef struct {
     int32_t *free, *count;
     uint64_t pages;
@@ -549,10 +560,13 @@ int qh_paged_plan(qh_ctx *ctx, const qh_pool_t *pool, int32_t *table, size_t tab
  * strides, with the same tables), to the slots behind the context, in order.
  * Outputs: new_length[batch] = length - nodes + accepted; accepted[batch] (root
  * included); path[n]: the accepted nodes' numbers from the sequence's first row on, -1
- * in all other rows; next[batch] = chosen at the last of them.  A sequence without
+ * in its other rows and in those in front of first[0] and behind first[batch];
+ * next[batch] = chosen at the last of them.  A sequence without
  * nodes, with more than 64, or whose length, bounds or pages (those of its nodes) are
- * out of range: length as it was, 0 accepted, next -1, nothing moves.  No output may
- * lie where the call reads, and no two sequences hold the same page. */
+ * out of range: length as it was, 0 accepted, next -1, nothing moves (and
+ * the rows of one whose bounds do not ascend within 0 .. n are left as they were).  No
+ * output may lie where the call reads, no cache is given twice, and the pages that hold
+ * a sequence's nodes are in no other sequence. */
 int qh_paged_accept(qh_ctx *ctx, const qh_pages_t *caches, size_t layers, const qh_sequences_t *seqs,
                     const int32_t *first, size_t n, const int32_t *parents, const int32_t *tokens,
                     const int32_t *chosen, int32_t *new_length, int32_t *accepted, int32_t *path, int32_t *next,

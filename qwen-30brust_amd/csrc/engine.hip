@@ -2948,6 +2948,10 @@ int qh_paged_accept(qh_ctx* c, const qh_pages_t* caches, size_t layers, const qh
                 p.count != a.c.count || p.ps != a.c.ps || p.ts != a.c.ts || p.hs != a.c.hs)
                 throw Error("caches differ in shape, kind or strides");
         }
+        std::vector<const void*> keys(layers);
+        for (size_t i = 0; i < layers; i++) keys[i] = caches[i].k;
+        std::sort(keys.begin(), keys.end());
+        if (std::adjacent_find(keys.begin(), keys.end()) != keys.end()) throw Error("a cache is given twice");
         if (n > (1u << 24)) throw Error("at most 16777216 tokens");
         if (!a.r.batch) return;
         need_ptr(first, 4, "first tokens");

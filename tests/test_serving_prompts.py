@@ -113,6 +113,30 @@ def test_plan(kw, text):
     assert text in message(plan(**kw))
 
 
+@pytest.mark.parametrize("call", [prompts, tree])
+def test_workspace(call):
+    size = C.c_size_t()
+    assert engine.lib().qh_paged_prompts_bytes(None, cache(), seqs(), 5, 4, size) == 0 and size.value > 0
+    assert "null workspace" in message(call(work=(None, size.value)))
+    assert "workspace is not aligned" in message(call(work=(A + 8, size.value)))
+    assert "bytes, " in message(call(work=(A, 0)))
+    assert message(call(work=(A, size.value))) == "null context"
+
+
+@pytest.mark.parametrize("call", [prompts, tree])
+def test_more_work_than_is_counted(call):
+    pages = 1 << 26
+    big = dict(s=seqs(batch=1, table_pages=pages, table_stride=pages, most=(1 << 30) - 1))
+    assert message(call(c=cache(kvheads=1), n=1 << 23, h=250, **big)) == "too many tokens, heads and keys"
+    assert message(call(c=cache(kvheads=1), n=1 << 23, h=32, **big)) == "null context"
+
+
+def test_one_cache_twice():
+    three = (engine._Pages * 3)(cache(), cache(k=9 * A, v=10 * A), cache())
+    assert message(accept(c=three, layers=3)) == "a cache is given twice"
+    assert message(accept(c=three, layers=2)) == "null context"
+
+
 def test_null_structures():
     lib = engine.lib()
     assert "null cache" in message(lib.qh_paged_prompts(None, None, seqs(), A, 5, heads(), 4, 1.0, heads(), None, 0, None))
