@@ -492,7 +492,8 @@ int qh_paged_evict(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *s
  * ones.  BF16 queries and out over Q8_0 (heads up to 128 wide, a multiple of 8, rows
  * aligned to 8 bytes) are taken in F16 products: weights and values (code times
  * scale) are rounded to F16, so a value past 65504 comes out not finite, and an
- * element of a query below 2^-39 of the largest of its row is lost.  All other mixes
+ * element of a query is rounded below 2^-31 of the largest of its row and lost below
+ * 2^-39.  All other mixes
  * and an F32 out are in 32 bits.  q and out may be the same.  A call whose tokens
  * times heads pass 2^31, or with the keys 2^62, is refused. */
 int qh_paged_prompts(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,

@@ -6,7 +6,9 @@
 namespace qh {
 
 constexpr uint32_t kPlanBlock = 1024, kPlanWaves = kPlanBlock / 64;
-constexpr uint32_t kPlanHere = 4096;  // tokens that k_page_plan itself fills in
+// Tokens that k_page_plan itself fills in: a launch less (two plans of 64 sequences 39 us rather
+// than 42), but one workgroup (48 prompts of 50,000 tokens 76 us rather than 38).
+constexpr uint32_t kPlanHere = 4096;
 
 // What sequence b asks for.
 struct Ask {
@@ -120,7 +122,8 @@ __device__ __forceinline__ void fill_tree(const PagePlan& a, const Filled& q, ui
 // One workgroup: three passes over the sequences (pages given back, the sums that
 // decide who grows, pages claimed), 1,024 of them at a time with a sum over the
 // workgroup, the pages themselves dealt to all threads by a search in the sums; then
-// the tokens, where they are few.  Bound by latency: each pass waits for its reads.
+// the tokens, where they are few.  Bound by latency, each pass waits for its reads: 7.5 us
+// for 64 sequences with a token each, 8.4 for 48 with up to 2,100 (k_page_fill 4 more).
 __global__ __launch_bounds__(kPlanBlock) void k_page_plan(PagePlan a, uint32_t fill) {
     __shared__ Sum part[kPlanWaves];
     __shared__ uint32_t upto[kPlanBlock];  // pages up to and with each sequence of the chunk

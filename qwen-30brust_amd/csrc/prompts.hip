@@ -12,6 +12,17 @@
 // fill the chip.  A run may hold several tiles; one that it holds whole goes straight
 // to out, and of the first and the last it may hold a part: its (m, l, o) go to the
 // workgroup's two slots, and k_page_many_join folds them.
+//
+// Bound by the products, but for few rows over a long context, which wait for the cache's
+// bytes.  Measured, with 32 query heads over 4 KV heads of 128 values, on a card whose
+// large products reach 1,104 TFLOP/s in f16, 1,160 in bf16 and 153 in f32, and whose large
+// copies 4.6 TB/s (products that a causal row sees, join included):
+//   16,381 tokens, f16                         2.29 ms   960 TFLOP/s; the clock falls to 1.9 GHz
+//   24 prompts of 1 to 2,100 tokens, bf16      0.60 ms   599 TFLOP/s
+//   2 x 512 tokens behind 12,000 to 15,000, Q8_0   0.67 ms   344 TFLOP/s; turning codes to f16 is most
+//   517 tokens, f32                              59 us    37 TFLOP/s; runs of 4 to 5 steps
+//   2 trees of 64 nodes behind 65,473 keys, f16 175 us   788 TFLOP/s, 1.5 TB/s
+//   48 trees behind up to 4,096 keys, bf16       79 us   2.7 TB/s
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -258,7 +269,11 @@ constexpr uint32_t kDirect = 100, kAny = 101;
 // row's scores (of the keys 8 i + 4 (lane / 32) + j), its maximum and sum need one
 // exchange, and the weights lie where O^T = V^T P^T wants its second operand: for 16-bit
 // types keys 16 c + 8 (e / 4) + 4 (lane / 32) + e % 4 are element e, for V^T read by the
-// transposing LDS read.  K and V of the next step come in while one is worked on.
+// transposing LDS read.  K and V of the next step come in while one is worked on, asked
+// for between the products of the scores (16,381 tokens 2.73 -> 2.55 ms).  The weights are
+// rounded once to T, at most half a step of it each, and the sum is of the rounded ones;
+// everything else between the products is in 32 bits.  Written so that none of the kernels
+// spills vector registers: what is wanted once a tile is computed there anew.
 template <class T, uint32_t D, uint32_t SRC>
 __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std::is_same<T, _Float16>::value) ? 1 : 2) void k_page_many(PageMany a) {
     constexpr bool F = std::is_same<T, float>::value, H = std::is_same<T, _Float16>::value;
@@ -736,7 +751,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 #pragma unroll
                 for (uint32_t g = 0; g < NQ; g++) xq[g] = (xq[g] ^ flip) & keep;
                 if constexpr (Q8) {
-                    // bf16 queries as f16, the row's largest value in [2^14, 2^15): what lies below 2^-38
+                    // bf16 queries as f16, the row's largest value in [2^14, 2^15): what lies below 2^-39
                     // of it is lost, what is not finite stays so
                     uint32_t top = 0;
 #pragma unroll
@@ -887,7 +902,8 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 
 // out of the tiles that several workgroups hold parts of: a workgroup for the first
 // run that begins inside a tile and 1,024 of its values, four a thread.  The parts: the
-// second slot of the run in front, and the first slot of those up to the last.
+// second slot of the run in front, and the first slot of those up to the last.  Bound by
+// what it reads, which is in the caches: 10 to 13 us behind a full grid.
 __global__ __launch_bounds__(kBlock) void k_page_many_join(PageMany a) {
     const uint32_t D = a.wide, w = blockIdx.x + 1;
     const uint32_t runs = min(*runs_of(a), a.runs);
@@ -939,9 +955,15 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.q_wide = d % 8 == 0 && aligned(a.q, 16);
     a.out_wide = aligned(a.out, a.out.kind == F32 ? 16 : 8);
     a.kv_wide = d % 8 == 0 && (((uintptr_t)a.c.k | (uintptr_t)a.c.v | (a.c.ps | a.c.ts | a.c.hs) * es) % std::min(8 * es, 16u)) == 0;
-    // products of 16 bits: of the cache's own type, or of f16 where bf16 queries read Q8_0
+    // Products of 16 bits: of the cache's own type, or of f16 where bf16 queries read Q8_0 (the two
+    // prompts over Q8_0 0.67 ms, 2.27 in 32 bits); wider heads' codes and registers do not fit.
     a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
                (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && d <= 128 && a.q.kind == BF16 && a.out.kind == BF16));
+    // What a tile's start and end cost, in keys: queries in, values out (256 rather than 32: 16,381
+    // tokens 2.67 -> 2.31 ms, 24 prompts 0.81 -> 0.59, 48 trees 103 -> 77 us), and the least that a run
+    // is worth having (128, of four steps less than one for its start: a tree behind 517 keys 22.4 us,
+    // with 64 25.3, with 256 23.3, with 1,024 38.4; f32, where a key costs eight times as much, 32:
+    // 517 tokens 64 us, with 256 84).
     a.tile_keys = a.narrow ? 256 : 32;
     a.run_keys = a.narrow ? 128 : 32;
     a.one_page = a.c.page % std::max(1024 / (a.wide * es), 1u) == 0 && a.c.ps * es >> 32 == 0 && (unsigned __int128)a.c.page * a.c.ts * es >> 32 == 0;
@@ -953,7 +975,11 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.c2 = a.scale == 0.f ? 1.f : std::max(std::fabs(a.scale) * kLog2e, 1.17549435e-38f);
     const uint64_t tiles = ((uint64_t)a.n * a.group / kTileRows + a.r.batch) * a.c.kvheads;
     const uint64_t most = tiles * (a.r.most / a.run_keys + 2);
-    a.runs = (uint32_t)std::min<uint64_t>(cus * (a.wide == 256 || (a.narrow && a.c.kind == Q8_0 && a.wide == 128) ? 1 : 2), std::max<uint64_t>(most, 1));
+    // A run for each workgroup that is there at once: two a unit by registers (one: 16,381 tokens 2.31 ->
+    // 3.22 ms), and one of the kernels with 256 values, or Q8_0's codes of 128, which hold more (two:
+    // 48 trees of 256 values 192 -> 207 us, Q8_0 0.675 -> 0.69 ms; 24 prompts of 256 1.38 -> 1.35).
+    const bool alone = a.wide == 256 || (a.narrow && a.c.kind == Q8_0 && a.wide == 128);
+    a.runs = (uint32_t)std::min<uint64_t>(cus * (alone ? 1 : 2), std::max<uint64_t>(most, 1));
 }
 
 template <class T, uint32_t SRC> static void launch_many(const PageMany& a, hipStream_t s) {
@@ -963,6 +989,8 @@ template <class T, uint32_t SRC> static void launch_many(const PageMany& a, hipS
     else if constexpr (SRC == kDirect || SRC == kAny || (SRC == Q8_0 && std::is_same<T, float>::value)) hipLaunchKernelGGL((k_page_many<T, 256, SRC>), grid, block, 0, s, a);
 }
 void launch_page_many(const PageMany& a, hipStream_t s) {
+    // Rows straight to LDS (16,381 tokens 2.31 ms, value by value 3.36; 48 trees 77 us, 114) where a
+    // wave's load of them lies in one page, which it finds once.
     const bool direct = a.kv_wide && a.one_page && a.c.dim == a.wide;
     if (a.narrow) {
         if (a.c.kind == Q8_0) launch_many<_Float16, Q8_0>(a, s);

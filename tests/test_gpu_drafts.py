@@ -421,3 +421,54 @@ def test_rounds(dev, kv):
                 a, o = (int(table[b, t // page]), t % page), (int(table1[b, t // page]), t % page)
                 assert torch.equal(c.k[a], d.k[o]) and torch.equal(c.v[a], d.v[o])
                 assert c.k_scale is None or torch.equal(c.k_scale[a], d.k_scale[o])
+
+
+@pytest.mark.parametrize("kv", ["f16", "q8_0"])
+def test_round_in_a_graph(dev, kv):
+    """A round captured whole (plan, append, attend_tree, accept, plan) and replayed from states put back, with eager
+    rounds between: each replay leaves what the eager round left, bit for bit."""
+    G, H, dim, page, B, n = 2, 8, 64, 16, 4, 75
+    x = TYPES["bf16" if kv == "q8_0" else kv]
+    g = torch.Generator().manual_seed(5)
+    cache = serving.PagedCache(dev, *make_cache(g, 40, page, G, dim, kv))
+    pool = serving.PagePool(dev, 40, page)
+    table, held = torch.zeros(B, 12, dtype=torch.int32, device="cuda"), ints([0] * B)
+    lengths = pool.plan(table, held, ints([0] * B), ints([37, 0, 16, 100]), 153).lengths
+    nodes = [5, 1, 64, 3]  # two rows of 75 are no sequence's
+    parents, drafts, _ = drafted(sum(nodes), nodes, 3)
+    parents, drafts = ints(parents + [-1, -1]), ints(drafts + [0, 0])
+    chosen = torch.randint(0, 3, (n,), generator=g, dtype=torch.int32).cuda()
+    grow, none = ints(nodes), ints([0] * B)
+    k, v, q = (torch.randn(n, h, dim, generator=g).to(x).cuda() for h in (G, G, H))
+    rope = torch.randn(400, dim // 2, 2, generator=g).cuda()
+    out = torch.empty_like(q)
+
+    def one():
+        out.fill_(7)
+        plan = pool.plan(table, held, lengths, grow, n, parents=parents)
+        turned = cache.append(k, v, table, plan.lengths, plan.first, q=q, rope=rope, positions=plan.positions)
+        cache.attend_tree(turned, table, plan.lengths, plan.first, plan.ancestors, out=out)
+        new, accepted, path, following = serving.accept([cache], parents, drafts, chosen, table, plan.lengths, plan.first)
+        return [*plan, out, new, accepted, path, following, pool.plan(table, held, new, none, 0).lengths]
+
+    state = [t for t in (table, held, pool.free, pool.count, cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+    before = [t.clone() for t in state]
+
+    def back():
+        for t, b in zip(state, before):
+            t.copy_(b)
+
+    want = [t.clone() for t in one()]
+    after = [t.clone() for t in state]
+    assert want[6][-2:].eq(7).all() and not want[6][:-2].eq(7).all() and want[8].tolist()[1] == 1
+    back()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = one()
+    for _ in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(state, after))
+        back()
+        one()
+        back()
