@@ -539,25 +539,36 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                 };
                 auto k_part = [&](uint32_t g, uint32_t m) { return *reinterpret_cast<const T8*>(kt + ((Q8 ? opaque(k_at) : k_at) ^ g * 32) + m * 32 * D * 2); };
                 if constexpr (Q8) {
-                    // a block's codes are exact, its scale is the score's
+                    // A block's codes are exact, its scale is the score's: taken while the next block's products
+                    // run, whose parts and scales were read meanwhile.
+                    constexpr uint32_t N = NS * ND;
+                    T8 x[2][2];
+                    f4 f[2][4];
+                    f16v y[2];
+                    auto read = [&](uint32_t i) {
+                        const uint32_t g = i / NS, m = i % NS;
+                        x[i % 2][0] = k_part(2 * g, m), x[i % 2][1] = k_part(2 * g + 1, m);
 #pragma unroll
-                    for (uint32_t g = 0; g < D / 16; g += 2)
+                        for (uint32_t j = 0; j < 4; j++) f[i % 2][j] = *reinterpret_cast<const f4*>(&scales[buf][g][32 * m + 8 * j + 4 * half]);
+                    };
+                    auto scale = [&](uint32_t i) {
 #pragma unroll
-                        for (uint32_t m = 0; m < NS; m++) {
-                            f16v x;
+                        for (uint32_t j = 0; j < 16; j++) sc[i % NS][j] = fmaf(y[i % 2][j], f[i % 2][j / 4][j % 4], sc[i % NS][j]);
+                    };
+                    read(0);
+                    in_order();
 #pragma unroll
-                            for (int j = 0; j < 16; j++) x[j] = 0.f;
-                            x = product(k_part(g, m), q[g], x);
-                            x = product(k_part(g + 1, m), q[g + 1], x);
+                    for (uint32_t i = 0; i < N; i++) {
 #pragma unroll
-                            for (uint32_t i = 0; i < 4; i++) {
-                                const f4 f = *reinterpret_cast<const f4*>(&scales[buf][g / 2][32 * m + 8 * i + 4 * half]);
-#pragma unroll
-                                for (uint32_t j = 0; j < 4; j++) sc[m][4 * i + j] = fmaf(x[4 * i + j], f[j], sc[m][4 * i + j]);
-                            }
-                            between(g / 2 * NS + m, NS * D / 32);
-                            in_order();
-                        }
+                        for (int j = 0; j < 16; j++) y[i % 2][j] = 0.f;
+                        y[i % 2] = product(x[i % 2][0], q[2 * (i / NS)], y[i % 2]);
+                        y[i % 2] = product(x[i % 2][1], q[2 * (i / NS) + 1], y[i % 2]);
+                        if (i) scale(i - 1);
+                        if (i + 1 < N) read(i + 1);
+                        between(i, N);
+                        in_order();
+                    }
+                    scale(N - 1);
                 } else {
                     // four parts of K are on their way ahead of a product
                     constexpr uint32_t N = NS * D / 16, AHEAD = 4;
