@@ -423,11 +423,11 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                 }
             }
         };
-        // To LDS, as the products take it.
-        auto store = [&](uint32_t buf) {
-            if constexpr (DIRECT || SRC == kAny) return;
-#pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; r++) {
+        // To LDS, as the products take it: part i of PARTS (a round, of Q8_0's codes its K or its V).
+        constexpr uint32_t PARTS = DIRECT || SRC == kAny ? 0 : Q8 ? 2 * ROUNDS : ROUNDS;
+        auto store_part = [&](uint32_t buf, uint32_t i) {
+            if constexpr (PARTS != 0) {
+                const uint32_t r = Q8 ? i / 2 : i;
                 const uint32_t u = r * kBlock + tid, line = u / PER;
                 auto put = [&](const u4* w, uint32_t b) {
 #pragma unroll
@@ -446,11 +446,15 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                         }
                         return w;
                     };
-                    const h2 f = h2(__builtin_bit_cast(_Float16, (uint16_t)vf[r]));
-                    const u4 k = values(kc[r], [](h2 x) { return x; }), v = values(vc[r], [&](h2 x) { return x * f; });
-                    put(&k, buf);
-                    put(&v, 2 + buf);
-                    if (u % PER % 4 == 0) scales[buf][u % PER / 4][line] = h2f(kf[r]);
+                    if (i % 2 == 0) {
+                        const u4 k = values(kc[r], [](h2 x) { return x; });
+                        put(&k, buf);
+                        if (u % PER % 4 == 0) scales[buf][u % PER / 4][line] = h2f(kf[r]);
+                    } else {
+                        const h2 f = h2(__builtin_bit_cast(_Float16, (uint16_t)vf[r]));
+                        const u4 v = values(vc[r], [&](h2 x) { return x * f; });
+                        put(&v, 2 + buf);
+                    }
                 } else if constexpr (SRC == Q8_0) {
                     auto one = [&](uint2 c, uint32_t f16, uint32_t b) {
                         u4 w[2];
@@ -475,6 +479,10 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                     one(vw[r], 2 + buf);
                 }
             }
+        };
+        auto store = [&](uint32_t buf) {
+#pragma unroll
+            for (uint32_t i = 0; i < PARTS; i++) store_part(buf, i);
         };
         // kAny: a value at a time, straight to LDS (16-bit rows aligned to 8 values: eight)
         auto bring = [&](uint32_t k0, uint32_t buf) {
@@ -517,7 +525,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
         const uint32_t vrow = 4 * half + lane % 16 / 4;
         const uint32_t v_at = F ? 4 * half * D * 4 + n % 4 * 4
                                 : vrow * D * 2 + (((lane >> 4 & 1) * 2 + (lane % 4 >> 1)) ^ turn<CH>(vrow)) * 16 + lane % 2 * 8;
-        auto step = [&](uint32_t k0, auto masked, auto buf, auto between) {
+        auto step = [&](uint32_t k0, auto masked, auto buf, auto between, auto behind) {
             const uint8_t *kt = lds[buf], *vt = lds[2 + buf];
             f16v sc[NS];
 #pragma unroll
@@ -708,6 +716,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 #pragma unroll
                             for (uint32_t i = d * 4 / ND; i < (d + 1) * 4 / ND; i++) weights(c + 1, i);
                         }
+                        behind(c * ND + d, C * ND);
                         in_order();
                     }
             }
@@ -808,9 +817,14 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
         auto both = [&](uint32_t k0, auto buf) {
             step(k0, std::false_type(), buf, [&](uint32_t i, uint32_t n) {
                 if constexpr (EARLY) loads(k0, buf, i, n);
+            }, [&](uint32_t i, uint32_t n) {
+                if constexpr (Q8 && PARTS != 0)
+#pragma unroll
+                    for (uint32_t j = 0; j < PARTS; j++)
+                        if (i == (2 * j + 1) * n / (2 * PARTS)) store_part(buf ^ 1, j);
             });
             late(k0, buf);
-            store(buf ^ 1);
+            if constexpr (!Q8) store(buf ^ 1);
             meet();
         };
         uint32_t k0 = lo;
@@ -824,7 +838,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
             const bool more = k0 + KT < hi;
             if (EARLY && more)
                 for (uint32_t i = 0; i < ROUNDS; i++) loads(k0, buf, i, ROUNDS);
-            if (k0 < most) step(k0, std::true_type(), buf, [](uint32_t, uint32_t) {});
+            if (k0 < most) step(k0, std::true_type(), buf, [](uint32_t, uint32_t) {}, [](uint32_t, uint32_t) {});
             if (more) {
                 late(k0, buf);
                 store(buf ^ 1);
