@@ -339,6 +339,10 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
         for (uint32_t d = 0; d < ND; d++)
 #pragma unroll
             for (int j = 0; j < 16; j++) o[d][j] = 0.f;
+        f16v zeros;  // in registers, as sixteen moves a product would not be free
+        if constexpr (Q8)
+#pragma unroll
+            for (int j = 0; j < 16; j++) zeros[j] = __uint_as_float(opaque(0u));
         float M = -INFINITY, L = 0.f;
         // the first step with a value that is not finite beside keys that some row does not
         // see: 0 times it is no 0, so from there on the products are taken key by key, below
@@ -567,9 +571,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                     in_order();
 #pragma unroll
                     for (uint32_t i = 0; i < N; i++) {
-#pragma unroll
-                        for (int j = 0; j < 16; j++) y[i % 2][j] = 0.f;
-                        y[i % 2] = product(x[i % 2][0], q[2 * (i / NS)], y[i % 2]);
+                        y[i % 2] = product(x[i % 2][0], q[2 * (i / NS)], zeros);
                         y[i % 2] = product(x[i % 2][1], q[2 * (i / NS) + 1], y[i % 2]);
                         if (i) scale(i - 1);
                         if (i + 1 < N) read(i + 1);
