@@ -19,7 +19,7 @@
 // copies 4.6 TB/s (products that a causal row sees, join included):
 //   16,381 tokens, f16                         2.29 ms   960 TFLOP/s; the clock falls to 1.9 GHz
 //   24 prompts of 1 to 2,100 tokens, bf16      0.60 ms   599 TFLOP/s
-//   2 x 512 tokens behind 12,000 to 15,000, Q8_0   0.67 ms   344 TFLOP/s; turning codes to f16 is most
+//   2 x 512 tokens behind 12,000 to 15,000, Q8_0   0.56 ms   414 TFLOP/s; the vector units: codes to f16, scales
 //   517 tokens, f32                              59 us    37 TFLOP/s; runs of 4 to 5 steps
 //   2 trees of 64 nodes behind 65,473 keys, f16 175 us   788 TFLOP/s, 1.5 TB/s
 //   48 trees behind up to 4,096 keys, bf16       79 us   2.7 TB/s
@@ -552,7 +552,8 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                 auto k_part = [&](uint32_t g, uint32_t m) { return *reinterpret_cast<const T8*>(kt + ((Q8 ? opaque(k_at) : k_at) ^ g * 32) + m * 32 * D * 2); };
                 if constexpr (Q8) {
                     // A block's codes are exact, its scale is the score's: taken while the next block's products
-                    // run, whose parts and scales were read meanwhile.
+                    // run, whose parts and scales were read meanwhile (two prompts behind 12,000 to 15,000 keys 0.67 ->
+                    // 0.57 ms).
                     constexpr uint32_t N = NS * ND;
                     T8 x[2][2];
                     f4 f[2][4];
@@ -983,7 +984,7 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.out_wide = aligned(a.out, a.out.kind == F32 ? 16 : 8);
     a.kv_wide = d % 8 == 0 && (((uintptr_t)a.c.k | (uintptr_t)a.c.v | (a.c.ps | a.c.ts | a.c.hs) * es) % std::min(8 * es, 16u)) == 0;
     // Products of 16 bits: of the cache's own type, or of f16 where bf16 queries read Q8_0 (the two
-    // prompts over Q8_0 0.67 ms, 2.27 in 32 bits); wider heads' codes and registers do not fit.
+    // prompts over Q8_0 0.56 ms, 2.27 in 32 bits); wider heads' codes and registers do not fit.
     a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
                (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && d <= 128 && a.q.kind == BF16 && a.out.kind == BF16));
     // What a tile's start and end cost, in keys: queries in, values out (256 rather than 32: 16,381
@@ -1004,7 +1005,7 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     const uint64_t most = tiles * (a.r.most / a.run_keys + 2);
     // A run for each workgroup that is there at once: two a unit by registers (one: 16,381 tokens 2.31 ->
     // 3.22 ms), and one of the kernels with 256 values, or Q8_0's codes of 128, which hold more (two:
-    // 48 trees of 256 values 192 -> 207 us, Q8_0 0.675 -> 0.69 ms; 24 prompts of 256 1.38 -> 1.35).
+    // 48 trees of 256 values 192 -> 207 us, Q8_0 0.56 -> 0.575 ms; 24 prompts of 256 1.38 -> 1.35).
     const bool alone = a.wide == 256 || (a.narrow && a.c.kind == Q8_0 && a.wide == 128);
     a.runs = (uint32_t)std::min<uint64_t>(cus * (alone ? 1 : 2), std::max<uint64_t>(most, 1));
 }
