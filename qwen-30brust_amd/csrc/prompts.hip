@@ -33,6 +33,7 @@
 namespace qh {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeast = 1.17549435e-38f, kMost = 3.40282347e38f;  // f32's normal numbers
 constexpr uint32_t kTileRows = 128;  // query rows of a tile, 32 a wave
 constexpr uint32_t kXcds = 8;
 
@@ -783,7 +784,10 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                         for (int j = 0; j < 4; j++) top = max(top, max(xq[g][j] << 16 & 0x7fff0000u, xq[g][j] & 0x7fff0000u));
                     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64)) >> 23;
                     const int up = top == 0 || top == 255 ? 0 : 141 - (int)top;
+                    // kept where -inf times it is -inf, and 0 times it 0; what leaves that range is no score that
+                    // counts (below 2^-80), or one that is past every other (two that differ, by 2^79 at least)
                     c2 = ldexpf(c2, -up);
+                    c2 = c2 < kLeast ? kLeast : c2 > kMost && a.c2 <= kMost ? kMost : c2;
 #pragma unroll
                     for (uint32_t g = 0; g < NQ; g++) {
 #pragma unroll
@@ -1000,7 +1004,7 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     while ((1ull << a.page_log) < a.c.page) a.page_log++;
     a.page_mul = (uint32_t)(((1ull << (31 + a.page_log)) + a.c.page - 1) / a.c.page);
     a.sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
-    a.c2 = a.scale == 0.f ? 1.f : std::max(std::fabs(a.scale) * kLog2e, 1.17549435e-38f);
+    a.c2 = a.scale == 0.f ? 1.f : std::max(std::fabs(a.scale) * kLog2e, kLeast);
     const uint64_t tiles = ((uint64_t)a.n * a.group / kTileRows + a.r.batch) * a.c.kvheads;
     const uint64_t most = tiles * (a.r.most / a.run_keys + 2);
     // A run for each workgroup that is there at once: two a unit by registers (one: 16,381 tokens 2.31 ->

@@ -1,0 +1,48 @@
+"""Attention of several new tokens where the range of its types ends: small and large queries, scales and values, codes
+whose values pass f16, values that are not finite; and 8-bit caches under bf16 queries at the lengths and masks of the
+other kinds."""
+import importlib
+import math
+
+import pytest
+import torch
+
+from prompts_reference import attend_many, close, make, signed, split_of, trees
+from serving_reference import values
+from test_gpu_prompts import at, ints, run
+
+engine = importlib.import_module("qwen-30brust_amd")
+serving = importlib.import_module("qwen-30brust_amd.serving")
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = engine.Device(0)
+    yield d
+    d.close()
+
+
+# ------------------------------------------------------- queries and scales of any size over codes
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("scale,size", [(1e-30, 1e-12), (2.0 ** -12, 2.0 ** -126), (1e-30, 1.0), (0.0, 1.0), (-0.3, 1.0), (3.0, 1.0)])
+def test_queries_of_any_size_over_codes(dev, tree, dim, scale, size):
+    """The factor that takes a row's queries into f16's range, and its inverse in the scale, change no score, also where
+    the product with the scale leaves 32 bits' range."""
+    def change(cache, table, lengths, first, query):
+        query.copy_((query.float().clamp(-3.9, 3.9) / 4 * size).to(query.dtype))
+        query[:, 0] = (query[:, 0].float() / 64).to(query.dtype)  # rows of different sizes
+
+    run(dev, [70, 0, 400], [33, 20, 40], 4, 2, dim, 16, "bf16", "q8_0", tree=tree, scale=scale, change=change)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_large_scale_over_codes(dev, dim):
+    """Scores of 0 under a scale whose product with the queries' factor passes 32 bits: the mean of the values."""
+    def change(cache, table, lengths, first, query):
+        query.copy_((query.float().clamp(-3.9, 3.9) * 2.0 ** 125).to(query.dtype))
+        cache[0].zero_()
+
+    run(dev, [70, 0], [33, 60], 4, 2, dim, 16, "bf16", "q8_0", scale=2.0 ** 20, change=change)
