@@ -283,8 +283,9 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
     constexpr uint32_t NS = KT / 32, ND = D / 32, CH = D * sizeof(T) / 16, TILE = KT * D * sizeof(T);
     constexpr uint32_t NQ = F ? D / 2 : D / 16;
     constexpr uint32_t QKIND = F ? F32 : H && !Q8 ? F16 : BF16;  // of queries that are loaded as they are
-    // weights are at most 2^(kAhead + kUp), so that f16 holds them and small ones too
-    constexpr float kAhead = 8.f, kUp = H ? 7.f : 0.f;
+    // weights are at most 2^(kAhead + kUp): in f16 2^15, so that small ones have their bits; in bf16, which has f32's
+    // exponents, 1, so that sums of values up to 2^128 / keys fit
+    constexpr float kAhead = 8.f, kUp = H ? 7.f : F ? 0.f : -kAhead;
     typedef typename std::conditional<H, h8, b8>::type T8;
     typedef typename std::conditional<F, float, T8>::type Q;
     __shared__ __align__(16) uint8_t lds[4][TILE];  // K, K, V, V; in front and behind a part for each wave

@@ -46,3 +46,25 @@ def test_large_scale_over_codes(dev, dim):
         cache[0].zero_()
 
     run(dev, [70, 0], [33, 60], 4, 2, dim, 16, "bf16", "q8_0", scale=2.0 ** 20, change=change)
+
+
+# ------------------------------------------------------- values near the end of their range
+@pytest.mark.parametrize("dim", [64, 128, 256, 96])
+@pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32"), ("f16", "f16")])
+def test_sums_that_fit(dev, q, kv, dim):
+    """Values of 2^128 / keys, under scores that run 7.5 powers of two ahead of those in front: no weight passes 1, so
+    the sum stays in range."""
+    n, new = 440, 40
+    most = 60000.0 if kv == "f16" else 2.0 ** 119
+
+    def change(cache, table, lengths, first, query):
+        query.zero_()
+        query[:, :, 0] = 1.0
+        cache[0].zero_()
+        cache[1].copy_((cache[1].float().sign() * most).to(cache[1].dtype))
+        cache[1][..., 0] = most
+        for t in range(64, n + new):
+            cache[0][at(table, 0, t)][:, 0] = 5.1875  # 7.48 ln 2
+
+    got = run(dev, [n], [new], 4, 2, dim, 16, q, kv, scale=1.0, change=change)
+    assert torch.isfinite(got).all()
