@@ -784,7 +784,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 #pragma unroll
                         for (int j = 0; j < 4; j++) top = max(top, max(xq[g][j] << 16 & 0x7fff0000u, xq[g][j] & 0x7fff0000u));
                     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64)) >> 23;
-                    const int up = top == 0 || top == 255 ? 0 : 141 - (int)top;
+                    const int up = top == 255 ? 0 : 141 - (int)top;  // subnormal rows too: they lie below 2^-126
                     // kept where -inf times it is -inf, and 0 times it 0; what leaves that range is no score that
                     // counts (below 2^-80), or one that is past every other (two that differ, by 2^79 at least)
                     c2 = ldexpf(c2, -up);

@@ -38,6 +38,17 @@ def test_queries_of_any_size_over_codes(dev, tree, dim, scale, size):
     run(dev, [70, 0, 400], [33, 20, 40], 4, 2, dim, 16, "bf16", "q8_0", tree=tree, scale=scale, change=change)
 
 
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_subnormal_queries_over_codes(dev, tree, dim):
+    """Rows of nothing but subnormal numbers, under a scale that brings the scores back."""
+    def change(cache, table, lengths, first, query):
+        query.copy_((query.float().clamp(-3.9, 3.9) / 4 * 2.0 ** -126).to(query.dtype))
+        query[:, 0] = (query[:, 0].float() / 16).to(query.dtype)
+
+    run(dev, [70, 0, 400], [33, 20, 40], 4, 2, dim, 16, "bf16", "q8_0", tree=tree, scale=2.0 ** 125, change=change)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_large_scale_over_codes(dev, dim):
     """Scores of 0 under a scale whose product with the queries' factor passes 32 bits: the mean of the values."""
