@@ -776,15 +776,17 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 #pragma unroll
                 for (uint32_t g = 0; g < NQ; g++) xq[g] = (xq[g] ^ flip) & keep;
                 if constexpr (Q8) {
-                    // bf16 queries as f16, the row's largest value in [2^14, 2^15): what lies below 2^-39
+                    // bf16 queries as f16, the row's largest finite value in [2^14, 2^15): what lies below 2^-39
                     // of it is lost, what is not finite stays so
                     uint32_t top = 0;
+                    auto finite = [](uint32_t x) { return x < 0x7f800000u ? x : 0u; };
 #pragma unroll
                     for (uint32_t g = 0; g < NQ; g++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) top = max(top, max(xq[g][j] << 16 & 0x7fff0000u, xq[g][j] & 0x7fff0000u));
+                        for (int j = 0; j < 4; j++)
+                            top = max(top, max(finite(xq[g][j] << 16 & 0x7fff0000u), finite(xq[g][j] & 0x7fff0000u)));
                     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64)) >> 23;
-                    const int up = top == 255 ? 0 : 141 - (int)top;  // subnormal rows too: they lie below 2^-126
+                    const int up = 141 - (int)top;  // subnormal rows too: they lie below 2^-126
                     // kept where -inf times it is -inf, and 0 times it 0; what leaves that range is no score that
                     // counts (below 2^-80), or one that is past every other (two that differ, by 2^79 at least)
                     c2 = ldexpf(c2, -up);

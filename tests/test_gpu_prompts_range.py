@@ -59,6 +59,20 @@ def test_large_scale_over_codes(dev, dim):
     run(dev, [70, 0], [33, 60], 4, 2, dim, 16, "bf16", "q8_0", scale=2.0 ** 20, change=change)
 
 
+def test_infinite_queries_over_codes(dev):
+    """An infinity beside large elements: the scores are its alone, -inf for codes above 0 under -inf."""
+    cache, table, lengths, first, query = make(3, [20], [40], 4, 2, 64, 16, "bf16", "q8_0")
+    query.copy_((query.float().sign() * 2.0 ** 100).to(query.dtype))
+    cache[0][..., 5] = 3
+    query[:, 0, 5], query[:, 1, 5] = -math.inf, math.inf
+    c = serving.PagedCache(dev, *cache)
+    got = c.attend_prompts(query.cuda(), table.cuda(), ints(lengths), ints(first), scale=2.0 ** -100)
+    assert (got[:, 0] == 0).all() and got[:, 1].isnan().all()
+    want, bound = attend_many(query[:, 2:], values(cache[0], cache[2])[:, :, 1:], values(cache[1], cache[3])[:, :, 1:], table,
+                              lengths, first, 2.0 ** -100, None, split_of("bf16", "q8_0"))
+    close(got[:, 2:], want, bound)
+
+
 # ------------------------------------------------------- values near the end of their range
 @pytest.mark.parametrize("dim", [64, 128, 256, 96])
 @pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32"), ("f16", "f16")])
