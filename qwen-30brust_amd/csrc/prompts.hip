@@ -772,9 +772,17 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 #pragma unroll
                 for (uint32_t i = 0; i < NQ; i++) q[i] = __uint_as_float(xq[i / 4][i % 4]) * a.sign;
             } else {
-                const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u, keep = a.sign == 0.f ? 0u : ~0u;
+                const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-                for (uint32_t g = 0; g < NQ; g++) xq[g] = (xq[g] ^ flip) & keep;
+                for (uint32_t g = 0; g < NQ; g++) xq[g] ^= flip;
+                if (a.sign == 0.f) {  // 0 times what is not finite is NaN
+                    constexpr uint32_t top = QKIND == F16 ? 0x7c00u : 0x7f80u;
+                    auto none = [](uint32_t x) { return (x & top) == top ? 0x7fffu : 0u; };
+#pragma unroll
+                    for (uint32_t g = 0; g < NQ; g++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) xq[g][j] = none(xq[g][j]) | none(xq[g][j] >> 16) << 16;
+                }
                 if constexpr (Q8) {
                     // bf16 queries as f16, the row's largest finite value in [2^14, 2^15): what lies below 2^-39
                     // of it is lost, what is not finite stays so

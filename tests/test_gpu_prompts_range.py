@@ -73,6 +73,24 @@ def test_infinite_queries_over_codes(dev):
     close(got[:, 2:], want, bound)
 
 
+@pytest.mark.parametrize("q,kv,dim", [("bf16", "bf16", 64), ("f16", "f16", 128), ("bf16", "q8_0", 64), ("f32", "f32", 64), ("f32", "bf16", 64),
+                                      ("bf16", "bf16", 96)])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_scale_of_zero(dev, q, kv, dim, what):
+    """0 times what is not finite is NaN; the other rows are means."""
+    cache, table, lengths, first, query = make(3, [20, 0], [40, 9], 4, 2, dim, 16, q, kv)
+    query[7, 1, 3] = query[45, 2, dim - 1] = what
+    c = serving.PagedCache(dev, *cache)
+    got = c.attend_prompts(query.cuda(), table.cuda(), ints(lengths), ints(first), scale=0.0)
+    assert got[7, 1].isnan().all() and got[45, 2].isnan().all()
+    query[7, 1, 3] = query[45, 2, dim - 1] = 0
+    got[7, 1] = got[45, 2] = 0
+    want, bound = attend_many(query, values(cache[0], cache[2]), values(cache[1], cache[3]), table, lengths, first, 0.0, None,
+                              split_of(q, kv))
+    want[7, 1] = want[45, 2] = 0
+    close(got, want, bound)
+
+
 # ------------------------------------------------------- values near the end of their range
 @pytest.mark.parametrize("dim", [64, 128, 256, 96])
 @pytest.mark.parametrize("q,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32"), ("f16", "f16")])
