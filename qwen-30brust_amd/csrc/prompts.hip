@@ -889,6 +889,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                 for (uint32_t d = lane; d < D; d += 64) {
                     part[d] = d < dim ? value(a.c.k, a.c.ks, at + d) : 0.f;
                     part[D + d] = d < dim ? value(a.c.v, a.c.vs, at + d) : 0.f;
+                    if constexpr (Q8) part[D + d] = (float)(_Float16)part[D + d];  // as in the other steps
                 }
                 settle();
                 float x = 0.f;

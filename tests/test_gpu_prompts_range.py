@@ -111,3 +111,26 @@ def test_sums_that_fit(dev, q, kv, dim):
 
     got = run(dev, [n], [new], 4, 2, dim, 16, q, kv, scale=1.0, change=change)
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_codes_past_f16(dev, tree, dim):
+    """Code times scale past 65504 is not finite in every row that sees it, wherever it lies, and in no other."""
+    context, new = [300, 40, 0], [40, 60, 64]
+    cache, table, lengths, first, query = make(4, context, new, 4, 2, dim, 16, "bf16", "q8_0")
+    for b, (c, n) in enumerate(zip(context, new)):
+        for t in {c // 3, c + n // 2, c + n - 1}:
+            cache[1][at(table, b, t)][b % 2, 1 + t % 9] = 127 if t % 2 else -127
+            cache[3][at(table, b, t)][b % 2, 0] = 700.0
+    k, v = values(cache[0], cache[2]), values(cache[1], cache[3])
+    assert (v.abs() > 65520).sum() > 0 and (v.abs() > 65504).sum() == (v.abs() > 65520).sum()
+    bits = trees(torch.Generator().manual_seed(1), new)[1] if tree else None
+    rounded = v.float().half().double()
+    want, bound = attend_many(query, k, rounded, table, lengths, first, 0.01, bits, split_of("bf16", "q8_0"))
+    c = serving.PagedCache(dev, *cache)
+    args = (query.cuda(), table.cuda(), ints(lengths), ints(first))
+    got = c.attend_tree(*args, signed(bits).cuda(), scale=0.01) if tree else c.attend_prompts(*args, scale=0.01)
+    assert not torch.isfinite(want).all()
+    # values of up to 65504 beside the infinite ones, rounded as `rounded` is
+    close(got, want, bound)
