@@ -561,8 +561,8 @@ int qh_paged_plan(qh_ctx *ctx, const qh_pool_t *pool, int32_t *table, size_t tab
  * strides, with the same tables), to the slots behind the context, in order.
  * Outputs: new_length[batch] = length - nodes + accepted; accepted[batch] (root
  * included); path[n]: the accepted nodes' numbers from the sequence's first row on, -1
- * in its other rows and in those in front of first[0] and behind first[batch];
- * next[batch] = chosen at the last of them.  A sequence without
+ * in its other rows and in those in front of first[0] and behind first[batch] (a
+ * batch of 0 writes nothing); next[batch] = chosen at the last of them.  A sequence without
  * nodes, with more than 64, or whose length, bounds or pages (those of its nodes) are
  * out of range: length as it was, 0 accepted, next -1, nothing moves (and
  * the rows of one whose bounds do not ascend within 0 .. n are left as they were).  No

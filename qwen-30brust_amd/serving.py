@@ -364,8 +364,10 @@ def accept(caches, parents, tokens, chosen, table, lengths, first):
     n = parents.shape[0]
     _need(tokens.shape[0] == n and chosen.shape[0] == n, "a drafted and a chosen token for each node")
     _need(first.shape[0] == batch + 1, "first tokens: one more than sequences is needed")
-    new, accepted, following, path = torch.empty(3 * batch + n, dtype=torch.int32,
-                                                 device=table.device).split_with_sizes((batch, batch, batch, n))
+    held = torch.empty(3 * batch + n, dtype=torch.int32, device=table.device)
+    if not batch:
+        held.fill_(-1)  # nothing is launched: rows of no sequence
+    new, accepted, following, path = held.split_with_sizes((batch, batch, batch, n))
     pages = (engine._Pages * len(caches))(*(c._pages for c in caches))
     dev._check(engine.lib().qh_paged_accept(_live(dev), pages, len(caches), seqs, first.data_ptr(), n, parents.data_ptr(),
                                             tokens.data_ptr(), chosen.data_ptr(), new.data_ptr(), accepted.data_ptr(),

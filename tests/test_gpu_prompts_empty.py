@@ -1,11 +1,11 @@
-"""Sequences without new tokens between those that have some."""
+"""Sequences without new tokens between those that have some, and batches without sequences."""
 import importlib
 
 import pytest
 import torch
 
 from prompts_reference import attend_many, close, make, split_of
-from serving_reference import values
+from serving_reference import make_cache, values
 from test_gpu_prompts import ints
 
 engine = importlib.import_module("qwen-30brust_amd")
@@ -61,3 +61,15 @@ def test_sequences_without_tokens_take_no_turns(dev):
     apart = gaps(dev, [0, 20000, 40000, 60000, 65534], batch, "bf16", "bf16")[0]
     beside = gaps(dev, [65530, 65531, 65532, 65533, 65534], batch, "bf16", "bf16")[0]
     assert took(apart) < 5 * took(beside)
+
+
+def test_acceptance_without_sequences(dev):
+    """No sequences, and rows of none: no node is accepted."""
+    g = torch.Generator().manual_seed(1)
+    cache = serving.PagedCache(dev, *make_cache(g, 4, 16, 2, 64, "f32"))
+    x = ints([-1, 0, 0, 1, 2])
+    held = torch.full((20,), 77, dtype=torch.int32, device="cuda")  # memory that the outputs may get
+    del held
+    new, accepted, path, following = serving.accept([cache], x, x, x, torch.zeros(0, 2, dtype=torch.int32, device="cuda"),
+                                                    ints([]), ints([0]))
+    assert new.shape == accepted.shape == following.shape == (0,) and path.tolist() == [-1] * 5
