@@ -59,6 +59,21 @@ def test_large_scale_over_codes(dev, dim):
     run(dev, [70, 0], [33, 60], 4, 2, dim, 16, "bf16", "q8_0", scale=2.0 ** 20, change=change)
 
 
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_wide_query_rows_over_codes(dev, tree, dim):
+    """Rows whose largest element meets codes of 0: the others, 2^-45 to 2^-20 of it, decide, and what is below 2^-39 is lost."""
+    def change(cache, table, lengths, first, query):
+        g = torch.Generator().manual_seed(7)
+        power = torch.randint(-45, -19, query.shape, generator=g)
+        power[..., 0] = 0
+        query.copy_((query.double().clamp(-2, 2) * 2.0 ** power.double()).to(query.dtype))
+        query[..., 0] = 2.0
+        cache[0][..., 0] = 0
+
+    run(dev, [70, 0, 300], [33, 20, 40], 4, 2, dim, 16, "bf16", "q8_0", tree=tree, scale=2.0 ** 18, change=change)
+
+
 def test_infinite_queries_over_codes(dev):
     """An infinity beside large elements: the scores are its alone, -inf for codes above 0 under -inf."""
     cache, table, lengths, first, query = make(3, [20], [40], 4, 2, 64, 16, "bf16", "q8_0")
@@ -134,3 +149,49 @@ def test_codes_past_f16(dev, tree, dim):
     assert not torch.isfinite(want).all()
     # values of up to 65504 beside the infinite ones, rounded as `rounded` is
     close(got, want, bound)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_masked_scales(dev, tree, dim):
+    """NaN and infinite scales of keys and values that a row does not see change nothing; those of values that it sees
+    come out as the formula has them, and a NaN key scale as NaN."""
+    context, new = [100, 0, 33], [40, 60, 30]
+    cache, table, lengths, first, query = make(4, context, new, 8, 2, dim, 16, "bf16", "q8_0")
+    ks, vs = cache[2], cache[3]
+    for b, (c, n) in enumerate(zip(context, new)):
+        for t, (x, value) in zip((c + n - 1, c + n // 2, c + n // 3, c + 5),
+                                 ((vs, math.nan), (vs, math.inf), (vs, -math.inf), (ks, math.nan))):
+            x[at(table, b, t)][b % 2, t % (dim // 32)] = value
+        for t in range(c + n, -(-(c + n) // 16) * 16):
+            ks[at(table, b, t)] = math.nan
+            vs[at(table, b, t)] = math.inf
+    k, v = values(cache[0], cache[2]), values(cache[1], cache[3])
+    bits = trees(torch.Generator().manual_seed(1), new)[1] if tree else None
+    more = table, lengths, first, 0.1, bits, split_of("bf16", "q8_0")
+    want = attend_many(query, k, v, *more)[0]
+    # rows that see a NaN key are NaN; the others' error has no part of it
+    bound = attend_many(query, k.nan_to_num(0), v, *more)[1]
+    c = serving.PagedCache(dev, *cache)
+    args = (query.cuda(), table.cuda(), ints(lengths), ints(first))
+    got = c.attend_tree(*args, signed(bits).cuda(), scale=0.1) if tree else c.attend_prompts(*args, scale=0.1)
+    close(got, want, bound)
+
+
+# ------------------------------------------------------- lengths over codes
+@pytest.mark.parametrize("heads,kvheads,dim", [(8, 2, 128), (8, 1, 64), (16, 2, 64)])
+@pytest.mark.parametrize("context,new", [([0], [1500]), ([3100], [400]), ([0, 2900, 17], [700, 130, 450])])
+def test_longer_over_codes(dev, heads, kvheads, dim, context, new):
+    run(dev, context, new, heads, kvheads, dim, 16, "bf16", "q8_0")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("context,new", [([30001], [3]), ([9000, 3, 500], [64, 64, 1])])
+def test_tree_long_over_codes(dev, dim, context, new):
+    run(dev, context, new, 8, 1, dim, 64, "bf16", "q8_0", tree=True)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("heads", [1, 3, 130])
+def test_groups_over_codes(dev, tree, heads):
+    run(dev, [50, 0], [20, 9], heads, 1, 64, 16, "bf16", "q8_0", tree=tree)
