@@ -415,7 +415,9 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
         auto fetch = [&](uint32_t k0, uint32_t buf, uint32_t r) {
             if constexpr (DIRECT) {
                 // 16 bytes a lane from its own address to LDS.  In assembly, as the compiler lets every
-                // later LDS read wait for such loads, of whatever buffer; meet() waits for them.
+                // later LDS read wait for such loads, of whatever buffer; meet() waits for them.  With the move
+                // five wait states, as a load needs behind a vector instruction that writes its scalar
+                // address (one read back from a spilled lane, which the compiler does not see read here).
                 if (r == 0) found();
                 const uint32_t line = lane / PER, t = __builtin_amdgcn_readlane(first, r);
                 const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(first_at >> 32), r) << 32 |
@@ -426,8 +428,8 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                 const uint32_t off = min(line, end - 1 - t) * (uint32_t)(sizeof(T) * a.c.ts) + chunk;
 #if defined(__HIP_DEVICE_COMPILE__)
                 const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds[buf] + (r * kWaves + wv) * 1024;
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(kbase + at) : "memory");
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + 2 * TILE), "v"(off), "s"(vbase + at) : "memory");
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(kbase + at) : "memory", "m0");
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + 2 * TILE), "v"(off), "s"(vbase + at) : "memory", "m0");
 #else
                 (void)at, (void)off;
 #endif
