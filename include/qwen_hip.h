@@ -492,10 +492,11 @@ int qh_paged_evict(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *s
  * ones.  BF16 queries and out over Q8_0 (heads up to 128 wide, a multiple of 8, rows
  * aligned to 8 bytes) are taken in F16 products: weights and values (code times
  * scale) are rounded to F16, so a value past 65504 comes out not finite, and an
- * element of a query is rounded below 2^-31 of the largest of its row and lost below
- * 2^-39.  All other mixes
- * and an F32 out are in 32 bits.  q and out may be the same.  A call whose tokens
- * times heads pass 2^31, or with the keys 2^62, is refused. */
+ * element of a query is rounded below 2^-31 of the largest finite one of its row and
+ * lost below 2^-39.  All other mixes and an F32 out are in 32 bits.  Rows that the bounds
+ * give to two sequences hold what either makes of them, values of both mixed.  q and
+ * out may be the same.  A call whose tokens times heads pass 2^31, or with the keys
+ * 2^62, is refused. */
 int qh_paged_prompts(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *seqs, const int32_t *first, size_t n,
                      const qh_heads_t *q, uint32_t heads, float scale, const qh_heads_t *out, void *workspace,
                      size_t workspace_bytes, void *stream);
@@ -538,6 +539,8 @@ typedef struct {
  * ([batch][table_pages], table_stride apart) of which held[b] entries are in use get
  * pages from the pool, or give those back that the new length does not need, all in
  * place.  Pages that are given back may go to a sequence that grows in the same call.
+ * A sequence that grows keeps the pages that it holds beyond its new length; one whose
+ * grow is 0 or less gives back all that its new length does not need.
  * Growth is served in the sequences' order, and from the first on that asks for more
  * pages than are left, or brings the new tokens past n, no sequence grows: it keeps
  * its length and gets no tokens (first tells).  So does one whose length, held pages or
@@ -565,7 +568,9 @@ int qh_paged_plan(qh_ctx *ctx, const qh_pool_t *pool, int32_t *table, size_t tab
  * batch of 0 writes nothing); next[batch] = chosen at the last of them.  A sequence without
  * nodes, with more than 64, or whose length, bounds or pages (those of its nodes) are
  * out of range: length as it was, 0 accepted, next -1, nothing moves (and
- * the rows of one whose bounds do not ascend within 0 .. n are left as they were).  No
+ * the rows of one whose bounds do not ascend within 0 .. n are left as they were; rows
+ * that the bounds give to two, or that lie in a sequence and in front of first[0] or
+ * behind first[batch], hold what either has there).  No
  * output may lie where the call reads, no cache is given twice, and the pages that hold
  * a sequence's nodes are in no other sequence. */
 int qh_paged_accept(qh_ctx *ctx, const qh_pages_t *caches, size_t layers, const qh_sequences_t *seqs,

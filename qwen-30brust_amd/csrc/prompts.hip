@@ -17,12 +17,13 @@
 // bytes.  Measured, with 32 query heads over 4 KV heads of 128 values, on a card whose
 // large products reach 1,104 TFLOP/s in f16, 1,160 in bf16 and 153 in f32, and whose large
 // copies 4.6 TB/s (products that a causal row sees, join included):
-//   16,381 tokens, f16                         2.29 ms   960 TFLOP/s; the clock falls to 1.9 GHz
-//   24 prompts of 1 to 2,100 tokens, bf16      0.60 ms   599 TFLOP/s
-//   2 x 512 tokens behind 12,000 to 15,000, Q8_0   0.56 ms   414 TFLOP/s; the vector units: codes to f16, scales
+//   16,381 tokens, f16                         2.26 ms   974 TFLOP/s; the clock falls to 1.9 GHz
+//   24 prompts of 1 to 2,100 tokens, bf16      0.59 ms   607 TFLOP/s
+//   2 x 512 tokens behind 12,000 to 15,000, Q8_0   0.545 ms   424 TFLOP/s; the vector units: codes to f16, scales
 //   517 tokens, f32                              59 us    37 TFLOP/s; runs of 4 to 5 steps
-//   2 trees of 64 nodes behind 65,473 keys, f16 175 us   788 TFLOP/s, 1.5 TB/s
-//   48 trees behind up to 4,096 keys, bf16       79 us   2.7 TB/s
+//   2 trees of 64 nodes behind 65,537 keys, f16 173 us   797 TFLOP/s, 1.6 TB/s
+//   48 trees behind up to 4,096 keys, bf16       79 us   203 MB of keys and values, of which trees of more than 128
+//                                                        rows read theirs once a tile: 324 MB in the kernel's 62 us
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -292,7 +293,9 @@ constexpr uint32_t kDirect = 100, kAny = 101;
 // types keys 16 c + 8 (e / 4) + 4 (lane / 32) + e % 4 are element e, for V^T read by the
 // transposing LDS read.  K and V of the next step come in while one is worked on, asked
 // for between the products of the scores (16,381 tokens 2.73 -> 2.55 ms).  The weights are
-// rounded once to T, at most half a step of it each, and the sum is of the rounded ones;
+// rounded once to T, at most half a step of it each, and the sum is of the rounded ones (in two
+// parts, as the attention of single tokens has them, another product of the values for each:
+// 16,381 tokens 2.26 -> 3.28 ms, 24 prompts 0.59 -> 0.72, 48 trees 79 -> 93 us);
 // everything else between the products is in 32 bits.  Written so that none of the kernels
 // spills vector registers: what is wanted once a tile is computed there anew.
 template <class T, uint32_t D, uint32_t SRC>
@@ -969,7 +972,7 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 // out of the tiles that several workgroups hold parts of: a workgroup for the first
 // run that begins inside a tile and 1,024 of its values, four a thread.  The parts: the
 // second slot of the run in front, and the first slot of those up to the last.  Bound by
-// what it reads, which is in the caches: 10 to 13 us behind a full grid.
+// what it reads, which is in the caches: 9 to 18 us behind a full grid.
 __global__ __launch_bounds__(kBlock) void k_page_many_join(PageMany a) {
     const uint32_t D = a.wide, w = blockIdx.x + 1;
     const uint32_t runs = min(*runs_of(a), a.runs);
@@ -1022,14 +1025,14 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.out_wide = aligned(a.out, a.out.kind == F32 ? 16 : 8);
     a.kv_wide = d % 8 == 0 && (((uintptr_t)a.c.k | (uintptr_t)a.c.v | (a.c.ps | a.c.ts | a.c.hs) * es) % std::min(8 * es, 16u)) == 0;
     // Products of 16 bits: of the cache's own type, or of f16 where bf16 queries read Q8_0 (the two
-    // prompts over Q8_0 0.56 ms, 2.27 in 32 bits); wider heads' codes and registers do not fit.
+    // prompts over Q8_0 0.545 ms, 2.27 in 32 bits); wider heads' codes and registers do not fit.
     a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
                (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && d <= 128 && a.q.kind == BF16 && a.out.kind == BF16));
     // What a tile's start and end cost, in keys: queries in, values out (256 rather than 32: 16,381
     // tokens 2.67 -> 2.31 ms, 24 prompts 0.81 -> 0.59, 48 trees 103 -> 77 us), and the least that a run
     // is worth having (128, of four steps less than one for its start: a tree behind 517 keys 22.4 us,
-    // with 64 25.3, with 256 23.3, with 1,024 38.4; f32, where a key costs eight times as much, 32:
-    // 517 tokens 64 us, with 256 84).
+    // with 64 25.3, with 256 23.3, with 1,024 38.4; f32, where a key costs eight times as much, 32, and
+    // 16 or 64 take as long: 517 tokens 64 us, with 256 84).
     a.tile_keys = a.narrow ? 256 : 32;
     a.run_keys = a.narrow ? 128 : 32;
     a.one_page = a.c.page % std::max(1024 / (a.wide * es), 1u) == 0 && a.c.ps * es >> 32 == 0 && (unsigned __int128)a.c.page * a.c.ts * es >> 32 == 0;
@@ -1042,8 +1045,9 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     const uint64_t tiles = ((uint64_t)a.n * a.group / kTileRows + a.r.batch) * a.c.kvheads;
     const uint64_t most = tiles * (a.r.most / a.run_keys + 2);
     // A run for each workgroup that is there at once: two a unit by registers (one: 16,381 tokens 2.31 ->
-    // 3.22 ms), and one of the kernels with 256 values, or Q8_0's codes of 128, which hold more (two:
-    // 48 trees of 256 values 192 -> 207 us, Q8_0 0.56 -> 0.575 ms; 24 prompts of 256 1.38 -> 1.35).
+    // 3.22 ms), and one of the kernels with 256 values, or Q8_0's codes of 128, whose registers leave room
+    // for one (two, one behind the other: 48 trees of 256 values 192 -> 207 us, Q8_0 0.545 -> 0.559 ms; 24
+    // prompts of 256 1.38 -> 1.35).
     const bool alone = a.wide == 256 || (a.narrow && a.c.kind == Q8_0 && a.wide == 128);
     a.runs = (uint32_t)std::min<uint64_t>(cus * (alone ? 1 : 2), std::max<uint64_t>(most, 1));
 }

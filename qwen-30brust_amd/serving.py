@@ -219,7 +219,10 @@ class PagedCache:
         last of its `lengths[b]` keys (appended before) their own, and each sees
         the keys up to its own.  A whole prompt, the next piece of one, or a single
         token.  out like q (allocated if not given); rows of no sequence are left as
-        they were.  most and scale as in attend."""
+        they were.  most and scale as in attend.  With 16-bit q and out over a
+        cache of their type, or bf16 ones over Q8_0, softmax weights (over Q8_0 the
+        values too) are rounded once to 16 bits, fewer than the 17 to 23 of attend; an f32 out
+        keeps 32."""
         return self._many(q, table, lengths, first, None, most, scale, out)
 
     def attend_tree(self, q, table, lengths, first, ancestors, most=None, *, scale=None, out=None):
@@ -309,8 +312,10 @@ class PagePool:
     def plan(self, table, held, lengths, grow, n, *, parents=None, out=None):
         """Grows sequences by `grow` tokens (shrinks them where it is negative):
         table [batch][pages] and held [batch], the entries of its rows in use, get pages
-        or give them back in place.  n: room for new tokens; growth ends with the
-        first sequence that does not fit into n or the free pages.  Returns a Plan:
+        or give them back in place.  One that grows keeps pages held beyond its
+        length; with 0 or less all that its new length does not need go back.  n: room
+        for new tokens; growth ends with the first sequence that does not fit into n
+        or the free pages.  Returns a Plan:
         lengths [batch] (out, which may be lengths; allocated if not given), first
         [batch + 1], and for each of n rows, packed by first, slots (int64: page id * page
         + slot), positions, sequences (-1 behind the last token) and, with parents
