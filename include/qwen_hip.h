@@ -487,12 +487,12 @@ int qh_paged_evict(qh_ctx *ctx, const qh_pages_t *cache, const qh_sequences_t *s
  * or of a sequence whose bounds do not ascend within 0 .. n) are left as they were.
  * Keys and values that a row does not see take no part in it, whatever they hold.
  * Sums and maxima in 32 bits, out rounded once to its kind.  With queries and out of
- * 16 bits over a cache of the queries' kind, each softmax weight is rounded once to
- * that kind before it meets its value, and the sum it is divided by is of the rounded
- * ones (F16: steps of at least 2^-31 of a row's largest weight, so one below 2^-32 of it
- * counts nothing).  BF16 queries and out over Q8_0 (heads up to 128 wide, a multiple of 8, rows
- * aligned to 8 bytes) are taken in F16 products: weights and values (code times
- * scale) are rounded to F16, so a value past 65504 comes out not finite, and an
+ * 16 bits over a cache of the queries' kind a key's softmax weight enters the products
+ * with 17 bits (BF16) or 23 (F16, in steps no finer than 2^-35 of a row's largest weight, so
+ * that one below 2^-36 of it may count nothing).  BF16 queries and out over Q8_0 (heads up
+ * to 128 wide, a multiple of 8, rows aligned to 8 bytes) are taken in F16 products:
+ * weights (in steps no finer than 2^-31 of the largest) and values (code times scale) are
+ * rounded once to F16, so a value past 65504 comes out not finite, and an
  * element of a query is rounded below 2^-31 of the largest finite one of its row and
  * lost below 2^-39.  All other mixes and an F32 out are in 32 bits.  Rows that the bounds
  * give to two sequences hold what either makes of them, values of both mixed.  q and

@@ -17,13 +17,13 @@
 // bytes.  Measured, with 32 query heads over 4 KV heads of 128 values, on a card whose
 // large products reach 1,104 TFLOP/s in f16, 1,160 in bf16 and 153 in f32, and whose large
 // copies 4.6 TB/s (products that a causal row sees, join included):
-//   16,381 tokens, f16                         2.26 ms   974 TFLOP/s; the clock falls to 1.9 GHz
-//   24 prompts of 1 to 2,100 tokens, bf16      0.59 ms   607 TFLOP/s
+//   16,381 tokens, f16                         3.18 ms   691 TFLOP/s, with the weights' second parts 1,037
+//   24 prompts of 1 to 2,100 tokens, bf16      0.69 ms   522 TFLOP/s, 783
 //   2 x 512 tokens behind 12,000 to 15,000, Q8_0   0.545 ms   424 TFLOP/s; the vector units: codes to f16, scales
 //   517 tokens, f32                              59 us    37 TFLOP/s; runs of 4 to 5 steps
-//   2 trees of 64 nodes behind 65,537 keys, f16 173 us   797 TFLOP/s, 1.6 TB/s
-//   48 trees behind up to 4,096 keys, bf16       79 us   203 MB of keys and values, of which trees of more than 128
-//                                                        rows read theirs once a tile: 324 MB in the kernel's 62 us
+//   2 trees of 64 nodes behind 65,537 keys, f16 228 us   605 TFLOP/s, 910; 1.2 TB/s
+//   48 trees behind up to 4,096 keys, bf16       89 us   326 TFLOP/s, 489; 203 MB of keys and values, of which trees of
+//                                                        more than 128 rows read theirs once a tile: 324 MB
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -292,11 +292,13 @@ constexpr uint32_t kDirect = 100, kAny = 101;
 // exchange, and the weights lie where O^T = V^T P^T wants its second operand: for 16-bit
 // types keys 16 c + 8 (e / 4) + 4 (lane / 32) + e % 4 are element e, for V^T read by the
 // transposing LDS read.  K and V of the next step come in while one is worked on, asked
-// for between the products of the scores (16,381 tokens 2.73 -> 2.55 ms).  The weights are
-// rounded once to T, at most half a step of it each, and the sum is of the rounded ones (in two
-// parts, as the attention of single tokens has them, another product of the values for each:
-// 16,381 tokens 2.26 -> 3.28 ms, 24 prompts 0.59 -> 0.72, 48 trees 79 -> 93 us);
-// everything else between the products is in 32 bits.  Written so that none of the kernels
+// for between the products of the scores (16,381 tokens 2.73 -> 2.55 ms).  A weight meets its
+// values in two parts of T, rounded and what that left: 17 bits in bf16, 23 in f16, as in the
+// attention of single tokens, so that an output is off by its own rounding alone.  One part would
+// be faster (16,381 tokens 2.26 ms rather than 3.18, 24 prompts 0.59 rather than 0.69, 48 trees 79
+// rather than 89 us) and 1.2 to 1.4 times as far off.  Everything else between the products is in
+// 32 bits, but over Q8_0, in f16 products under outputs of bf16, whose weights and values are rounded
+// once, three bits finer than the outputs.  Written so that none of the kernels
 // spills vector registers: what is wanted once a tile is computed there anew.
 template <class T, uint32_t D, uint32_t SRC>
 __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std::is_same<T, _Float16>::value) ? 1 : 2) void k_page_many(PageMany a) {
@@ -306,9 +308,11 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
     constexpr uint32_t NS = KT / 32, ND = D / 32, CH = D * sizeof(T) / 16, TILE = KT * D * sizeof(T);
     constexpr uint32_t NQ = F ? D / 2 : D / 16;
     constexpr uint32_t QKIND = F ? F32 : H && !Q8 ? F16 : BF16;  // of queries that are loaded as they are
-    // weights are at most 2^(kAhead + kUp): in f16 2^15, so that small ones have their bits; in bf16, which has f32's
-    // exponents, 1, so that sums of values up to 2^128 / keys fit
-    constexpr float kAhead = 8.f, kUp = H ? 7.f : F ? 0.f : -kAhead;
+    constexpr bool TWO = !F && !Q8;  // parts of a weight
+    // weights are at most 2^(kAhead + kUp): in f16 2^15, so that small ones have their bits, the more the closer the
+    // reference stays to the maximum (4 and 8 take as long; over Q8_0 4 0.573 ms rather than 0.549); in bf16, which has
+    // f32's exponents, 1, so that sums of values up to 2^128 / keys fit
+    constexpr float kAhead = TWO ? 4.f : 8.f, kUp = F ? 0.f : H ? 15.f - kAhead : -kAhead;
     typedef typename std::conditional<H, h8, b8>::type T8;
     typedef typename std::conditional<F, float, T8>::type Q;
     __shared__ __align__(16) uint8_t lds[4][TILE];  // K, K, V, V; in front and behind a part for each wave
@@ -708,19 +712,20 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                 }
             } else {
                 constexpr uint32_t C = 2 * NS;
-                T8 p[C];
-                // weights 2 i and 2 i + 1 of p[c]; the sum is of the rounded ones, so that equal errors of all cancel
+                T8 p[C], rest[TWO ? C : 1];
+                // weights 2 i and 2 i + 1 of p[c], and of rest[c] what their rounding left
                 auto weights = [&](uint32_t c, uint32_t i) {
                     const uint32_t m = c / 2, j = c % 2 * 8 + 2 * i;
                     const float x = exp2_of(fmaf(sc[m][j], c2, -Mf)), y = exp2_of(fmaf(sc[m][j + 1], c2, -Mf));
-                    if constexpr (H) {
-                        const h2 z = {(_Float16)x, (_Float16)y}, ones = {(_Float16)1.f, (_Float16)1.f};
-                        L = __builtin_amdgcn_fdot2(z, ones, L, false);
-                        p[c][2 * i] = z[0], p[c][2 * i + 1] = z[1];
+                    typedef typename std::conditional<H, h2, b2>::type T2;
+                    const T2 z = {(T)x, (T)y};
+                    p[c][2 * i] = z[0], p[c][2 * i + 1] = z[1];
+                    if constexpr (TWO) {
+                        L += x + y;
+                        const T2 r = {(T)fmaf((float)z[0], -1.f, x), (T)fmaf((float)z[1], -1.f, y)};
+                        rest[c][2 * i] = r[0], rest[c][2 * i + 1] = r[1];
                     } else {
-                        const b2 z = {(bf16_t)x, (bf16_t)y}, ones = {(bf16_t)1.f, (bf16_t)1.f};
-                        L = __builtin_amdgcn_fdot2_f32_bf16(z, ones, L, false);
-                        p[c][2 * i] = z[0], p[c][2 * i + 1] = z[1];
+                        L = __builtin_amdgcn_fdot2(z, T2{(T)1.f, (T)1.f}, L, false);
                     }
                 };
                 if (masked() && odd != ~0u) {
@@ -728,6 +733,10 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
                     for (uint32_t i = 0; i < 4 * C; i++) weights(i / 4, i % 4);
                     return;
                 }
+                auto add = [&](uint32_t d, const T8& v, const T8& w) {
+                    if constexpr (H) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w, o[d], 0, 0, 0);
+                    else o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w, o[d], 0, 0, 0);
+                };
                 // a step of 16 keys: V's parts and the weights of the next between its products
                 if constexpr (Q8)
 #pragma unroll
@@ -735,18 +744,19 @@ __global__ __launch_bounds__(kBlock, D == 256 || (SRC == Q8_0 && D == 128 && std
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) weights(0, i);
                 in_order();
+                constexpr uint32_t EACH = TWO ? 2 * ND : ND;  // products of 16 keys
 #pragma unroll
                 for (uint32_t c = 0; c < C; c++)
 #pragma unroll
-                    for (uint32_t d = 0; d < ND; d++) {
-                        if constexpr (H) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[c % 2][d], p[c], o[d], 0, 0, 0);
-                        else o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c % 2][d], p[c], o[d], 0, 0, 0);
+                    for (uint32_t u = 0; u < EACH; u++) {
+                        const uint32_t d = u % ND;
+                        add(d, x[c % 2][d], u < ND ? p[c] : rest[TWO ? c : 0]);
                         if (c + 1 < C) {
-                            x[(c + 1) % 2][d] = v_part(c + 1, d);
+                            if (u < ND) x[(c + 1) % 2][d] = v_part(c + 1, d);
 #pragma unroll
-                            for (uint32_t i = d * 4 / ND; i < (d + 1) * 4 / ND; i++) weights(c + 1, i);
+                            for (uint32_t i = u * 4 / EACH; i < (u + 1) * 4 / EACH; i++) weights(c + 1, i);
                         }
-                        behind(c * ND + d, C * ND);
+                        behind(c * EACH + u, C * EACH);
                         in_order();
                     }
             }

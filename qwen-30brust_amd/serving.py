@@ -220,9 +220,9 @@ class PagedCache:
         the keys up to its own.  A whole prompt, the next piece of one, or a single
         token.  out like q (allocated if not given); rows of no sequence are left as
         they were.  most and scale as in attend.  With 16-bit q and out over a
-        cache of their type, or bf16 ones over Q8_0, softmax weights (over Q8_0 the
-        values too) are rounded once to 16 bits, fewer than the 17 to 23 of attend; an f32 out
-        keeps 32."""
+        cache of their type softmax weights keep attend's 17 bits (bf16) or 23 (f16);
+        with bf16 ones over Q8_0 weights and values keep 11, where attend has 23; an
+        f32 out keeps 32."""
         return self._many(q, table, lengths, first, None, most, scale, out)
 
     def attend_tree(self, q, table, lengths, first, ancestors, most=None, *, scale=None, out=None):
