@@ -17,11 +17,11 @@
 // bytes.  Measured, with 32 query heads over 4 KV heads of 128 values, on a card whose
 // large products reach 1,104 TFLOP/s in f16, 1,160 in bf16 and 153 in f32, and whose large
 // copies 4.6 TB/s (products that a causal row sees, join included):
-//   16,381 tokens, f16                         3.18 ms   691 TFLOP/s, with the weights' second parts 1,037
-//   24 prompts of 1 to 2,100 tokens, bf16      0.69 ms   522 TFLOP/s, 783
+//   16,381 tokens, f16                         3.17 ms   694 TFLOP/s, with the weights' second parts 1,041
+//   24 prompts of 1 to 2,100 tokens, bf16      0.68 ms   523 TFLOP/s, 785
 //   2 x 512 tokens behind 12,000 to 15,000, Q8_0   0.545 ms   424 TFLOP/s; the vector units: codes to f16, scales
 //   517 tokens, f32                              59 us    37 TFLOP/s; runs of 4 to 5 steps
-//   2 trees of 64 nodes behind 65,537 keys, f16 228 us   605 TFLOP/s, 910; 1.2 TB/s
+//   2 trees of 64 nodes behind 65,537 keys, f16 231 us   595 TFLOP/s, 893; 1.2 TB/s
 //   48 trees behind up to 4,096 keys, bf16       89 us   326 TFLOP/s, 489; 203 MB of keys and values, of which trees of
 //                                                        more than 128 rows read theirs once a tile: 324 MB
 #include <algorithm>
@@ -292,10 +292,11 @@ constexpr uint32_t kDirect = 100, kAny = 101;
 // exchange, and the weights lie where O^T = V^T P^T wants its second operand: for 16-bit
 // types keys 16 c + 8 (e / 4) + 4 (lane / 32) + e % 4 are element e, for V^T read by the
 // transposing LDS read.  K and V of the next step come in while one is worked on, asked
-// for between the products of the scores (16,381 tokens 2.73 -> 2.55 ms).  A weight meets its
+// for between the products of the scores (16,381 tokens 2.73 -> 2.55 ms before a weight had two
+// parts).  A weight meets its
 // values in two parts of T, rounded and what that left: 17 bits in bf16, 23 in f16, as in the
 // attention of single tokens, so that an output is off by its own rounding alone.  One part would
-// be faster (16,381 tokens 2.26 ms rather than 3.18, 24 prompts 0.59 rather than 0.69, 48 trees 79
+// be faster (16,381 tokens 2.26 ms rather than 3.17, 24 prompts 0.59 rather than 0.68, 48 trees 79
 // rather than 89 us) and 1.2 to 1.4 times as far off.  Everything else between the products is in
 // 32 bits, but over Q8_0, in f16 products under outputs of bf16, whose weights and values are rounded
 // once, three bits finer than the outputs (both in two parts: two prompts behind 12,000 to 15,000 keys
@@ -1040,10 +1041,10 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.narrow = a.q.kind != F32 && a.out.kind != F32 &&
                (a.c.kind == a.q.kind || (a.c.kind == Q8_0 && a.kv_wide && d <= 128 && a.q.kind == BF16 && a.out.kind == BF16));
     // What a tile's start and end cost, in keys: queries in, values out (256 rather than 32: 16,381
-    // tokens 2.67 -> 2.31 ms, 24 prompts 0.81 -> 0.59, 48 trees 103 -> 77 us), and the least that a run
-    // is worth having (128, of four steps less than one for its start: a tree behind 517 keys 22.4 us,
-    // with 64 25.3, with 256 23.3, with 1,024 38.4; f32, where a key costs eight times as much, 32, and
-    // 16 or 64 take as long: 517 tokens 64 us, with 256 84).
+    // tokens 3.29 -> 3.23 ms, 24 prompts 0.93 -> 0.69, 48 trees 107 -> 89 us), and the least that a run
+    // is worth having (128, of four steps less than one for its start: a tree behind 517 keys 20.6 us,
+    // with 64 23.4, with 256 22.2; f32, where a key costs eight times as much, 32, and 16 or 64 take
+    // as long: 517 tokens 60 us).
     a.tile_keys = a.narrow ? 256 : 32;
     a.run_keys = a.narrow ? 128 : 32;
     a.one_page = a.c.page % std::max(1024 / (a.wide * es), 1u) == 0 && a.c.ps * es >> 32 == 0 && (unsigned __int128)a.c.page * a.c.ts * es >> 32 == 0;
@@ -1055,10 +1056,10 @@ void page_many_plan(PageMany& a, uint32_t cus) {
     a.c2 = a.scale == 0.f ? 1.f : std::max(std::fabs(a.scale) * kLog2e, kLeast);
     const uint64_t tiles = ((uint64_t)a.n * a.group / kTileRows + a.r.batch) * a.c.kvheads;
     const uint64_t most = tiles * (a.r.most / a.run_keys + 2);
-    // A run for each workgroup that is there at once: two a unit by registers (one: 16,381 tokens 2.31 ->
-    // 3.22 ms), and one of the kernels with 256 values, or Q8_0's codes of 128, whose registers leave room
-    // for one (two, one behind the other: 48 trees of 256 values 192 -> 207 us, Q8_0 0.545 -> 0.559 ms; 24
-    // prompts of 256 1.38 -> 1.35).
+    // A run for each workgroup that is there at once: two a unit by registers (one: 16,381 tokens 3.23 ->
+    // 4.04 ms, 24 prompts 0.69 -> 0.90), and one of the kernels with 256 values, or Q8_0's codes of 128, whose
+    // registers leave room for one (two, one behind the other: 48 trees of 256 values 194 -> 212 us, Q8_0 0.545 ->
+    // 0.559 ms; 24 prompts of 256 1.68 either way).
     const bool alone = a.wide == 256 || (a.narrow && a.c.kind == Q8_0 && a.wide == 128);
     a.runs = (uint32_t)std::min<uint64_t>(cus * (alone ? 1 : 2), std::max<uint64_t>(most, 1));
 }
@@ -1070,7 +1071,7 @@ template <class T, uint32_t SRC> static void launch_many(const PageMany& a, hipS
     else if constexpr (SRC == kDirect || SRC == kAny || (SRC == Q8_0 && std::is_same<T, float>::value)) hipLaunchKernelGGL((k_page_many<T, 256, SRC>), grid, block, 0, s, a);
 }
 void launch_page_many(const PageMany& a, hipStream_t s) {
-    // Rows straight to LDS (16,381 tokens 2.31 ms, value by value 3.36; 48 trees 77 us, 114) where a
+    // Rows straight to LDS (16,381 tokens 3.23 ms, value by value 4.44; 48 trees 89 us, 121) where a
     // wave's load of them lies in one page, which it finds once.
     const bool direct = a.kv_wide && a.one_page && a.c.dim == a.wide;
     if (a.narrow) {
